@@ -251,6 +251,8 @@ def prepare(case, seed):
             s["out"] = torch.empty(case["tokens"], case["q_heads"], case["head_dim"], device="cuda", dtype=torch.bfloat16)
         else:
             s["out"] = torch.empty_like(s["q"])
+        if kind in ("append", "attention"):
+            s["cache"] = sq.PagedCache(s["k_cache"], s["v_cache"], s["k_scale"], s["v_scale"])
     return s
 
 
@@ -273,11 +275,11 @@ def _run_own(case, s):
         return ctx.product_f8_quantized(s["x"], s["w"], s["scale"], bias=s["bias"], epilogue=case["epilogue"], out=s["out"])
     if kind == "append":
         q, k, v = s["heads"]
-        out = ctx.append_kv(q, k, v, s["k_cache"], s["v_cache"], s["positions"], s["slots"], s["table"], q_out=s["out"],
-                            interleaved=case["interleaved"], k_scale=s["k_scale"], v_scale=s["v_scale"])
+        out = ctx.append_kv(q, k, v, s["cache"], s["positions"], s["slots"], s["table"], q_out=s["out"],
+                            interleaved=case["interleaved"])
         return {"q": out, "k_cache": s["k_cache"], "v_cache": s["v_cache"]}
-    return ctx.paged_attention(s["q"], s["k_cache"], s["v_cache"], s["pages"], s["lengths"], softcap=case["softcap"],
-                               window=case["window"], k_scale=s["k_scale"], v_scale=s["v_scale"], out=s["out"])
+    return ctx.paged_attention(s["q"], s["cache"], s["pages"], s["lengths"], softcap=case["softcap"],
+                               window=case["window"], out=s["out"])
 
 
 def _norm_outputs(codes, scales, stream):
