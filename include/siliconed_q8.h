@@ -384,6 +384,90 @@ int sq8_rms_rows(sq8_ctx *ctx, uint16_t *t, int64_t ld, int64_t rows, int cols, 
 int sq8_gated_residual(sq8_ctx *ctx, float *x, int64_t ldx, const void *y, int y_dtype, int64_t ldy,
                        const float *gate, int64_t rows, int cols);
 
+/* ---- a text decoder's operators on block-scaled fp8 weights and a paged cache. No counterpart in the reference,
+ * whose text models run on the widened route: published fp8 checkpoints hold e4m3 codes with one scale per 128 × 128
+ * block, and their products take activations in e4m3 with one scale per 128 values of a row. All are queued on the
+ * context's stream; device values they read as indices (slots, positions, pages, lengths) are checked on the device,
+ * never trusted. ---- */
+
+/* **The norm of the residual stream's new sum, writing the next product's 8-bit operand.** For each of `rows` rows,
+ * s = r + x (x SQ8_BF16 or SQ8_F32, the stream `residual` SQ8_BF16 or SQ8_F32, or NULL: s = x), y = (s · 1/sqrt(mean(s²)
+ * + eps)) · w in fp32; s rounded to the stream's type goes to `residual_out` unless NULL (it may be `residual` itself;
+ * no other overlap) — the norm takes s before that rounding.
+ *   `codes_dtype` SQ8_FP8_E4M3: per 128 columns a scale t = max(max|y| / 448, 1e-30) and codes e4m3(y · (1/t)), nearest
+ *   even; scales [rows, ⌈cols/128⌉] with leading dimension lds — sq8_linear_f8's operand;
+ *   SQ8_INT8: per row t = max(max|y| / 127, 1e-30) and codes clamp(rint(y / t), −128, 127); scales [rows], lds unused —
+ *   sq8_linear_w8a8's operand.
+ * w fp32 [cols]; codes [rows, cols] with leading dimension ldq. Any cols to 32 768 (else SQ8_EUNSUPPORTED); rows that
+ * are not 16-byte aligned or a multiple of 8 wide are read one value at a time. */
+int sq8_add_norm_quantized(sq8_ctx *ctx, const void *x, int x_dtype, int64_t ldx,
+                           const void *residual, int r_dtype, int64_t ldr, void *residual_out, int64_t ldro,
+                           const float *w, float eps, void *codes, int codes_dtype, int64_t ldq,
+                           float *scales, int64_t lds, int rows, int cols);
+
+/* **The same quantization alone**: x [rows, cols] (SQ8_BF16 or SQ8_F32) to e4m3 codes and a scale per 128 columns, as
+ * sq8_add_norm_quantized writes them from y. Any cols. */
+int sq8_quantize_groups(sq8_ctx *ctx, const void *x, int x_dtype, int64_t ldx, int rows, int cols,
+                        void *codes, int64_t ldq, float *scales, int64_t lds);
+
+/* **The product of e4m3 codes by e4m3 codes.** C[i, j] = act(Σ_b sx[i, b] · sw[j/128, b] · (Σ_{k in b} A[i, k] ·
+ * W[j, k]) + bias[j]), b the blocks of 128 of K (the last may be short), sums fp32; for a bf16 C the matrix cores'
+ * e4m3 instructions drop, within each 8 consecutive K, what is under 2^-13 of the largest product's power of two (1.4e-5
+ * of a result's size on normal operands); for an fp32 C they do not. A: codes [m, k], leading dimension
+ * lda; sx fp32 [m, ⌈k/128⌉], ldsx. W: codes [n, k] as published, ldw; sw fp32 [⌈n/128⌉, ⌈k/128⌉], ldsw. `epilogue`
+ * SQ8_EPI_NONE, or SQ8_EPI_SILU_GLU (n = 2h, output h: silu(gate)·up): the halves are then blocked each by itself, sw
+ * [2·⌈h/128⌉, ⌈k/128⌉], gate's rows first (else SQ8_EUNSUPPORTED). bias fp32 [n] or NULL. C SQ8_BF16 or SQ8_F32, ldc.
+ * Codes are read in place where rows are 16-byte aligned and k is a multiple of 16, and copied padded into the
+ * context's buffers first where not (sq8_linear says when those grow). `gpu_seconds` as sq8_linear. */
+int sq8_linear_f8(sq8_ctx *ctx, const void *a, int64_t lda, const float *sx, int64_t ldsx,
+                  const void *w, int64_t ldw, const float *sw, int64_t ldsw,
+                  const float *bias, int epilogue, void *c, int c_dtype, int64_t ldc,
+                  int m, int k, int n, double *gpu_seconds);
+
+/* The same from an activation in SQ8_BF16 or SQ8_F32, quantized (sq8_quantize_groups) into the context's scratch. */
+int sq8_linear_f8_quantized(sq8_ctx *ctx, const void *a, int a_dtype, int64_t lda,
+                            const void *w, int64_t ldw, const float *sw, int64_t ldsw,
+                            const float *bias, int epilogue, void *c, int c_dtype, int64_t ldc,
+                            int m, int k, int n, double *gpu_seconds);
+
+/* A paged cache: two pools of `pages` pages of `page` tokens, [pages, page, kv_heads, dim] with the strides given
+ * (elements; dim contiguous), SQ8_BF16, or SQ8_FP8_E4M3 standing for code · scale[kv head] (fp32 [kv_heads] device
+ * arrays, NULL: 1; not read for bf16). */
+typedef struct sq8_paged_cache {
+    void *k, *v;
+    int64_t k_page, k_token, k_head, v_page, v_token, v_head;
+    const float *k_scale, *v_scale;
+    int dtype, pages, page, kv_heads, dim;
+} sq8_paged_cache;
+
+/* **Appending to a paged cache, the position rotation on the way.** For each of `tokens` tokens (bf16 q [tokens,
+ * q_heads, dim], k and v [tokens, kv_heads, dim], token and head strides in elements): q and k turned by the angles of
+ * positions[token] — pairs (i, i + rot/2) of a head's first `rot` values, or (2i, 2i + 1) with `interleaved`, by row
+ * `position` of `table` (fp32 [max_position, rot]: rot/2 cosines, then the sines; leading dimension table_row) — q to
+ * q_out (bf16, may be q itself), k and v to slot slots[token] = page index · page + place, rounded once (e4m3: of value
+ * · (1/scale), saturated at ±448). A slot outside [0, pages · page) writes nothing (an idle row's −1); a position
+ * outside the table takes its last row. dim and rot even, rot ≤ dim (else SQ8_EUNSUPPORTED). Two tokens with one slot
+ * race. */
+int sq8_append_kv(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head,
+                  const uint16_t *k, int64_t k_token, int64_t k_head, const uint16_t *v, int64_t v_token, int64_t v_head,
+                  uint16_t *q_out, int64_t qo_token, int64_t qo_head, const sq8_paged_cache *cache,
+                  const int32_t *positions, const int32_t *slots, const float *table, int64_t table_row,
+                  int max_position, int rot, int interleaved, int tokens, int q_heads);
+
+/* **Attention of one new token per sequence over a paged cache.** o[b, h] = Σ_t softmax_t(s_t) · v_t over tokens t in
+ * [max(0, len − window), len) (`window` 0: all) of sequence b, s_t = scale · q·k_t, capped to softcap · tanh(s_t /
+ * softcap) unless softcap is 0; query head h reads kv head h / (q_heads / kv_heads). q, out bf16 [batch, q_heads, dim];
+ * table int32 [batch, max_pages] (page indices in order; leading dimension table_row), lengths int32 [batch], cut to
+ * [0, max_pages · page]. A length of 0 gives zeros; tokens on a page index outside the pools count as masked; masked
+ * rows may hold anything. Scores, maxima and sums fp32; the probabilities are rounded to bf16 for their product with v.
+ * dim up to 256, a multiple of 8 (past 128 and for e4m3: of 16); 16-byte aligned rows (else SQ8_EUNSUPPORTED). Partial
+ * results of split sequences go to the context's scratch (sq8_linear says when it grows; its size follows from the
+ * arguments here, not from the lengths). */
+int sq8_paged_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head, const sq8_paged_cache *cache,
+                        const int32_t *table, int64_t table_row, int max_pages, const int32_t *lengths,
+                        float scale, float softcap, int window,
+                        uint16_t *out, int64_t o_token, int64_t o_head, int batch, int q_heads);
+
 /* ---- codes with a scale per block of rows and column: GGUF Q8_0 (w = q · d, one fp16 d per 32
  * consecutive K of an output; Sources/Siliconed/Forge/GGUF.swift, `deinterleaveQ8_0`) ---- */
 

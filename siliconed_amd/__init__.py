@@ -8,6 +8,7 @@ its host side. There is no CPU fallback: without the library, importing the oper
 from . import _abi as abi
 from .tensor_gemm import (PackedWeight, TensorGEMM, context, dequantize, dequantize_rotated, linear, linear_qkv, pack,
                           rotate, round_bf16)
+from .text_ops import PagedCache
 
-__all__ = ["abi", "PackedWeight", "TensorGEMM", "context", "linear", "linear_qkv", "pack", "dequantize",
+__all__ = ["abi", "PackedWeight", "PagedCache", "TensorGEMM", "context", "linear", "linear_qkv", "pack", "dequantize",
            "dequantize_rotated", "rotate", "round_bf16"]

@@ -20,6 +20,17 @@ EPI_NONE, EPI_GELU_TANH, EPI_SILU_GLU, EPI_SITU_GLU = 0, 1, 2, 3
 
 # Every symbol the header declares, with (restype, argtypes).
 _P, _I, _I64, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_double
+
+
+class PagedCacheArgs(ctypes.Structure):
+    """struct sq8_paged_cache."""
+
+    _fields_ = [("k", _P), ("v", _P),
+                *((name, _I64) for name in ("k_page", "k_token", "k_head", "v_page", "v_token", "v_head")),
+                ("k_scale", _P), ("v_scale", _P),
+                *((name, _I) for name in ("dtype", "pages", "page", "kv_heads", "dim"))]
+
+
 SIGNATURES = {
     "sq8_create": (_I, [_I, _P, ctypes.POINTER(_P)]),
     "sq8_destroy": (_I, [_P]),
@@ -63,6 +74,17 @@ SIGNATURES = {
     "sq8_norm_modulate": (_I, [_P, _P, _I64, _P, _P, _P, ctypes.c_float, _P, _I64, _I, _I]),
     "sq8_rms_rows": (_I, [_P, _P, _I64, _I64, _I, _P, ctypes.c_float]),
     "sq8_gated_residual": (_I, [_P, _P, _I64, _P, _I, _I64, _P, _I64, _I]),
+    "sq8_add_norm_quantized": (_I, [_P, _P, _I, _I64, _P, _I, _I64, _P, _I64, _P, ctypes.c_float, _P, _I, _I64, _P, _I64,
+                                    _I, _I]),
+    "sq8_quantize_groups": (_I, [_P, _P, _I, _I64, _I, _I, _P, _I64, _P, _I64]),
+    "sq8_linear_f8": (_I, [_P, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I, _P, _I, _I64, _I, _I, _I,
+                           ctypes.POINTER(_D)]),
+    "sq8_linear_f8_quantized": (_I, [_P, _P, _I, _I64, _P, _I64, _P, _I64, _P, _I, _P, _I, _I64, _I, _I, _I,
+                                     ctypes.POINTER(_D)]),
+    "sq8_append_kv": (_I, [_P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64,
+                           ctypes.POINTER(PagedCacheArgs), _P, _P, _P, _I64, _I, _I, _I, _I, _I]),
+    "sq8_paged_attention": (_I, [_P, _P, _I64, _I64, ctypes.POINTER(PagedCacheArgs), _P, _I64, _I, _P, ctypes.c_float,
+                                 ctypes.c_float, _I, _P, _I64, _I64, _I, _I]),
     "sq8_synchronize": (_I, [_P]),
     "sq8_status_string": (ctypes.c_char_p, [_I]),
     "sq8_abi_version": (_I, []),

@@ -4,7 +4,6 @@
 #include "siliconed_q8.h"
 
 #include <hip/hip_runtime.h>
-#include <rocblas/rocblas.h>
 #include <stdint.h>
 #include <stdlib.h>
 #include <string.h>
@@ -14,7 +13,7 @@
 #include <mutex>
 #include <new>
 
-#include "sq8_buffers.h"
+#include "sq8_context.h"
 #include "sq8_gemm.h"
 
 // The allocation-free entry point's device memory (sq8_linear_quantized_static): one array per GPU,
@@ -23,25 +22,12 @@
 // once per device (static_scratch_of) and used wherever a kernel or a copy needs the memory.
 static __device__ __align__(256) uint8_t scratch[SQ8_STATIC_SCRATCH_BYTES];
 
-struct sq8_ctx {
-    int device;
-    hipStream_t stream;
-    hipEvent_t begin, end;
-    sq8::Buffer scratch;    // bf16 copy of an fp32 activation (the reference's rounding scratch)
-    sq8::Buffer wpack;      // [K, N] codes repacked for the weight-direct kernels, per product
-    sq8::Buffer part;       // the skinny kernel's partial sums of a K split
-    sq8::SetAside *aside;   // what these outgrew while a captured graph may use it
-    rocblas_handle blas;    // the bf16-weight product's library GEMM (created on its first call)
-    int wd_tile;            // measurement knobs, read once at sq8_create (SQ8_TILE, SQ8_Q8_TILE, SQ8_SPLITS): a
-    int q8_tile;            // forced weight-direct / block-scale tile, or -1 (the product's own choice); the
-    int i8_tile;            // the W8A8 tile SQ8_TILE forces (the K-group tiles only), or -1
-    int splits;             // skinny kernel's K split count (1: none, the default)
-    int cus;                // the device's compute units, read once here: the tile rules' rounds
-};
-
 namespace {
 
-int hip_status(hipError_t e) { return e == hipSuccess ? SQ8_OK : -(int)e; }
+using sq8::aligned;
+using sq8::DeviceScope;
+using sq8::hip_status;
+using sq8::reserve;
 
 // The static scratch's device address per device ordinal, looked up once with that device current.
 constexpr int kMaxDevices = 64;
@@ -63,22 +49,6 @@ hipError_t static_scratch_of(int device, uint8_t **out) {
     *out = g_static_ptr[device];
     return hipSuccess;
 }
-
-// Makes the context's device current for the scope, restoring the caller's afterwards.
-struct DeviceScope {
-    int previous = -1;
-    hipError_t error = hipSuccess;
-    explicit DeviceScope(int device) {
-        error = hipGetDevice(&previous);
-        if (error == hipSuccess && previous != device) error = hipSetDevice(device);
-    }
-    ~DeviceScope() {
-        int now = -1;
-        if (previous >= 0 && hipGetDevice(&now) == hipSuccess && now != previous) (void)hipSetDevice(previous);
-    }
-};
-
-bool aligned(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 
 // A measurement knob's value (an environment variable read when a context is created): the tile named,
 // or -1 when unset or unknown (the product's own choice).
@@ -133,11 +103,6 @@ int check_config(int a_dtype, int w_dtype, int w_layout, int scale_layout, int c
     if (c_dtype != SQ8_BF16 && c_dtype != SQ8_F32) return SQ8_EUNSUPPORTED;
     if (epilogue < SQ8_EPI_NONE || epilogue > SQ8_EPI_SITU_GLU) return SQ8_EINVAL;
     return SQ8_OK;
-}
-
-// Grows one of the context's buffers to `bytes` (never shrinks; freed with the context).
-int reserve(sq8_ctx *ctx, sq8::Buffer &b, size_t bytes) {
-    return hip_status(sq8::reserve(b, bytes, ctx->stream, ctx->aside));
 }
 
 struct Product {

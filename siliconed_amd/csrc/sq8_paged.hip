@@ -1,0 +1,658 @@
+// sq8_paged.hip — a paged key-value cache: appending new keys and values with the position rotation applied, and
+// attention of one new token per sequence over it.
+//
+// A cache is two pools [pages, page, kv_heads, dim] of bf16 or e4m3 (times a scale per head), any strides with the
+// values of a head contiguous. Offsets into them are 64-bit. No index read from device memory is trusted: a slot
+// outside the pools is not written, a position outside the table reads its last row, a page outside the pools
+// counts as masked, a length past the page table's end is cut to it.
+#include <hip/hip_runtime.h>
+
+#include "sq8_device.h"
+#include "sq8_text.h"
+
+namespace sq8 {
+namespace {
+
+__device__ __forceinline__ float bf16_f32(uint32_t bits) { return __uint_as_float(bits << 16); }
+
+// ---- append ------------------------------------------------------------------------------------------------------
+//
+// q' = rot(q), k' = rot(k): with (cos, sin) of the token's position, pair i of the first `rot` values of a head,
+// (a, b) → (a·cos − b·sin, b·cos + a·sin); pairs (i, i + rot/2), or (2i, 2i + 1) when interleaved. Products and sums
+// in fp32, one rounding. e4m3: code = e4m3(v · (1/scale)), saturated at ±448 (a NaN stays one).
+//
+// Bound by memory: every value is read once and written once. A thread takes one unit of a token: two runs of W
+// values, the two halves of W pairs (or W values of one run and the next where there is nothing to turn), so a wave
+// reads whole 16-byte runs on both sides (W = 8). W = 1 serves what is not aligned for that.
+template <int W>
+__device__ __forceinline__ void load_run(const uint16_t *src, float (&v)[W]) {
+    if constexpr (W == 8) {
+        const u32x4 d = *reinterpret_cast<const u32x4 *>(src);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[2 * e] = bf16_f32(d[e] & 0xFFFFu);
+            v[2 * e + 1] = __uint_as_float(d[e] & 0xFFFF0000u);
+        }
+    } else {
+        v[0] = bf16_f32(src[0]);
+    }
+}
+
+template <int W>
+__device__ __forceinline__ void load_angles(const float *src, float (&v)[W]) {
+    if constexpr (W == 8) {
+        const f32x4 a = reinterpret_cast<const f32x4 *>(src)[0], b = reinterpret_cast<const f32x4 *>(src)[1];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+    } else {
+        v[0] = src[0];
+    }
+}
+
+template <int W>
+__device__ __forceinline__ void store_bf16(uint16_t *dst, const float (&v)[W]) {
+    if constexpr (W == 8)
+        *reinterpret_cast<u32x4 *>(dst) = u32x4{pack_bf16_rne(v[0], v[1]), pack_bf16_rne(v[2], v[3]), pack_bf16_rne(v[4], v[5]),
+                                                pack_bf16_rne(v[6], v[7])};
+    else
+        dst[0] = (uint16_t)(pack_bf16_rne(v[0], v[0]) & 0xFFFFu);
+}
+
+template <int W>
+__device__ __forceinline__ void store_e4m3(uint8_t *dst, const float (&v)[W], float recip) {
+    float q[W];
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+        const float t = v[e] * recip;
+        q[e] = t != t ? t : fminf(fmaxf(t, -448.0f), 448.0f);
+    }
+    if constexpr (W == 8) {
+        uint32_t lo = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+        lo = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], (int)lo, true);
+        uint32_t hi = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
+        hi = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], (int)hi, true);
+        *reinterpret_cast<u32x2 *>(dst) = u32x2{lo, hi};
+    } else {
+        dst[0] = (uint8_t)((uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[0], 0, false) & 0xFFu);
+    }
+}
+
+template <int W, bool E4M3>
+__global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs p) {
+    const unsigned per_head = (unsigned)p.dim / (2 * W);
+    const unsigned units = (unsigned)(p.q_heads + 2 * p.kv_heads) * per_head;
+    const int64_t first = (int64_t)blockIdx.x * 256;  // of this workgroup's units over all tokens
+    const int64_t token0 = first / units;
+    const unsigned local = (unsigned)(first - token0 * units) + threadIdx.x;
+    const int64_t token = token0 + local / units;
+    if (token >= p.tokens) return;
+    const unsigned unit = local % units;
+    int head = (int)(unit / per_head);
+    const int u = (int)(unit % per_head);
+    const int32_t slot = p.slots[token];
+    const int kind = head < p.q_heads ? 0 : head < p.q_heads + p.kv_heads ? 1 : 2;  // q, k, v
+    head -= kind == 0 ? 0 : kind == 1 ? p.q_heads : p.q_heads + p.kv_heads;
+    const bool live = slot >= 0 && slot < p.slot_count;
+    if (kind != 0 && !live) return;
+    const uint16_t *src = kind == 0   ? p.q + token * p.q_tok + head * p.q_head
+                          : kind == 1 ? p.k + token * p.k_tok + head * p.k_head
+                                      : p.v + token * p.v_tok + head * p.v_head;
+    const int turned = p.rot / (2 * W);  // units of a head that are turned
+    const bool turns = kind != 2 && u < turned;
+    const int at0 = turns && !p.interleaved ? W * u : 2 * W * u;
+    const int at1 = turns && !p.interleaved ? at0 + p.rot / 2 : at0 + W;
+    float a[W], b[W];
+    load_run<W>(src + at0, a);
+    load_run<W>(src + at1, b);
+    if (turns) {
+        int position = p.positions[token];
+        position = position < 0 || position >= p.max_position ? p.max_position - 1 : position;
+        float cs[W], sn[W];
+        const float *row = p.table + (int64_t)position * p.table_row + W * u;
+        load_angles<W>(row, cs);
+        load_angles<W>(row + p.rot / 2, sn);
+        if (p.interleaved && W > 1) {
+            // Pair i of the unit's 2W values is values 2i and 2i + 1: both in `a` or both in `b`.
+#pragma unroll
+            for (int i = 0; i < W / 2; ++i) {
+                const float x = a[2 * i], y = a[2 * i + 1], z = b[2 * i], t = b[2 * i + 1];
+                a[2 * i] = x * cs[i] - y * sn[i];
+                a[2 * i + 1] = y * cs[i] + x * sn[i];
+                b[2 * i] = z * cs[W / 2 + i] - t * sn[W / 2 + i];
+                b[2 * i + 1] = t * cs[W / 2 + i] + z * sn[W / 2 + i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const float x = a[i], y = b[i];
+                a[i] = x * cs[i] - y * sn[i];
+                b[i] = y * cs[i] + x * sn[i];
+            }
+        }
+    }
+    if (kind == 0) {
+        uint16_t *dst = p.q_out + token * p.qo_tok + head * p.qo_head;
+        store_bf16<W>(dst + at0, a);
+        store_bf16<W>(dst + at1, b);
+        return;
+    }
+    const int64_t page = slot / p.page, in = slot - page * p.page;
+    const int64_t to = kind == 1 ? page * p.kc_page + in * p.kc_tok + head * p.kc_head
+                                 : page * p.vc_page + in * p.vc_tok + head * p.vc_head;
+    void *pool = kind == 1 ? p.kc : p.vc;
+    if constexpr (E4M3) {
+        const float *scales = kind == 1 ? p.k_scale : p.v_scale;
+        const float recip = scales ? __fdiv_rn(1.0f, scales[head]) : 1.0f;
+        uint8_t *dst = static_cast<uint8_t *>(pool) + to;
+        store_e4m3<W>(dst + at0, a, recip);
+        store_e4m3<W>(dst + at1, b, recip);
+    } else {
+        uint16_t *dst = static_cast<uint16_t *>(pool) + to;
+        store_bf16<W>(dst + at0, a);
+        store_bf16<W>(dst + at1, b);
+    }
+}
+
+// ---- attention of one new token ------------------------------------------------------------------------------------
+//
+//   o[b, h] = Σ_t softmax_t(s_t) · v_t,  s_t = cap(scale · q·k_t),  t in [max(0, len − window), len)
+//
+// One pass over the cache with the running maximum and sum of the softmax, both fp32; the probabilities are rounded
+// to bf16 for their product with v (the sum is of the unrounded ones): at most 2^-8 of each, random over the tokens.
+//
+// Bound by the cache's bytes. The query heads of one kv head (up to 16; more take several passes) are the columns of
+// both products, on v_mfma_f32_16x16x32_bf16:
+//   S[token, head] = K · Qᵀ   (first operand: 16 tokens × 32 values)
+//   O[value, head] += Vᵀ · P  (first operand: 16 values × 32 tokens)
+// A lane (c = lane mod 16, h = lane / 16) ends with S of tokens 4h..4h+3 of each 16-token tile for head c, and the
+// second product takes its 32 tokens in the order (4h + r of the first tile, 4h + r of the second), so a lane's eight
+// probabilities are its operand as they lie: nothing crosses lanes between the products. Its V operand is those eight
+// tokens' rows at values DV·c .. DV·c + DV − 1 (DV = dim / 16): one contiguous load a token, transposed within the
+// lane, value DV·c + i going to instruction i. So both pools go from memory to registers in whole rows, without LDS.
+//
+// Work is split over tiles of 128 tokens (a wave takes 32) of every (sequence, kv head, 16 query heads), numbered in
+// that order; workgroup g of G takes tiles [T·g/G, T·(g+1)/G), whatever sequences they belong to, so ragged lengths
+// load the card evenly and the host needs no lengths. A sequence's head whose tiles lie in several workgroups leaves
+// its maximum, sum and unnormalised output in each one's slot; a second launch joins them in tile order.
+
+constexpr int TILE = 128;   // tokens a workgroup takes at a time
+constexpr int WAVES = 4;
+
+struct Span {
+    int first, last;  // tokens [first, last), from the window's first
+    int base;         // `first` rounded down to 32
+    int tiles;
+};
+
+__device__ __forceinline__ Span span_of(const PagedArgs &p, int length) {
+    const int64_t most = (int64_t)p.max_pages * p.page;
+    Span s;
+    s.last = (int)(length < 0 ? 0 : length > most ? most : length);
+    s.first = p.window > 0 && s.last > p.window ? s.last - p.window : 0;
+    s.base = s.first & ~31;
+    s.tiles = (s.last - s.base + TILE - 1) / TILE;
+    return s;
+}
+
+// The sum of v over this lane and those before it.
+__device__ __forceinline__ int wave_scan(int v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(v, o, 64);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+
+// The batch's tiles of one head, by 64 sequences at a time in every wave.
+__device__ __forceinline__ int64_t batch_tiles(const PagedArgs &p, int lane) {
+    int64_t total = 0;
+    for (int b = 0; b < p.batch; b += 64) {
+        int v = b + lane < p.batch ? span_of(p, p.lengths[b + lane]).tiles : 0;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+        total += v;
+    }
+    return total;
+}
+
+// The sequence that holds per-head tile number `at`, and the tiles of the sequences before it.
+__device__ __forceinline__ int sequence_of(const PagedArgs &p, int64_t at, int lane, int64_t &before) {
+    int64_t base = 0;
+    for (int b = 0; b < p.batch; b += 64) {
+        const int v = b + lane < p.batch ? span_of(p, p.lengths[b + lane]).tiles : 0;
+        const int upto = wave_scan(v, lane);
+        const uint64_t past = __ballot(base + upto > at);
+        if (past) {
+            const int l = __ffsll((unsigned long long)past) - 1;
+            before = base + (l > 0 ? __shfl(upto, l - 1, 64) : 0);
+            return b + l;
+        }
+        base += __shfl(upto, 63, 64);
+    }
+    before = base;
+    return -1;
+}
+
+__host__ __device__ constexpr int part_floats(int dp) { return 32 + 16 * dp; }  // maxima, sums, outputs [16][dp]
+
+// A head's values past `dim` (a head narrower than DP) read as zeros.
+template <int N>
+struct Raw {
+    uint32_t d[N];
+};
+
+template <int N>
+__device__ __forceinline__ Raw<N> load_raw(const uint8_t *src) {
+    Raw<N> r;
+    if constexpr (N == 1) {
+        r.d[0] = *reinterpret_cast<const uint32_t *>(src);
+    } else if constexpr (N == 2) {
+        const u32x2 v = *reinterpret_cast<const u32x2 *>(src);
+        r.d[0] = v[0]; r.d[1] = v[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const u32x4 v = reinterpret_cast<const u32x4 *>(src)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.d[4 * i + e] = v[e];
+        }
+    }
+    return r;
+}
+
+// Two e4m3 codes (bytes 2W, 2W + 1) as a bf16 pair, exactly.
+template <int W>
+__device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t d) {
+    float lo, hi;
+    fp8_pair<W>(d, lo, hi);
+    return pack_exact_bf16(lo, hi);
+}
+
+template <int DP, bool E4M3, bool PAGE16>
+__global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) paged_attention_kernel(const PagedArgs p) {
+    constexpr int ES = E4M3 ? 1 : 2;
+    constexpr int STEPS = DP / 32;                // MFMAs of a 16-token tile's scores
+    constexpr int KRUNS = DP * ES / 64;           // 16-byte runs of a key a lane reads
+    constexpr int DV = DP / 16;                   // values of a token a lane reads: MFMAs of the second product
+    constexpr int VN = DV * ES / 4;               // and their dwords
+    __shared__ __attribute__((aligned(16))) f32x4 joined[WAVES - 1][DV][64];
+    __shared__ float tops[WAVES][16], totals[WAVES][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, h = lane >> 4;
+    const int group = p.q_heads / p.kv_heads;
+    const int passes = (group + 15) / 16;
+    const int heads = p.kv_heads * passes;
+
+    // Sequences without a token: zeros.
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        if (span_of(p, p.lengths[b]).tiles != 0) continue;
+        for (int i = threadIdx.x; i < p.q_heads * p.dim; i += 64 * WAVES)
+            p.out[b * p.o_tok + (i / p.dim) * p.o_head + i % p.dim] = 0;
+    }
+
+    const int64_t per_head = batch_tiles(p, lane);
+    const int64_t total = per_head * heads;
+    const int64_t start = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
+    if (start >= end) return;
+    // Tiles are numbered sequence by sequence, `heads` runs of a sequence's tiles each.
+    int64_t before = 0;
+    int b = sequence_of(p, start / heads, lane, before);
+    if (b < 0) return;
+    b = __builtin_amdgcn_readfirstlane(b);
+    Span span = span_of(p, p.lengths[b]);
+    int64_t seq0 = before * heads;  // the sequence's first tile
+
+    for (int64_t pos = start; pos < end;) {
+        while (pos >= seq0 + (int64_t)span.tiles * heads) {
+            seq0 += (int64_t)span.tiles * heads;
+            ++b;
+            span = span_of(p, p.lengths[b]);
+        }
+        const int in_seq = (int)(pos - seq0);
+        const int head = in_seq / span.tiles;
+        const int tile0 = in_seq - head * span.tiles;
+        const int run = (int)min((int64_t)(span.tiles - tile0), end - pos);
+        const int kvh = head / passes, pass = head - kvh * passes;
+        const int q0 = kvh * group + pass * 16;
+        const int live = min(16, group - pass * 16);  // query heads of this pass
+
+        // ---- the queries: head c's values in the order the keys' lanes hold them ----
+        bf16x8 q[STEPS];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            const int d = E4M3 ? 64 * (s >> 1) + 16 * h + 8 * (s & 1) : 32 * s + 8 * h;
+            u32x4 v = {0, 0, 0, 0};
+            if (c < live && d < p.dim) v = *reinterpret_cast<const u32x4 *>(p.q + b * p.q_tok + (q0 + c) * p.q_head + d);
+            q[s] = __builtin_bit_cast(bf16x8, v);
+        }
+        const float score_scale = p.scale * (E4M3 && p.k_scale ? p.k_scale[kvh] : 1.0f);
+        const uint8_t *kbase = p.kc + (int64_t)kvh * p.kc_head * ES;
+        const uint8_t *vbase = p.vc + (int64_t)kvh * p.vc_head * ES;
+        const int32_t *pages = p.pages + (int64_t)b * p.pages_row;
+
+        // Where the rows of a subtile's tokens lie. PAGE16: each 16-token tile in one page, its page uniform.
+        struct Where {
+            int64_t k[2], v[PAGE16 ? 2 : 8];  // row offsets in elements
+            uint32_t bad;                     // tokens (bit: order of the lane's eight) on a page outside the pools
+        };
+        auto locate = [&](int token) {
+            Where w;
+            w.bad = 0;
+            if constexpr (PAGE16) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int at = min(token + 16 * t, (span.last - 1) & ~15);
+                    const int page = at / p.page, in = at - page * p.page;
+                    int id = pages[page];
+                    if ((unsigned)id >= (unsigned)p.page_count) { id = 0; w.bad |= 0xFu << (4 * t); }
+                    w.k[t] = id * p.kc_page + in * p.kc_tok;
+                    w.v[t] = id * p.vc_page + in * p.vc_tok;
+                }
+            } else {
+                auto row = [&](int t, int64_t page_stride, int64_t tok_stride, bool &bad) {
+                    const int at = min(t, span.last - 1);
+                    const int page = at / p.page, in = at - page * p.page;
+                    int id = pages[page];
+                    bad = (unsigned)id >= (unsigned)p.page_count;
+                    if (bad) id = 0;
+                    return id * page_stride + in * tok_stride;
+                };
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    bool bad;
+                    w.k[t] = row(token + 16 * t + c, p.kc_page, p.kc_tok, bad);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    bool bad;
+                    w.v[i] = row(token + 16 * (i >> 2) + 4 * h + (i & 3), p.vc_page, p.vc_tok, bad);
+                    w.bad |= bad ? 1u << i : 0u;
+                }
+            }
+            return w;
+        };
+        Raw<4> k[2][KRUNS];
+        auto load_k = [&](const Where &w) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint8_t *row = kbase + (PAGE16 ? w.k[t] + c * p.kc_tok : w.k[t]) * ES;
+#pragma unroll
+                for (int s = 0; s < KRUNS; ++s) {
+                    const int d = E4M3 ? 64 * s + 16 * h : 32 * s + 8 * h;
+                    k[t][s] = Raw<4>{{0, 0, 0, 0}};
+                    if (d < p.dim) k[t][s] = load_raw<4>(row + d * ES);
+                }
+            }
+        };
+        Raw<VN> v[8];
+        auto load_v = [&](const Where &w) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint8_t *row = vbase + (PAGE16 ? w.v[PAGE16 ? i >> 2 : 0] + (4 * h + (i & 3)) * p.vc_tok : w.v[PAGE16 ? 0 : i]) * ES;
+#pragma unroll
+                for (int e = 0; e < VN; ++e) v[i].d[e] = 0;
+                if (DV * c < p.dim) v[i] = load_raw<VN>(row + DV * c * ES);
+            }
+        };
+
+        float top = -INFINITY, sum = 0.0f;  // of head c, in units of log2: the sum over this lane's tokens
+        f32x4 o[DV];
+#pragma unroll
+        for (int i = 0; i < DV; ++i) o[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+        int token = span.base + tile0 * TILE + wave * 32;
+        Where at = locate(token);
+        load_k(at);
+        load_v(at);
+        Where next = locate(token + TILE);
+        for (int i = 0; i < run; ++i, token += TILE) {
+            const bool more = i + 1 < run;
+            f32x4 s[2] = {};
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < STEPS; ++j) {
+                    bf16x8 kk;
+                    if constexpr (E4M3) {
+                        const uint32_t d0 = k[t][j >> 1].d[2 * (j & 1)], d1 = k[t][j >> 1].d[2 * (j & 1) + 1];
+                        kk = __builtin_bit_cast(bf16x8, u32x4{bf16_of_e4m3<0>(d0), bf16_of_e4m3<1>(d0), bf16_of_e4m3<0>(d1),
+                                                              bf16_of_e4m3<1>(d1)});
+                    } else {
+                        kk = __builtin_bit_cast(bf16x8, k[t][j]);
+                    }
+                    s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[j], s[t], 0, 0, 0);
+                }
+            if (more) load_k(next);
+            const uint32_t bad = at.bad;
+            const Where later = more ? locate(token + 2 * TILE) : next;
+
+            // Scores in units of log2, tokens 16t + 4h + r.
+            float e[8];
+            constexpr float LOG2E = 1.4426950408889634f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = s[j >> 2][j & 3] * score_scale;
+                e[j] = (p.softcap > 0.0f ? p.softcap * tanh_rel(x / p.softcap) : x) * LOG2E;
+            }
+            const bool edge = token < span.first || token + 32 > span.last;
+            if (edge || __any(bad != 0)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int t = token + 16 * (j >> 2) + 4 * h + (j & 3);
+                    if (t < span.first || t >= span.last || (bad >> j & 1)) {
+                        e[j] = -INFINITY;
+                        // A masked row may hold anything, and 0 · NaN is one.
+#pragma unroll
+                        for (int d = 0; d < VN; ++d) v[j].d[d] = 0;
+                    }
+                }
+            }
+            float m = e[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) m = fmaxf(m, e[j]);
+            m = fmaxf(m, __shfl_xor(m, 16, 64));
+            m = fmaxf(m, __shfl_xor(m, 32, 64));
+            if (__any(m > top)) {
+                m = fmaxf(m, top);
+                const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - m);
+                top = m;
+                sum *= keep;
+#pragma unroll
+                for (int d = 0; d < DV; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[d][r] *= keep;
+            }
+            const float from = top == -INFINITY ? 0.0f : top;
+            float w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[j] = __builtin_amdgcn_exp2f(e[j] - from);
+                sum += w[j];
+            }
+            const bf16x8 prob = __builtin_bit_cast(
+                bf16x8, u32x4{pack_bf16_rne(w[0], w[1]), pack_bf16_rne(w[2], w[3]), pack_bf16_rne(w[4], w[5]), pack_bf16_rne(w[6], w[7])});
+            // Value DV·c + d of the lane's eight tokens, two tokens a dword.
+#pragma unroll
+            for (int d = 0; d < DV; ++d) {
+                u32x4 t;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (E4M3) {
+                        const uint32_t x = v[2 * j].d[d >> 2], y = v[2 * j + 1].d[d >> 2];
+                        // bytes (x[d], y[d]) → a bf16 pair
+                        const uint32_t two = __builtin_amdgcn_perm(y, x, 0x0c0c0400u + 0x0101u * (d & 3));
+                        t[j] = bf16_of_e4m3<0>(two);
+                    } else {
+                        t[j] = __builtin_amdgcn_perm(v[2 * j + 1].d[d >> 1], v[2 * j].d[d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+                    }
+                }
+                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t), prob, o[d], 0, 0, 0);
+            }
+            if (more) load_v(next);
+            at = next;
+            next = later;
+        }
+
+        // ---- the waves' results joined, by the first ----
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        __syncthreads();  // the segment before has been read
+        if (h == 0) { tops[wave][c] = top; totals[wave][c] = sum; }
+        if (wave > 0) {
+#pragma unroll
+            for (int d = 0; d < DV; ++d) joined[wave - 1][d][lane] = o[d];
+        }
+        __syncthreads();
+        if (wave == 0) {
+            float all = top;
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) all = fmaxf(all, tops[w][c]);
+            const float from = all == -INFINITY ? 0.0f : all;
+            float weight = __builtin_amdgcn_exp2f(top - from);
+            float l = sum * weight;
+#pragma unroll
+            for (int d = 0; d < DV; ++d)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[d][r] *= weight;
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) {
+                weight = __builtin_amdgcn_exp2f(tops[w][c] - from);
+                l += totals[w][c] * weight;
+#pragma unroll
+                for (int d = 0; d < DV; ++d) {
+                    const f32x4 t = joined[w - 1][d][lane];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[d][r] = __builtin_fmaf(t[r], weight, o[d][r]);
+                }
+            }
+            if (c < live) {
+                if (run == span.tiles) {
+                    const float scale = (l > 0.0f ? __fdiv_rn(1.0f, l) : l == 0.0f ? 0.0f : l) * (E4M3 && p.v_scale ? p.v_scale[kvh] : 1.0f);
+                    uint16_t *dst = p.out + b * p.o_tok + (q0 + c) * p.o_head;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int at = DV * (4 * h + r);
+                        if (at >= p.dim) continue;
+#pragma unroll
+                        for (int d = 0; d < DV; d += 2)
+                            *reinterpret_cast<uint32_t *>(dst + at + d) = pack_bf16_rne(o[d][r] * scale, o[d + 1][r] * scale);
+                    }
+                } else {
+                    float *slot = p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * part_floats(DP);
+                    if (h == 0) { slot[c] = all; slot[16 + c] = l; }
+                    float *dst = slot + 32 + c * DP;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int d = 0; d < DV; d += 4)
+                            *reinterpret_cast<f32x4 *>(dst + DV * (4 * h + r) + d) = f32x4{o[d][r], o[d + 1][r], o[d + 2][r], o[d + 3][r]};
+                }
+            }
+        }
+        pos += run;
+    }
+}
+
+// One workgroup a (sequence, kv head, 16 query heads): the slots of the workgroups its tiles lay in, in tile order.
+template <int DP, bool E4M3>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs p, int groups) {
+    const int lane = threadIdx.x & 63;
+    const int group = p.q_heads / p.kv_heads;
+    const int passes = (group + 15) / 16;
+    const int heads = p.kv_heads * passes;
+    const int b = blockIdx.x / heads, head = blockIdx.x - b * heads;
+    const int tiles = span_of(p, p.lengths[b]).tiles;
+    if (tiles == 0) return;
+    int64_t before = 0, total = 0;
+    for (int i = 0; i < p.batch; i += 64) {
+        int v = i + lane < p.batch ? span_of(p, p.lengths[i + lane]).tiles : 0;
+        int u = i + lane < b ? v : 0;
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+            v += __shfl_xor(v, o, 64);
+            u += __shfl_xor(u, o, 64);
+        }
+        total += v;
+        before += u;
+    }
+    total *= heads;
+    const int64_t first = before * heads + (int64_t)head * tiles;
+    // Workgroup g took tiles from floor(total · g / groups) on.
+    const int g0 = (int)(((first + 1) * groups - 1) / total), g1 = (int)(((first + tiles) * groups - 1) / total);
+    if (g0 == g1) return;  // one workgroup had them all, and wrote the result
+    const int kvh = head / passes, pass = head - kvh * passes;
+    const int live = min(16, group - pass * 16);
+    const float v_scale = E4M3 && p.v_scale ? p.v_scale[kvh] : 1.0f;
+    for (int i = threadIdx.x; i < live * (p.dim / 2); i += 256) {
+        const int c = i / (p.dim / 2), d = 2 * (i - c * (p.dim / 2));
+        float top = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
+        for (int g = g0; g <= g1; ++g) {
+            if (total * g / groups == total * (g + 1) / groups) continue;  // fewer tiles than workgroups: it had none
+            const float *slot = p.part + (int64_t)(2 * g + (total * g / groups < first ? 1 : 0)) * part_floats(DP);
+            const float m = fmaxf(top, slot[c]), from = m == -INFINITY ? 0.0f : m;
+            const float keep = __builtin_amdgcn_exp2f(top - from), weight = __builtin_amdgcn_exp2f(slot[c] - from);
+            l = l * keep + slot[16 + c] * weight;
+            x = x * keep + slot[32 + c * DP + d] * weight;
+            y = y * keep + slot[32 + c * DP + d + 1] * weight;
+            top = m;
+        }
+        const float scale = (l > 0.0f ? __fdiv_rn(1.0f, l) : l == 0.0f ? 0.0f : l) * v_scale;
+        *reinterpret_cast<uint32_t *>(p.out + b * p.o_tok + (kvh * group + pass * 16 + c) * p.o_head + d) =
+            pack_bf16_rne(x * scale, y * scale);
+    }
+}
+
+int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+template <int DP, bool E4M3>
+hipError_t launch_attention(const PagedArgs &p, int groups, hipStream_t stream) {
+    if (p.page % 16 == 0)
+        hipLaunchKernelGGL((paged_attention_kernel<DP, E4M3, true>), dim3(groups), dim3(64 * WAVES), 0, stream, p);
+    else
+        hipLaunchKernelGGL((paged_attention_kernel<DP, E4M3, false>), dim3(groups), dim3(64 * WAVES), 0, stream, p);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || groups == 1) return e;
+    const int passes = (p.q_heads / p.kv_heads + 15) / 16;
+    hipLaunchKernelGGL((paged_join_kernel<DP, E4M3>), dim3(p.batch * p.kv_heads * passes), dim3(256), 0, stream, p, groups);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_append_kv(const AppendArgs &p, bool e4m3, bool vec, hipStream_t stream) {
+    if (p.tokens == 0) return hipSuccess;
+    const int64_t units = (int64_t)(p.q_heads + 2 * p.kv_heads) * (p.dim / (vec ? 16 : 2)) * p.tokens;
+    const int64_t blocks = (units + 255) / 256;
+    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)blocks);
+    if (e4m3 && vec) hipLaunchKernelGGL((append_kv_kernel<8, true>), grid, dim3(256), 0, stream, p);
+    else if (e4m3) hipLaunchKernelGGL((append_kv_kernel<1, true>), grid, dim3(256), 0, stream, p);
+    else if (vec) hipLaunchKernelGGL((append_kv_kernel<8, false>), grid, dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((append_kv_kernel<1, false>), grid, dim3(256), 0, stream, p);
+    return hipGetLastError();
+}
+
+int paged_groups(const PagedArgs &p, int cus) {
+    const int passes = (p.q_heads / p.kv_heads + 15) / 16;
+    int64_t tokens = (int64_t)p.max_pages * p.page;
+    if (p.window > 0 && tokens > p.window + 31) tokens = p.window + 31;
+    const int64_t most = (int64_t)p.batch * p.kv_heads * passes * ((tokens + TILE - 1) / TILE);
+    const int64_t full = 2 * (int64_t)cus;
+    return (int)(most < 1 ? 1 : most < full ? most : full);
+}
+
+int64_t paged_part_bytes(const PagedArgs &p, int groups) {
+    return groups == 1 ? 0 : (int64_t)2 * groups * part_floats(padded_dim(p.dim)) * 4;
+}
+
+hipError_t launch_paged_attention(const PagedArgs &p, bool e4m3, int groups, hipStream_t stream) {
+    if (p.batch == 0) return hipSuccess;
+    switch (padded_dim(p.dim)) {
+        case 64: return e4m3 ? launch_attention<64, true>(p, groups, stream) : launch_attention<64, false>(p, groups, stream);
+        case 128: return e4m3 ? launch_attention<128, true>(p, groups, stream) : launch_attention<128, false>(p, groups, stream);
+        default: return e4m3 ? launch_attention<256, true>(p, groups, stream) : launch_attention<256, false>(p, groups, stream);
+    }
+}
+
+}  // namespace sq8

@@ -1,0 +1,86 @@
+// sq8_text.h — host/device interface of a text decoder's operators: the norm that adds the residual stream and
+// writes 8-bit codes, products of e4m3 codes with a scale per 128 of K, the paged cache's append with the position
+// rotation, and attention of one new token over that cache.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace sq8 {
+
+constexpr int F8_GROUP = 128;  // values of K that share a scale
+
+// sq8_text_norm.hip. Element types by flag: bf16 or fp32.
+struct AddNormArgs {
+    const void *x;          // [rows, cols]
+    const void *r;          // the residual stream, or null
+    void *ro;               // the stream's sum (r's type), or null; may be r
+    const float *w;         // [cols]
+    uint8_t *codes;         // e4m3 or int8 [rows, cols]
+    float *scales;          // e4m3: [rows, ⌈cols/128⌉]; int8: [rows]
+    int64_t ldx, ldr, ldro, ldq, lds;
+    float eps;
+    int rows, cols;
+    int x_bf16, r_bf16;
+};
+constexpr int kAddNormCols = 32768;
+hipError_t launch_add_norm(const AddNormArgs &p, bool int8, int cus, hipStream_t stream);
+hipError_t launch_quantize_groups(const void *x, bool x_bf16, int64_t ldx, int rows, int cols, uint8_t *codes, int64_t ldq,
+                                  float *scales, int64_t lds, hipStream_t stream);
+// rows × n bytes read lds apart → written ldd apart (n ≤ ldd; bytes [n, ldd) zero).
+hipError_t launch_pad_bytes(const void *src, int64_t lds, void *dst, int64_t ldd, int64_t rows, int64_t n,
+                            hipStream_t stream);
+
+// sq8_f8_gemm.hip.
+struct F8Args {
+    const uint8_t *a;       // e4m3 [M, K], rows lda apart, 16-byte aligned rows
+    const float *sx;        // [M, KB], rows ldsx apart
+    const uint8_t *w;       // e4m3 [N, K], rows ldw apart, 16-byte aligned rows
+    const float *sw;        // [⌈N/128⌉ (GLU: 2⌈H/128⌉), KB], rows ldsw apart
+    const float *bias;      // [N] or null
+    void *c;                // [M, n_out]
+    int64_t lda, ldsx, ldw, ldsw, ldc;
+    int M, N, K;            // K a multiple of 16
+    int KB;                 // ⌈K/128⌉
+    int H;                  // the output's width: N, or N/2 for GLU
+    int up_block;           // GLU: the up half's first scale row, ⌈H/128⌉
+    int c_vec;              // four outputs a store allowed (aligned base and rows)
+    int sx_vec;             // four scales a load allowed
+};
+hipError_t launch_f8_product(const F8Args &p, bool glu, bool out_f32, int cus, hipStream_t stream);
+
+// sq8_paged.hip. Strides in elements.
+struct AppendArgs {
+    const uint16_t *q, *k, *v;          // bf16 [tokens, heads, dim]
+    uint16_t *q_out;
+    void *kc, *vc;                      // [pages, page, kv_heads, dim], bf16 or e4m3
+    const float *k_scale, *v_scale;     // [kv_heads] or null (1); e4m3 only
+    const float *table;                 // [positions, rot]: rot/2 cosines, then as many sines
+    const int32_t *positions, *slots;
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head;
+    int64_t kc_page, kc_tok, kc_head, vc_page, vc_tok, vc_head, table_row;
+    int64_t slot_count;                 // pages · page
+    int tokens, q_heads, kv_heads, dim, rot, page, max_position;
+    int interleaved;
+};
+hipError_t launch_append_kv(const AppendArgs &p, bool e4m3, bool vec, hipStream_t stream);
+
+struct PagedArgs {
+    const uint16_t *q;                  // bf16 [batch, q_heads, dim]
+    const uint8_t *kc, *vc;             // as AppendArgs
+    const float *k_scale, *v_scale;
+    const int32_t *pages;               // [batch, max_pages], rows pages_row apart
+    const int32_t *lengths;             // [batch]
+    uint16_t *out;
+    float *part;                        // partial results of split sequences: paged_part_bytes() bytes
+    int64_t q_tok, q_head, o_tok, o_head;
+    int64_t kc_page, kc_tok, kc_head, vc_page, vc_tok, vc_head, pages_row;
+    float scale, softcap;
+    int batch, q_heads, kv_heads, dim, page, page_count, max_pages, window;
+};
+// The workgroups a call of these sizes takes, and the partial results' bytes they need.
+int paged_groups(const PagedArgs &p, int cus);
+int64_t paged_part_bytes(const PagedArgs &p, int groups);
+hipError_t launch_paged_attention(const PagedArgs &p, bool e4m3, int groups, hipStream_t stream);
+
+}  // namespace sq8

@@ -1,0 +1,323 @@
+// sq8_text_norm.hip — the passes that write a product's 8-bit operand in a text decoder: the RMS norm of the
+// residual stream's new sum, and the quantization alone.
+//
+//   s' = r + x,  y = (s' · 1/sqrt(mean(s'²) + eps)) · w
+//   e4m3: per 128 columns s = max(max|y| / 448, 1e-30), code = e4m3(y · (1/s)), nearest even
+//   int8: per row s = max(max|y| / 127, 1e-30), code = clamp(rint(y / s), −128, 127)
+//
+// The sums, the norm and the scales are fp32; s' is rounded to the stream's type only where it is stored, so the
+// norm sees the sum before that rounding. y/s of an e4m3 code is the product with the rounded reciprocal: the two
+// differ by an ulp of fp32, which moves a code only on a tie of its 4 significant bits; int8 codes are those of
+// the division, as sq8_quantize_rows writes them. 448·fl(1/s)·s stays below 464, so no code overflows to NaN.
+// An infinity in a group (e4m3) or row (int8) makes its scale infinite.
+#include <hip/hip_runtime.h>
+
+#include "sq8_device.h"
+#include "sq8_quant.h"
+#include "sq8_text.h"
+
+namespace sq8 {
+namespace {
+
+// Eight consecutive values from element `at` of a bf16 or fp32 array as fp32; element e of the row is real when
+// col + e < cols (VEC: all of them, and 16-byte aligned).
+template <bool VEC>
+__device__ __forceinline__ void load8(const void *base, bool bf16, int64_t at, int col, int cols, float (&v)[8]) {
+    if constexpr (VEC) {
+        if (bf16) {
+            const u32x4 d = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(base) + at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[2 * e] = __uint_as_float(d[e] << 16);
+                v[2 * e + 1] = __uint_as_float(d[e] & 0xFFFF0000u);
+            }
+        } else {
+            const f32x4 *src = reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + at);
+            const f32x4 a = src[0], b = src[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[e] = 0.0f;
+            if (col + e < cols)
+                v[e] = bf16 ? __uint_as_float((uint32_t)static_cast<const uint16_t *>(base)[at + e] << 16)
+                            : static_cast<const float *>(base)[at + e];
+        }
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store8(void *base, bool bf16, int64_t at, int col, int cols, const float (&v)[8]) {
+    if constexpr (VEC) {
+        if (bf16) {
+            *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(base) + at) =
+                u32x4{pack_bf16_rne(v[0], v[1]), pack_bf16_rne(v[2], v[3]), pack_bf16_rne(v[4], v[5]), pack_bf16_rne(v[6], v[7])};
+        } else {
+            f32x4 *dst = reinterpret_cast<f32x4 *>(static_cast<float *>(base) + at);
+            dst[0] = f32x4{v[0], v[1], v[2], v[3]};
+            dst[1] = f32x4{v[4], v[5], v[6], v[7]};
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (col + e < cols) {
+                if (bf16) static_cast<uint16_t *>(base)[at + e] = (uint16_t)round_bf16(v[e]);
+                else static_cast<float *>(base)[at + e] = v[e];
+            }
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store_codes8(uint8_t *dst, int col, int cols, uint32_t lo, uint32_t hi) {
+    if constexpr (VEC) {
+        *reinterpret_cast<u32x2 *>(dst) = u32x2{lo, hi};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (col + e < cols) dst[e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
+    }
+}
+
+__device__ __forceinline__ float max8(const float (&v)[8]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
+    return m;
+}
+
+// The largest of 16 consecutive lanes (a group of 128 columns, eight a lane): four row rotations.
+__device__ __forceinline__ float max_of_16(float m) {
+    auto turn = [](float f, auto by) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(f), 0x120 + decltype(by)::value, 0xF, 0xF, true));
+    };
+    m = fmaxf(m, turn(m, std::integral_constant<int, 8>{}));
+    m = fmaxf(m, turn(m, std::integral_constant<int, 4>{}));
+    m = fmaxf(m, turn(m, std::integral_constant<int, 2>{}));
+    return fmaxf(m, turn(m, std::integral_constant<int, 1>{}));
+}
+
+__device__ __forceinline__ float group_scale(float m) {
+    const float q = __fdiv_rn(m, 448.0f);
+    return q > 1e-30f ? q : 1e-30f;
+}
+
+__device__ __forceinline__ void e4m3_codes(const float (&y)[8], float scale, uint32_t &lo, uint32_t &hi) {
+    const float recip = __fdiv_rn(1.0f, scale);
+    float q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = y[e] * recip;
+    lo = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    lo = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], (int)lo, true);
+    hi = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
+    hi = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], (int)hi, true);
+}
+
+// clamp(rint(y / s)) from the reciprocal's product where that surely rounds alike (quant::store_codes).
+__device__ __forceinline__ void int8_codes(const float (&y)[8], float scale, uint32_t &lo, uint32_t &hi) {
+    const float recip = __fdiv_rn(1.0f, scale);
+    float c[8];
+    bool hard = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float q = y[e] * recip;
+        c[e] = rintf(q);
+        hard |= fabsf(q - c[e]) > 0.5f - 0x1p-14f;
+    }
+    if (hard) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = rintf(__fdiv_rn(y[e], scale));
+    }
+    lo = hi = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        lo |= (uint32_t)(uint8_t)(int8_t)(int)fminf(fmaxf(c[e], -128.0f), 127.0f) << (8 * e);
+        hi |= (uint32_t)(uint8_t)(int8_t)(int)fminf(fmaxf(c[4 + e], -128.0f), 127.0f) << (8 * e);
+    }
+}
+
+// Rows in turn over the grid, T threads a row, each holding IT runs of 8 columns 8·T apart in registers: one read
+// of x and r, w once a workgroup.
+template <bool INT8, int T, int IT, bool VEC>
+__global__ void __launch_bounds__(T) add_norm_kernel(const AddNormArgs p) {
+    constexpr int WAVES = T / 64;
+    __shared__ float sums[2][WAVES], tops[2][WAVES];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    float w[IT][8];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int col = 8 * (tid + T * i);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[i][e] = 0.0f;
+        if (col < p.cols) load8<VEC>(p.w, false, col, col, p.cols, w[i]);
+    }
+    int turn = 0;
+    for (unsigned row = blockIdx.x; row < (unsigned)p.rows; row += gridDim.x, turn ^= 1) {
+        float v[IT][8];
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+            const int col = 8 * (tid + T * i);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
+            if (col < p.cols) load8<VEC>(p.x, p.x_bf16, (int64_t)row * p.ldx + col, col, p.cols, v[i]);
+        }
+        if (p.r) {
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const int col = 8 * (tid + T * i);
+                if (col < p.cols) {
+                    float r[8];
+                    load8<VEC>(p.r, p.r_bf16, (int64_t)row * p.ldr + col, col, p.cols, r);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[i][e] = r[e] + v[i][e];
+                    if (p.ro) store8<VEC>(p.ro, p.r_bf16, (int64_t)row * p.ldro + col, col, p.cols, v[i]);
+                }
+            }
+        }
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < IT; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(v[i][e], v[i][e], ss);
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
+        if constexpr (WAVES > 1) {
+            // One barrier a row: a wave is at most one row ahead, and writes the other half of `sums` there.
+            if (lane == 0) sums[turn][wave] = ss;
+            __syncthreads();
+            ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) ss += sums[turn][i];
+        }
+        const float r = __fdiv_rn(1.0f, __fsqrt_rn(__fdiv_rn(ss, (float)p.cols) + p.eps));
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < IT; ++i) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = (v[i][e] * r) * w[i][e];
+            if constexpr (INT8) top = fmaxf(top, max8(v[i]));
+        }
+        if constexpr (INT8) {
+#pragma unroll
+            for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+            if constexpr (WAVES > 1) {
+                if (lane == 0) tops[turn][wave] = top;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < WAVES; ++i) top = fmaxf(top, tops[turn][i]);
+            }
+            const float scale = quant::row_scale(top);
+            if (tid == 0) p.scales[row] = scale;
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const int col = 8 * (tid + T * i);
+                if (col >= p.cols) break;
+                uint32_t lo, hi;
+                int8_codes(v[i], scale, lo, hi);
+                store_codes8<VEC>(p.codes + (int64_t)row * p.ldq + col, col, p.cols, lo, hi);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < IT; ++i) {
+                const int col = 8 * (tid + T * i);
+                const float scale = group_scale(max_of_16(max8(v[i])));  // in every lane: the 16 agree
+                if (col >= p.cols) continue;
+                uint32_t lo, hi;
+                e4m3_codes(v[i], scale, lo, hi);
+                store_codes8<VEC>(p.codes + (int64_t)row * p.ldq + col, col, p.cols, lo, hi);
+                if ((tid & 15) == 0) p.scales[(int64_t)row * p.lds + col / F8_GROUP] = scale;
+            }
+        }
+    }
+}
+
+// Sixteen lanes a group of 128 columns, groups in order over the grid.
+template <bool VEC>
+__global__ void __launch_bounds__(256) quantize_groups_kernel(const void *x, bool x_bf16, int64_t ldx, unsigned total,
+                                                              unsigned groups, int cols, uint8_t *codes, int64_t ldq,
+                                                              float *scales, int64_t lds) {
+    const unsigned sub = threadIdx.x & 15;
+    for (unsigned g = blockIdx.x * 16 + (threadIdx.x >> 4); g < total; g += gridDim.x * 16) {
+        const unsigned row = g / groups, group = g - row * groups;
+        const int col = (int)(group * F8_GROUP + sub * 8);
+        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        if (col < cols) load8<VEC>(x, x_bf16, (int64_t)row * ldx + col, col, cols, v);
+        const float scale = group_scale(max_of_16(max8(v)));
+        if (col < cols) {
+            uint32_t lo, hi;
+            e4m3_codes(v, scale, lo, hi);
+            store_codes8<VEC>(codes + (int64_t)row * ldq + col, col, cols, lo, hi);
+        }
+        if (sub == 0) scales[(int64_t)row * lds + group] = scale;
+    }
+}
+
+// A thread a 4-byte word of the destination.
+__global__ void __launch_bounds__(256) pad_bytes_kernel(const uint8_t *src, int64_t lds, uint8_t *dst, int64_t ldd,
+                                                        int64_t words, unsigned row_words, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / row_words;
+        const int64_t at = (i - row * row_words) * 4;
+        uint32_t word = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (at + e < n) word |= (uint32_t)src[row * lds + at + e] << (8 * e);
+        *reinterpret_cast<uint32_t *>(dst + row * ldd + at) = word;
+    }
+}
+
+bool at_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+hipError_t launch_add_norm(const AddNormArgs &p, bool int8, int cus, hipStream_t stream) {
+    if (p.rows == 0 || p.cols == 0) return hipSuccess;
+    const bool vec = p.cols % 8 == 0 && at_16(p.x) && p.ldx % 8 == 0 && at_16(p.w) && (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0 &&
+                     p.ldq % 8 == 0 && (!p.r || (at_16(p.r) && p.ldr % 8 == 0)) && (!p.ro || (at_16(p.ro) && p.ldro % 8 == 0));
+#define SQ8_ADD_NORM(T, IT)                                                                                          \
+    do {                                                                                                             \
+        const int most = cus * (2048 / T), grid = p.rows < most ? p.rows : most;                                      \
+        if (int8 && vec) hipLaunchKernelGGL((add_norm_kernel<true, T, IT, true>), dim3(grid), dim3(T), 0, stream, p); \
+        else if (int8) hipLaunchKernelGGL((add_norm_kernel<true, T, IT, false>), dim3(grid), dim3(T), 0, stream, p);  \
+        else if (vec) hipLaunchKernelGGL((add_norm_kernel<false, T, IT, true>), dim3(grid), dim3(T), 0, stream, p);   \
+        else hipLaunchKernelGGL((add_norm_kernel<false, T, IT, false>), dim3(grid), dim3(T), 0, stream, p);           \
+        return hipGetLastError();                                                                                    \
+    } while (0)
+    if (p.cols <= 512) SQ8_ADD_NORM(64, 1);
+    if (p.cols <= 1024) SQ8_ADD_NORM(64, 2);
+    if (p.cols <= 4096) SQ8_ADD_NORM(256, 2);
+    if (p.cols <= 8192) SQ8_ADD_NORM(256, 4);
+    if (p.cols <= 16384) SQ8_ADD_NORM(1024, 2);
+    if (p.cols <= kAddNormCols) SQ8_ADD_NORM(1024, 4);
+#undef SQ8_ADD_NORM
+    return hipErrorInvalidValue;
+}
+
+hipError_t launch_quantize_groups(const void *x, bool x_bf16, int64_t ldx, int rows, int cols, uint8_t *codes, int64_t ldq,
+                                  float *scales, int64_t lds, hipStream_t stream) {
+    if (rows == 0 || cols == 0) return hipSuccess;
+    const int64_t groups = (cols + F8_GROUP - 1) / F8_GROUP, total = rows * groups;
+    if (total > INT32_MAX - 65536 * 16) return hipErrorInvalidValue;
+    const bool vec = cols % 8 == 0 && at_16(x) && ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && ldq % 8 == 0;
+    const int64_t want = (total + 15) / 16;
+    const dim3 grid((unsigned)(want < 65536 ? want : 65536));
+    if (vec)
+        hipLaunchKernelGGL(quantize_groups_kernel<true>, grid, dim3(256), 0, stream, x, x_bf16, ldx, (unsigned)total,
+                           (unsigned)groups, cols, codes, ldq, scales, lds);
+    else
+        hipLaunchKernelGGL(quantize_groups_kernel<false>, grid, dim3(256), 0, stream, x, x_bf16, ldx, (unsigned)total,
+                           (unsigned)groups, cols, codes, ldq, scales, lds);
+    return hipGetLastError();
+}
+
+hipError_t launch_pad_bytes(const void *src, int64_t lds, void *dst, int64_t ldd, int64_t rows, int64_t n,
+                            hipStream_t stream) {
+    if (rows == 0 || ldd == 0) return hipSuccess;
+    const int64_t words = rows * (ldd / 4), want = (words + 255) / 256;
+    hipLaunchKernelGGL(pad_bytes_kernel, dim3((unsigned)(want < 65536 ? want : 65536)), dim3(256), 0, stream,
+                       static_cast<const uint8_t *>(src), lds, static_cast<uint8_t *>(dst), ldd, words, (unsigned)(ldd / 4), n);
+    return hipGetLastError();
+}
+
+}  // namespace sq8

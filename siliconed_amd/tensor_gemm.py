@@ -17,6 +17,7 @@ from typing import Optional
 import torch
 
 from . import _abi as abi
+from .text_ops import TextOps
 
 _EPILOGUES = {
     None: abi.EPI_NONE, "none": abi.EPI_NONE,
@@ -118,8 +119,9 @@ def _block_scales(scale: Optional[torch.Tensor], lay: int, n: int, k: int, block
                          f"(it has strides {tuple(scale.stride())})")
 
 
-class TensorGEMM:
-    """One context (device + stream) of the library: `TensorGEMM` of the reference."""
+class TensorGEMM(TextOps):
+    """One context (device + stream) of the library: `TensorGEMM` of the reference, and a text decoder's operators
+    (text_ops.py)."""
 
     def __init__(self, handle: ctypes.c_void_p, device: int):
         self._h = handle
