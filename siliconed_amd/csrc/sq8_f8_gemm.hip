@@ -21,8 +21,11 @@
 // and weight rows past the last read the last one; their results are not stored.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "sq8_device.h"
 #include "sq8_text.h"
+#include "sq8_wdirect_kernel.h"
 
 namespace sq8 {
 namespace {
@@ -62,6 +65,37 @@ __device__ __forceinline__ i32x8 load_f8(const uint8_t *row, int kb, int h, int 
     return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
 }
 
+// N consecutive outputs, the first `real` of them, from element `at` of C.
+template <int N, bool F32>
+__device__ __forceinline__ void store_run(void *c, int64_t at, int real, int vec, const float (&y)[N]) {
+    if (vec && real == N) {
+        if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < N; e += 4)
+                *reinterpret_cast<f32x4 *>(static_cast<float *>(c) + at + e) = f32x4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+        } else {
+            uint16_t *to = static_cast<uint16_t *>(c) + at;
+            if (N == 4 || vec < 8) {
+#pragma unroll
+                for (int e = 0; e < N; e += 4)
+                    *reinterpret_cast<u32x2 *>(to + e) = u32x2{pack_bf16_rne(y[e], y[e + 1]), pack_bf16_rne(y[e + 2], y[e + 3])};
+            } else {
+#pragma unroll
+                for (int e = 0; e + 8 <= N; e += 8)
+                    *reinterpret_cast<u32x4 *>(to + e) = u32x4{pack_bf16_rne(y[e], y[e + 1]), pack_bf16_rne(y[e + 2], y[e + 3]),
+                                                               pack_bf16_rne(y[e + 4], y[e + 5]), pack_bf16_rne(y[e + 6], y[e + 7])};
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            if (e < real) {
+                if constexpr (F32) static_cast<float *>(c)[at + e] = y[e];
+                else static_cast<uint16_t *>(c)[at + e] = (uint16_t)(pack_bf16_rne(y[e], y[e]) & 0xFFFFu);
+            }
+    }
+}
+
 // Four consecutive outputs from column `col` of row `row`: bias, activation, store.
 template <bool GLU, bool F32>
 __device__ __forceinline__ void store4(const F8Args &p, int row, int col, f32x4 x, f32x4 u) {
@@ -70,44 +104,30 @@ __device__ __forceinline__ void store4(const F8Args &p, int row, int col, f32x4 
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int n = min(col + e, p.H - 1);
-        float v = x[e];
-        if (p.bias) v += p.bias[n];
-        if constexpr (GLU) {
-            float w = u[e];
-            if (p.bias) w += p.bias[p.H + n];
-            v = silu_glu(v, w);
-        }
-        y[e] = v;
+        y[e] = x[e];
+        if (p.bias) y[e] += p.bias[n];
+        if constexpr (GLU) y[e] = silu_glu(y[e], p.bias ? u[e] + p.bias[p.H + n] : u[e]);
     }
-    const int64_t at = (int64_t)row * p.ldc + col;
-    if (p.c_vec && col + 4 <= p.H) {
-        if constexpr (F32) *reinterpret_cast<f32x4 *>(static_cast<float *>(p.c) + at) = f32x4{y[0], y[1], y[2], y[3]};
-        else *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(p.c) + at) = u32x2{pack_bf16_rne(y[0], y[1]), pack_bf16_rne(y[2], y[3])};
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (col + e < p.H) {
-                if constexpr (F32) static_cast<float *>(p.c)[at + e] = y[e];
-                else static_cast<uint16_t *>(p.c)[at + e] = (uint16_t)(pack_bf16_rne(y[e], y[e]) & 0xFFFFu);
-            }
-    }
+    store_run<4, F32>(p.c, (int64_t)row * p.ldc + col, p.H - col < 4 ? p.H - col : 4, p.c_vec, y);
 }
 
-// Few rows: a workgroup of NW waves takes 16 output columns (GLU: of both halves) and TM tiles of 16 rows; the
-// waves take the K blocks in turn, both operands straight from memory, and add up through LDS.
-template <int TM, int NW, bool GLU, bool F32>
+// Few rows: a workgroup of NW waves takes NO × 16 output columns (GLU: of both halves) and TM tiles of 16 rows; the
+// waves take the K blocks in turn, both operands straight from memory, U blocks' loads in flight, and add up through
+// LDS.
+template <int TM, int NO, int NW, int U, bool GLU, bool F32>
 __global__ void __launch_bounds__(64 * NW) f8_short_kernel(const F8Args p) {
-    constexpr int NT = GLU ? 2 : 1;
+    constexpr int NT = GLU ? 2 * NO : NO;
     __shared__ __attribute__((aligned(16))) f32x4 sums[NW][TM * NT][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, h = lane >> 4;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * TM);
+    const int n0 = blockIdx.x * (16 * NO), m0 = blockIdx.y * (16 * TM);
     const uint8_t *wrow[NT];
     const float *sw[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        wrow[j] = p.w + ((int64_t)min(n0 + c, p.H - 1) + (int64_t)j * p.H) * p.ldw;
-        sw[j] = p.sw + (int64_t)(n0 / F8_GROUP + j * p.up_block) * p.ldsw;
+        const int half = j / NO, at = n0 + 16 * (j - half * NO);
+        wrow[j] = p.w + ((int64_t)min(at + c, p.H - 1) + (int64_t)half * p.H) * p.ldw;
+        sw[j] = p.sw + (int64_t)(min(at, p.H - 1) / F8_GROUP + half * p.up_block) * p.ldsw;
     }
     const uint8_t *arow[TM];
     const float *sx[TM];
@@ -122,21 +142,35 @@ __global__ void __launch_bounds__(64 * NW) f8_short_kernel(const F8Args p) {
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int kb = wave; kb < p.KB; kb += NW) {
-        i32x8 w[NT];
+    for (int k0 = wave; k0 < p.KB; k0 += U * NW) {
+        i32x8 w[U][NT], a[U][TM];
+        float s_x[U][TM], s_w[U][NT];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) w[j] = load_f8(wrow[j], kb, h, p.K);
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const i32x8 a = load_f8(arow[i], kb, h, p.K);
-            const float s = sx[i][kb];
+        for (int u = 0; u < U; ++u) {
+            const int kb = min(k0 + u * NW, p.KB - 1);  // past the last: its scales are zeroed below
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const f32x4 part = block_sums<F32>(w[j], a);
-                const float both = s * sw[j][kb];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(part[e], both, acc[i][j][e]);
+                w[u][j] = load_f8(wrow[j], kb, h, p.K);
+                s_w[u][j] = sw[j][kb];
             }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                a[u][i] = load_f8(arow[i], kb, h, p.K);
+                s_x[u][i] = sx[i][kb];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 + u * NW >= p.KB) break;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const f32x4 part = block_sums<F32>(w[u][j], a[u][i]);
+                    const float both = s_x[u][i] * s_w[u][j];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(part[e], both, acc[i][j][e]);
+                }
         }
     }
 #pragma unroll
@@ -144,40 +178,431 @@ __global__ void __launch_bounds__(64 * NW) f8_short_kernel(const F8Args p) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) sums[wave][i * NT + j][lane] = acc[i][j];
     __syncthreads();
-    for (int i = wave; i < TM; i += NW) {
+    for (int q = wave; q < TM * NO; q += NW) {
+        const int i = q / NO, j = q - i * NO;
         f32x4 x[2] = {};
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            f32x4 v = sums[0][i * NT + j][lane];
+        for (int half = 0; half < NT / NO; ++half) {
+            f32x4 v = sums[0][i * NT + half * NO + j][lane];
 #pragma unroll
-            for (int g = 1; g < NW; ++g) v += sums[g][i * NT + j][lane];
-            x[j] = v;
+            for (int g = 1; g < NW; ++g) v += sums[g][i * NT + half * NO + j][lane];
+            x[half] = v;
         }
-        store4<GLU, F32>(p, m0 + 16 * i + c, n0 + 4 * h, x[0], x[1]);
+        store4<GLU, F32>(p, m0 + 16 * i + c, n0 + 16 * j + 4 * h, x[0], x[1]);
     }
 }
 
-template <int TM, bool GLU, bool F32>
-hipError_t launch_short(const F8Args &p, hipStream_t stream) {
-    constexpr int NW = 8;
-    const dim3 grid((unsigned)((p.H + 15) / 16), (unsigned)((p.M + 16 * TM - 1) / (16 * TM)));
-    hipLaunchKernelGGL((f8_short_kernel<TM, NW, GLU, F32>), grid, dim3(64 * NW), 0, stream, p);
+// Many rows: tiles of BM rows by BN weight rows (GLU: half of them of each half), WM × WN waves.
+//
+// Both operands go to LDS by direct loads, a block (128 bytes) of each row a step, in two stages. 16-byte runs of a
+// row are permuted within it (by key_a, key_w) so that the eight rows a fragment read touches at once lie on different
+// banks. The rows' scales go to LDS too, four blocks at a time where they can be read so.
+//
+// Each wave multiplies (BM/WM) × (BN/WN) in 16 × 16 parts, a row of TN parts at a time, the weight's fragments held for
+// the step and the rows' read two parts ahead; the multiply-adds that scale one row of parts go between the matrix
+// instructions of the next. The step's one barrier stands before its last two rows of parts, whose fragments are in
+// registers by then: the stage is free for the loads of the step after next, the next step's loads have landed, and
+// its first fragments are read under the last matrix instructions of this one.
+//
+// The weight row an instruction's row stands for is chosen so that a lane ends with consecutive outputs: lane group
+// h, register r of part j is output 4·NTO·h + 4j + r of the wave's (NTO parts wide).
+template <int BM, int BN, int WM, int WN, int NS, bool GLU, bool F32>
+struct TileShape {
+    static constexpr int THREADS = 64 * WM * WN;
+    static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;  // parts of a wave
+    static constexpr int NTO = GLU ? TN / 2 : TN;               // and those of one half
+    static constexpr int OUT = GLU ? BN / 2 : BN;               // outputs of a tile
+    static constexpr int STAGE = (BM + BN) * F8_GROUP;
+    // The rows' scales: two buffers of four blocks', or with more stages one block's a stage (and room for the
+    // waves that have no row).
+    static constexpr int SCALES = NS == 2 ? BM * 16 : WM * WN * 256;
+    static constexpr int LDS = NS * (STAGE + SCALES);
+    static_assert(TM * 16 * WM == BM && TN * 16 * WN == BN && (!GLU || TN % 2 == 0), "whole parts");
+    static_assert(NTO == 1 || NTO == 2 || NTO == 4, "a lane's outputs");
+};
+
+__device__ __forceinline__ int key_a(int row) { return row & 7; }
+// Rows 4·NTO·(c / 4) + 4j + c mod 4 of eight consecutive c: different keys.
+template <int NTO>
+__device__ __forceinline__ int key_w(int row) {
+    constexpr int SHIFT = NTO == 4 ? 4 : NTO == 2 ? 3 : 2;
+    return (row & 3) | ((row >> SHIFT) & 1) << 2;
+}
+
+// Columns of a row of partial sums: whole runs of a lane's outputs.
+__host__ __device__ constexpr int part_columns(int h) { return (h + 15) / 16 * 16; }
+
+template <int BM, int BN, int WM, int WN, int NS, bool GLU, bool F32>
+__global__ void __attribute__((amdgpu_flat_work_group_size(64 * WM * WN, 64 * WM * WN), amdgpu_waves_per_eu(2, 2)))
+f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
+    using S = TileShape<BM, BN, WM, WN, NS, GLU, F32>;
+    constexpr int TM = S::TM, TN = S::TN, NTO = S::NTO, WAVES = WM * WN;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[S::LDS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, h = lane >> 4;
+    int tm, tn;
+    kern::tile_of(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    // This workgroup's blocks of K: all, or one of gridDim.y parts.
+    const int t0 = (int)((int64_t)p.KB * blockIdx.y / gridDim.y), t1 = (int)((int64_t)p.KB * (blockIdx.y + 1) / gridDim.y);
+    const int m0 = tm * BM, n0 = tn * S::OUT;
+    const int wm = wave % WM, wn = wave / WM;
+
+    // ---- loads: a wave instruction fills 8 rows; lane → row lane / 8, run (lane mod 8) ^ key ----
+    constexpr int A_LOADS = BM / 8 / WAVES, W_LOADS = BN / 8 / WAVES;
+    static_assert(A_LOADS * 8 * WAVES == BM && W_LOADS * 8 * WAVES == BN, "loads spread evenly");
+    const wd::i32x4 a_rsrc = wd::buffer_rsrc(p.a + (int64_t)m0 * p.lda), w_rsrc = wd::buffer_rsrc(p.w + (int64_t)n0 * p.ldw);
+    uint32_t a_off[A_LOADS], w_off[W_LOADS];
+    const int a_run = ((lane & 7) ^ key_a(lane >> 3)) * 16;
+    auto w_run = [&](int i) { return ((lane & 7) ^ key_w<NTO>((wave * W_LOADS + i) * 8 + (lane >> 3))) * 16; };
+#pragma unroll
+    for (int i = 0; i < A_LOADS; ++i)
+        a_off[i] = (uint32_t)(min((wave * A_LOADS + i) * 8 + (lane >> 3), p.M - 1 - m0) * p.lda) + a_run;
+#pragma unroll
+    for (int i = 0; i < W_LOADS; ++i) {
+        const int row = (wave * W_LOADS + i) * 8 + (lane >> 3);
+        const int half = GLU && row >= BN / 2 ? 1 : 0;
+        const int64_t n = min(row - half * (BN / 2), p.H - 1 - n0) + (int64_t)half * p.H;
+        w_off[i] = (uint32_t)(n * p.ldw) + w_run(i);
+    }
+    const int left = p.K & (F8_GROUP - 1);  // of a last block that K ends inside
+    uint8_t *const scales = lds + NS * S::STAGE;
+    const wd::i32x4 sx_rsrc = wd::buffer_rsrc(p.sx + (int64_t)m0 * p.ldsx);
+    // NS > 2: one row's scale a lane; the waves past BM rows read row 0's, so that every wave's loads are as many.
+    const uint32_t sx_off = (uint32_t)min(wave * 64 < BM ? wave * 64 + lane : 0, p.M - 1 - m0) * (uint32_t)p.ldsx * 4;
+    constexpr int LOADS = A_LOADS + W_LOADS + 1;  // a wave's of one block (NS > 2)
+    auto issue = [&](int t, int stage) {
+        const int at = t * F8_GROUP;
+        uint8_t *const to = lds + stage;
+        if (left == 0 || t != p.KB - 1) {
+#pragma unroll
+            for (int i = 0; i < A_LOADS; ++i)
+                wd::raw_buffer_load_lds(a_rsrc, (wd::lds_u32)(to + (wave * A_LOADS + i) * 1024), 16, (int)a_off[i], at, 0, 0);
+#pragma unroll
+            for (int i = 0; i < W_LOADS; ++i)
+                wd::raw_buffer_load_lds(w_rsrc, (wd::lds_u32)(to + BM * F8_GROUP + (wave * W_LOADS + i) * 1024), 16, (int)w_off[i], at, 0, 0);
+        } else {
+            // Runs past K are read from the block's first. (Nothing of this is worth registers over the loop: the
+            // empty statement keeps it here.)
+            int end = left;
+            asm volatile("" : "+s"(end));
+#pragma unroll
+            for (int i = 0; i < A_LOADS; ++i)
+                wd::raw_buffer_load_lds(a_rsrc, (wd::lds_u32)(to + (wave * A_LOADS + i) * 1024), 16,
+                                        (int)(a_off[i] - (a_run >= end ? a_run : 0)), at, 0, 0);
+#pragma unroll
+            for (int i = 0; i < W_LOADS; ++i)
+                wd::raw_buffer_load_lds(w_rsrc, (wd::lds_u32)(to + BM * F8_GROUP + (wave * W_LOADS + i) * 1024), 16,
+                                        (int)(w_off[i] - (w_run(i) >= end ? w_run(i) : 0)), at, 0, 0);
+        }
+        if constexpr (NS > 2) {
+            wd::raw_buffer_load_lds(sx_rsrc, (wd::lds_u32)(scales + (stage / S::STAGE) * S::SCALES + wave * 256), 4, (int)sx_off, t * 4, 0, 0);
+        } else if (!p.sx_vec || (t & 3) == 0 || t == t0) {
+            // A lane a row; sx_vec: blocks t .. t + 3 as [row][4], else one block as [4][row].
+            uint8_t *const s = scales + ((t >> 2) & 1) * S::SCALES;
+            int last_row = p.M - 1 - m0;
+            asm volatile("" : "+s"(last_row));
+            for (int r = wave * 64; r < BM; r += 64 * WAVES) {
+                const int from = (int)(min(r + lane, last_row) * (uint32_t)p.ldsx * 4);
+                if (p.sx_vec) wd::raw_buffer_load_lds(sx_rsrc, (wd::lds_u32)(s + r * 16), 16, from, (t & ~3) * 4, 0, 0);
+                else wd::raw_buffer_load_lds(sx_rsrc, (wd::lds_u32)(s + ((t & 3) * BM + r) * 4), 4, from, t * 4, 0, 0);
+            }
+        }
+    };
+    // Block t's loads are done, this wave's and then all; those of NS − 2 later ones may be under way, where there are
+    // as many (`more`). The activation's runs past K become zeros in between.
+    auto landed = [&](int t, int stage, bool more) {
+        if (NS > 2 && more) wd::wait_vmcnt<NS == 2 ? 0 : (NS - 2) * LOADS>();
+        else wd::wait_vmcnt<0>();
+        if (left != 0 && t == p.KB - 1 && a_run >= left) {
+#pragma unroll
+            for (int i = 0; i < A_LOADS; ++i)
+                *reinterpret_cast<u32x4 *>(lds + stage + (wave * A_LOADS + i) * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
+        }
+        __syncthreads();
+    };
+    const int scale_row = NS == 2 && p.sx_vec ? 16 : 4, scale_block = p.sx_vec ? 4 : BM * 4;
+
+    // ---- fragment addresses: neither key depends on the part, whose rows lie at fixed distances ----
+    int a_at[2], w_at[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int ra = wm * (BM / WM) + c, rw = wn * (16 * NTO) + 4 * NTO * (c >> 2) + (c & 3);
+        a_at[u] = ra * F8_GROUP + (((4 * u + h) ^ key_a(ra)) << 4);
+        w_at[u] = BM * F8_GROUP + rw * F8_GROUP + (((4 * u + h) ^ key_w<NTO>(rw)) << 4);
+    }
+    const int sx_at = NS * S::STAGE + (wm * (BM / WM) + c) * scale_row;
+    // A wave's outputs of one half lie in one block of 128 columns (past the last: none are stored). Lane l keeps the
+    // scale of block l of each 64.
+    const float *const sw0 = p.sw + (int64_t)min((n0 + wn * 16 * NTO) / F8_GROUP, p.up_block - 1) * p.ldsw;
+    float sw_of[2];
+    auto load_sw = [&](int t) {
+#pragma unroll
+        for (int g = 0; g < (GLU ? 2 : 1); ++g) sw_of[g] = sw0[(int64_t)g * p.up_block * p.ldsw + min(t + lane, t1 - 1)];
+        wd::wait_vmcnt<0>();
+    };
+
+    f32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    i32x8 w[TN], a[2];
+    float s_x[2], both[2][2];
+    f32x4 part[TN];
+    auto fragment = [&](int lo, int hi) {
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(lds + lo), y = *reinterpret_cast<const u32x4 *>(lds + hi);
+        return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+    };
+    int stage = 0;  // the offset in LDS of the stage whose fragments are read, and of its scales
+    auto scales_of = [&](int t, int stage) {
+        return NS == 2 ? sx_at + (t & 3) * scale_block + ((t >> 2) & 1) * S::SCALES : sx_at + (stage / S::STAGE) * S::SCALES;
+    };
+    int sx_now = scales_of(t0, 0);
+    auto read_a = [&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        a[i & 1] = fragment(a_at[0] + stage + i * 16 * F8_GROUP, a_at[1] + stage + i * 16 * F8_GROUP);
+        s_x[i & 1] = *reinterpret_cast<const float *>(lds + sx_now + i * 16 * scale_row);
+    };
+    auto read_w = [&](auto jc) {
+        constexpr int j = decltype(jc)::value, from = ((j / NTO) * (BN / 2) + 4 * (j % NTO)) * F8_GROUP;
+        w[j] = fragment(w_at[0] + stage + from, w_at[1] + stage + from);
+    };
+    auto add = [&](auto ic, auto jc) {
+        constexpr int i = decltype(ic)::value, j = decltype(jc)::value;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(part[j][e], both[i & 1][j / NTO & 1], acc[i][j][e]);
+        // Kept where it stands: moved down past the step's branches it would hold on to its part's registers.
+        asm volatile("" : "+v"(acc[i][j][0]), "+v"(acc[i][j][1]), "+v"(acc[i][j][2]), "+v"(acc[i][j][3]));
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using Last = std::integral_constant<int, TM - 1>;
+    static_assert(TM >= 2 && TM % 2 == 0, "fragments of two rows of parts in turn");
+
+    if (t0 < t1) {
+        load_sw(t0);
+        static_for<0, NS>([&](auto sc) {
+            constexpr int s = decltype(sc)::value;
+            if (s == 0 || t0 + s < t1) issue(t0 + s, s * S::STAGE);
+            // With two stages the first is waited for alone, as the loop does.
+            if constexpr (NS == 2 && s == 0) landed(t0, 0, false);
+        });
+        if constexpr (NS > 2) {
+            landed(t0, 0, t0 + NS <= t1);
+        }
+        static_for<0, TN>([&](auto jc) { read_w(jc); });
+        read_a(I0{});
+        read_a(I1{});
+#pragma unroll
+        for (int j = 0; j < TN; ++j) part[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        both[1][0] = both[1][1] = 0.0f;
+    }
+#pragma clang loop unroll(disable)
+    for (int t = t0; t < t1; ++t) {
+        float s_w[2];
+        if (t != t0 && ((t - t0) & 63) == 0) load_sw(t);
+#pragma unroll
+        for (int g = 0; g < (GLU ? 2 : 1); ++g) s_w[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sw_of[g]), (t - t0) & 63));
+        static_for<0, TM>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            using Before = std::integral_constant<int, (i + TM - 1) % TM>;
+            if constexpr (i == TM - 2) {
+                // Every fragment of this stage is in registers (or on its way there: the barrier waits for those).
+                const int from = stage;
+                stage = stage == (NS - 1) * S::STAGE ? 0 : stage + S::STAGE;
+                landed(t + 1, stage, t + NS <= t1);
+                if (t + NS < t1) issue(t + NS, from);
+                sx_now = scales_of(t + 1, stage);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int g = 0; g < (GLU ? 2 : 1); ++g) both[i & 1][g] = s_x[i & 1] * s_w[g];
+            static_for<0, TN>([&](auto jc) {
+                constexpr int j = decltype(jc)::value;
+                add(Before{}, jc);
+                part[j] = block_sums<F32>(w[j], a[i & 1]);
+                if constexpr (i == TM - 1) read_w(jc);
+            });
+            read_a(std::integral_constant<int, (i + 2) % TM>{});
+            if constexpr (!F32) {
+                // The multiply-adds of a part of the row before, the matrix instruction that takes its place, its reads.
+                static_for<0, TN>([&](auto) {
+                    __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if constexpr (i == TM - 1) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                });
+                __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+    }
+    if (t0 < t1) static_for<0, TN>([&](auto jc) { add(Last{}, jc); });
+
+    // ---- outputs: N consecutive ones of each of TM rows ----
+    constexpr int N = 4 * NTO;
+    const int col = n0 + wn * 16 * NTO + N * h;
+    const int real = min(N, p.H - col);  // of them
+    const int row0 = m0 + wm * (BM / WM) + c;
+    if (gridDim.y > 1) {
+        // One part of K: its sums as they are, to be added up by f8_join_kernel.
+        const int wide = part_columns(p.H);
+        if (col >= wide) return;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            if (row0 + 16 * i >= p.M) continue;
+#pragma unroll
+            for (int g = 0; g < (GLU ? 2 : 1); ++g) {
+                float *to = p.part + (((int64_t)blockIdx.y * p.M + row0 + 16 * i) * (GLU ? 2 : 1) + g) * wide + col;
+#pragma unroll
+                for (int j = 0; j < NTO; ++j) *reinterpret_cast<f32x4 *>(to + 4 * j) = acc[i][g * NTO + j];
+            }
+        }
+        return;
+    }
+    float bias[GLU ? 2 : 1][N];
+    if (p.bias) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            bias[0][e] = p.bias[min(col + e, p.H - 1)];
+            if constexpr (GLU) bias[1][e] = p.bias[min(col + e, p.H - 1) + p.H];
+        }
+    }
+    static_for<0, TM>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        float y[N];
+        static_for<0, N>([&](auto ec) {
+            constexpr int e = decltype(ec)::value;
+            float x = acc[i][e / 4][e % 4];
+            if (p.bias) x += bias[0][e];
+            if constexpr (GLU) {
+                float u = acc[i][NTO + e / 4][e % 4];
+                if (p.bias) u += bias[1][e];
+                x = silu_glu(x, u);
+            }
+            y[e] = x;
+        });
+        if (row0 + 16 * i < p.M) store_run<N, F32>(p.c, (int64_t)(row0 + 16 * i) * p.ldc + col, real, p.c_vec, y);
+        __builtin_amdgcn_sched_barrier(0);
+    });
+}
+
+// The parts' sums of a product whose K was split, added in order, then as ever: four outputs a thread.
+template <bool GLU, bool F32>
+__global__ void __launch_bounds__(256) f8_join_kernel(const F8Args p, int splits) {
+    constexpr int HALVES = GLU ? 2 : 1;
+    const int wide = part_columns(p.H), quads = wide / 4;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < (int64_t)p.M * quads; q += (int64_t)gridDim.x * 256) {
+        const int row = (int)(q / quads), col = 4 * (int)(q - (int64_t)row * quads);
+        f32x4 x[2] = {};
+        for (int s = 0; s < splits; ++s)
+#pragma unroll
+            for (int g = 0; g < HALVES; ++g)
+                x[g] += *reinterpret_cast<const f32x4 *>(p.part + (((int64_t)s * p.M + row) * HALVES + g) * wide + col);
+        store4<GLU, F32>(p, row, col, x[0], x[1]);
+    }
+}
+
+template <int BM, int BN, int WM, int WN, int NS, bool GLU, bool F32>
+hipError_t launch_tile(const F8Args &p, int splits, hipStream_t stream) {
+    using S = TileShape<BM, BN, WM, WN, NS, GLU, F32>;
+    const int64_t tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.H + S::OUT - 1) / S::OUT;
+    if (tiles_m * tiles_n > INT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((f8_tile_kernel<BM, BN, WM, WN, NS, GLU, F32>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)splits),
+                       dim3(S::THREADS), 0, stream, p, (int)tiles_m, (int)tiles_n);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || splits == 1) return e;
+    const int64_t blocks = ((int64_t)p.M * (part_columns(p.H) / 4) + 255) / 256;
+    hipLaunchKernelGGL((f8_join_kernel<GLU, F32>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, p, splits);
     return hipGetLastError();
 }
 
+template <int TM, int NO, int NW, int U, bool GLU, bool F32>
+hipError_t launch_short(const F8Args &p, hipStream_t stream) {
+    const dim3 grid((unsigned)((p.H + 16 * NO - 1) / (16 * NO)), (unsigned)((p.M + 16 * TM - 1) / (16 * TM)));
+    hipLaunchKernelGGL((f8_short_kernel<TM, NO, NW, U, GLU, F32>), grid, dim3(64 * NW), 0, stream, p);
+    return hipGetLastError();
+}
+
+// The tile kernels: rows, weight rows, waves, stages; workgroups a CU holds; microseconds a step of one block takes
+// with one workgroup on a CU and with as many as it holds.
+struct TileCost {
+    int rows, columns, held;
+    float one, all;
+};
+enum { T_256 = 0, T_128, T_64x128, T_64, TILES };
+// Measured over M 32 to 8192, K 4096 and 12288, N 4096 to 24576, plain and GLU: within 15 %.
+constexpr TileCost kTiles[TILES] = {{256, 256, 1, 1.6f, 1.95f}, {128, 128, 2, 0.8f, 1.15f}, {64, 128, 2, 0.58f, 0.78f}, {64, 64, 2, 0.43f, 0.57f}};
+// A launch and its first loads; the weight's bytes at the rate they are read with; what adding up the parts of a split
+// K takes beside their bytes.
+constexpr float kLaunch = 2.5f, kBytesMicrosecond = 4.5e6f, kJoin = 3.0f;
+
 template <bool GLU, bool F32>
-hipError_t launch(const F8Args &p, int cus, hipStream_t stream) {
-    if (p.M <= 16) return launch_short<1, GLU, F32>(p, stream);
-    if (p.M <= 32) return launch_short<2, GLU, F32>(p, stream);
-    return launch_short<4, GLU, F32>(p, stream);
+hipError_t launch(const F8Args &p, const F8Plan &plan, hipStream_t stream) {
+    switch (plan.kernel) {
+        case 0: return launch_tile<256, 256, 2, 4, 2, GLU, false>(p, plan.splits, stream);
+        case 1: return launch_tile<128, 128, 2, 2, 2, GLU, F32>(p, plan.splits, stream);
+        case 2: return launch_tile<64, 128, 1, 4, 3, GLU, F32>(p, plan.splits, stream);
+        case 3: return launch_tile<64, 64, 2, 2, 4, GLU, F32>(p, plan.splits, stream);
+        case 4: return launch_short<1, 1, 8, 4, GLU, F32>(p, stream);
+        case 5: return launch_short<1, 2, 8, 4, GLU, F32>(p, stream);
+        default: return launch_short<4, 1, 8, 2, GLU, F32>(p, stream);
+    }
 }
 
 }  // namespace
 
-hipError_t launch_f8_product(const F8Args &p, bool glu, bool out_f32, int cus, hipStream_t stream) {
+// Up to 16 rows the short kernel: each of its workgroups reads its weight rows and all of A, and a CU takes in a bounded
+// number of bytes a cycle, so 16 or 32 columns a workgroup by the bytes that the fullest CU takes. At M = 16, K = 4096:
+// N = 6144 11.3 µs by 16 and 8.8 by 32, N = 4096 7.1 and 8.7, N = 24576 (GLU) 25.8 and 29.0.
+// Above, the tile and the split of K with the least estimated time: rounds of workgroups times steps, not under the
+// time the bytes take. At M = 64, K = 12288, N = 4096: 64 × 64 tiles 45.4 µs whole and 20.9 in four parts; at M = 2048 of the same
+// 256 × 256 165 and 128 × 128 122; at M = 8192, K = 4096, N = 24576 752 and 885.
+// Rows too far apart for the tile kernels' 32-bit offsets go to the short kernel.
+F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
+    F8Plan plan = {6, 1, 0};
+    if (p.M <= 0 || p.H <= 0) return plan;
+    const int halves = glu ? 2 : 1;
+    if (p.M <= 16) {
+        auto fullest = [&](int columns) {
+            const int64_t groups = (p.H + columns - 1) / columns;
+            return ((groups + cus - 1) / cus) * (columns * halves + p.M);
+        };
+        plan.kernel = fullest(32) < fullest(16) ? 5 : 4;
+        return plan;
+    }
+    const bool near = 256 * std::max(std::max(p.lda, p.ldw), 4 * p.ldsx) + p.K <= INT32_MAX &&
+                      (!glu || ((int64_t)p.H + 256) * p.ldw + p.K <= INT32_MAX);
+    if (!near) return plan;
+    const int wide = part_columns(p.H);
+    float best = 0.0f;
+    for (int t = out_f32 ? T_128 : T_256; t < TILES; ++t) {
+        const TileCost &c = kTiles[t];
+        const int64_t tiles = (int64_t)((p.M + c.rows - 1) / c.rows) * ((p.H * halves + c.columns - 1) / c.columns);
+        for (int splits = 1; splits <= 8; ++splits) {
+            // Two stages read four blocks' scales at once: not split (a part may begin inside four).
+            if (splits > 1 && (t <= T_128 || p.KB < 8 * splits)) break;
+            const int64_t groups = tiles * splits, slots = (int64_t)cus * c.held, rest = groups % slots;
+            const int steps = (p.KB + splits - 1) / splits;
+            float us = steps * ((float)(groups / slots) * c.all + (rest == 0 ? 0.0f : rest > cus ? c.all : c.one));
+            us = std::max(us, ((float)p.N * p.K + (float)p.M * p.K) / kBytesMicrosecond);
+            const float part = (float)p.M * wide * halves * 4.0f * splits;
+            if (splits > 1) us += kJoin + 2.0f * part / kBytesMicrosecond;
+            us += kLaunch;
+            if (best == 0.0f || us < best) {
+                best = us;
+                plan = F8Plan{t, splits, splits > 1 ? (int64_t)part : 0};
+            }
+        }
+    }
+    if (plan.splits > 1) plan.part_bytes = (int64_t)plan.splits * p.M * wide * halves * 4;
+    return plan;
+}
+
+hipError_t launch_f8_product(const F8Args &p, const F8Plan &plan, bool glu, bool out_f32, hipStream_t stream) {
     if (p.M == 0 || p.H == 0) return hipSuccess;
-    if (glu) return out_f32 ? launch<true, true>(p, cus, stream) : launch<true, false>(p, cus, stream);
-    return out_f32 ? launch<false, true>(p, cus, stream) : launch<false, false>(p, cus, stream);
+    if (glu) return out_f32 ? launch<true, true>(p, plan, stream) : launch<true, false>(p, plan, stream);
+    return out_f32 ? launch<false, true>(p, plan, stream) : launch<false, false>(p, plan, stream);
 }
 
 }  // namespace sq8

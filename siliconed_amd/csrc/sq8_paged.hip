@@ -19,7 +19,7 @@ __device__ __forceinline__ float bf16_f32(uint32_t bits) { return __uint_as_floa
 //
 // q' = rot(q), k' = rot(k): with (cos, sin) of the token's position, pair i of the first `rot` values of a head,
 // (a, b) → (a·cos − b·sin, b·cos + a·sin); pairs (i, i + rot/2), or (2i, 2i + 1) when interleaved. Products and sums
-// in fp32, one rounding. e4m3: code = e4m3(v · (1/scale)), saturated at ±448 (a NaN stays one).
+// in fp32, one rounding. e4m3: code = e4m3(v / scale), saturated at ±448 (a NaN stays one).
 //
 // Bound by memory: every value is read once and written once. A thread takes one unit of a token: two runs of W
 // values, the two halves of W pairs (or W values of one run and the next where there is nothing to turn), so a wave
@@ -59,11 +59,12 @@ __device__ __forceinline__ void store_bf16(uint16_t *dst, const float (&v)[W]) {
 }
 
 template <int W>
-__device__ __forceinline__ void store_e4m3(uint8_t *dst, const float (&v)[W], float recip) {
+__device__ __forceinline__ void store_e4m3(uint8_t *dst, const float (&v)[W], const Quotient &by) {
     float q[W];
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-        const float t = v[e] * recip;
+        const float near = v[e] * by.r;
+        const float t = fabsf(near) < INFINITY ? by.of(v[e]) : near;
         q[e] = t != t ? t : fminf(fmaxf(t, -448.0f), 448.0f);
     }
     if constexpr (W == 8) {
@@ -142,10 +143,10 @@ __global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs p) {
     void *pool = kind == 1 ? p.kc : p.vc;
     if constexpr (E4M3) {
         const float *scales = kind == 1 ? p.k_scale : p.v_scale;
-        const float recip = scales ? __fdiv_rn(1.0f, scales[head]) : 1.0f;
+        const Quotient by(scales ? scales[head] : 1.0f);
         uint8_t *dst = static_cast<uint8_t *>(pool) + to;
-        store_e4m3<W>(dst + at0, a, recip);
-        store_e4m3<W>(dst + at1, b, recip);
+        store_e4m3<W>(dst + at0, a, by);
+        store_e4m3<W>(dst + at1, b, by);
     } else {
         uint16_t *dst = static_cast<uint16_t *>(pool) + to;
         store_bf16<W>(dst + at0, a);

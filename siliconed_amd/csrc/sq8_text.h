@@ -10,6 +10,20 @@ namespace sq8 {
 
 constexpr int F8_GROUP = 128;  // values of K that share a scale
 
+// Correctly rounded quotients by one divisor s: from r = fl(1/s), q0 = fl(y·r) is within two ulps, one step
+// q1 = q0 + r·(y − q0·s) within one, and the next is then the rounded quotient (Markstein 1990: r correctly rounded,
+// q1 faithful, both steps fused). Four multiply-adds where a division is ten instructions. An infinite s: 0, or NaN
+// for an infinite y (the remainder takes s as 0 there, as 0 · ∞ is NaN).
+struct Quotient {
+    float s, r;
+    __device__ __forceinline__ explicit Quotient(float by) : s(fabsf(by) == INFINITY ? 0.0f : by), r(__fdiv_rn(1.0f, by)) {}
+    __device__ __forceinline__ float of(float y) const {
+        const float q0 = y * r;
+        const float q1 = __builtin_fmaf(__builtin_fmaf(-q0, s, y), r, q0);
+        return __builtin_fmaf(__builtin_fmaf(-q1, s, y), r, q1);
+    }
+};
+
 // sq8_text_norm.hip. Element types by flag: bf16 or fp32.
 struct AddNormArgs {
     const void *x;          // [rows, cols]
@@ -39,15 +53,22 @@ struct F8Args {
     const float *sw;        // [⌈N/128⌉ (GLU: 2⌈H/128⌉), KB], rows ldsw apart
     const float *bias;      // [N] or null
     void *c;                // [M, n_out]
+    float *part;            // the sums of a split K's parts
     int64_t lda, ldsx, ldw, ldsw, ldc;
     int M, N, K;            // K a multiple of 16
     int KB;                 // ⌈K/128⌉
     int H;                  // the output's width: N, or N/2 for GLU
-    int up_block;           // GLU: the up half's first scale row, ⌈H/128⌉
-    int c_vec;              // four outputs a store allowed (aligned base and rows)
-    int sx_vec;             // four scales a load allowed
+    int up_block;           // ⌈H/128⌉: the scale rows of a half, and the up half's first
+    int c_vec;              // outputs a store may take: 8 or 4 (aligned base and rows), 0 for one at a time
+    int sx_vec;             // four scales a load allowed (rows of whole fours)
 };
-hipError_t launch_f8_product(const F8Args &p, bool glu, bool out_f32, int cus, hipStream_t stream);
+// Which kernel a product runs on, and the parts its K is split in; part_bytes: what F8Args::part needs.
+struct F8Plan {
+    int kernel, splits;
+    int64_t part_bytes;
+};
+F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus);
+hipError_t launch_f8_product(const F8Args &p, const F8Plan &plan, bool glu, bool out_f32, hipStream_t stream);
 
 // sq8_paged.hip. Strides in elements.
 struct AppendArgs {

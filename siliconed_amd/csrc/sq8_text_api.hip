@@ -60,7 +60,7 @@ int run_f8(sq8_ctx *ctx, const F8Product &q, double *gpu_seconds) {
     p.M = q.m; p.N = q.n; p.K = q.k; p.KB = kb; p.H = h;
     p.up_block = (h + F8_GROUP - 1) / F8_GROUP;
     const size_t esz = q.c_dtype == SQ8_F32 ? 4 : 2;
-    p.c_vec = aligned(q.c, 4 * esz) && q.ldc % 4 == 0;
+    p.c_vec = aligned(q.c, 8 * esz) && q.ldc % 8 == 0 ? 8 : aligned(q.c, 4 * esz) && q.ldc % 4 == 0 ? 4 : 0;
 
     // What the kernel does not read in place is copied first, rows padded with zero codes to whole 16-byte runs.
     const bool ragged = q.k % 16 != 0;
@@ -77,6 +77,16 @@ int run_f8(sq8_ctx *ctx, const F8Product &q, double *gpu_seconds) {
         const int st = reserve(ctx, ctx->wpack, (size_t)(q.n * kp));
         if (st != SQ8_OK) return st;
     }
+    if (quantize) p.lda = kp, p.ldsx = scales_row;
+    if (pad_a) p.lda = kp;
+    if (pad_w) p.ldw = kp;
+    p.K = (int)kp;
+    const sq8::F8Plan plan = sq8::f8_plan(p, glu, q.c_dtype == SQ8_F32, ctx->cus);
+    if (plan.part_bytes > 0) {
+        const int st = reserve(ctx, ctx->part, (size_t)plan.part_bytes);
+        if (st != SQ8_OK) return st;
+        p.part = static_cast<float *>(ctx->part.at);
+    }
     hipError_t e = hipSuccess;
     if (gpu_seconds) e = hipEventRecord(ctx->begin, ctx->stream);
     if (e != hipSuccess) return hip_status(e);
@@ -91,23 +101,20 @@ int run_f8(sq8_ctx *ctx, const F8Product &q, double *gpu_seconds) {
         }
         e = sq8::launch_quantize_groups(q.a, q.a_dtype == SQ8_BF16, q.lda, q.m, q.k, codes, kp, scales, scales_row, ctx->stream);
         if (e != hipSuccess) return e == hipErrorInvalidValue ? SQ8_EUNSUPPORTED : hip_status(e);
-        p.a = codes; p.lda = kp;
-        p.sx = scales; p.ldsx = scales_row;
+        p.a = codes;
+        p.sx = scales;
     } else if (pad_a) {
         e = sq8::launch_pad_bytes(q.a, q.lda, ctx->scratch.at, kp, q.m, q.k, ctx->stream);
         if (e != hipSuccess) return hip_status(e);
         p.a = static_cast<const uint8_t *>(ctx->scratch.at);
-        p.lda = kp;
     }
     if (pad_w) {
         e = sq8::launch_pad_bytes(q.w, q.ldw, ctx->wpack.at, kp, q.n, q.k, ctx->stream);
         if (e != hipSuccess) return hip_status(e);
         p.w = static_cast<const uint8_t *>(ctx->wpack.at);
-        p.ldw = kp;
     }
-    p.K = (int)kp;
-    p.sx_vec = aligned(p.sx, 16) && p.ldsx % 4 == 0;
-    e = sq8::launch_f8_product(p, glu, q.c_dtype == SQ8_F32, ctx->cus, ctx->stream);
+    p.sx_vec = aligned(p.sx, 16) && p.ldsx % 4 == 0 && (quantize || kb % 4 == 0);
+    e = sq8::launch_f8_product(p, plan, glu, q.c_dtype == SQ8_F32, ctx->stream);
     if (e != hipSuccess) return e == hipErrorInvalidValue ? SQ8_EUNSUPPORTED : hip_status(e);
     if (gpu_seconds) {
         e = hipEventRecord(ctx->end, ctx->stream);

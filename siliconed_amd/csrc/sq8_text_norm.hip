@@ -2,14 +2,14 @@
 // residual stream's new sum, and the quantization alone.
 //
 //   s' = r + x,  y = (s' · 1/sqrt(mean(s'²) + eps)) · w
-//   e4m3: per 128 columns s = max(max|y| / 448, 1e-30), code = e4m3(y · (1/s)), nearest even
+//   e4m3: per 128 columns s = max(max|y| / 448, 1e-30), code = e4m3(y / s), nearest even
 //   int8: per row s = max(max|y| / 127, 1e-30), code = clamp(rint(y / s), −128, 127)
 //
 // The sums, the norm and the scales are fp32; s' is rounded to the stream's type only where it is stored, so the
-// norm sees the sum before that rounding. y/s of an e4m3 code is the product with the rounded reciprocal: the two
-// differ by an ulp of fp32, which moves a code only on a tie of its 4 significant bits; int8 codes are those of
-// the division, as sq8_quantize_rows writes them. 448·fl(1/s)·s stays below 464, so no code overflows to NaN.
-// An infinity in a group (e4m3) or row (int8) makes its scale infinite.
+// norm sees the sum before that rounding. Both quotients are correctly rounded: an ulp of y/s decides a code where
+// y/s lies halfway between two, and among bf16 values that is common (448 = 7 · 64: y = 3·2^j · max|y| is such a
+// tie). y/s is under 449, which rounds to the largest code: none overflows to NaN. An infinity in a group (e4m3) or
+// row (int8) makes its scale infinite, and its finite values' codes 0.
 #include <hip/hip_runtime.h>
 
 #include "sq8_device.h"
@@ -104,10 +104,10 @@ __device__ __forceinline__ float group_scale(float m) {
 }
 
 __device__ __forceinline__ void e4m3_codes(const float (&y)[8], float scale, uint32_t &lo, uint32_t &hi) {
-    const float recip = __fdiv_rn(1.0f, scale);
+    const Quotient by(scale);
     float q[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = y[e] * recip;
+    for (int e = 0; e < 8; ++e) q[e] = by.of(y[e]);
     lo = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
     lo = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], (int)lo, true);
     hi = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);

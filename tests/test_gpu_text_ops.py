@@ -230,6 +230,22 @@ def test_product_f8(gemm, m, k, n, out):
     run_product(gemm, m, k, 2 * n, True, m % 2 == 0, out)
 
 
+@pytest.mark.parametrize("m,k,n", [(48, 8192, 40), (64, 9216 + 48, 130), (300, 12288, 96), (20, 16384 + 16, 64), (700, 2560, 1100),
+                                   (1537, 640, 2570), (2049, 1296, 1300), (3000, 256, 4100)])
+@pytest.mark.parametrize("out", [BF, torch.float32], ids=["bf16", "f32"])
+def test_product_f8_large(gemm, m, k, n, out):
+    """Long sums split over workgroups, more than 64 blocks of K, and each of the tiles: rows, columns and K that end
+    inside them. Checked at rows and columns taken from all over, and the edges."""
+    for glu in (False, True):
+        g = gen(m + k + n)
+        a, sx, w, sw = operands(g, m, k, 2 * n if glu else n, glu)
+        rows = torch.unique(torch.cat([torch.randint(0, m, (40,), generator=g), torch.arange(max(0, m - 18), m), torch.arange(min(18, m))]))
+        print(f"f8 product {m} x {k} x {n} glu {glu} {out}", flush=True)
+        want, tol = product_oracle(a[rows], sx[rows], w, sw, None, glu, out)
+        got = gemm.product_f8(a.to(DEV), sx.to(DEV), w.to(DEV), sw.to(DEV), epilogue="silu_glu" if glu else None, out_dtype=out)
+        within(got[rows.to(DEV)], want, tol, "product")
+
+
 @pytest.mark.parametrize("k", [1, 8, 17, 100, 130, 1001])
 @pytest.mark.parametrize("m", [2, 70])
 def test_product_f8_ragged_k(gemm, m, k):
