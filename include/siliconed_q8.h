@@ -394,7 +394,7 @@ int sq8_gated_residual(sq8_ctx *ctx, float *x, int64_t ldx, const void *y, int y
  * s = r + x (x SQ8_BF16 or SQ8_F32, the stream `residual` SQ8_BF16 or SQ8_F32, or NULL: s = x), y = (s · 1/sqrt(mean(s²)
  * + eps)) · w in fp32; s rounded to the stream's type goes to `residual_out` unless NULL (it may be `residual` itself;
  * no other overlap) — the norm takes s before that rounding.
- *   `codes_dtype` SQ8_FP8_E4M3: per 128 columns a scale t = max(max|y| / 448, 1e-30) and codes e4m3(y / t), nearest
+ *   `codes_dtype` SQ8_FP8_E4M3: per 128 columns a scale t = max(max|y| · fl(1/448), 1e-30) and codes e4m3(y / t), nearest
  *   even; scales [rows, ⌈cols/128⌉] with leading dimension lds — sq8_linear_f8's operand;
  *   SQ8_INT8: per row t = max(max|y| / 127, 1e-30) and codes clamp(rint(y / t), −128, 127); scales [rows], lds unused —
  *   sq8_linear_w8a8's operand.

@@ -798,6 +798,7 @@ int sq8_destroy(sq8_ctx *ctx) {
     sq8::release(ctx->scratch);
     sq8::release(ctx->wpack);
     sq8::release(ctx->part);
+    sq8::release(ctx->marks);
     sq8::release(ctx->aside);
     if (ctx->blas) (void)rocblas_destroy_handle(ctx->blas);
     (void)hipEventDestroy(ctx->begin);

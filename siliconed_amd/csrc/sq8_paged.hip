@@ -7,6 +7,8 @@
 // counts as masked, a length past the page table's end is cut to it.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "sq8_device.h"
 #include "sq8_text.h"
 
@@ -158,8 +160,10 @@ __global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs p) {
 //
 //   o[b, h] = Σ_t softmax_t(s_t) · v_t,  s_t = cap(scale · q·k_t),  t in [max(0, len − window), len)
 //
-// One pass over the cache with the running maximum and sum of the softmax, both fp32; the probabilities are rounded
-// to bf16 for their product with v (the sum is of the unrounded ones): at most 2^-8 of each, random over the tokens.
+// One pass over the cache with the running maximum and sum of the softmax, both fp32. The maximum is moved only when a
+// score passes it by 8 powers of two, so a probability may be up to 2^8 of what it will be divided by: the same bits
+// of it, and the sums rescaled hardly ever. The probabilities are rounded to bf16 for their product with v (the sum is of
+// the unrounded ones): at most 2^-8 of each, random over the tokens.
 //
 // Bound by the cache's bytes. The query heads of one kv head (up to 16; more take several passes) are the columns of
 // both products, on v_mfma_f32_16x16x32_bf16:
@@ -172,12 +176,19 @@ __global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs p) {
 // lane, value DV·c + i going to instruction i. So both pools go from memory to registers in whole rows, without LDS.
 //
 // Work is split over tiles of 128 tokens (a wave takes 32) of every (sequence, kv head, 16 query heads), numbered in
-// that order; workgroup g of G takes tiles [T·g/G, T·(g+1)/G), whatever sequences they belong to, so ragged lengths
-// load the card evenly and the host needs no lengths. A sequence's head whose tiles lie in several workgroups leaves
-// its maximum, sum and unnormalised output in each one's slot; a second launch joins them in tile order.
+// that order and shared out evenly (Share), whatever sequences they belong to, so ragged lengths load the card evenly and
+// the host needs no lengths. A sequence's head whose tiles lie in several workgroups leaves its maximum, sum and
+// unnormalised output in each one's slot, and the workgroup that finishes last, as a counter tells it, joins them in
+// tile order: the result does not depend on which one that is. It also sets the counter back to zero, as every call
+// finds it.
 
 constexpr int TILE = 128;   // tokens a workgroup takes at a time
 constexpr int WAVES = 4;
+
+// Token / tokens a page, by a multiplication (page_divisor).
+__device__ __forceinline__ int page_of(const PagedArgs &p, int token) {
+    return (int)(((uint64_t)(uint32_t)token * p.page_mul) >> p.page_shift);
+}
 
 struct Span {
     int first, last;  // tokens [first, last), from the window's first
@@ -195,6 +206,23 @@ __device__ __forceinline__ Span span_of(const PagedArgs &p, int length) {
     return s;
 }
 
+// How a batch's tiles are shared out: the first `more` of `groups` workgroups take each + 1, the others `each`, in
+// order. (Fewer workgroups of four tiles or more where there are not enough for all: slower, 20 µs against 12 at one
+// sequence of 777.)
+struct Share {
+    int groups, each, more;
+    __device__ __forceinline__ Share() {}
+    __device__ __forceinline__ Share(int total, int most) {
+        groups = min(most, total);
+        each = groups > 0 ? total / groups : 0;
+        more = groups > 0 ? total - each * groups : 0;
+    }
+    __device__ __forceinline__ int first(int g) const { return g * each + min(g, more); }
+    __device__ __forceinline__ int of(int tile) const {
+        return tile < more * (each + 1) ? tile / (each + 1) : more + (tile - more * (each + 1)) / each;
+    }
+};
+
 // The sum of v over this lane and those before it.
 __device__ __forceinline__ int wave_scan(int v, int lane) {
 #pragma unroll
@@ -206,8 +234,8 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
 }
 
 // The batch's tiles of one head, by 64 sequences at a time in every wave.
-__device__ __forceinline__ int64_t batch_tiles(const PagedArgs &p, int lane) {
-    int64_t total = 0;
+__device__ __forceinline__ int batch_tiles(const PagedArgs &p, int lane) {
+    int total = 0;
     for (int b = 0; b < p.batch; b += 64) {
         int v = b + lane < p.batch ? span_of(p, p.lengths[b + lane]).tiles : 0;
 #pragma unroll
@@ -218,8 +246,8 @@ __device__ __forceinline__ int64_t batch_tiles(const PagedArgs &p, int lane) {
 }
 
 // The sequence that holds per-head tile number `at`, and the tiles of the sequences before it.
-__device__ __forceinline__ int sequence_of(const PagedArgs &p, int64_t at, int lane, int64_t &before) {
-    int64_t base = 0;
+__device__ __forceinline__ int sequence_of(const PagedArgs &p, int at, int lane, int &before) {
+    int base = 0;
     for (int b = 0; b < p.batch; b += 64) {
         const int v = b + lane < p.batch ? span_of(p, p.lengths[b + lane]).tiles : 0;
         const int upto = wave_scan(v, lane);
@@ -232,12 +260,22 @@ __device__ __forceinline__ int sequence_of(const PagedArgs &p, int64_t at, int l
         base += __shfl(upto, 63, 64);
     }
     before = base;
-    return -1;
+    return 0;  // not reached: `at` is under the batch's tiles
 }
 
-__host__ __device__ constexpr int part_floats(int dp) { return 32 + 16 * dp; }  // maxima, sums, outputs [16][dp]
+// The larger (the sum) of a value over the four lanes of a head (16 apart): the swaps leave each row's neighbour's, and
+// each half's other's, in the second of the pair.
+template <bool SUM>
+__device__ __forceinline__ float over_rows(float v) {
+    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+    auto both = [](u32x2_t r) {
+        const float a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+        return SUM ? a + b : fmaxf(a, b);
+    };
+    v = both(__builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return both(__builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+}
 
-// A head's values past `dim` (a head narrower than DP) read as zeros.
 template <int N>
 struct Raw {
     uint32_t d[N];
@@ -265,55 +303,139 @@ __device__ __forceinline__ Raw<N> load_raw(const uint8_t *src) {
 // Two e4m3 codes (bytes 2W, 2W + 1) as a bf16 pair, exactly.
 template <int W>
 __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t d) {
-    float lo, hi;
-    fp8_pair<W>(d, lo, hi);
-    return pack_exact_bf16(lo, hi);
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d, 1.0f, W != 0));
 }
 
+// A slot: maxima [16], sums [16], outputs [16][dp].
+__host__ __device__ constexpr int part_floats(int dp) { return 32 + 16 * dp; }
+
+// The slots lie where every XCD sees them: written and read past its own L2 (agent-scope accesses), so the join needs no
+// fence, which would write back and drop that cache under everything still streaming through it (with fences the
+// kernel took twice as long at 48 sequences of up to 8192).
+__device__ __forceinline__ void put(float *to, float v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float get(const float *from) { return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// 1 / l, or 0 where nothing was added (a NaN stays one).
+__device__ __forceinline__ float inverse(float l) { return l > 0.0f ? __fdiv_rn(1.0f, l) : l == 0.0f ? 0.0f : l; }
+
+// The results of workgroups g0 .. g1 over one sequence's head, in that order: the first's in slot `slot0`, the others' in
+// 2g (where a workgroup's tiles begin with that sequence's). A thread takes two values of a query head; its loads of
+// eight slots are under way at once.
+template <int DP>
+__device__ __forceinline__ void join_slots(const PagedArgs &p, int slot0, int g0, int g1, int live, float v_scale, uint16_t *out) {
+    const int pairs = p.dim / 2;
+    auto slot_of = [&](int g) { return p.part + (int64_t)(g == g0 ? slot0 : 2 * g) * part_floats(DP); };
+    for (int i = threadIdx.x; i < live * pairs; i += 64 * WAVES) {
+        const int c = i / pairs, d = 2 * (i - c * pairs);
+        float top = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
+        for (int g = g0; g <= g1; g += 8) {
+            float m[8], n[8], u[8], v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float *slot = slot_of(min(g + e, g1));
+                m[e] = get(slot + c);
+                n[e] = get(slot + 16 + c);
+                u[e] = get(slot + 32 + c * DP + d);
+                v[e] = get(slot + 32 + c * DP + d + 1);
+            }
+            float most = top;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, m[e]);
+            const float from = most == -INFINITY ? 0.0f : most;
+            const float keep = __builtin_amdgcn_exp2f(top - from);
+            top = most;
+            l *= keep;
+            x *= keep;
+            y *= keep;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (g + e > g1) break;
+                const float weight = __builtin_amdgcn_exp2f(m[e] - from);
+                l = __builtin_fmaf(n[e], weight, l);
+                x = __builtin_fmaf(u[e], weight, x);
+                y = __builtin_fmaf(v[e], weight, y);
+            }
+        }
+        const float scale = inverse(l) * v_scale;
+        *reinterpret_cast<uint32_t *>(out + c * p.o_head + d) = pack_bf16_rne(x * scale, y * scale);
+    }
+}
+
+// Workgroups a CU holds (by their registers).
+constexpr int held(int dp) { return dp <= 128 ? 2 : 1; }
+
 template <int DP, bool E4M3, bool PAGE16>
-__global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) paged_attention_kernel(const PagedArgs p) {
+__global__ void __launch_bounds__(64 * WAVES, held(DP)) paged_attention_kernel(const PagedArgs p) {
     constexpr int ES = E4M3 ? 1 : 2;
     constexpr int STEPS = DP / 32;                // MFMAs of a 16-token tile's scores
     constexpr int KRUNS = DP * ES / 64;           // 16-byte runs of a key a lane reads
     constexpr int DV = DP / 16;                   // values of a token a lane reads: MFMAs of the second product
     constexpr int VN = DV * ES / 4;               // and their dwords
+    constexpr float LOG2E = 1.4426950408889634f;
     __shared__ __attribute__((aligned(16))) f32x4 joined[WAVES - 1][DV][64];
     __shared__ float tops[WAVES][16], totals[WAVES][16];
+    __shared__ int joins[2];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, h = lane >> 4;
     const int group = p.q_heads / p.kv_heads;
     const int passes = (group + 15) / 16;
     const int heads = p.kv_heads * passes;
-
-    // Sequences without a token: zeros.
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-        if (span_of(p, p.lengths[b]).tiles != 0) continue;
-        for (int i = threadIdx.x; i < p.q_heads * p.dim; i += 64 * WAVES)
-            p.out[b * p.o_tok + (i / p.dim) * p.o_head + i % p.dim] = 0;
+    const bool full = p.dim == DP;
+    const bool capped = p.softcap > 0.0f;
+    // The bytes of a row a lane reads (past `dim`, the row's first), and PAGE16: with its row's place from the 16-token
+    // tile's first.
+    uint32_t k_run[KRUNS], k_lane[KRUNS], v_lane[4];
+#pragma unroll
+    for (int s = 0; s < KRUNS; ++s) {
+        const int d = E4M3 ? 64 * s + 16 * h : 32 * s + 8 * h;
+        k_run[s] = d < p.dim ? d * ES : 0;
+        k_lane[s] = (uint32_t)(c * p.kc_tok * ES) + k_run[s];
     }
+    const uint32_t v_run = DV * c < p.dim ? DV * c * ES : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v_lane[i] = (uint32_t)((4 * h + i) * p.vc_tok * ES) + v_run;
 
-    const int64_t per_head = batch_tiles(p, lane);
-    const int64_t total = per_head * heads;
-    const int64_t start = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
-    if (start >= end) return;
+    // This workgroup's tiles, and the sequence they begin in; all uniform. Up to 64 sequences lie in a wave's lanes at once.
+    int total, before = 0, b = 0, length;
+    Share share;
+    int start, end;
+    auto mine = [&](int per_head) {
+        total = __builtin_amdgcn_readfirstlane(per_head) * heads;
+        share = Share(total, gridDim.x);
+        start = share.first(min((int)blockIdx.x, share.groups));
+        end = share.first(min((int)blockIdx.x + 1, share.groups));
+    };
+    if (p.batch <= 64) {
+        const int n = lane < p.batch ? p.lengths[lane] : 0;
+        const int v = span_of(p, n).tiles;
+        const int upto = wave_scan(v, lane);
+        mine(__builtin_amdgcn_readlane(upto, 63));
+        const uint64_t past = __ballot(upto > start / heads);
+        b = past ? __ffsll((unsigned long long)past) - 1 : 0;
+        before = __builtin_amdgcn_readlane(upto - v, b);
+        length = __builtin_amdgcn_readlane(n, b);
+    } else {
+        mine(batch_tiles(p, lane));
+        if (start < end) b = __builtin_amdgcn_readfirstlane(sequence_of(p, start / heads, lane, before));
+        length = p.lengths[b];
+    }
     // Tiles are numbered sequence by sequence, `heads` runs of a sequence's tiles each.
-    int64_t before = 0;
-    int b = sequence_of(p, start / heads, lane, before);
-    if (b < 0) return;
-    b = __builtin_amdgcn_readfirstlane(b);
-    Span span = span_of(p, p.lengths[b]);
-    int64_t seq0 = before * heads;  // the sequence's first tile
+    Span span = span_of(p, __builtin_amdgcn_readfirstlane(length));
+    int seq0 = __builtin_amdgcn_readfirstlane(before) * heads;  // the sequence's first tile
 
-    for (int64_t pos = start; pos < end;) {
-        while (pos >= seq0 + (int64_t)span.tiles * heads) {
-            seq0 += (int64_t)span.tiles * heads;
+    struct Part {
+        int b, head, first, tiles;  // tiles 0: none
+    } parts[2] = {};
+    for (int pos = start; pos < end;) {
+        while (pos >= seq0 + span.tiles * heads) {
+            seq0 += span.tiles * heads;
             ++b;
-            span = span_of(p, p.lengths[b]);
+            span = span_of(p, __builtin_amdgcn_readfirstlane(p.lengths[b]));
         }
-        const int in_seq = (int)(pos - seq0);
+        const int in_seq = pos - seq0;
         const int head = in_seq / span.tiles;
         const int tile0 = in_seq - head * span.tiles;
-        const int run = (int)min((int64_t)(span.tiles - tile0), end - pos);
+        const int run = min(span.tiles - tile0, end - pos);
         const int kvh = head / passes, pass = head - kvh * passes;
         const int q0 = kvh * group + pass * 16;
         const int live = min(16, group - pass * 16);  // query heads of this pass
@@ -327,15 +449,19 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) paged_attention
             if (c < live && d < p.dim) v = *reinterpret_cast<const u32x4 *>(p.q + b * p.q_tok + (q0 + c) * p.q_head + d);
             q[s] = __builtin_bit_cast(bf16x8, v);
         }
-        const float score_scale = p.scale * (E4M3 && p.k_scale ? p.k_scale[kvh] : 1.0f);
+        // Scores in units of log2, or where they are capped, in those of the cap.
+        const float score_scale = p.scale * (E4M3 && p.k_scale ? p.k_scale[kvh] : 1.0f) * (capped ? 1.0f / p.softcap : LOG2E);
         const uint8_t *kbase = p.kc + (int64_t)kvh * p.kc_head * ES;
         const uint8_t *vbase = p.vc + (int64_t)kvh * p.vc_head * ES;
-        const int32_t *pages = p.pages + (int64_t)b * p.pages_row;
+        // Read as constant memory: scalar loads, for which the vector loads under way need not be waited for.
+        const auto pages = (const __attribute__((address_space(4))) int32_t *)(p.pages + (int64_t)b * p.pages_row);
 
-        // Where the rows of a subtile's tokens lie. PAGE16: each 16-token tile in one page, its page uniform.
+        // The rows of a subtile's 32 tokens. PAGE16: each 16-token tile lies in one page, whose index is uniform and read
+        // one subtile before its use. Else each lane looks up its own rows.
         struct Where {
-            int64_t k[2], v[PAGE16 ? 2 : 8];  // row offsets in elements
-            uint32_t bad;                     // tokens (bit: order of the lane's eight) on a page outside the pools
+            int id[2], in[2];                              // PAGE16: the page's index as read, and the first row in it
+            int64_t k[PAGE16 ? 1 : 2], v[PAGE16 ? 1 : 8];  // else the rows' offsets in elements
+            uint32_t bad;                                  // and tokens on a page outside the pools (in the order of the lane's eight)
         };
         auto locate = [&](int token) {
             Where w;
@@ -344,56 +470,51 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) paged_attention
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     const int at = min(token + 16 * t, (span.last - 1) & ~15);
-                    const int page = at / p.page, in = at - page * p.page;
-                    int id = pages[page];
-                    if ((unsigned)id >= (unsigned)p.page_count) { id = 0; w.bad |= 0xFu << (4 * t); }
-                    w.k[t] = id * p.kc_page + in * p.kc_tok;
-                    w.v[t] = id * p.vc_page + in * p.vc_tok;
+                    const int page = page_of(p, at);
+                    w.in[t] = at - page * p.page;
+                    w.id[t] = pages[page];
                 }
             } else {
                 auto row = [&](int t, int64_t page_stride, int64_t tok_stride, bool &bad) {
                     const int at = min(t, span.last - 1);
-                    const int page = at / p.page, in = at - page * p.page;
+                    const int page = page_of(p, at), in = at - page * p.page;
                     int id = pages[page];
                     bad = (unsigned)id >= (unsigned)p.page_count;
                     if (bad) id = 0;
                     return id * page_stride + in * tok_stride;
                 };
+                bool bad;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    bool bad;
-                    w.k[t] = row(token + 16 * t + c, p.kc_page, p.kc_tok, bad);
-                }
+                for (int t = 0; t < 2; ++t) w.k[t] = row(token + 16 * t + c, p.kc_page, p.kc_tok, bad);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    bool bad;
                     w.v[i] = row(token + 16 * (i >> 2) + 4 * h + (i & 3), p.vc_page, p.vc_tok, bad);
                     w.bad |= bad ? 1u << i : 0u;
                 }
             }
             return w;
         };
+        auto inside = [&](int id) { return (unsigned)id < (unsigned)p.page_count; };
+        auto bad_of = [&](const Where &w) {
+            return PAGE16 ? (inside(w.id[0]) ? 0u : 0x0Fu) | (inside(w.id[1]) ? 0u : 0xF0u) : w.bad;
+        };
         Raw<4> k[2][KRUNS];
         auto load_k = [&](const Where &w) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const uint8_t *row = kbase + (PAGE16 ? w.k[t] + c * p.kc_tok : w.k[t]) * ES;
+                const uint8_t *row = PAGE16 ? kbase + ((inside(w.id[t]) ? w.id[t] : 0) * p.kc_page + w.in[t] * p.kc_tok) * ES
+                                            : kbase + w.k[PAGE16 ? 0 : t] * ES;
 #pragma unroll
-                for (int s = 0; s < KRUNS; ++s) {
-                    const int d = E4M3 ? 64 * s + 16 * h : 32 * s + 8 * h;
-                    k[t][s] = Raw<4>{{0, 0, 0, 0}};
-                    if (d < p.dim) k[t][s] = load_raw<4>(row + d * ES);
-                }
+                for (int s = 0; s < KRUNS; ++s) k[t][s] = load_raw<4>(row + (PAGE16 ? k_lane[s] : k_run[s]));
             }
         };
         Raw<VN> v[8];
         auto load_v = [&](const Where &w) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const uint8_t *row = vbase + (PAGE16 ? w.v[PAGE16 ? i >> 2 : 0] + (4 * h + (i & 3)) * p.vc_tok : w.v[PAGE16 ? 0 : i]) * ES;
-#pragma unroll
-                for (int e = 0; e < VN; ++e) v[i].d[e] = 0;
-                if (DV * c < p.dim) v[i] = load_raw<VN>(row + DV * c * ES);
+                const int t = i >> 2;
+                v[i] = load_raw<VN>(PAGE16 ? vbase + ((inside(w.id[t]) ? w.id[t] : 0) * p.vc_page + w.in[t] * p.vc_tok) * ES + v_lane[i & 3]
+                                           : vbase + w.v[PAGE16 ? 0 : i] * ES + v_run);
             }
         };
 
@@ -407,13 +528,22 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) paged_attention
         load_k(at);
         load_v(at);
         Where next = locate(token + TILE);
-        for (int i = 0; i < run; ++i, token += TILE) {
-            const bool more = i + 1 < run;
+        // One subtile, and the loads of the next: the keys' once the scores are done with this one's, the values' after the
+        // second product. A run's last one loads nothing (a copy of its own, so that the waits of the others are for
+        // what they use).
+        auto subtile = [&](auto last) {
+            constexpr bool more = !decltype(last)::value;
             f32x4 s[2] = {};
+            if (!full) {
+                // Keys past `dim`, which were read from the row's first values, are zeros (such values give no output).
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+                for (int j = 0; j < KRUNS; ++j)
+                    if ((E4M3 ? 64 * j + 16 * h : 32 * j + 8 * h) >= p.dim) k[0][j] = k[1][j] = Raw<4>{{0, 0, 0, 0}};
+            }
 #pragma unroll
-                for (int j = 0; j < STEPS; ++j) {
+            for (int j = 0; j < STEPS; ++j)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
                     bf16x8 kk;
                     if constexpr (E4M3) {
                         const uint32_t d0 = k[t][j >> 1].d[2 * (j & 1)], d1 = k[t][j >> 1].d[2 * (j & 1) + 1];
@@ -425,37 +555,32 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) paged_attention
                     s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[j], s[t], 0, 0, 0);
                 }
             if (more) load_k(next);
-            const uint32_t bad = at.bad;
-            const Where later = more ? locate(token + 2 * TILE) : next;
+            const uint32_t bad = bad_of(at);
+            const Where later = more ? locate(token + 2 * TILE) : at;
 
-            // Scores in units of log2, tokens 16t + 4h + r.
+            // Tokens 16t + 4h + r.
             float e[8];
-            constexpr float LOG2E = 1.4426950408889634f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = s[j >> 2][j & 3] * score_scale;
-                e[j] = (p.softcap > 0.0f ? p.softcap * tanh_rel(x / p.softcap) : x) * LOG2E;
+            for (int j = 0; j < 8; ++j) e[j] = s[j >> 2][j & 3] * score_scale;
+            if (capped) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) e[j] = p.softcap * LOG2E * tanh_rel(e[j]);
             }
             const bool edge = token < span.first || token + 32 > span.last;
-            if (edge || __any(bad != 0)) {
+            if (edge || (PAGE16 ? bad != 0 : __any(bad != 0))) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int t = token + 16 * (j >> 2) + 4 * h + (j & 3);
-                    if (t < span.first || t >= span.last || (bad >> j & 1)) {
-                        e[j] = -INFINITY;
-                        // A masked row may hold anything, and 0 · NaN is one.
+                    const bool dead = t < span.first || t >= span.last || (bad >> j & 1);
+                    e[j] = dead ? -INFINITY : e[j];
+                    // A masked row may hold anything, and 0 · NaN is one.
 #pragma unroll
-                        for (int d = 0; d < VN; ++d) v[j].d[d] = 0;
-                    }
+                    for (int d = 0; d < VN; ++d) v[j].d[d] = dead ? 0 : v[j].d[d];
                 }
             }
-            float m = e[0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) m = fmaxf(m, e[j]);
-            m = fmaxf(m, __shfl_xor(m, 16, 64));
-            m = fmaxf(m, __shfl_xor(m, 32, 64));
-            if (__any(m > top)) {
-                m = fmaxf(m, top);
+            float m = fmaxf(fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])), fmaxf(fmaxf(e[4], e[5]), fmaxf(e[6], e[7])));
+            if (__any(m > top + 8.0f)) {
+                m = fmaxf(over_rows<false>(m), top);
                 const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - m);
                 top = m;
                 sum *= keep;
@@ -467,38 +592,42 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) paged_attention
             const float from = top == -INFINITY ? 0.0f : top;
             float w[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                w[j] = __builtin_amdgcn_exp2f(e[j] - from);
-                sum += w[j];
-            }
+            for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(e[j] - from);
+            sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
             const bf16x8 prob = __builtin_bit_cast(
                 bf16x8, u32x4{pack_bf16_rne(w[0], w[1]), pack_bf16_rne(w[2], w[3]), pack_bf16_rne(w[4], w[5]), pack_bf16_rne(w[6], w[7])});
-            // Value DV·c + d of the lane's eight tokens, two tokens a dword.
+            // Value DV·c + d of the lane's eight tokens, two tokens a dword, two values at a time.
 #pragma unroll
-            for (int d = 0; d < DV; ++d) {
-                u32x4 t;
+            for (int d = 0; d < DV; d += 2) {
+                u32x4 t[2];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if constexpr (E4M3) {
-                        const uint32_t x = v[2 * j].d[d >> 2], y = v[2 * j + 1].d[d >> 2];
-                        // bytes (x[d], y[d]) → a bf16 pair
-                        const uint32_t two = __builtin_amdgcn_perm(y, x, 0x0c0c0400u + 0x0101u * (d & 3));
-                        t[j] = bf16_of_e4m3<0>(two);
+                        // bytes (x[d], y[d], x[d + 1], y[d + 1]), then as bf16
+                        const uint32_t four = __builtin_amdgcn_perm(v[2 * j + 1].d[d >> 2], v[2 * j].d[d >> 2], d & 2 ? 0x07030602u : 0x05010400u);
+                        t[0][j] = bf16_of_e4m3<0>(four);
+                        t[1][j] = bf16_of_e4m3<1>(four);
                     } else {
-                        t[j] = __builtin_amdgcn_perm(v[2 * j + 1].d[d >> 1], v[2 * j].d[d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+                        const uint32_t x = v[2 * j].d[d >> 1], y = v[2 * j + 1].d[d >> 1];
+                        t[0][j] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+                        t[1][j] = __builtin_amdgcn_perm(y, x, 0x07060302u);
                     }
                 }
-                o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t), prob, o[d], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    o[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t[i]), prob, o[d + i], 0, 0, 0);
             }
             if (more) load_v(next);
             at = next;
             next = later;
-        }
+            token += TILE;
+        };
+        for (int i = 1; i < run; ++i) subtile(std::false_type{});
+        subtile(std::true_type{});
 
         // ---- the waves' results joined, by the first ----
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        __syncthreads();  // the segment before has been read
+        sum = over_rows<true>(sum);
+        __syncthreads();  // the run before has been read
         if (h == 0) { tops[wave][c] = top; totals[wave][c] = sum; }
         if (wave > 0) {
 #pragma unroll
@@ -529,7 +658,7 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) paged_attention
             }
             if (c < live) {
                 if (run == span.tiles) {
-                    const float scale = (l > 0.0f ? __fdiv_rn(1.0f, l) : l == 0.0f ? 0.0f : l) * (E4M3 && p.v_scale ? p.v_scale[kvh] : 1.0f);
+                    const float scale = inverse(l) * (E4M3 && p.v_scale ? p.v_scale[kvh] : 1.0f);
                     uint16_t *dst = p.out + b * p.o_tok + (q0 + c) * p.o_head;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
@@ -541,81 +670,78 @@ __global__ void __launch_bounds__(64 * WAVES, DP <= 128 ? 2 : 1) paged_attention
                     }
                 } else {
                     float *slot = p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * part_floats(DP);
-                    if (h == 0) { slot[c] = all; slot[16 + c] = l; }
+                    if (h == 0) {
+                        put(slot + c, all);
+                        put(slot + 16 + c, l);
+                    }
                     float *dst = slot + 32 + c * DP;
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
-                        for (int d = 0; d < DV; d += 4)
-                            *reinterpret_cast<f32x4 *>(dst + DV * (4 * h + r) + d) = f32x4{o[d][r], o[d + 1][r], o[d + 2][r], o[d + 3][r]};
+                        for (int d = 0; d < DV; ++d) put(dst + DV * (4 * h + r) + d, o[d][r]);
                 }
             }
         }
+        // A part of a sequence's head: at most the first and the last of a workgroup's runs are.
+        if (run != span.tiles) {
+            Part &part = pos == start ? parts[0] : parts[1];
+            part.b = b;
+            part.head = head;
+            part.first = seq0 + head * span.tiles;
+            part.tiles = span.tiles;
+        }
         pos += run;
+    }
+
+    // Sequences without a token: zeros.
+    for (int i = blockIdx.x; i < p.batch; i += gridDim.x) {
+        if (span_of(p, p.lengths[i]).tiles != 0) continue;
+        for (int j = threadIdx.x; j < p.q_heads * p.dim; j += 64 * WAVES)
+            p.out[i * p.o_tok + (j / p.dim) * p.o_head + j % p.dim] = 0;
+    }
+
+    // The parts' slots are written (by the first wave) before their counters say so; the last to count joins.
+    if (parts[0].tiles == 0 && parts[1].tiles == 0) return;
+    if (wave == 0) __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        const Part part = threadIdx.x == 0 ? parts[0] : parts[1];
+        bool last = false;
+        if (part.tiles != 0) {
+            int *const mark = p.marks + part.b * heads + part.head;
+            const int others = share.of(part.first + part.tiles - 1) - share.of(part.first);
+            last = __hip_atomic_fetch_add(mark, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == others;
+            if (last) __hip_atomic_store(mark, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        joins[threadIdx.x] = last;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (!joins[i]) continue;
+        const Part part = parts[i];
+        const int g0 = share.of(part.first), g1 = share.of(part.first + part.tiles - 1);
+        const int kvh = part.head / passes, pass = part.head - kvh * passes;
+        join_slots<DP>(p, 2 * g0 + (share.first(g0) < part.first ? 1 : 0), g0, g1, min(16, group - pass * 16),
+                       E4M3 && p.v_scale ? p.v_scale[kvh] : 1.0f, p.out + part.b * p.o_tok + (kvh * group + pass * 16) * p.o_head);
     }
 }
 
-// One workgroup a (sequence, kv head, 16 query heads): the slots of the workgroups its tiles lay in, in tile order.
-template <int DP, bool E4M3>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs p, int groups) {
-    const int lane = threadIdx.x & 63;
-    const int group = p.q_heads / p.kv_heads;
-    const int passes = (group + 15) / 16;
-    const int heads = p.kv_heads * passes;
-    const int b = blockIdx.x / heads, head = blockIdx.x - b * heads;
-    const int tiles = span_of(p, p.lengths[b]).tiles;
-    if (tiles == 0) return;
-    int64_t before = 0, total = 0;
-    for (int i = 0; i < p.batch; i += 64) {
-        int v = i + lane < p.batch ? span_of(p, p.lengths[i + lane]).tiles : 0;
-        int u = i + lane < b ? v : 0;
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
-            v += __shfl_xor(v, o, 64);
-            u += __shfl_xor(u, o, 64);
-        }
-        total += v;
-        before += u;
-    }
-    total *= heads;
-    const int64_t first = before * heads + (int64_t)head * tiles;
-    // Workgroup g took tiles from floor(total · g / groups) on.
-    const int g0 = (int)(((first + 1) * groups - 1) / total), g1 = (int)(((first + tiles) * groups - 1) / total);
-    if (g0 == g1) return;  // one workgroup had them all, and wrote the result
-    const int kvh = head / passes, pass = head - kvh * passes;
-    const int live = min(16, group - pass * 16);
-    const float v_scale = E4M3 && p.v_scale ? p.v_scale[kvh] : 1.0f;
-    for (int i = threadIdx.x; i < live * (p.dim / 2); i += 256) {
-        const int c = i / (p.dim / 2), d = 2 * (i - c * (p.dim / 2));
-        float top = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
-        for (int g = g0; g <= g1; ++g) {
-            if (total * g / groups == total * (g + 1) / groups) continue;  // fewer tiles than workgroups: it had none
-            const float *slot = p.part + (int64_t)(2 * g + (total * g / groups < first ? 1 : 0)) * part_floats(DP);
-            const float m = fmaxf(top, slot[c]), from = m == -INFINITY ? 0.0f : m;
-            const float keep = __builtin_amdgcn_exp2f(top - from), weight = __builtin_amdgcn_exp2f(slot[c] - from);
-            l = l * keep + slot[16 + c] * weight;
-            x = x * keep + slot[32 + c * DP + d] * weight;
-            y = y * keep + slot[32 + c * DP + d + 1] * weight;
-            top = m;
-        }
-        const float scale = (l > 0.0f ? __fdiv_rn(1.0f, l) : l == 0.0f ? 0.0f : l) * v_scale;
-        *reinterpret_cast<uint32_t *>(p.out + b * p.o_tok + (kvh * group + pass * 16 + c) * p.o_head + d) =
-            pack_bf16_rne(x * scale, y * scale);
-    }
+__global__ void __launch_bounds__(256) zero_marks_kernel(int *marks, int64_t count) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) marks[i] = 0;
 }
+
+// Whether 16-token tiles lie in one page each, and a lane's offsets within one in 32 bits.
+bool by_pages(const PagedArgs &p) { return p.page % 16 == 0 && 32 * std::max(p.kc_tok, p.vc_tok) <= INT32_MAX; }
 
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 template <int DP, bool E4M3>
 hipError_t launch_attention(const PagedArgs &p, int groups, hipStream_t stream) {
-    if (p.page % 16 == 0)
+    if (by_pages(p))
         hipLaunchKernelGGL((paged_attention_kernel<DP, E4M3, true>), dim3(groups), dim3(64 * WAVES), 0, stream, p);
     else
         hipLaunchKernelGGL((paged_attention_kernel<DP, E4M3, false>), dim3(groups), dim3(64 * WAVES), 0, stream, p);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || groups == 1) return e;
-    const int passes = (p.q_heads / p.kv_heads + 15) / 16;
-    hipLaunchKernelGGL((paged_join_kernel<DP, E4M3>), dim3(p.batch * p.kv_heads * passes), dim3(256), 0, stream, p, groups);
     return hipGetLastError();
 }
 
@@ -634,17 +760,34 @@ hipError_t launch_append_kv(const AppendArgs &p, bool e4m3, bool vec, hipStream_
     return hipGetLastError();
 }
 
+// n / page for n < 2^31 as (n · mul) >> shift: s with 2^(s-1) < page ≤ 2^s, mul = floor(2^(31+s) / page) + 1 ≤ 2^32 + 1,
+// the product's excess under n / 2^(31+s) < 2^-s ≤ 1/page.
+void page_divisor(PagedArgs &p) {
+    int s = 0;
+    while ((1ll << s) < p.page) ++s;
+    p.page_shift = 31 + s;
+    p.page_mul = ((1ull << (31 + s)) / (uint64_t)p.page) + 1;
+}
+
 int paged_groups(const PagedArgs &p, int cus) {
     const int passes = (p.q_heads / p.kv_heads + 15) / 16;
     int64_t tokens = (int64_t)p.max_pages * p.page;
     if (p.window > 0 && tokens > p.window + 31) tokens = p.window + 31;
     const int64_t most = (int64_t)p.batch * p.kv_heads * passes * ((tokens + TILE - 1) / TILE);
-    const int64_t full = 2 * (int64_t)cus;
+    const int64_t full = held(padded_dim(p.dim)) * (int64_t)cus;
     return (int)(most < 1 ? 1 : most < full ? most : full);
 }
 
 int64_t paged_part_bytes(const PagedArgs &p, int groups) {
     return groups == 1 ? 0 : (int64_t)2 * groups * part_floats(padded_dim(p.dim)) * 4;
+}
+
+int64_t paged_marks(const PagedArgs &p) { return (int64_t)p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16); }
+
+hipError_t launch_zero_marks(int *marks, int64_t count, hipStream_t stream) {
+    const int64_t blocks = (count + 255) / 256;
+    hipLaunchKernelGGL(zero_marks_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, stream, marks, count);
+    return hipGetLastError();
 }
 
 hipError_t launch_paged_attention(const PagedArgs &p, bool e4m3, int groups, hipStream_t stream) {

@@ -94,14 +94,20 @@ struct PagedArgs {
     const int32_t *lengths;             // [batch]
     uint16_t *out;
     float *part;                        // partial results of split sequences: paged_part_bytes() bytes
+    int *marks;                         // paged_marks() counters, zero before and after every call
     int64_t q_tok, q_head, o_tok, o_head;
     int64_t kc_page, kc_tok, kc_head, vc_page, vc_tok, vc_head, pages_row;
     float scale, softcap;
     int batch, q_heads, kv_heads, dim, page, page_count, max_pages, window;
+    uint64_t page_mul;                  // page_divisor()'s
+    int page_shift;
 };
+void page_divisor(PagedArgs &p);
 // The workgroups a call of these sizes takes, and the partial results' bytes they need.
 int paged_groups(const PagedArgs &p, int cus);
 int64_t paged_part_bytes(const PagedArgs &p, int groups);
+int64_t paged_marks(const PagedArgs &p);
+hipError_t launch_zero_marks(int *marks, int64_t count, hipStream_t stream);
 hipError_t launch_paged_attention(const PagedArgs &p, bool e4m3, int groups, hipStream_t stream);
 
 }  // namespace sq8

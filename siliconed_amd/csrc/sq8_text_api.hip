@@ -240,9 +240,9 @@ int sq8_paged_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_
     if (q_heads % cache->kv_heads != 0) return SQ8_EINVAL;
     const bool e4m3 = cache->dtype == SQ8_FP8_E4M3;
     if (cache->dim > 256 || cache->dim % (e4m3 || cache->dim > 128 ? 16 : 8) != 0) return SQ8_EUNSUPPORTED;
-    // Token numbers, and tiles of a sequence over its heads, are 32-bit.
+    // Token numbers, and the tiles of a batch over its heads, are 32-bit.
     if ((int64_t)max_pages * cache->page > INT32_MAX - 4096 ||
-        ((int64_t)max_pages * cache->page / 128 + 1) * q_heads > INT32_MAX)
+        (double)((int64_t)max_pages * cache->page / 128 + 2) * q_heads * batch > INT32_MAX)
         return SQ8_EUNSUPPORTED;
     if (batch == 0) return SQ8_OK;
     if (!q || !out || !lengths || q_token < 0 || q_head < 0 || o_token < 0 || o_head < 0) return SQ8_EINVAL;
@@ -269,12 +269,25 @@ int sq8_paged_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_
     p.scale = scale; p.softcap = softcap;
     p.batch = batch; p.q_heads = q_heads; p.kv_heads = cache->kv_heads; p.dim = cache->dim;
     p.page = cache->page; p.page_count = cache->pages; p.max_pages = max_pages; p.window = window;
+    sq8::page_divisor(p);
     const int groups = sq8::paged_groups(p, ctx->cus);
     const int64_t bytes = sq8::paged_part_bytes(p, groups);
     if (bytes > 0) {
         st = reserve(ctx, ctx->part, (size_t)bytes);
         if (st != SQ8_OK) return st;
         p.part = static_cast<float *>(ctx->part.at);
+        const size_t marks = (size_t)sq8::paged_marks(p) * sizeof(int);
+        if (ctx->marks.bytes < marks) {
+            // New counters are cleared once, and no graph may hold that.
+            if (sq8::capturing(ctx->stream)) return hip_status(hipErrorStreamCaptureUnsupported);
+            st = reserve(ctx, ctx->marks, marks < 65536 ? 65536 : marks);
+            if (st != SQ8_OK) return st;
+            const hipError_t e = sq8::launch_zero_marks(static_cast<int *>(ctx->marks.at), (int64_t)(ctx->marks.bytes / sizeof(int)), ctx->stream);
+            if (e != hipSuccess) return hip_status(e);
+        } else if (!ctx->marks.in_graph && sq8::capturing(ctx->stream)) {
+            ctx->marks.in_graph = true;
+        }
+        p.marks = static_cast<int *>(ctx->marks.at);
     }
     return hip_status(sq8::launch_paged_attention(p, e4m3, groups, ctx->stream));
 }

@@ -2,13 +2,13 @@
 // residual stream's new sum, and the quantization alone.
 //
 //   s' = r + x,  y = (s' · 1/sqrt(mean(s'²) + eps)) · w
-//   e4m3: per 128 columns s = max(max|y| / 448, 1e-30), code = e4m3(y / s), nearest even
+//   e4m3: per 128 columns s = max(max|y| · fl(1/448), 1e-30), code = e4m3(y / s), nearest even
 //   int8: per row s = max(max|y| / 127, 1e-30), code = clamp(rint(y / s), −128, 127)
 //
 // The sums, the norm and the scales are fp32; s' is rounded to the stream's type only where it is stored, so the
-// norm sees the sum before that rounding. Both quotients are correctly rounded: an ulp of y/s decides a code where
-// y/s lies halfway between two, and among bf16 values that is common (448 = 7 · 64: y = 3·2^j · max|y| is such a
-// tie). y/s is under 449, which rounds to the largest code: none overflows to NaN. An infinity in a group (e4m3) or
+// norm sees the sum before that rounding. y/s is correctly rounded: an ulp of it decides a code where it lies
+// halfway between two, and among bf16 values that is common (448 = 7 · 64: y = 3·2^j · max|y| is such a
+// tie). It is under 449, which rounds to the largest code: none overflows to NaN. An infinity in a group (e4m3) or
 // row (int8) makes its scale infinite, and its finite values' codes 0.
 #include <hip/hip_runtime.h>
 
@@ -99,7 +99,7 @@ __device__ __forceinline__ float max_of_16(float m) {
 }
 
 __device__ __forceinline__ float group_scale(float m) {
-    const float q = __fdiv_rn(m, 448.0f);
+    const float q = m * (1.0f / 448.0f);
     return q > 1e-30f ? q : 1e-30f;
 }
 
