@@ -306,7 +306,7 @@ __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t d) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d, 1.0f, W != 0));
 }
 
-// A slot: maxima [16], sums [16], outputs [16][dp].
+// A slot: maxima [16], sums [16], outputs [dp / 16][4][64] as the first wave's lanes hold them.
 __host__ __device__ constexpr int part_floats(int dp) { return 32 + 16 * dp; }
 
 // The slots lie where every XCD sees them: written and read past its own L2 (agent-scope accesses), so the join needs no
@@ -319,14 +319,18 @@ __device__ __forceinline__ float get(const float *from) { return __hip_atomic_lo
 __device__ __forceinline__ float inverse(float l) { return l > 0.0f ? __fdiv_rn(1.0f, l) : l == 0.0f ? 0.0f : l; }
 
 // The results of workgroups g0 .. g1 over one sequence's head, in that order: the first's in slot `slot0`, the others' in
-// 2g (where a workgroup's tiles begin with that sequence's). A thread takes two values of a query head; its loads of
-// eight slots are under way at once.
+// 2g (where a workgroup's tiles begin with that sequence's). A thread takes two values of a query head, as neighbours of
+// the lane that wrote them; its loads of eight slots are under way at once.
 template <int DP>
 __device__ __forceinline__ void join_slots(const PagedArgs &p, int slot0, int g0, int g1, int live, float v_scale, uint16_t *out) {
-    const int pairs = p.dim / 2;
+    constexpr int DV = DP / 16;
     auto slot_of = [&](int g) { return p.part + (int64_t)(g == g0 ? slot0 : 2 * g) * part_floats(DP); };
-    for (int i = threadIdx.x; i < live * pairs; i += 64 * WAVES) {
-        const int c = i / pairs, d = 2 * (i - c * pairs);
+    // An item a thread: head c, row h of the lanes and register r, values d and d + 1.
+    for (int i = threadIdx.x; i < live * 8 * DV; i += 64 * WAVES) {
+        const int rest = i / live, c = i - rest * live;
+        const int h = rest & 3, r = rest >> 2 & 3, d = 2 * (rest >> 4);
+        const int lane = 16 * h + c, at = DV * (4 * h + r) + d;
+        if (at >= p.dim) continue;
         float top = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
         for (int g = g0; g <= g1; g += 8) {
             float m[8], n[8], u[8], v[8];
@@ -335,8 +339,8 @@ __device__ __forceinline__ void join_slots(const PagedArgs &p, int slot0, int g0
                 const float *slot = slot_of(min(g + e, g1));
                 m[e] = get(slot + c);
                 n[e] = get(slot + 16 + c);
-                u[e] = get(slot + 32 + c * DP + d);
-                v[e] = get(slot + 32 + c * DP + d + 1);
+                u[e] = get(slot + 32 + (4 * d + r) * 64 + lane);
+                v[e] = get(slot + 32 + (4 * d + 4 + r) * 64 + lane);
             }
             float most = top;
 #pragma unroll
@@ -357,7 +361,7 @@ __device__ __forceinline__ void join_slots(const PagedArgs &p, int slot0, int g0
             }
         }
         const float scale = inverse(l) * v_scale;
-        *reinterpret_cast<uint32_t *>(out + c * p.o_head + d) = pack_bf16_rne(x * scale, y * scale);
+        *reinterpret_cast<uint32_t *>(out + c * p.o_head + at) = pack_bf16_rne(x * scale, y * scale);
     }
 }
 
@@ -674,11 +678,10 @@ __global__ void __launch_bounds__(64 * WAVES, held(DP)) paged_attention_kernel(c
                         put(slot + c, all);
                         put(slot + 16 + c, l);
                     }
-                    float *dst = slot + 32 + c * DP;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
+                    for (int d = 0; d < DV; ++d)
 #pragma unroll
-                        for (int d = 0; d < DV; ++d) put(dst + DV * (4 * h + r) + d, o[d][r]);
+                        for (int r = 0; r < 4; ++r) put(slot + 32 + (4 * d + r) * 64 + lane, o[d][r]);
                 }
             }
         }
