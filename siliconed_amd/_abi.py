@@ -90,7 +90,12 @@ SIGNATURES = {
     "sq8_abi_version": (_I, []),
 }
 
+# The entries that text_bind.cpp calls, in the order of its Entries.
+TEXT_ENTRIES = ("sq8_add_norm_quantized", "sq8_quantize_groups", "sq8_linear_f8", "sq8_linear_f8_quantized",
+                "sq8_append_kv", "sq8_paged_attention")
+
 _lib = None
+text = None  # the text decoder's operators' native calls (text_bind.cpp), once the library is loaded
 
 
 class SQ8Error(RuntimeError):
@@ -106,7 +111,7 @@ class Unsupported(SQ8Error):
 
 
 def load() -> ctypes.CDLL:
-    global _lib
+    global _lib, text
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise ImportError(f"{LIB_PATH} is not built: run `python -c 'import __graft_entry__ as g; g.build()'`")
@@ -115,7 +120,11 @@ def load() -> ctypes.CDLL:
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
-        _lib = lib
+        import torch  # noqa: F401  (the libraries that the module is linked against)
+
+        from . import _text_bind
+        _text_bind.bind(*(ctypes.cast(getattr(lib, name), _P).value for name in TEXT_ENTRIES))
+        _lib, text = lib, _text_bind
     return _lib
 
 

@@ -1,4 +1,5 @@
-"""Builds the gfx950 library libsiliconed_q8.so in-tree with hipcc.
+"""Builds the gfx950 library libsiliconed_q8.so in-tree with hipcc, and the host module _text_bind.so
+(text_bind.cpp, the text decoder's operators' calls on torch tensors) with g++.
 
 Each .hip source is compiled to an object in parallel, then linked. The flags every HIP object
 gets: --offload-arch=gfx950 only, -O3, and packed-fp32 instructions disabled for the device code
@@ -11,12 +12,14 @@ import concurrent.futures
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libsiliconed_q8.so")
+BIND = os.path.join(PKG, "_text_bind.so")
 # (source, object name, extra defines): the FAST kernel set is one source compiled per weight type
 # and layout, so the sets compile in parallel, the longest first.
 SOURCES = [
@@ -97,13 +100,30 @@ def _stale(item) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _bind() -> None:
+    import torch
+
+    at = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           "-I", os.path.join(ROOT, "include"), "-isystem", os.path.join(at, "include"),
+           "-isystem", os.path.join(at, "include", "torch", "csrc", "api", "include"),
+           "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, "text_bind.cpp"), "-o", BIND + ".tmp",
+           "-L", os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"the host module failed:\n{r.stderr}")
+    os.replace(BIND + ".tmp", BIND)
+
+
 def build(verbose: bool = False, incremental: bool = False) -> str:
     """Compiles the sources and links the library; returns its path. Always recompiles every source,
     unless `incremental` (then only those whose object is older than the source or a header)."""
     os.makedirs(OBJ, exist_ok=True)
     todo = [it for it in SOURCES if _stale(it)] if incremental else SOURCES
-    with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, min(len(todo), os.cpu_count() or 1))) as pool:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, min(len(todo) + 1, os.cpu_count() or 1))) as pool:
+        bind = pool.submit(_bind)
         list(pool.map(_compile, todo))
+        bind.result()
     objs = [os.path.join(OBJ, name + ".o") for _, name, _ in SOURCES]
     tmp = LIB + ".tmp"
     # rocBLAS: the bf16-weight product's plain GEMM.
