@@ -32,13 +32,16 @@ namespace {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// A lane's codes 8·J .. 8·J + 7 of a block as bf16, exactly.
+// A lane's codes 8·J .. 8·J + 7 of a block as bf16, exactly (the conversion's scale is 1): two codes an instruction.
 template <int J>
 __device__ __forceinline__ bf16x8 widen_f8(const i32x8 &x) {
-    uint32_t d0, d1, d2, d3;
-    widen4<(int)W_FP8>((uint32_t)x[2 * J], d0, d1);
-    widen4<(int)W_FP8>((uint32_t)x[2 * J + 1], d2, d3);
-    return __builtin_bit_cast(bf16x8, u32x4{d0, d1, d2, d3});
+    u32x4 y;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        y[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)x[2 * J + i], 1.0f, false));
+        y[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((uint32_t)x[2 * J + i], 1.0f, true));
+    }
+    return __builtin_bit_cast(bf16x8, y);
 }
 
 // One block's sums of 16 weight rows by 16 activation rows.
@@ -114,6 +117,11 @@ __device__ __forceinline__ void store4(const F8Args &p, int row, int col, f32x4 
 // Few rows: a workgroup of NW waves takes NO × 16 output columns (GLU: of both halves) and TM tiles of 16 rows; the
 // waves take the K blocks in turn, both operands straight from memory, U blocks' loads in flight, and add up through
 // LDS.
+//
+// The weight's bytes bound it: one row by K = 4096, N = 6144 (25 MB) takes 7.1 µs, 3.5 TB/s with 2.5 of them the launch,
+// and a gate and up product of N = 24576 (101 MB) 20 to 22, 4.6 to 5 TB/s. Fragments that lanes load from 16 rows at
+// once come in at 34 KB/µs a CU (whole rows of 128 bytes: 115), which is above a CU's share of the memory's rate but
+// not by much: past 16 rows, whose loads then outweigh the weight's, the tile kernel's way through LDS is the faster.
 template <int TM, int NO, int NW, int U, bool GLU, bool F32>
 __global__ void __launch_bounds__(64 * NW) f8_short_kernel(const F8Args p) {
     constexpr int NT = GLU ? 2 * NO : NO;
@@ -194,15 +202,23 @@ __global__ void __launch_bounds__(64 * NW) f8_short_kernel(const F8Args p) {
 
 // Many rows: tiles of BM rows by BN weight rows (GLU: half of them of each half), WM × WN waves.
 //
-// Both operands go to LDS by direct loads, a block (128 bytes) of each row a step, in two stages. 16-byte runs of a
+// Both operands go to LDS by direct loads, a block (128 bytes) of each row a step, in NS stages. 16-byte runs of a
 // row are permuted within it (by key_a, key_w) so that the eight rows a fragment read touches at once lie on different
-// banks. The rows' scales go to LDS too, four blocks at a time where they can be read so.
+// banks. The rows' scales go to LDS too, four blocks at a time where they can be read so (a load of one block's scales
+// a step, a line for each row, cost the small tiles a tenth).
 //
 // Each wave multiplies (BM/WM) × (BN/WN) in 16 × 16 parts, a row of TN parts at a time, the weight's fragments held for
 // the step and the rows' read two parts ahead; the multiply-adds that scale one row of parts go between the matrix
 // instructions of the next. The step's one barrier stands before its last two rows of parts, whose fragments are in
-// registers by then: the stage is free for the loads of the step after next, the next step's loads have landed, and
-// its first fragments are read under the last matrix instructions of this one.
+// registers by then: the stage is free for the loads of NS steps on, which go between the last matrix instructions (in
+// one burst behind the barrier they held up the small tiles' steps by a seventh), the next step's loads have landed,
+// and its first fragments are read under those instructions too.
+//
+// What bounds it: at M = 8192, K = 4096, N = 24576 (GLU) the 256 × 256 tile's matrix instructions and their power,
+// 757 µs or 2.18 PFLOP/s (a library's product of such codes with one scale a tensor, no GLU: 650). A 64-row tile's step
+// is a chain of a barrier, reads, four to eight matrix instructions a wave and their scaling, 0.36 µs where the
+// instructions alone are 0.06, so few rows want many workgroups: N = 24576 (GLU) has 192 of 64 × 128, 27.6 µs at M = 48
+// (100 MB, 3.7 TB/s), and N = 4096 takes its K in four parts, 10.1 µs at M = 64, K = 4096, and 17.7 at K = 12288.
 //
 // The weight row an instruction's row stands for is chosen so that a lane ends with consecutive outputs: lane group
 // h, register r of part j is output 4·NTO·h + 4j + r of the wave's (NTO parts wide).
@@ -213,10 +229,10 @@ struct TileShape {
     static constexpr int NTO = GLU ? TN / 2 : TN;               // and those of one half
     static constexpr int OUT = GLU ? BN / 2 : BN;               // outputs of a tile
     static constexpr int STAGE = (BM + BN) * F8_GROUP;
-    // The rows' scales: two buffers of four blocks', or with more stages one block's a stage (and room for the
-    // waves that have no row).
-    static constexpr int SCALES = NS == 2 ? BM * 16 : WM * WN * 256;
-    static constexpr int LDS = NS * (STAGE + SCALES);
+    static constexpr int SCALES = BM * 16;                      // four blocks' scales of the rows
+    static constexpr int LDS = NS * STAGE + 2 * SCALES;
+    static constexpr bool SPLIT = NS > 2;                       // K may be split
+    static_assert(NS <= 4, "two buffers of scales hold the blocks under way");
     static_assert(TM * 16 * WM == BM && TN * 16 * WN == BN && (!GLU || TN % 2 == 0), "whole parts");
     static_assert(NTO == 1 || NTO == 2 || NTO == 4, "a lane's outputs");
 };
@@ -228,9 +244,6 @@ __device__ __forceinline__ int key_w(int row) {
     constexpr int SHIFT = NTO == 4 ? 4 : NTO == 2 ? 3 : 2;
     return (row & 3) | ((row >> SHIFT) & 1) << 2;
 }
-
-// Columns of a row of partial sums: whole runs of a lane's outputs.
-__host__ __device__ constexpr int part_columns(int h) { return (h + 15) / 16 * 16; }
 
 template <int BM, int BN, int WM, int WN, int NS, bool GLU, bool F32>
 __global__ void __attribute__((amdgpu_flat_work_group_size(64 * WM * WN, 64 * WM * WN), amdgpu_waves_per_eu(2, 2)))
@@ -267,36 +280,23 @@ f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
     const int left = p.K & (F8_GROUP - 1);  // of a last block that K ends inside
     uint8_t *const scales = lds + NS * S::STAGE;
     const wd::i32x4 sx_rsrc = wd::buffer_rsrc(p.sx + (int64_t)m0 * p.ldsx);
-    // NS > 2: one row's scale a lane; the waves past BM rows read row 0's, so that every wave's loads are as many.
-    const uint32_t sx_off = (uint32_t)min(wave * 64 < BM ? wave * 64 + lane : 0, p.M - 1 - m0) * (uint32_t)p.ldsx * 4;
-    constexpr int LOADS = A_LOADS + W_LOADS + 1;  // a wave's of one block (NS > 2)
-    auto issue = [&](int t, int stage) {
-        const int at = t * F8_GROUP;
-        uint8_t *const to = lds + stage;
-        if (left == 0 || t != p.KB - 1) {
+    constexpr int LOADS = A_LOADS + W_LOADS;  // a wave's of one block, besides those of scales
+    // Block t's loads into a stage: first `ahead`, then each of LOADS. Past t1 the buffers have no bytes: nothing is
+    // read, but the loads under way stay as many.
+    wd::i32x4 a_from = a_rsrc, w_from = w_rsrc;
+    auto ahead = [&](int t) {
+        int under = t - t1;
+        asm volatile("" : "+s"(under));  // (a comparison's result would go through vector registers)
+        a_from[2] = w_from[2] = under >> 31;
+        if (t >= t1) return;
+        if (left != 0 && t == p.KB - 1) {
+            // Runs past K are read from the block's first: it is the last that these offsets are for.
 #pragma unroll
-            for (int i = 0; i < A_LOADS; ++i)
-                wd::raw_buffer_load_lds(a_rsrc, (wd::lds_u32)(to + (wave * A_LOADS + i) * 1024), 16, (int)a_off[i], at, 0, 0);
+            for (int i = 0; i < A_LOADS; ++i) a_off[i] -= a_run >= left ? a_run : 0;
 #pragma unroll
-            for (int i = 0; i < W_LOADS; ++i)
-                wd::raw_buffer_load_lds(w_rsrc, (wd::lds_u32)(to + BM * F8_GROUP + (wave * W_LOADS + i) * 1024), 16, (int)w_off[i], at, 0, 0);
-        } else {
-            // Runs past K are read from the block's first. (Nothing of this is worth registers over the loop: the
-            // empty statement keeps it here.)
-            int end = left;
-            asm volatile("" : "+s"(end));
-#pragma unroll
-            for (int i = 0; i < A_LOADS; ++i)
-                wd::raw_buffer_load_lds(a_rsrc, (wd::lds_u32)(to + (wave * A_LOADS + i) * 1024), 16,
-                                        (int)(a_off[i] - (a_run >= end ? a_run : 0)), at, 0, 0);
-#pragma unroll
-            for (int i = 0; i < W_LOADS; ++i)
-                wd::raw_buffer_load_lds(w_rsrc, (wd::lds_u32)(to + BM * F8_GROUP + (wave * W_LOADS + i) * 1024), 16,
-                                        (int)(w_off[i] - (w_run(i) >= end ? w_run(i) : 0)), at, 0, 0);
+            for (int i = 0; i < W_LOADS; ++i) w_off[i] -= w_run(i) >= left ? w_run(i) : 0;
         }
-        if constexpr (NS > 2) {
-            wd::raw_buffer_load_lds(sx_rsrc, (wd::lds_u32)(scales + (stage / S::STAGE) * S::SCALES + wave * 256), 4, (int)sx_off, t * 4, 0, 0);
-        } else if (!p.sx_vec || (t & 3) == 0 || t == t0) {
+        if (!p.sx_vec || (t & 3) == 0 || t == t0) {
             // A lane a row; sx_vec: blocks t .. t + 3 as [row][4], else one block as [4][row].
             uint8_t *const s = scales + ((t >> 2) & 1) * S::SCALES;
             int last_row = p.M - 1 - m0;
@@ -308,19 +308,27 @@ f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
             }
         }
     };
-    // Block t's loads are done, this wave's and then all; those of NS − 2 later ones may be under way, where there are
-    // as many (`more`). The activation's runs past K become zeros in between.
-    auto landed = [&](int t, int stage, bool more) {
-        if (NS > 2 && more) wd::wait_vmcnt<NS == 2 ? 0 : (NS - 2) * LOADS>();
-        else wd::wait_vmcnt<0>();
+    auto load = [&](auto nc, int t, int stage) {
+        constexpr int n = decltype(nc)::value, i = n < A_LOADS ? n : n - A_LOADS;
+        uint8_t *const to = lds + stage;
+        if constexpr (n < A_LOADS)
+            wd::raw_buffer_load_lds(a_from, (wd::lds_u32)(to + (wave * A_LOADS + i) * 1024), 16, (int)a_off[i], t * F8_GROUP, 0, 0);
+        else
+            wd::raw_buffer_load_lds(w_from, (wd::lds_u32)(to + BM * F8_GROUP + (wave * W_LOADS + i) * 1024), 16, (int)w_off[i], t * F8_GROUP, 0, 0);
+    };
+    // Block t's loads are done, this wave's and then all; those of NS − 2 later ones may be under way. The activation's
+    // runs past K become zeros in between.
+    auto landed = [&](int t, int stage) {
+        wd::wait_vmcnt<(NS - 2) * LOADS>();
         if (left != 0 && t == p.KB - 1 && a_run >= left) {
 #pragma unroll
             for (int i = 0; i < A_LOADS; ++i)
                 *reinterpret_cast<u32x4 *>(lds + stage + (wave * A_LOADS + i) * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
         }
-        __syncthreads();
+        // No fence: one would wait for the later blocks' loads too. What LDS this wave still reads has come.
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
-    const int scale_row = NS == 2 && p.sx_vec ? 16 : 4, scale_block = p.sx_vec ? 4 : BM * 4;
+    const int scale_row = p.sx_vec ? 16 : 4, scale_block = p.sx_vec ? 4 : BM * 4;
 
     // ---- fragment addresses: neither key depends on the part, whose rows lie at fixed distances ----
     int a_at[2], w_at[2];
@@ -355,10 +363,8 @@ f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
         return i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
     };
     int stage = 0;  // the offset in LDS of the stage whose fragments are read, and of its scales
-    auto scales_of = [&](int t, int stage) {
-        return NS == 2 ? sx_at + (t & 3) * scale_block + ((t >> 2) & 1) * S::SCALES : sx_at + (stage / S::STAGE) * S::SCALES;
-    };
-    int sx_now = scales_of(t0, 0);
+    auto scales_of = [&](int t) { return sx_at + (t & 3) * scale_block + ((t >> 2) & 1) * S::SCALES; };
+    int sx_now = scales_of(t0);
     auto read_a = [&](auto ic) {
         constexpr int i = decltype(ic)::value;
         a[i & 1] = fragment(a_at[0] + stage + i * 16 * F8_GROUP, a_at[1] + stage + i * 16 * F8_GROUP);
@@ -384,13 +390,10 @@ f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
         load_sw(t0);
         static_for<0, NS>([&](auto sc) {
             constexpr int s = decltype(sc)::value;
-            if (s == 0 || t0 + s < t1) issue(t0 + s, s * S::STAGE);
-            // With two stages the first is waited for alone, as the loop does.
-            if constexpr (NS == 2 && s == 0) landed(t0, 0, false);
+            ahead(t0 + s);
+            static_for<0, LOADS>([&](auto nc) { load(nc, t0 + s, s * S::STAGE); });
+            if constexpr (s == NS - 2) landed(t0, 0);
         });
-        if constexpr (NS > 2) {
-            landed(t0, 0, t0 + NS <= t1);
-        }
         static_for<0, TN>([&](auto jc) { read_w(jc); });
         read_a(I0{});
         read_a(I1{});
@@ -401,6 +404,7 @@ f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
 #pragma clang loop unroll(disable)
     for (int t = t0; t < t1; ++t) {
         float s_w[2];
+        int from = 0;  // the stage that is free after this step's barrier
         if (t != t0 && ((t - t0) & 63) == 0) load_sw(t);
 #pragma unroll
         for (int g = 0; g < (GLU ? 2 : 1); ++g) s_w[g] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sw_of[g]), (t - t0) & 63));
@@ -409,11 +413,11 @@ f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
             using Before = std::integral_constant<int, (i + TM - 1) % TM>;
             if constexpr (i == TM - 2) {
                 // Every fragment of this stage is in registers (or on its way there: the barrier waits for those).
-                const int from = stage;
+                from = stage;
                 stage = stage == (NS - 1) * S::STAGE ? 0 : stage + S::STAGE;
-                landed(t + 1, stage, t + NS <= t1);
-                if (t + NS < t1) issue(t + NS, from);
-                sx_now = scales_of(t + 1, stage);
+                landed(t + 1, stage);
+                ahead(t + NS);
+                sx_now = scales_of(t + 1);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -422,14 +426,20 @@ f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
                 constexpr int j = decltype(jc)::value;
                 add(Before{}, jc);
                 part[j] = block_sums<F32>(w[j], a[i & 1]);
+                if constexpr (i >= TM - 2) {
+                    constexpr int SLOT = (i - (TM - 2)) * TN + j, SLOTS = 2 * TN;
+                    static_for<LOADS * SLOT / SLOTS, LOADS * (SLOT + 1) / SLOTS>([&](auto nc) { load(nc, t + NS, from); });
+                }
                 if constexpr (i == TM - 1) read_w(jc);
             });
             read_a(std::integral_constant<int, (i + 2) % TM>{});
             if constexpr (!F32) {
                 // The multiply-adds of a part of the row before, the matrix instruction that takes its place, its reads.
-                static_for<0, TN>([&](auto) {
+                static_for<0, TN>([&](auto jc) {
+                    constexpr int SLOT = (i - (TM - 2)) * TN + decltype(jc)::value, SLOTS = 2 * TN;
                     __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    if constexpr (SLOT >= 0) __builtin_amdgcn_sched_group_barrier(0x010, LOADS * (SLOT + 1) / SLOTS - LOADS * SLOT / SLOTS, 0);
                     if constexpr (i == TM - 1) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
                 });
                 __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
@@ -438,27 +448,55 @@ f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
         });
     }
     if (t0 < t1) static_for<0, TN>([&](auto jc) { add(Last{}, jc); });
+    wd::wait_vmcnt<0>();  // a load's write to LDS may not outlive the workgroup
 
     // ---- outputs: N consecutive ones of each of TM rows ----
     constexpr int N = 4 * NTO;
     const int col = n0 + wn * 16 * NTO + N * h;
     const int real = min(N, p.H - col);  // of them
     const int row0 = m0 + wm * (BM / WM) + c;
-    if (gridDim.y > 1) {
-        // One part of K: its sums as they are, to be added up by f8_join_kernel.
-        const int wide = part_columns(p.H);
-        if (col >= wide) return;
+    if constexpr (S::SPLIT) {
+        if (gridDim.y > 1) {
+            // One part of K. Its sums go to its slot, past the caches that workgroups do not share, and the workgroup
+            // that a tile's counter finds last adds the slots up, in their order.
+            const int splits = gridDim.y, mine = blockIdx.y;
+            float *const slots = p.part + (int64_t)blockIdx.x * splits * (BM * BN) + threadIdx.x;
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            if (row0 + 16 * i >= p.M) continue;
+            for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int g = 0; g < (GLU ? 2 : 1); ++g) {
-                float *to = p.part + (((int64_t)blockIdx.y * p.M + row0 + 16 * i) * (GLU ? 2 : 1) + g) * wide + col;
+                for (int j = 0; j < TN; ++j)
 #pragma unroll
-                for (int j = 0; j < NTO; ++j) *reinterpret_cast<f32x4 *>(to + 4 * j) = acc[i][g * NTO + j];
+                    for (int e = 0; e < 4; ++e) put(slots + (int64_t)mine * (BM * BN) + ((i * TN + j) * 4 + e) * S::THREADS, acc[i][j][e]);
+            wd::wait_vmcnt<0>();
+            __syncthreads();
+            int *const joins = reinterpret_cast<int *>(lds);
+            if (threadIdx.x == 0) {
+                int *const mark = p.marks + blockIdx.x;
+                const bool last = __hip_atomic_fetch_add(mark, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
+                if (last) __hip_atomic_store(mark, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                *joins = last;
             }
+            __syncthreads();
+            if (!*joins) return;
+            f32x4 total[TM][TN];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) total[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int k = 0; k < splits; ++k) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            total[i][j][e] += get(slots + (int64_t)k * (BM * BN) + ((i * TN + j) * 4 + e) * S::THREADS);
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = total[i][j];
         }
-        return;
     }
     float bias[GLU ? 2 : 1][N];
     if (p.bias) {
@@ -487,22 +525,6 @@ f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
     });
 }
 
-// The parts' sums of a product whose K was split, added in order, then as ever: four outputs a thread.
-template <bool GLU, bool F32>
-__global__ void __launch_bounds__(256) f8_join_kernel(const F8Args p, int splits) {
-    constexpr int HALVES = GLU ? 2 : 1;
-    const int wide = part_columns(p.H), quads = wide / 4;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < (int64_t)p.M * quads; q += (int64_t)gridDim.x * 256) {
-        const int row = (int)(q / quads), col = 4 * (int)(q - (int64_t)row * quads);
-        f32x4 x[2] = {};
-        for (int s = 0; s < splits; ++s)
-#pragma unroll
-            for (int g = 0; g < HALVES; ++g)
-                x[g] += *reinterpret_cast<const f32x4 *>(p.part + (((int64_t)s * p.M + row) * HALVES + g) * wide + col);
-        store4<GLU, F32>(p, row, col, x[0], x[1]);
-    }
-}
-
 template <int BM, int BN, int WM, int WN, int NS, bool GLU, bool F32>
 hipError_t launch_tile(const F8Args &p, int splits, hipStream_t stream) {
     using S = TileShape<BM, BN, WM, WN, NS, GLU, F32>;
@@ -510,10 +532,6 @@ hipError_t launch_tile(const F8Args &p, int splits, hipStream_t stream) {
     if (tiles_m * tiles_n > INT32_MAX) return hipErrorInvalidValue;
     hipLaunchKernelGGL((f8_tile_kernel<BM, BN, WM, WN, NS, GLU, F32>), dim3((unsigned)(tiles_m * tiles_n), (unsigned)splits),
                        dim3(S::THREADS), 0, stream, p, (int)tiles_m, (int)tiles_n);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || splits == 1) return e;
-    const int64_t blocks = ((int64_t)p.M * (part_columns(p.H) / 4) + 255) / 256;
-    hipLaunchKernelGGL((f8_join_kernel<GLU, F32>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream, p, splits);
     return hipGetLastError();
 }
 
@@ -524,25 +542,28 @@ hipError_t launch_short(const F8Args &p, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// The tile kernels: rows, weight rows, waves, stages; workgroups a CU holds; microseconds a step of one block takes
-// with one workgroup on a CU and with as many as it holds.
+// The tile kernels: rows, weight rows, workgroups a CU holds; microseconds a step of one block takes with one workgroup
+// on a CU and with as many as it holds, for a bf16 C and for an fp32 one.
 struct TileCost {
     int rows, columns, held;
-    float one, all;
+    float one, all, one_f32, all_f32;
 };
 enum { T_256 = 0, T_128, T_64x128, T_64, TILES };
-// Measured over M 32 to 8192, K 4096 and 12288, N 4096 to 24576, plain and GLU: within 15 %.
-constexpr TileCost kTiles[TILES] = {{256, 256, 1, 1.6f, 1.95f}, {128, 128, 2, 0.8f, 1.15f}, {64, 128, 2, 0.58f, 0.78f}, {64, 64, 2, 0.43f, 0.57f}};
-// A launch and its first loads; the weight's bytes at the rate they are read with; what adding up the parts of a split
-// K takes beside their bytes.
-constexpr float kLaunch = 2.5f, kBytesMicrosecond = 4.5e6f, kJoin = 3.0f;
+// Measured over M 20 to 8192, K 512 to 12288, N 512 to 24576, plain and GLU: within 15 %.
+constexpr TileCost kTiles[TILES] = {{256, 256, 1, 1.9f, 1.9f, 0.0f, 0.0f},
+                                    {128, 128, 2, 0.85f, 1.36f, 1.25f, 2.2f},
+                                    {64, 128, 2, 0.47f, 0.82f, 0.78f, 1.29f},
+                                    {64, 64, 2, 0.36f, 0.49f, 0.52f, 0.77f}};
+// A launch and its first loads; the weight's bytes at the rate they are read with; adding up the parts of a split K:
+// once, for each part, and their bytes.
+constexpr float kLaunch = 3.0f, kBytesMicrosecond = 5.0e6f, kJoin = 0.7f, kJoinPart = 0.5f, kPartMicrosecond = 5.0e6f;
 
 template <bool GLU, bool F32>
 hipError_t launch(const F8Args &p, const F8Plan &plan, hipStream_t stream) {
     switch (plan.kernel) {
         case 0: return launch_tile<256, 256, 2, 4, 2, GLU, false>(p, plan.splits, stream);
         case 1: return launch_tile<128, 128, 2, 2, 2, GLU, F32>(p, plan.splits, stream);
-        case 2: return launch_tile<64, 128, 1, 4, 3, GLU, F32>(p, plan.splits, stream);
+        case 2: return launch_tile<64, 128, 2, 2, 3, GLU, F32>(p, plan.splits, stream);
         case 3: return launch_tile<64, 64, 2, 2, 4, GLU, F32>(p, plan.splits, stream);
         case 4: return launch_short<1, 1, 8, 4, GLU, F32>(p, stream);
         case 5: return launch_short<1, 2, 8, 4, GLU, F32>(p, stream);
@@ -556,11 +577,11 @@ hipError_t launch(const F8Args &p, const F8Plan &plan, hipStream_t stream) {
 // number of bytes a cycle, so 16 or 32 columns a workgroup by the bytes that the fullest CU takes. At M = 16, K = 4096:
 // N = 6144 11.3 µs by 16 and 8.8 by 32, N = 4096 7.1 and 8.7, N = 24576 (GLU) 25.8 and 29.0.
 // Above, the tile and the split of K with the least estimated time: rounds of workgroups times steps, not under the
-// time the bytes take. At M = 64, K = 12288, N = 4096: 64 × 64 tiles 45.4 µs whole and 20.9 in four parts; at M = 2048 of the same
-// 256 × 256 165 and 128 × 128 122; at M = 8192, K = 4096, N = 24576 752 and 885.
+// time the bytes take. At M = 64, K = 12288, N = 4096: 64 × 64 tiles 37.6 µs whole and 17.5 in four parts; at M = 2048
+// of the same 256 × 256 160 and 128 × 128 120; at M = 8192, K = 4096, N = 24576 752 and 885.
 // Rows too far apart for the tile kernels' 32-bit offsets go to the short kernel.
 F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
-    F8Plan plan = {6, 1, 0};
+    F8Plan plan = {6, 1, 0, 0};
     if (p.M <= 0 || p.H <= 0) return plan;
     const int halves = glu ? 2 : 1;
     if (p.M <= 16) {
@@ -574,28 +595,27 @@ F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
     const bool near = 256 * std::max(std::max(p.lda, p.ldw), 4 * p.ldsx) + p.K <= INT32_MAX &&
                       (!glu || ((int64_t)p.H + 256) * p.ldw + p.K <= INT32_MAX);
     if (!near) return plan;
-    const int wide = part_columns(p.H);
     float best = 0.0f;
     for (int t = out_f32 ? T_128 : T_256; t < TILES; ++t) {
         const TileCost &c = kTiles[t];
         const int64_t tiles = (int64_t)((p.M + c.rows - 1) / c.rows) * ((p.H * halves + c.columns - 1) / c.columns);
         for (int splits = 1; splits <= 8; ++splits) {
-            // Two stages read four blocks' scales at once: not split (a part may begin inside four).
-            if (splits > 1 && (t <= T_128 || p.KB < 8 * splits)) break;
+            if (splits > 1 && (t <= T_128 || p.KB < 4 * splits)) break;
             const int64_t groups = tiles * splits, slots = (int64_t)cus * c.held, rest = groups % slots;
             const int steps = (p.KB + splits - 1) / splits;
-            float us = steps * ((float)(groups / slots) * c.all + (rest == 0 ? 0.0f : rest > cus ? c.all : c.one));
+            const float one = out_f32 ? c.one_f32 : c.one, all = out_f32 ? c.all_f32 : c.all;
+            const float last = rest == 0 ? 0.0f : rest <= cus ? one : one + (all - one) * (float)(rest - cus) / (float)(slots - cus);
+            float us = steps * ((float)(groups / slots) * all + last);
             us = std::max(us, ((float)p.N * p.K + (float)p.M * p.K) / kBytesMicrosecond);
-            const float part = (float)p.M * wide * halves * 4.0f * splits;
-            if (splits > 1) us += kJoin + 2.0f * part / kBytesMicrosecond;
+            const int64_t part = groups * c.rows * c.columns * 4;
+            if (splits > 1) us += kJoin + kJoinPart * splits + (float)part / kPartMicrosecond;
             us += kLaunch;
             if (best == 0.0f || us < best) {
                 best = us;
-                plan = F8Plan{t, splits, splits > 1 ? (int64_t)part : 0};
+                plan = F8Plan{t, splits, splits > 1 ? part : 0, splits > 1 ? (int)tiles : 0};
             }
         }
     }
-    if (plan.splits > 1) plan.part_bytes = (int64_t)plan.splits * p.M * wide * halves * 4;
     return plan;
 }
 

@@ -309,12 +309,6 @@ __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t d) {
 // A slot: maxima [16], sums [16], outputs [dp / 16][4][64] as the first wave's lanes hold them.
 __host__ __device__ constexpr int part_floats(int dp) { return 32 + 16 * dp; }
 
-// The slots lie where every XCD sees them: written and read past its own L2 (agent-scope accesses), so the join needs no
-// fence, which would write back and drop that cache under everything still streaming through it (with fences the
-// kernel took twice as long at 48 sequences of up to 8192).
-__device__ __forceinline__ void put(float *to, float v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float get(const float *from) { return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
 // 1 / l, or 0 where nothing was added (a NaN stays one).
 __device__ __forceinline__ float inverse(float l) { return l > 0.0f ? __fdiv_rn(1.0f, l) : l == 0.0f ? 0.0f : l; }
 

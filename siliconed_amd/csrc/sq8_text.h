@@ -24,6 +24,12 @@ struct Quotient {
     }
 };
 
+// Partial results lie where every XCD sees them: written and read past its own L2 (agent-scope accesses), so that the
+// workgroup that joins them needs no fence, which would write back and drop that cache under everything still
+// streaming through it (with fences the attention took twice as long at 48 sequences of up to 8192).
+__device__ __forceinline__ void put(float *to, float v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ float get(const float *from) { return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
 // sq8_text_norm.hip. Element types by flag: bf16 or fp32.
 struct AddNormArgs {
     const void *x;          // [rows, cols]
@@ -54,6 +60,7 @@ struct F8Args {
     const float *bias;      // [N] or null
     void *c;                // [M, n_out]
     float *part;            // the sums of a split K's parts
+    int *marks;             // the tiles' counters of parts that are done, zero between calls
     int64_t lda, ldsx, ldw, ldsw, ldc;
     int M, N, K;            // K a multiple of 16
     int KB;                 // ⌈K/128⌉
@@ -62,10 +69,11 @@ struct F8Args {
     int c_vec;              // outputs a store may take: 8 or 4 (aligned base and rows), 0 for one at a time
     int sx_vec;             // four scales a load allowed (rows of whole fours)
 };
-// Which kernel a product runs on, and the parts its K is split in; part_bytes: what F8Args::part needs.
+// Which kernel a product runs on, and the parts its K is split in; part_bytes, marks: what F8Args::part and ::marks need.
 struct F8Plan {
     int kernel, splits;
     int64_t part_bytes;
+    int marks;
 };
 F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus);
 hipError_t launch_f8_product(const F8Args &p, const F8Plan &plan, bool glu, bool out_f32, hipStream_t stream);

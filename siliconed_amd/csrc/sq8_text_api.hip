@@ -21,6 +21,23 @@ bool is_activation(int dtype) { return dtype == SQ8_BF16 || dtype == SQ8_F32; }
 int groups_of(int k) { return (int)(((int64_t)k + F8_GROUP - 1) / F8_GROUP); }
 int64_t up_to(int64_t v, int64_t step) { return (v + step - 1) / step * step; }
 
+// `count` of the context's counters, zero between the calls that use them.
+int reserve_marks(sq8_ctx *ctx, int64_t count, int *&marks) {
+    const size_t bytes = (size_t)count * sizeof(int);
+    if (ctx->marks.bytes < bytes) {
+        // New counters are cleared once, and no graph may hold that.
+        if (sq8::capturing(ctx->stream)) return hip_status(hipErrorStreamCaptureUnsupported);
+        const int st = reserve(ctx, ctx->marks, bytes < 65536 ? 65536 : bytes);
+        if (st != SQ8_OK) return st;
+        const hipError_t e = sq8::launch_zero_marks(static_cast<int *>(ctx->marks.at), (int64_t)(ctx->marks.bytes / sizeof(int)), ctx->stream);
+        if (e != hipSuccess) return hip_status(e);
+    } else if (!ctx->marks.in_graph && sq8::capturing(ctx->stream)) {
+        ctx->marks.in_graph = true;
+    }
+    marks = static_cast<int *>(ctx->marks.at);
+    return SQ8_OK;
+}
+
 struct F8Product {
     const void *a; int a_dtype; int64_t lda;    // SQ8_FP8_E4M3: codes with sx; else quantized here
     const float *sx; int64_t ldsx;
@@ -86,6 +103,8 @@ int run_f8(sq8_ctx *ctx, const F8Product &q, double *gpu_seconds) {
         const int st = reserve(ctx, ctx->part, (size_t)plan.part_bytes);
         if (st != SQ8_OK) return st;
         p.part = static_cast<float *>(ctx->part.at);
+        const int counted = reserve_marks(ctx, plan.marks, p.marks);
+        if (counted != SQ8_OK) return counted;
     }
     hipError_t e = hipSuccess;
     if (gpu_seconds) e = hipEventRecord(ctx->begin, ctx->stream);
@@ -276,18 +295,8 @@ int sq8_paged_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_
         st = reserve(ctx, ctx->part, (size_t)bytes);
         if (st != SQ8_OK) return st;
         p.part = static_cast<float *>(ctx->part.at);
-        const size_t marks = (size_t)sq8::paged_marks(p) * sizeof(int);
-        if (ctx->marks.bytes < marks) {
-            // New counters are cleared once, and no graph may hold that.
-            if (sq8::capturing(ctx->stream)) return hip_status(hipErrorStreamCaptureUnsupported);
-            st = reserve(ctx, ctx->marks, marks < 65536 ? 65536 : marks);
-            if (st != SQ8_OK) return st;
-            const hipError_t e = sq8::launch_zero_marks(static_cast<int *>(ctx->marks.at), (int64_t)(ctx->marks.bytes / sizeof(int)), ctx->stream);
-            if (e != hipSuccess) return hip_status(e);
-        } else if (!ctx->marks.in_graph && sq8::capturing(ctx->stream)) {
-            ctx->marks.in_graph = true;
-        }
-        p.marks = static_cast<int *>(ctx->marks.at);
+        st = reserve_marks(ctx, sq8::paged_marks(p), p.marks);
+        if (st != SQ8_OK) return st;
     }
     return hip_status(sq8::launch_paged_attention(p, e4m3, groups, ctx->stream));
 }
