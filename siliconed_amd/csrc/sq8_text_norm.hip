@@ -19,32 +19,40 @@
 namespace sq8 {
 namespace {
 
-// Eight consecutive values from element `at` of a bf16 or fp32 array as fp32; element e of the row is real when
-// col + e < cols (VEC: all of them, and 16-byte aligned).
+// Eight consecutive values from element `at` of a bf16 or fp32 array: as they lie, so that every load of a row is under
+// way before the first is waited for, then as fp32; element e of the row is real when col + e < cols (VEC: all of
+// them, and 16-byte aligned).
+struct Raw8 {
+    u32x4 a, b;  // bf16: a
+};
+
 template <bool VEC>
-__device__ __forceinline__ void load8(const void *base, bool bf16, int64_t at, int col, int cols, float (&v)[8]) {
+__device__ __forceinline__ Raw8 load8(const void *base, bool bf16, int64_t at, int col, int cols) {
+    Raw8 v = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
+    if (col >= cols) return v;
     if constexpr (VEC) {
-        if (bf16) {
-            const u32x4 d = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(base) + at);
+        const uint32_t *src = static_cast<const uint32_t *>(base) + (bf16 ? at >> 1 : at);
+        v.a = *reinterpret_cast<const u32x4 *>(src);
+        if (!bf16) v.b = *reinterpret_cast<const u32x4 *>(src + 4);
+    } else if (bf16) {
+        const uint16_t *src = static_cast<const uint16_t *>(base) + at;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[2 * e] = __uint_as_float(d[e] << 16);
-                v[2 * e + 1] = __uint_as_float(d[e] & 0xFFFF0000u);
-            }
-        } else {
-            const f32x4 *src = reinterpret_cast<const f32x4 *>(static_cast<const float *>(base) + at);
-            const f32x4 a = src[0], b = src[1];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
-        }
+        for (int e = 0; e < 8; ++e)
+            if (col + e < cols) v.a[e >> 1] |= (uint32_t)src[e] << (16 * (e & 1));
     } else {
+        const uint32_t *src = static_cast<const uint32_t *>(base) + at;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[e] = 0.0f;
-            if (col + e < cols)
-                v[e] = bf16 ? __uint_as_float((uint32_t)static_cast<const uint16_t *>(base)[at + e] << 16)
-                            : static_cast<const float *>(base)[at + e];
-        }
+        for (int e = 0; e < 8; ++e)
+            if (col + e < cols) (e < 4 ? v.a : v.b)[e & 3] = src[e];
+    }
+    return v;
+}
+
+__device__ __forceinline__ void widen8(const Raw8 &x, bool bf16, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        v[e] = __uint_as_float(bf16 ? (e & 1 ? x.a[e >> 1] & 0xFFFF0000u : x.a[e >> 1] << 16) : x.a[e]);
+        v[4 + e] = __uint_as_float(bf16 ? (e & 1 ? x.a[2 + (e >> 1)] & 0xFFFF0000u : x.a[2 + (e >> 1)] << 16) : x.b[e]);
     }
 }
 
@@ -148,32 +156,36 @@ __global__ void __launch_bounds__(T) add_norm_kernel(const AddNormArgs p) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
         const int col = 8 * (tid + T * i);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[i][e] = 0.0f;
-        if (col < p.cols) load8<VEC>(p.w, false, col, col, p.cols, w[i]);
+        widen8(load8<VEC>(p.w, false, col, col, p.cols), false, w[i]);
     }
     int turn = 0;
     for (unsigned row = blockIdx.x; row < (unsigned)p.rows; row += gridDim.x, turn ^= 1) {
         float v[IT][8];
+        // All of a row's loads at once, or a thousand threads of 128 registers each, half.
+        constexpr int AT_ONCE = T * IT > 2048 ? IT / 2 : IT;
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
-            const int col = 8 * (tid + T * i);
+        for (int i0 = 0; i0 < IT; i0 += AT_ONCE) {
+            Raw8 x[AT_ONCE], r[AT_ONCE];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
-            if (col < p.cols) load8<VEC>(p.x, p.x_bf16, (int64_t)row * p.ldx + col, col, p.cols, v[i]);
-        }
-        if (p.r) {
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int col = 8 * (tid + T * (i0 + i));
+                x[i] = load8<VEC>(p.x, p.x_bf16, (int64_t)row * p.ldx + col, col, p.cols);
+                if (p.r) r[i] = load8<VEC>(p.r, p.r_bf16, (int64_t)row * p.ldr + col, col, p.cols);
+            }
 #pragma unroll
-            for (int i = 0; i < IT; ++i) {
-                const int col = 8 * (tid + T * i);
-                if (col < p.cols) {
-                    float r[8];
-                    load8<VEC>(p.r, p.r_bf16, (int64_t)row * p.ldr + col, col, p.cols, r);
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int col = 8 * (tid + T * (i0 + i));
+                float (&y)[8] = v[i0 + i];
+                widen8(x[i], p.x_bf16, y);
+                if (p.r) {
+                    float old[8];
+                    widen8(r[i], p.r_bf16, old);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[i][e] = r[e] + v[i][e];
-                    if (p.ro) store8<VEC>(p.ro, p.r_bf16, (int64_t)row * p.ldro + col, col, p.cols, v[i]);
+                    for (int e = 0; e < 8; ++e) y[e] = old[e] + y[e];
+                    if (p.ro && col < p.cols) store8<VEC>(p.ro, p.r_bf16, (int64_t)row * p.ldro + col, col, p.cols, y);
                 }
             }
+            if constexpr (AT_ONCE < IT) __builtin_amdgcn_sched_barrier(0);
         }
         float ss = 0.0f;
 #pragma unroll
@@ -241,8 +253,8 @@ __global__ void __launch_bounds__(256) quantize_groups_kernel(const void *x, boo
     for (unsigned g = blockIdx.x * 16 + (threadIdx.x >> 4); g < total; g += gridDim.x * 16) {
         const unsigned row = g / groups, group = g - row * groups;
         const int col = (int)(group * F8_GROUP + sub * 8);
-        float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        if (col < cols) load8<VEC>(x, x_bf16, (int64_t)row * ldx + col, col, cols, v);
+        float v[8];
+        widen8(load8<VEC>(x, x_bf16, (int64_t)row * ldx + col, col, cols), x_bf16, v);
         const float scale = group_scale(max_of_16(max8(v)));
         if (col < cols) {
             uint32_t lo, hi;
