@@ -418,7 +418,9 @@ int sq8_quantize_groups(sq8_ctx *ctx, const void *x, int x_dtype, int64_t ldx, i
  * SQ8_EPI_NONE, or SQ8_EPI_SILU_GLU (n = 2h, output h: silu(gate)·up): the halves are then blocked each by itself, sw
  * [2·⌈h/128⌉, ⌈k/128⌉], gate's rows first (else SQ8_EUNSUPPORTED). bias fp32 [n] or NULL. C SQ8_BF16 or SQ8_F32, ldc.
  * Codes are read in place where rows are 16-byte aligned and k is a multiple of 16, and copied padded into the
- * context's buffers first where not (sq8_linear says when those grow). `gpu_seconds` as sq8_linear. */
+ * context's buffers first where not (sq8_linear says when those grow). Few rows may have their K split, the parts' sums in
+ * those buffers too, and counters beside them, which the first call that needs more clears: under stream capture that
+ * call is refused, so sizes run once before they are captured. `gpu_seconds` as sq8_linear. */
 int sq8_linear_f8(sq8_ctx *ctx, const void *a, int64_t lda, const float *sx, int64_t ldsx,
                   const void *w, int64_t ldw, const float *sw, int64_t ldsw,
                   const float *bias, int epilogue, void *c, int c_dtype, int64_t ldc,
@@ -462,7 +464,7 @@ int sq8_append_kv(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_he
  * rows may hold anything. Scores, maxima and sums fp32; the probabilities are rounded to bf16 for their product with v.
  * dim up to 256, a multiple of 8 (past 128 and for e4m3: of 16); 16-byte aligned rows (else SQ8_EUNSUPPORTED). Partial
  * results of split sequences go to the context's scratch (sq8_linear says when it grows; its size follows from the
- * arguments here, not from the lengths). */
+ * arguments here, not from the lengths), with sq8_linear_f8's counters. */
 int sq8_paged_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head, const sq8_paged_cache *cache,
                         const int32_t *table, int64_t table_row, int max_pages, const int32_t *lengths,
                         float scale, float softcap, int window,
