@@ -25,6 +25,7 @@
 
 #include "sq8_device.h"
 #include "sq8_text.h"
+#include "sq8_text_quant.h"
 #include "sq8_wdirect_kernel.h"
 
 namespace sq8 {
@@ -114,6 +115,31 @@ __device__ __forceinline__ void store4(const F8Args &p, int row, int col, f32x4 
     store_run<4, F32>(p.c, (int64_t)row * p.ldc + col, p.H - col < 4 ? p.H - col : 4, p.c_vec, y);
 }
 
+// The waves' sums, in their order, and the outputs of TM tiles of 16 rows by NO × 16 columns.
+template <int TM, int NO, int NW, bool GLU, bool F32>
+__device__ __forceinline__ void add_waves(const F8Args &p, f32x4 (*sums)[TM * (GLU ? 2 * NO : NO)][64],
+                                          const f32x4 (&acc)[TM][GLU ? 2 * NO : NO], int m0, int n0, int wave, int lane) {
+    constexpr int NT = GLU ? 2 * NO : NO;
+    const int c = lane & 15, h = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sums[wave][i * NT + j][lane] = acc[i][j];
+    __syncthreads();
+    for (int q = wave; q < TM * NO; q += NW) {
+        const int i = q / NO, j = q - i * NO;
+        f32x4 x[2] = {};
+#pragma unroll
+        for (int half = 0; half < NT / NO; ++half) {
+            f32x4 v = sums[0][i * NT + half * NO + j][lane];
+#pragma unroll
+            for (int g = 1; g < NW; ++g) v += sums[g][i * NT + half * NO + j][lane];
+            x[half] = v;
+        }
+        store4<GLU, F32>(p, m0 + 16 * i + c, n0 + 16 * j + 4 * h, x[0], x[1]);
+    }
+}
+
 // Few rows: a workgroup of NW waves takes NO × 16 output columns (GLU: of both halves) and TM tiles of 16 rows; the
 // waves take the K blocks in turn, both operands straight from memory, U blocks' loads in flight, and add up through
 // LDS.
@@ -181,23 +207,115 @@ __global__ void __launch_bounds__(64 * NW) f8_short_kernel(const F8Args p) {
                 }
         }
     }
+    add_waves<TM, NO, NW, GLU, F32>(p, sums, acc, m0, n0, wave, lane);
+}
+
+// A few rows of values that are still to be quantized: as the short kernel, but the workgroup first makes its rows' codes
+// and scales, GROUPS groups of 128 at most, in LDS, so that no other kernel runs before (a launch is 2.4 µs, among
+// other kernels nearly 5). The rows' loads go first, the weight's next: the codes are made while those are on their way.
+// Then U blocks of the weight are always under way, each asked for when its predecessor is used.
+template <int NO, int U, int GROUPS, bool F32>
+__global__ void __launch_bounds__(512) f8_staged_kernel(const F8Args p) {
+    constexpr int NW = 8, IT = GROUPS / 32;
+    __shared__ __attribute__((aligned(16))) uint8_t staged[GROUPS * F8_GROUP];
+    __shared__ float scales[GROUPS];
+    __shared__ __attribute__((aligned(16))) f32x4 sums[NW][NO][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, h = lane >> 4;
+    const int n0 = blockIdx.x * (16 * NO);
+
+    // ---- the rows' loads: sixteen threads a group, eight values each ----
+    const int groups = p.M * p.KB, sub = threadIdx.x & 15;
+    u32x4 raw[IT];
+    int to[IT];
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) sums[wave][i * NT + j][lane] = acc[i][j];
-    __syncthreads();
-    for (int q = wave; q < TM * NO; q += NW) {
-        const int i = q / NO, j = q - i * NO;
-        f32x4 x[2] = {};
-#pragma unroll
-        for (int half = 0; half < NT / NO; ++half) {
-            f32x4 v = sums[0][i * NT + half * NO + j][lane];
-#pragma unroll
-            for (int g = 1; g < NW; ++g) v += sums[g][i * NT + half * NO + j][lane];
-            x[half] = v;
-        }
-        store4<GLU, F32>(p, m0 + 16 * i + c, n0 + 16 * j + 4 * h, x[0], x[1]);
+    for (int i = 0; i < IT; ++i) {
+        const int g = 32 * i + (int)(threadIdx.x >> 4);
+        raw[i] = u32x4{0, 0, 0, 0};
+        to[i] = 0;
+        if (32 * i >= groups) continue;
+        const int row = g / p.KB, kb = g - row * p.KB, col = kb * F8_GROUP + 8 * sub;
+        to[i] = g * F8_GROUP + (((sub >> 1) ^ (row & 7)) << 4) + 8 * (sub & 1);  // 16-byte runs permuted: rows on other banks
+        if (g < groups && col < p.K) raw[i] = *reinterpret_cast<const u32x4 *>(p.x + row * p.ldx + col);
     }
+
+    // ---- the weight's ----
+    const uint8_t *wrow[NO];
+    const float *sw[NO];
+#pragma unroll
+    for (int j = 0; j < NO; ++j) {
+        wrow[j] = p.w + (int64_t)min(n0 + 16 * j + c, p.H - 1) * p.ldw;
+        sw[j] = p.sw + (int64_t)(min(n0 + 16 * j, p.H - 1) / F8_GROUP) * p.ldsw;
+    }
+    const int mine = p.KB > wave ? (p.KB - wave + NW - 1) / NW : 0;  // this wave's blocks
+    i32x8 w[U][NO];
+    float s_w[U][NO];
+    auto load = [&](auto uc, int n) {
+        constexpr int u = decltype(uc)::value;
+        const int kb = min(wave + n * NW, p.KB - 1);
+#pragma unroll
+        for (int j = 0; j < NO; ++j) {
+            w[u][j] = load_f8(wrow[j], kb, h, p.K);
+            s_w[u][j] = sw[j][kb];
+        }
+    };
+    if (mine > 0) static_for<0, U>([&](auto uc) { load(uc, min((int)decltype(uc)::value, mine - 1)); });
+
+    // ---- the rows' codes ----
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        if (32 * i >= groups) continue;
+        const int g = 32 * i + (int)(threadIdx.x >> 4);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(e & 1 ? raw[i][e >> 1] & 0xFFFF0000u : raw[i][e >> 1] << 16);
+        const float scale = group_scale(max_of_16(max8(v)));
+        uint32_t lo, hi;
+        e4m3_codes(v, scale, lo, hi);
+        if (g < groups) {
+            *reinterpret_cast<u32x2 *>(staged + to[i]) = u32x2{lo, hi};
+            if (sub == 0) scales[g] = scale;
+        }
+    }
+    __syncthreads();
+
+    f32x4 acc[1][NO];
+#pragma unroll
+    for (int j = 0; j < NO; ++j) acc[0][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int row = min(c, p.M - 1), runs[2] = {(h ^ (row & 7)) << 4, ((4 + h) ^ (row & 7)) << 4};
+    auto use = [&](auto uc, int n) {
+        constexpr int u = decltype(uc)::value;
+        const int g = row * p.KB + wave + n * NW;
+        const u32x4 lo = *reinterpret_cast<const u32x4 *>(staged + g * F8_GROUP + runs[0]);
+        const u32x4 hi = *reinterpret_cast<const u32x4 *>(staged + g * F8_GROUP + runs[1]);
+        const i32x8 a = {(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+        const float s_x = scales[g];
+#pragma unroll
+        for (int j = 0; j < NO; ++j) {
+            const f32x4 part = block_sums<F32>(w[u][j], a);
+            const float both = s_x * s_w[u][j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[0][j][e] = __builtin_fmaf(part[e], both, acc[0][j][e]);
+        }
+    };
+    int n = 0;
+    for (; n + 2 * U <= mine; n += U)
+        static_for<0, U>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            use(uc, n + u);
+            load(uc, n + U + u);
+        });
+    static_for<0, U>([&](auto uc) {
+        if (n + (int)decltype(uc)::value < mine) use(uc, n + decltype(uc)::value);
+    });
+    n += U;
+    if (n < mine) {
+        static_for<0, U>([&](auto uc) { load(uc, min(n + (int)decltype(uc)::value, mine - 1)); });
+        static_for<0, U>([&](auto uc) {
+            if (n + (int)decltype(uc)::value < mine) use(uc, n + decltype(uc)::value);
+        });
+    }
+    add_waves<1, NO, NW, false, F32>(p, sums, acc, 0, n0, wave, lane);
 }
 
 // Many rows: tiles of BM rows by BN weight rows (GLU: half of them of each half), WM × WN waves.
@@ -535,6 +653,8 @@ hipError_t launch_tile(const F8Args &p, int splits, hipStream_t stream) {
     return hipGetLastError();
 }
 
+constexpr int kStaged = 128;  // groups of 128 values that the staged kernel takes
+
 template <int TM, int NO, int NW, int U, bool GLU, bool F32>
 hipError_t launch_short(const F8Args &p, hipStream_t stream) {
     const dim3 grid((unsigned)((p.H + 16 * NO - 1) / (16 * NO)), (unsigned)((p.M + 16 * TM - 1) / (16 * TM)));
@@ -558,6 +678,12 @@ constexpr TileCost kTiles[TILES] = {{256, 256, 1, 1.9f, 1.9f, 0.0f, 0.0f},
 // once, for each part, and their bytes.
 constexpr float kLaunch = 3.0f, kBytesMicrosecond = 5.0e6f, kJoin = 0.7f, kJoinPart = 0.5f, kPartMicrosecond = 5.0e6f;
 
+template <int NO, bool F32>
+hipError_t launch_staged(const F8Args &p, hipStream_t stream) {
+    hipLaunchKernelGGL((f8_staged_kernel<NO, 4, kStaged, F32>), dim3((unsigned)((p.H + 16 * NO - 1) / (16 * NO))), dim3(512), 0, stream, p);
+    return hipGetLastError();
+}
+
 template <bool GLU, bool F32>
 hipError_t launch(const F8Args &p, const F8Plan &plan, hipStream_t stream) {
     switch (plan.kernel) {
@@ -567,21 +693,28 @@ hipError_t launch(const F8Args &p, const F8Plan &plan, hipStream_t stream) {
         case 3: return launch_tile<64, 64, 2, 2, 4, GLU, F32>(p, plan.splits, stream);
         case 4: return launch_short<1, 1, 8, 4, GLU, F32>(p, stream);
         case 5: return launch_short<1, 2, 8, 4, GLU, F32>(p, stream);
-        default: return launch_short<4, 1, 8, 2, GLU, F32>(p, stream);
+        default: break;
     }
+    if constexpr (!GLU) {
+        if (plan.kernel == 7) return launch_staged<1, F32>(p, stream);
+        if (plan.kernel == 8) return launch_staged<2, F32>(p, stream);
+    }
+    return launch_short<4, 1, 8, 2, GLU, F32>(p, stream);
 }
 
 }  // namespace
 
 // Up to 16 rows the short kernel: each of its workgroups reads its weight rows and all of A, and a CU takes in a bounded
 // number of bytes a cycle, so 16 or 32 columns a workgroup by the bytes that the fullest CU takes. At M = 16, K = 4096:
-// N = 6144 11.3 µs by 16 and 8.8 by 32, N = 4096 7.1 and 8.7, N = 24576 (GLU) 25.8 and 29.0.
+// N = 6144 11.3 µs by 16 and 8.8 by 32, N = 4096 7.1 and 8.7, N = 24576 (GLU) 25.8 and 29.0. Values of up to kStaged
+// groups are quantized there: one row of K = 4096 by N = 4096 takes 6.6 µs so and 8.2 in two kernels, of K = 12288 15.3
+// and 16.6, four rows of K = 4096 7.4 and 9.6. (GLUs, of three workgroups a CU and more, gain nothing: 25.0 and 24.2.)
 // Above, the tile and the split of K with the least estimated time: rounds of workgroups times steps, not under the
 // time the bytes take. At M = 64, K = 12288, N = 4096: 64 × 64 tiles 37.6 µs whole and 17.5 in four parts; at M = 2048
 // of the same 256 × 256 160 and 128 × 128 120; at M = 8192, K = 4096, N = 24576 752 and 885.
 // Rows too far apart for the tile kernels' 32-bit offsets go to the short kernel.
 F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
-    F8Plan plan = {6, 1, 0, 0};
+    F8Plan plan = {6, 1, 0, 0, false};
     if (p.M <= 0 || p.H <= 0) return plan;
     const int halves = glu ? 2 : 1;
     if (p.M <= 16) {
@@ -589,7 +722,9 @@ F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
             const int64_t groups = (p.H + columns - 1) / columns;
             return ((groups + cus - 1) / cus) * (columns * halves + p.M);
         };
-        plan.kernel = fullest(32) < fullest(16) ? 5 : 4;
+        const bool wide = fullest(32) < fullest(16);
+        plan.values = p.x && !glu && (int64_t)p.M * p.KB <= kStaged;
+        plan.kernel = (plan.values ? 7 : 4) + (wide ? 1 : 0);
         return plan;
     }
     const bool near = 256 * std::max(std::max(p.lda, p.ldw), 4 * p.ldsx) + p.K <= INT32_MAX &&
@@ -612,7 +747,7 @@ F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
             us += kLaunch;
             if (best == 0.0f || us < best) {
                 best = us;
-                plan = F8Plan{t, splits, splits > 1 ? part : 0, splits > 1 ? (int)tiles : 0};
+                plan = F8Plan{t, splits, splits > 1 ? part : 0, splits > 1 ? (int)tiles : 0, false};
             }
         }
     }

@@ -55,13 +55,14 @@ hipError_t launch_pad_bytes(const void *src, int64_t lds, void *dst, int64_t ldd
 struct F8Args {
     const uint8_t *a;       // e4m3 [M, K], rows lda apart, 16-byte aligned rows
     const float *sx;        // [M, KB], rows ldsx apart
+    const uint16_t *x;      // or null; bf16 [M, K], rows ldx apart, 16-byte aligned rows, that a and sx are to be of
     const uint8_t *w;       // e4m3 [N, K], rows ldw apart, 16-byte aligned rows
     const float *sw;        // [⌈N/128⌉ (GLU: 2⌈H/128⌉), KB], rows ldsw apart
     const float *bias;      // [N] or null
     void *c;                // [M, n_out]
     float *part;            // the sums of a split K's parts
     int *marks;             // the tiles' counters of parts that are done, zero between calls
-    int64_t lda, ldsx, ldw, ldsw, ldc;
+    int64_t lda, ldsx, ldx, ldw, ldsw, ldc;
     int M, N, K;            // K a multiple of 16
     int KB;                 // ⌈K/128⌉
     int H;                  // the output's width: N, or N/2 for GLU
@@ -74,6 +75,7 @@ struct F8Plan {
     int kernel, splits;
     int64_t part_bytes;
     int marks;
+    bool values;  // the kernel takes F8Args::x; else a and sx are to be there
 };
 F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus);
 hipError_t launch_f8_product(const F8Args &p, const F8Plan &plan, bool glu, bool out_f32, hipStream_t stream);

@@ -85,11 +85,6 @@ int run_f8(sq8_ctx *ctx, const F8Product &q, double *gpu_seconds) {
     const bool pad_w = q.k > 0 && (ragged || !aligned(q.w, 16) || q.ldw % 16 != 0);
     const bool pad_a = q.k > 0 && !quantize && (ragged || !aligned(q.a, 16) || q.lda % 16 != 0);
     const int64_t scales_row = up_to(kb, 4);
-    if (quantize || pad_a) {
-        const int64_t codes = up_to((int64_t)q.m * kp, 16);
-        const int st = reserve(ctx, ctx->scratch, (size_t)(codes + (quantize ? q.m * scales_row * 4 : 0) + 16));
-        if (st != SQ8_OK) return st;
-    }
     if (pad_w) {
         const int st = reserve(ctx, ctx->wpack, (size_t)(q.n * kp));
         if (st != SQ8_OK) return st;
@@ -98,7 +93,17 @@ int run_f8(sq8_ctx *ctx, const F8Product &q, double *gpu_seconds) {
     if (pad_a) p.lda = kp;
     if (pad_w) p.ldw = kp;
     p.K = (int)kp;
+    if (quantize && q.a_dtype == SQ8_BF16 && !ragged && aligned(q.a, 16) && q.lda % 8 == 0) {
+        p.x = static_cast<const uint16_t *>(q.a);
+        p.ldx = q.lda;
+    }
     const sq8::F8Plan plan = sq8::f8_plan(p, glu, q.c_dtype == SQ8_F32, ctx->cus);
+    const bool pass = quantize && !plan.values && q.k > 0;  // a quantization before the product
+    if (pass || pad_a) {
+        const int64_t codes = up_to((int64_t)q.m * kp, 16);
+        const int st = reserve(ctx, ctx->scratch, (size_t)(codes + (pass ? q.m * scales_row * 4 : 0) + 16));
+        if (st != SQ8_OK) return st;
+    }
     if (plan.part_bytes > 0) {
         const int st = reserve(ctx, ctx->part, (size_t)plan.part_bytes);
         if (st != SQ8_OK) return st;
@@ -109,7 +114,7 @@ int run_f8(sq8_ctx *ctx, const F8Product &q, double *gpu_seconds) {
     hipError_t e = hipSuccess;
     if (gpu_seconds) e = hipEventRecord(ctx->begin, ctx->stream);
     if (e != hipSuccess) return hip_status(e);
-    if (quantize && q.k > 0) {
+    if (pass) {
         uint8_t *codes = static_cast<uint8_t *>(ctx->scratch.at);
         float *scales = reinterpret_cast<float *>(codes + up_to((int64_t)q.m * kp, 16));
         // Codes past k in a row's last run meet the weight's zero codes (its copy is padded with them), but must
