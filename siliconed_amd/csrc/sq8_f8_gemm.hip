@@ -332,11 +332,13 @@ __global__ void __launch_bounds__(512) f8_staged_kernel(const F8Args p) {
 // one burst behind the barrier they held up the small tiles' steps by a seventh), the next step's loads have landed,
 // and its first fragments are read under those instructions too.
 //
-// What bounds it: at M = 8192, K = 4096, N = 24576 (GLU) the 256 × 256 tile's matrix instructions and their power,
-// 757 µs or 2.18 PFLOP/s (a library's product of such codes with one scale a tensor, no GLU: 650). A 64-row tile's step
-// is a chain of a barrier, reads, four to eight matrix instructions a wave and their scaling, 0.36 µs where the
-// instructions alone are 0.06, so few rows want many workgroups: N = 24576 (GLU) has 192 of 64 × 128, 27.6 µs at M = 48
-// (100 MB, 3.7 TB/s), and N = 4096 takes its K in four parts, 10.1 µs at M = 64, K = 4096, and 17.7 at K = 12288.
+// What bounds it: at M = 8192, K = 4096, N = 24576 (GLU) the 256 × 256 tile runs at the card's power limit, 703 to 757 µs
+// or 2.18 to 2.35 PFLOP/s on normal operands and 578 on zeros, its matrix instructions busy for 55 % of the cycles (a
+// library's product of such codes with one scale a tensor, no GLU: 650). A 64-row tile's step is a chain of a barrier, reads, four
+// to eight matrix instructions a wave and their scaling, 0.36 µs where the instructions alone are 0.06, so few rows want
+// many workgroups: N = 24576 (GLU) has 192 of 64 × 128, 27.6 µs at M = 48 (100 MB, 3.7 TB/s), and N = 4096 takes its K in
+// four parts, 10.1 µs at M = 64, K = 4096, and 17.7 at K = 12288. (More waves a tile, sets of waves on K parts of one
+// workgroup, deeper stages and fragments read a whole block ahead took as long or longer.)
 //
 // The weight row an instruction's row stands for is chosen so that a lane ends with consecutive outputs: lane group
 // h, register r of part j is output 4·NTO·h + 4j + r of the wave's (NTO parts wide).
@@ -676,7 +678,7 @@ constexpr TileCost kTiles[TILES] = {{256, 256, 1, 1.9f, 1.9f, 0.0f, 0.0f},
                                     {64, 64, 2, 0.36f, 0.49f, 0.52f, 0.77f}};
 // A launch and its first loads; the weight's bytes at the rate they are read with; adding up the parts of a split K:
 // once, for each part, and their bytes.
-constexpr float kLaunch = 3.0f, kBytesMicrosecond = 5.0e6f, kJoin = 0.7f, kJoinPart = 0.5f, kPartMicrosecond = 5.0e6f;
+constexpr float kLaunch = 3.0f, kBytesMicrosecond = 5.0e6f, kJoin = 1.6f, kJoinPart = 0.5f, kPartMicrosecond = 5.0e6f;
 
 template <int NO, bool F32>
 hipError_t launch_staged(const F8Args &p, hipStream_t stream) {

@@ -25,7 +25,9 @@ __device__ __forceinline__ float bf16_f32(uint32_t bits) { return __uint_as_floa
 //
 // Bound by memory: every value is read once and written once. A thread takes one unit of a token: two runs of W
 // values, the two halves of W pairs (or W values of one run and the next where there is nothing to turn), so a wave
-// reads whole 16-byte runs on both sides (W = 8). W = 1 serves what is not aligned for that.
+// reads whole 16-byte runs on both sides (W = 8). W = 1 serves what is not aligned for that. 8192 tokens of 32 query and
+// 8 key heads of 128 into a bf16 cache (206 MB) take 42.5 µs, 4.8 TB/s where a large copy runs at 5.0; 48 tokens
+// into an e4m3 one 3.2 µs, 2.3 of them the launch.
 template <int W>
 __device__ __forceinline__ void load_run(const uint16_t *src, float (&v)[W]) {
     if constexpr (W == 8) {
@@ -181,6 +183,13 @@ __global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs p) {
 // unnormalised output in each one's slot, and the workgroup that finishes last, as a counter tells it, joins them in
 // tile order: the result does not depend on which one that is. It also sets the counter back to zero, as every call
 // finds it.
+//
+// With 32 query heads on 8 of 128: two sequences of 131 072 tokens in bf16 (1074 MB) take 212 µs, 5.1 TB/s; 48 ragged ones of
+// up to 8192 in e4m3 (414 MB) 100, 4.1 TB/s, of which 13 are the start (the launch, the lengths, the first pages and
+// rows) and the join, and the rest runs at what 128-byte pieces a kilobyte apart come in at (by head [.., kv_heads,
+// page, dim] the same takes 89); one of 777 tokens 8.5, a chain of those latencies. The arithmetic is not felt: without it
+// the loads alone take as long. Neither are more workgroups a CU, or the heads of a sequence going through the same pages
+// at the same time.
 
 constexpr int TILE = 128;   // tokens a workgroup takes at a time
 constexpr int WAVES = 4;
