@@ -351,7 +351,7 @@ struct TileShape {
     static constexpr int STAGE = (BM + BN) * F8_GROUP;
     static constexpr int SCALES = BM * 16;                      // four blocks' scales of the rows
     static constexpr int LDS = NS * STAGE + 2 * SCALES;
-    static constexpr bool SPLIT = NS > 2;                       // K may be split
+    static constexpr bool SPLIT = BM == 64;                       // K may be split
     static_assert(NS <= 4, "two buffers of scales hold the blocks under way");
     static_assert(TM * 16 * WM == BM && TN * 16 * WN == BN && (!GLU || TN % 2 == 0), "whole parts");
     static_assert(NTO == 1 || NTO == 2 || NTO == 4, "a lane's outputs");
@@ -670,15 +670,19 @@ struct TileCost {
     int rows, columns, held;
     float one, all, one_f32, all_f32;
 };
-enum { T_256 = 0, T_128, T_64x128, T_64, TILES };
-// Measured over M 20 to 8192, K 512 to 12288, N 512 to 24576, plain and GLU: within 15 %.
+enum { T_256 = 0, T_128, T_128_ONE, T_64x128, T_64, TILES };
+// T_128_ONE has eight waves and four stages: 33 µs at M = 128, K = 4096, N = 24576 (GLU) where T_128 takes 40 and T_64x128
+// 37.5, while two rounds of it are no match for two workgroups of T_128 a CU (44 µs and 38 at M = 2048, K = N = 4096).
+// Over M 20 to 8192, K 512 to 12288, N 512 to 24576, plain, GLU and fp32 out (28 shapes), the tile and split that these
+// figures choose take at most a tenth longer than the best of all.
 constexpr TileCost kTiles[TILES] = {{256, 256, 1, 1.9f, 1.9f, 0.0f, 0.0f},
                                     {128, 128, 2, 0.85f, 1.36f, 1.25f, 2.2f},
+                                    {128, 128, 1, 0.66f, 0.66f, 1.15f, 1.15f},
                                     {64, 128, 2, 0.47f, 0.82f, 0.78f, 1.29f},
                                     {64, 64, 2, 0.36f, 0.49f, 0.52f, 0.77f}};
-// A launch and its first loads; the weight's bytes at the rate they are read with; adding up the parts of a split K:
-// once, for each part, and their bytes.
-constexpr float kLaunch = 3.0f, kBytesMicrosecond = 5.0e6f, kJoin = 1.6f, kJoinPart = 0.5f, kPartMicrosecond = 5.0e6f;
+// A launch and its first loads; the weight's bytes at the rate they are read with, and those that come into a CU with
+// either operand; adding up the parts of a split K: once, for each part, and their bytes.
+constexpr float kLaunch = 3.0f, kBytesMicrosecond = 5.0e6f, kIntoCU = 45.0e3f, kJoin = 1.6f, kJoinPart = 0.5f, kPartMicrosecond = 5.0e6f;
 
 template <int NO, bool F32>
 hipError_t launch_staged(const F8Args &p, hipStream_t stream) {
@@ -691,15 +695,16 @@ hipError_t launch(const F8Args &p, const F8Plan &plan, hipStream_t stream) {
     switch (plan.kernel) {
         case 0: return launch_tile<256, 256, 2, 4, 2, GLU, false>(p, plan.splits, stream);
         case 1: return launch_tile<128, 128, 2, 2, 2, GLU, F32>(p, plan.splits, stream);
-        case 2: return launch_tile<64, 128, 2, 2, 3, GLU, F32>(p, plan.splits, stream);
-        case 3: return launch_tile<64, 64, 2, 2, 4, GLU, F32>(p, plan.splits, stream);
-        case 4: return launch_short<1, 1, 8, 4, GLU, F32>(p, stream);
-        case 5: return launch_short<1, 2, 8, 4, GLU, F32>(p, stream);
+        case 2: return launch_tile<128, 128, 2, 4, 4, GLU, F32>(p, 1, stream);
+        case 3: return launch_tile<64, 128, 2, 2, 3, GLU, F32>(p, plan.splits, stream);
+        case 4: return launch_tile<64, 64, 2, 2, 4, GLU, F32>(p, plan.splits, stream);
+        case 5: return launch_short<1, 1, 8, 4, GLU, F32>(p, stream);
+        case 6: return launch_short<1, 2, 8, 4, GLU, F32>(p, stream);
         default: break;
     }
     if constexpr (!GLU) {
-        if (plan.kernel == 7) return launch_staged<1, F32>(p, stream);
-        if (plan.kernel == 8) return launch_staged<2, F32>(p, stream);
+        if (plan.kernel == 8) return launch_staged<1, F32>(p, stream);
+        if (plan.kernel == 9) return launch_staged<2, F32>(p, stream);
     }
     return launch_short<4, 1, 8, 2, GLU, F32>(p, stream);
 }
@@ -716,7 +721,7 @@ hipError_t launch(const F8Args &p, const F8Plan &plan, hipStream_t stream) {
 // of the same 256 × 256 160 and 128 × 128 120; at M = 8192, K = 4096, N = 24576 752 and 885.
 // Rows too far apart for the tile kernels' 32-bit offsets go to the short kernel.
 F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
-    F8Plan plan = {6, 1, 0, 0, false};
+    F8Plan plan = {7, 1, 0, 0, false};
     if (p.M <= 0 || p.H <= 0) return plan;
     const int halves = glu ? 2 : 1;
     if (p.M <= 16) {
@@ -726,7 +731,7 @@ F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
         };
         const bool wide = fullest(32) < fullest(16);
         plan.values = p.x && !glu && (int64_t)p.M * p.KB <= kStaged;
-        plan.kernel = (plan.values ? 7 : 4) + (wide ? 1 : 0);
+        plan.kernel = (plan.values ? 8 : 5) + (wide ? 1 : 0);
         return plan;
     }
     const bool near = 256 * std::max(std::max(p.lda, p.ldw), 4 * p.ldsx) + p.K <= INT32_MAX &&
@@ -737,13 +742,14 @@ F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
         const TileCost &c = kTiles[t];
         const int64_t tiles = (int64_t)((p.M + c.rows - 1) / c.rows) * ((p.H * halves + c.columns - 1) / c.columns);
         for (int splits = 1; splits <= 8; ++splits) {
-            if (splits > 1 && (t <= T_128 || p.KB < 4 * splits)) break;
+            if (splits > 1 && (t < T_64x128 || p.KB < 4 * splits)) break;
             const int64_t groups = tiles * splits, slots = (int64_t)cus * c.held, rest = groups % slots;
             const int steps = (p.KB + splits - 1) / splits;
             const float one = out_f32 ? c.one_f32 : c.one, all = out_f32 ? c.all_f32 : c.all;
             const float last = rest == 0 ? 0.0f : rest <= cus ? one : one + (all - one) * (float)(rest - cus) / (float)(slots - cus);
             float us = steps * ((float)(groups / slots) * all + last);
             us = std::max(us, ((float)p.N * p.K + (float)p.M * p.K) / kBytesMicrosecond);
+            us = std::max(us, (float)groups * steps * (float)((c.rows + c.columns) * F8_GROUP) / ((float)std::min<int64_t>(groups, cus) * kIntoCU));
             const int64_t part = groups * c.rows * c.columns * 4;
             if (splits > 1) us += kJoin + kJoinPart * splits + (float)part / kPartMicrosecond;
             us += kLaunch;
