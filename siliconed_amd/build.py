@@ -100,7 +100,10 @@ def _stale(item) -> bool:
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def _bind() -> None:
+def _bind(incremental: bool = False) -> None:
+    deps = (os.path.join(CSRC, "text_bind.cpp"), os.path.join(ROOT, "include", "siliconed_q8.h"))
+    if incremental and os.path.exists(BIND) and all(os.path.getmtime(BIND) >= os.path.getmtime(d) for d in deps):
+        return
     import torch
 
     at = os.path.dirname(torch.__file__)
@@ -116,12 +119,12 @@ def _bind() -> None:
 
 
 def build(verbose: bool = False, incremental: bool = False) -> str:
-    """Compiles the sources and links the library; returns its path. Always recompiles every source,
-    unless `incremental` (then only those whose object is older than the source or a header)."""
+    """Compiles the sources, links the library and builds the host module; returns the library's path. Always
+    recompiles every source, unless `incremental` (then only those whose object is older than the source or a header)."""
     os.makedirs(OBJ, exist_ok=True)
     todo = [it for it in SOURCES if _stale(it)] if incremental else SOURCES
     with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, min(len(todo) + 1, os.cpu_count() or 1))) as pool:
-        bind = pool.submit(_bind)
+        bind = pool.submit(_bind, incremental)
         list(pool.map(_compile, todo))
         bind.result()
     objs = [os.path.join(OBJ, name + ".o") for _, name, _ in SOURCES]
