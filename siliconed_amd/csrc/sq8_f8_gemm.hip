@@ -580,18 +580,19 @@ f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
             // One part of K. Its sums go to its slot, past the caches that workgroups do not share, and the workgroup
             // that a tile's counter finds last adds the slots up, in their order.
             const int splits = gridDim.y, mine = blockIdx.y;
-            float *const slots = p.part + (int64_t)blockIdx.x * splits * (BM * BN) + threadIdx.x;
+            float *const slots = p.part + (int64_t)blockIdx.x * splits * (BM * BN) + 2 * threadIdx.x;
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
                 for (int j = 0; j < TN; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) put(slots + (int64_t)mine * (BM * BN) + ((i * TN + j) * 4 + e) * S::THREADS, acc[i][j][e]);
+                    for (int e = 0; e < 4; e += 2)
+                        put(slots + (int64_t)mine * (BM * BN) + ((i * TN + j) * 4 + e) * S::THREADS, Pair{acc[i][j][e], acc[i][j][e + 1]});
             wd::wait_vmcnt<0>();
             __syncthreads();
             int *const joins = reinterpret_cast<int *>(lds);
             if (threadIdx.x == 0) {
-                int *const mark = p.marks + blockIdx.x;
+                int *const mark = p.marks + (int64_t)blockIdx.x * MARK;
                 const bool last = __hip_atomic_fetch_add(mark, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == splits - 1;
                 if (last) __hip_atomic_store(mark, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 *joins = last;
@@ -609,8 +610,11 @@ f8_tile_kernel(const F8Args p, int tiles_m, int tiles_n) {
 #pragma unroll
                     for (int j = 0; j < TN; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            total[i][j][e] += get(slots + (int64_t)k * (BM * BN) + ((i * TN + j) * 4 + e) * S::THREADS);
+                        for (int e = 0; e < 4; e += 2) {
+                            const Pair x = get(slots + (int64_t)k * (BM * BN) + ((i * TN + j) * 4 + e) * S::THREADS);
+                            total[i][j][e] += x.a;
+                            total[i][j][e + 1] += x.b;
+                        }
             }
 #pragma unroll
             for (int i = 0; i < TM; ++i)
@@ -755,7 +759,7 @@ F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
             us += kLaunch;
             if (best == 0.0f || us < best) {
                 best = us;
-                plan = F8Plan{t, splits, splits > 1 ? part : 0, splits > 1 ? (int)tiles : 0, false};
+                plan = F8Plan{t, splits, splits > 1 ? part : 0, splits > 1 ? tiles * MARK : 0, false};
             }
         }
     }

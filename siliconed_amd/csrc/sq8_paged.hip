@@ -184,12 +184,14 @@ __global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs p) {
 // tile order: the result does not depend on which one that is. It also sets the counter back to zero, as every call
 // finds it.
 //
-// With 32 query heads on 8 of 128: two sequences of 131 072 tokens in bf16 (1074 MB) take 212 µs, 5.1 TB/s; 48 ragged ones of
-// up to 8192 in e4m3 (414 MB) 100, 4.1 TB/s, of which 13 are the start (the launch, the lengths, the first pages and
-// rows) and the join, and the rest runs at what 128-byte pieces a kilobyte apart come in at (by head [.., kv_heads,
-// page, dim] the same takes 89); one of 777 tokens 8.5, a chain of those latencies. The arithmetic is not felt: without it
-// the loads alone take as long. Neither are more workgroups a CU, or the heads of a sequence going through the same pages
-// at the same time.
+// With 32 query heads on 8 of 128: two sequences of 131 072 tokens in bf16 (1074 MB) take 207 to 213 µs, 5.0 to 5.2 TB/s; 48
+// ragged ones of up to 8192 in e4m3 (414 MB) 96, 4.3 TB/s, of which some ten are the start (the launch, the lengths, the first
+// pages and rows) and the join, and the rest runs at what 128-byte pieces a kilobyte apart come in at; one of 777
+// tokens 8.6, a chain of those latencies (6.5 without a join), one of 4096 12.8 and of 16 384 25. The arithmetic is not
+// felt: without it the loads alone take as long. Neither are more workgroups a CU, or the heads of a sequence going through
+// the same pages at the same time. What the join costs is its slots' lines and its counters: with the values of a head's
+// lanes side by side (not by the 16 columns of the products), pairs to a load and a line for each counter the
+// sequence of 4096 went from 15.8 µs to 12.8, the ragged ones from 100 to 96.
 
 constexpr int TILE = 128;   // tokens a workgroup takes at a time
 constexpr int WAVES = 4;
@@ -315,53 +317,58 @@ __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t d) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d, 1.0f, W != 0));
 }
 
-// A slot: maxima [16], sums [16], outputs [dp / 16][4][64] as the first wave's lanes hold them.
+// A slot: maxima and sums [16][2], outputs [dp / 32][4][4][live][2]: pair, register and row of the first wave's lanes, head.
 __host__ __device__ constexpr int part_floats(int dp) { return 32 + 16 * dp; }
 
 // 1 / l, or 0 where nothing was added (a NaN stays one).
 __device__ __forceinline__ float inverse(float l) { return l > 0.0f ? __fdiv_rn(1.0f, l) : l == 0.0f ? 0.0f : l; }
 
 // The results of workgroups g0 .. g1 over one sequence's head, in that order: the first's in slot `slot0`, the others' in
-// 2g (where a workgroup's tiles begin with that sequence's). A thread takes two values of a query head, as neighbours of
-// the lane that wrote them; its loads of eight slots are under way at once.
+// 2g (where a workgroup's tiles begin with that sequence's). A thread takes two values of a query head, side by side in
+// every slot as its neighbours' are; its loads of up to 16 slots are under way at once.
 template <int DP>
 __device__ __forceinline__ void join_slots(const PagedArgs &p, int slot0, int g0, int g1, int live, float v_scale, uint16_t *out) {
-    constexpr int DV = DP / 16;
+    constexpr int DV = DP / 16, ROUND = 16;
     auto slot_of = [&](int g) { return p.part + (int64_t)(g == g0 ? slot0 : 2 * g) * part_floats(DP); };
     // An item a thread: head c, row h of the lanes and register r, values d and d + 1.
     for (int i = threadIdx.x; i < live * 8 * DV; i += 64 * WAVES) {
         const int rest = i / live, c = i - rest * live;
-        const int h = rest & 3, r = rest >> 2 & 3, d = 2 * (rest >> 4);
-        const int lane = 16 * h + c, at = DV * (4 * h + r) + d;
+        const int h = rest & 3, r = rest >> 2 & 3, d = 2 * (rest >> 4), at = DV * (4 * h + r) + d;
         if (at >= p.dim) continue;
         float top = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
-        for (int g = g0; g <= g1; g += 8) {
-            float m[8], n[8], u[8], v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float *slot = slot_of(min(g + e, g1));
-                m[e] = get(slot + c);
-                n[e] = get(slot + 16 + c);
-                u[e] = get(slot + 32 + (4 * d + r) * 64 + lane);
-                v[e] = get(slot + 32 + (4 * d + 4 + r) * 64 + lane);
-            }
+        for (int g = g0; g <= g1; g += ROUND) {
+            Pair s[ROUND], v[ROUND];
             float most = top;
+            static_for<0, ROUND / 8>([&](auto qc) {
+                constexpr int q = 8 * decltype(qc)::value;
+                if (g + q > g1) return;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = fmaxf(most, m[e]);
+                for (int e = q; e < q + 8; ++e) {
+                    const float *slot = slot_of(min(g + e, g1));
+                    s[e] = get(slot + 2 * c);
+                    v[e] = get(slot + 32 + 2 * i);
+                }
+            });
+            static_for<0, ROUND / 8>([&](auto qc) {
+                constexpr int q = 8 * decltype(qc)::value;
+                if (g + q > g1) return;
+#pragma unroll
+                for (int e = q; e < q + 8; ++e) most = fmaxf(most, s[e].a);
+            });
             const float from = most == -INFINITY ? 0.0f : most;
             const float keep = __builtin_amdgcn_exp2f(top - from);
             top = most;
             l *= keep;
             x *= keep;
             y *= keep;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (g + e > g1) break;
-                const float weight = __builtin_amdgcn_exp2f(m[e] - from);
-                l = __builtin_fmaf(n[e], weight, l);
-                x = __builtin_fmaf(u[e], weight, x);
-                y = __builtin_fmaf(v[e], weight, y);
-            }
+            static_for<0, ROUND>([&](auto ec) {
+                constexpr int e = decltype(ec)::value;
+                if (g + e > g1) return;
+                const float weight = __builtin_amdgcn_exp2f(s[e].a - from);
+                l = __builtin_fmaf(s[e].b, weight, l);
+                x = __builtin_fmaf(v[e].a, weight, x);
+                y = __builtin_fmaf(v[e].b, weight, y);
+            });
         }
         const float scale = inverse(l) * v_scale;
         *reinterpret_cast<uint32_t *>(out + c * p.o_head + at) = pack_bf16_rne(x * scale, y * scale);
@@ -677,14 +684,11 @@ __global__ void __launch_bounds__(64 * WAVES, held(DP)) paged_attention_kernel(c
                     }
                 } else {
                     float *slot = p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * part_floats(DP);
-                    if (h == 0) {
-                        put(slot + c, all);
-                        put(slot + 16 + c, l);
-                    }
+                    if (h == 0) put(slot + 2 * c, Pair{all, l});
 #pragma unroll
-                    for (int d = 0; d < DV; ++d)
+                    for (int d = 0; d < DV; d += 2)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) put(slot + 32 + (4 * d + r) * 64 + lane, o[d][r]);
+                        for (int r = 0; r < 4; ++r) put(slot + 32 + 2 * (((2 * d + r) * 4 + h) * live + c), Pair{o[d][r], o[d + 1][r]});
                 }
             }
         }
@@ -714,7 +718,7 @@ __global__ void __launch_bounds__(64 * WAVES, held(DP)) paged_attention_kernel(c
         const Part part = threadIdx.x == 0 ? parts[0] : parts[1];
         bool last = false;
         if (part.tiles != 0) {
-            int *const mark = p.marks + part.b * heads + part.head;
+            int *const mark = p.marks + ((int64_t)part.b * heads + part.head) * MARK;
             const int others = share.of(part.first + part.tiles - 1) - share.of(part.first);
             last = __hip_atomic_fetch_add(mark, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == others;
             if (last) __hip_atomic_store(mark, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -788,7 +792,7 @@ int64_t paged_part_bytes(const PagedArgs &p, int groups) {
     return groups == 1 ? 0 : (int64_t)2 * groups * part_floats(padded_dim(p.dim)) * 4;
 }
 
-int64_t paged_marks(const PagedArgs &p) { return (int64_t)p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16); }
+int64_t paged_marks(const PagedArgs &p) { return (int64_t)MARK * p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16); }
 
 hipError_t launch_zero_marks(int *marks, int64_t count, hipStream_t stream) {
     const int64_t blocks = (count + 255) / 256;

@@ -24,11 +24,22 @@ struct Quotient {
     }
 };
 
+// The counters that tell the last of several workgroups lie a line apart: side by side they held each other up (the
+// attention of two sequences of 8192 took 22 µs, and 18 so).
+constexpr int MARK = 32;
+
 // Partial results lie where every XCD sees them: written and read past its own L2 (agent-scope accesses), so that the
 // workgroup that joins them needs no fence, which would write back and drop that cache under everything still
 // streaming through it (with fences the attention took twice as long at 48 sequences of up to 8192).
-__device__ __forceinline__ void put(float *to, float v) { __hip_atomic_store(to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ float get(const float *from) { return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+struct Pair {
+    float a, b;
+};
+__device__ __forceinline__ void put(float *to, Pair v) {
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(to), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ Pair get(const float *from) {
+    return __builtin_bit_cast(Pair, __hip_atomic_load(reinterpret_cast<const uint64_t *>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
 
 // sq8_text_norm.hip. Element types by flag: bf16 or fp32.
 struct AddNormArgs {
@@ -73,8 +84,7 @@ struct F8Args {
 // Which kernel a product runs on, and the parts its K is split in; part_bytes, marks: what F8Args::part and ::marks need.
 struct F8Plan {
     int kernel, splits;
-    int64_t part_bytes;
-    int marks;
+    int64_t part_bytes, marks;
     bool values;  // the kernel takes F8Args::x; else a and sx are to be there
 };
 F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus);
