@@ -11,7 +11,7 @@ A layer takes and returns (y, x): the branch not yet added, and the fp32 residua
 Weights are e4m3 codes with an fp32 scale per 128 × 128 block, as published (random here); heads of a group share their
 keys and values. `step` runs one new token of each sequence and launches eight kernels (ten past a few sequences, whose
 operands two passes quantize), all of which a HIP graph can hold; `prompt` runs one sequence's first tokens. With the
-sizes below a step's layer takes 78 us for one sequence of 2000 tokens, 104 for 16 and 123 for 64 of 1000; the weights
+sizes below a step's layer takes 76 us for one sequence of 2000 tokens, 103 for 16 and 125 for 64 of 1000; the weights
 alone, 192 MB, are 38.
 
     python -m siliconed_amd.text_block --layers 4 --batch 16 --context 2000
