@@ -398,8 +398,8 @@ int sq8_gated_residual(sq8_ctx *ctx, float *x, int64_t ldx, const void *y, int y
  *   even; scales [rows, ⌈cols/128⌉] with leading dimension lds — sq8_linear_f8's operand;
  *   SQ8_INT8: per row t = max(max|y| / 127, 1e-30) and codes clamp(rint(y / t), −128, 127); scales [rows], lds unused —
  *   sq8_linear_w8a8's operand.
- * w fp32 [cols]; codes [rows, cols] with leading dimension ldq. Any cols to 32 768 (else SQ8_EUNSUPPORTED); rows that
- * are not 16-byte aligned or a multiple of 8 wide are read one value at a time. */
+ * w fp32 [cols]; codes [rows, cols] with leading dimension ldq. Any cols to 32 768 (else SQ8_EUNSUPPORTED), any
+ * alignment of the rows; the values past a row's last whole eight are read one at a time. */
 int sq8_add_norm_quantized(sq8_ctx *ctx, const void *x, int x_dtype, int64_t ldx,
                            const void *residual, int r_dtype, int64_t ldr, void *residual_out, int64_t ldro,
                            const float *w, float eps, void *codes, int codes_dtype, int64_t ldq,

@@ -11,6 +11,7 @@
 
 #include "sq8_device.h"
 #include "sq8_text.h"
+#include "sq8_text_quant.h"
 
 namespace sq8 {
 namespace {
@@ -25,39 +26,47 @@ __device__ __forceinline__ float bf16_f32(uint32_t bits) { return __uint_as_floa
 //
 // Bound by memory: every value is read once and written once. A thread takes one unit of a token: two runs of W
 // values, the two halves of W pairs (or W values of one run and the next where there is nothing to turn), so a wave
-// reads whole 16-byte runs on both sides (W = 8). W = 1 serves what is not aligned for that. 8192 tokens of 32 query and
+// reads whole 16-byte runs on both sides (W = 8, wherever the rows lie; W = 4 where heads or their turned part are no
+// multiple of 16, W = 1 where not of 8). 8192 tokens of 32 query and
 // 8 key heads of 128 into a bf16 cache (206 MB) take 42.5 µs, 4.8 TB/s where a large copy runs at 5.0; 48 tokens
 // into an e4m3 one 3.2 µs, 2.3 of them the launch.
 template <int W>
 __device__ __forceinline__ void load_run(const uint16_t *src, float (&v)[W]) {
-    if constexpr (W == 8) {
-        const u32x4 d = *reinterpret_cast<const u32x4 *>(src);
+    if constexpr (W == 1) {
+        v[0] = bf16_f32(src[0]);
+    } else {
+        typename std::conditional<W == 8, u32x4, u32x2>::type d;
+        if constexpr (W == 8) d = *reinterpret_cast<const u32x4_any *>(src);
+        else d = *reinterpret_cast<const u32x2_any *>(src);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < W / 2; ++e) {
             v[2 * e] = bf16_f32(d[e] & 0xFFFFu);
             v[2 * e + 1] = __uint_as_float(d[e] & 0xFFFF0000u);
         }
-    } else {
-        v[0] = bf16_f32(src[0]);
     }
 }
 
 template <int W>
 __device__ __forceinline__ void load_angles(const float *src, float (&v)[W]) {
-    if constexpr (W == 8) {
-        const f32x4 a = reinterpret_cast<const f32x4 *>(src)[0], b = reinterpret_cast<const f32x4 *>(src)[1];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
-    } else {
+    if constexpr (W == 1) {
         v[0] = src[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) {
+            const u32x4 d = reinterpret_cast<const u32x4_any *>(src)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * i + e] = __uint_as_float(d[e]);
+        }
     }
 }
 
 template <int W>
 __device__ __forceinline__ void store_bf16(uint16_t *dst, const float (&v)[W]) {
     if constexpr (W == 8)
-        *reinterpret_cast<u32x4 *>(dst) = u32x4{pack_bf16_rne(v[0], v[1]), pack_bf16_rne(v[2], v[3]), pack_bf16_rne(v[4], v[5]),
-                                                pack_bf16_rne(v[6], v[7])};
+        *reinterpret_cast<u32x4_any *>(dst) = u32x4{pack_bf16_rne(v[0], v[1]), pack_bf16_rne(v[2], v[3]), pack_bf16_rne(v[4], v[5]),
+                                                    pack_bf16_rne(v[6], v[7])};
+    else if constexpr (W == 4)
+        *reinterpret_cast<u32x2_any *>(dst) = u32x2{pack_bf16_rne(v[0], v[1]), pack_bf16_rne(v[2], v[3])};
     else
         dst[0] = (uint16_t)(pack_bf16_rne(v[0], v[0]) & 0xFFFFu);
 }
@@ -71,12 +80,13 @@ __device__ __forceinline__ void store_e4m3(uint8_t *dst, const float (&v)[W], co
         const float t = fabsf(near) < INFINITY ? by.of(v[e]) : near;
         q[e] = t != t ? t : fminf(fmaxf(t, -448.0f), 448.0f);
     }
-    if constexpr (W == 8) {
-        uint32_t lo = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-        lo = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], (int)lo, true);
-        uint32_t hi = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);
-        hi = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], (int)hi, true);
-        *reinterpret_cast<u32x2 *>(dst) = u32x2{lo, hi};
+    if constexpr (W > 1) {
+        auto four = [&](int e) {
+            const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[e], q[e + 1], 0, false);
+            return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[e + 2], q[e + 3], lo, true);
+        };
+        if constexpr (W == 8) *reinterpret_cast<u32x2_any *>(dst) = u32x2{four(0), four(4)};
+        else *reinterpret_cast<u32_any *>(dst) = four(0);
     } else {
         dst[0] = (uint8_t)((uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[0], 0, false) & 0xFFu);
     }
@@ -757,15 +767,18 @@ hipError_t launch_attention(const PagedArgs &p, int groups, hipStream_t stream) 
 
 }  // namespace
 
-hipError_t launch_append_kv(const AppendArgs &p, bool e4m3, bool vec, hipStream_t stream) {
+hipError_t launch_append_kv(const AppendArgs &p, bool e4m3, hipStream_t stream) {
     if (p.tokens == 0) return hipSuccess;
-    const int64_t units = (int64_t)(p.q_heads + 2 * p.kv_heads) * (p.dim / (vec ? 16 : 2)) * p.tokens;
+    const int run = (p.dim | p.rot) % 16 == 0 ? 8 : (p.dim | p.rot) % 8 == 0 ? 4 : 1;
+    const int64_t units = (int64_t)(p.q_heads + 2 * p.kv_heads) * (p.dim / (2 * run)) * p.tokens;
     const int64_t blocks = (units + 255) / 256;
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks);
-    if (e4m3 && vec) hipLaunchKernelGGL((append_kv_kernel<8, true>), grid, dim3(256), 0, stream, p);
+    if (e4m3 && run == 8) hipLaunchKernelGGL((append_kv_kernel<8, true>), grid, dim3(256), 0, stream, p);
+    else if (e4m3 && run == 4) hipLaunchKernelGGL((append_kv_kernel<4, true>), grid, dim3(256), 0, stream, p);
     else if (e4m3) hipLaunchKernelGGL((append_kv_kernel<1, true>), grid, dim3(256), 0, stream, p);
-    else if (vec) hipLaunchKernelGGL((append_kv_kernel<8, false>), grid, dim3(256), 0, stream, p);
+    else if (run == 8) hipLaunchKernelGGL((append_kv_kernel<8, false>), grid, dim3(256), 0, stream, p);
+    else if (run == 4) hipLaunchKernelGGL((append_kv_kernel<4, false>), grid, dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((append_kv_kernel<1, false>), grid, dim3(256), 0, stream, p);
     return hipGetLastError();
 }

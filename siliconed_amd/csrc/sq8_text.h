@@ -104,7 +104,7 @@ struct AppendArgs {
     int tokens, q_heads, kv_heads, dim, rot, page, max_position;
     int interleaved;
 };
-hipError_t launch_append_kv(const AppendArgs &p, bool e4m3, bool vec, hipStream_t stream);
+hipError_t launch_append_kv(const AppendArgs &p, bool e4m3, hipStream_t stream);
 
 struct PagedArgs {
     const uint16_t *q;                  // bf16 [batch, q_heads, dim]

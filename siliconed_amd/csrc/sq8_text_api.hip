@@ -245,13 +245,7 @@ int sq8_append_kv(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_he
     p.slot_count = (int64_t)cache->pages * cache->page;
     p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = cache->kv_heads; p.dim = cache->dim; p.rot = rot;
     p.page = cache->page; p.max_position = max_position; p.interleaved = interleaved != 0;
-    const int64_t all = q_token | q_head | k_token | k_head | v_token | v_head | qo_token | qo_head | p.kc_page | p.kc_tok |
-                        p.kc_head | p.vc_page | p.vc_tok | p.vc_head;
-    const size_t cache_align = e4m3 ? 8 : 16;
-    const bool vec = cache->dim % 16 == 0 && rot % 16 == 0 && all % 8 == 0 && aligned(q, 16) && aligned(k, 16) && aligned(v, 16) &&
-                     aligned(q_out, 16) && aligned(cache->k, cache_align) && aligned(cache->v, cache_align) &&
-                     (rot == 0 || (aligned(table, 16) && table_row % 4 == 0));
-    const hipError_t e = sq8::launch_append_kv(p, e4m3, vec, ctx->stream);
+    const hipError_t e = sq8::launch_append_kv(p, e4m3, ctx->stream);
     return e == hipErrorInvalidValue ? SQ8_EUNSUPPORTED : hip_status(e);
 }
 

@@ -21,30 +21,28 @@ namespace sq8 {
 namespace {
 
 // Eight consecutive values from element `at` of a bf16 or fp32 array: as they lie, so that every load of a row is under
-// way before the first is waited for, then as fp32; element e of the row is real when col + e < cols (VEC: all of
-// them, and 16-byte aligned).
+// way before the first is waited for, then as fp32; element e of the row is real when col + e < cols (WHOLE: rows are
+// whole runs of eight).
 struct Raw8 {
     u32x4 a, b;  // bf16: a
 };
 
-template <bool VEC>
+template <bool WHOLE>
 __device__ __forceinline__ Raw8 load8(const void *base, bool bf16, int64_t at, int col, int cols) {
     Raw8 v = {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}};
     if (col >= cols) return v;
-    if constexpr (VEC) {
-        const uint32_t *src = static_cast<const uint32_t *>(base) + (bf16 ? at >> 1 : at);
-        v.a = *reinterpret_cast<const u32x4 *>(src);
-        if (!bf16) v.b = *reinterpret_cast<const u32x4 *>(src + 4);
+    const uint8_t *const src = static_cast<const uint8_t *>(base) + at * (bf16 ? 2 : 4);
+    if (WHOLE || col + 8 <= cols) {
+        v.a = *reinterpret_cast<const u32x4_any *>(src);
+        if (!bf16) v.b = *reinterpret_cast<const u32x4_any *>(src + 16);
     } else if (bf16) {
-        const uint16_t *src = static_cast<const uint16_t *>(base) + at;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (col + e < cols) v.a[e >> 1] |= (uint32_t)src[e] << (16 * (e & 1));
+        for (int e = 0; e < 7; ++e)
+            if (col + e < cols) v.a[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(src)[e] << (16 * (e & 1));
     } else {
-        const uint32_t *src = static_cast<const uint32_t *>(base) + at;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (col + e < cols) (e < 4 ? v.a : v.b)[e & 3] = src[e];
+        for (int e = 0; e < 7; ++e)
+            if (col + e < cols) (e < 4 ? v.a : v.b)[e & 3] = reinterpret_cast<const uint32_t *>(src)[e];
     }
     return v;
 }
@@ -57,34 +55,36 @@ __device__ __forceinline__ void widen8(const Raw8 &x, bool bf16, float (&v)[8]) 
     }
 }
 
-template <bool VEC>
+template <bool WHOLE>
 __device__ __forceinline__ void store8(void *base, bool bf16, int64_t at, int col, int cols, const float (&v)[8]) {
-    if constexpr (VEC) {
+    uint8_t *const dst = static_cast<uint8_t *>(base) + at * (bf16 ? 2 : 4);
+    if (WHOLE || col + 8 <= cols) {
         if (bf16) {
-            *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(base) + at) =
+            *reinterpret_cast<u32x4_any *>(dst) =
                 u32x4{pack_bf16_rne(v[0], v[1]), pack_bf16_rne(v[2], v[3]), pack_bf16_rne(v[4], v[5]), pack_bf16_rne(v[6], v[7])};
         } else {
-            f32x4 *dst = reinterpret_cast<f32x4 *>(static_cast<float *>(base) + at);
-            dst[0] = f32x4{v[0], v[1], v[2], v[3]};
-            dst[1] = f32x4{v[4], v[5], v[6], v[7]};
+#pragma unroll
+            for (int e = 0; e < 8; e += 4)
+                *reinterpret_cast<u32x4_any *>(dst + 4 * e) = u32x4{__float_as_uint(v[e]), __float_as_uint(v[e + 1]),
+                                                                    __float_as_uint(v[e + 2]), __float_as_uint(v[e + 3])};
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < 7; ++e)
             if (col + e < cols) {
-                if (bf16) static_cast<uint16_t *>(base)[at + e] = (uint16_t)round_bf16(v[e]);
-                else static_cast<float *>(base)[at + e] = v[e];
+                if (bf16) reinterpret_cast<uint16_t *>(dst)[e] = (uint16_t)round_bf16(v[e]);
+                else reinterpret_cast<float *>(dst)[e] = v[e];
             }
     }
 }
 
-template <bool VEC>
+template <bool WHOLE>
 __device__ __forceinline__ void store_codes8(uint8_t *dst, int col, int cols, uint32_t lo, uint32_t hi) {
-    if constexpr (VEC) {
-        *reinterpret_cast<u32x2 *>(dst) = u32x2{lo, hi};
+    if (WHOLE || col + 8 <= cols) {
+        *reinterpret_cast<u32x2_any *>(dst) = u32x2{lo, hi};
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < 7; ++e)
             if (col + e < cols) dst[e] = (uint8_t)((e < 4 ? lo : hi) >> (8 * (e & 3)));
     }
 }
@@ -118,7 +118,7 @@ __device__ __forceinline__ void int8_codes(const float (&y)[8], float scale, uin
 // Memory bounds long ones: 8192 rows of 4096 on a bf16 stream (236 MB) take 42 to 45 µs, 5.2 to 5.6 TB/s where a large copy
 // runs at 5.0; on an fp32 stream (370 MB) 75. One row takes 3.0 µs, 2.3 of them the launch; the loads of x and r under
 // way together are 0.3 µs of that.
-template <bool INT8, int T, int IT, bool VEC>
+template <bool INT8, int T, int IT, bool WHOLE>
 __global__ void __launch_bounds__(T) add_norm_kernel(const AddNormArgs p) {
     constexpr int WAVES = T / 64;
     __shared__ float sums[2][WAVES], tops[2][WAVES];
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(T) add_norm_kernel(const AddNormArgs p) {
 #pragma unroll
     for (int i = 0; i < IT; ++i) {
         const int col = 8 * (tid + T * i);
-        widen8(load8<VEC>(p.w, false, col, col, p.cols), false, w[i]);
+        widen8(load8<WHOLE>(p.w, false, col, col, p.cols), false, w[i]);
     }
     int turn = 0;
     for (unsigned row = blockIdx.x; row < (unsigned)p.rows; row += gridDim.x, turn ^= 1) {
@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(T) add_norm_kernel(const AddNormArgs p) {
 #pragma unroll
             for (int i = 0; i < AT_ONCE; ++i) {
                 const int col = 8 * (tid + T * (i0 + i));
-                x[i] = load8<VEC>(p.x, p.x_bf16, (int64_t)row * p.ldx + col, col, p.cols);
-                if (p.r) r[i] = load8<VEC>(p.r, p.r_bf16, (int64_t)row * p.ldr + col, col, p.cols);
+                x[i] = load8<WHOLE>(p.x, p.x_bf16, (int64_t)row * p.ldx + col, col, p.cols);
+                if (p.r) r[i] = load8<WHOLE>(p.r, p.r_bf16, (int64_t)row * p.ldr + col, col, p.cols);
             }
 #pragma unroll
             for (int i = 0; i < AT_ONCE; ++i) {
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(T) add_norm_kernel(const AddNormArgs p) {
                     widen8(r[i], p.r_bf16, old);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) y[e] = old[e] + y[e];
-                    if (p.ro && col < p.cols) store8<VEC>(p.ro, p.r_bf16, (int64_t)row * p.ldro + col, col, p.cols, y);
+                    if (p.ro && col < p.cols) store8<WHOLE>(p.ro, p.r_bf16, (int64_t)row * p.ldro + col, col, p.cols, y);
                 }
             }
             if constexpr (AT_ONCE < IT) __builtin_amdgcn_sched_barrier(0);
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(T) add_norm_kernel(const AddNormArgs p) {
                 if (col >= p.cols) break;
                 uint32_t lo, hi;
                 int8_codes(v[i], scale, lo, hi);
-                store_codes8<VEC>(p.codes + (int64_t)row * p.ldq + col, col, p.cols, lo, hi);
+                store_codes8<WHOLE>(p.codes + (int64_t)row * p.ldq + col, col, p.cols, lo, hi);
             }
         } else {
 #pragma unroll
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(T) add_norm_kernel(const AddNormArgs p) {
                 if (col >= p.cols) continue;
                 uint32_t lo, hi;
                 e4m3_codes(v[i], scale, lo, hi);
-                store_codes8<VEC>(p.codes + (int64_t)row * p.ldq + col, col, p.cols, lo, hi);
+                store_codes8<WHOLE>(p.codes + (int64_t)row * p.ldq + col, col, p.cols, lo, hi);
                 if ((tid & 15) == 0) p.scales[(int64_t)row * p.lds + col / F8_GROUP] = scale;
             }
         }
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(T) add_norm_kernel(const AddNormArgs p) {
 
 // Sixteen lanes a group of 128 columns, groups in order over the grid: memory bounds it, 8192 rows of 12288 (305 MB) in
 // 61.7 µs, 4.9 TB/s; 48 rows of 4096 take 2.4 µs, a launch.
-template <bool VEC>
+template <bool WHOLE>
 __global__ void __launch_bounds__(256) quantize_groups_kernel(const void *x, bool x_bf16, int64_t ldx, unsigned total,
                                                               unsigned groups, int cols, uint8_t *codes, int64_t ldq,
                                                               float *scales, int64_t lds) {
@@ -226,45 +226,46 @@ __global__ void __launch_bounds__(256) quantize_groups_kernel(const void *x, boo
         const unsigned row = g / groups, group = g - row * groups;
         const int col = (int)(group * F8_GROUP + sub * 8);
         float v[8];
-        widen8(load8<VEC>(x, x_bf16, (int64_t)row * ldx + col, col, cols), x_bf16, v);
+        widen8(load8<WHOLE>(x, x_bf16, (int64_t)row * ldx + col, col, cols), x_bf16, v);
         const float scale = group_scale(max_of_16(max8(v)));
         if (col < cols) {
             uint32_t lo, hi;
             e4m3_codes(v, scale, lo, hi);
-            store_codes8<VEC>(codes + (int64_t)row * ldq + col, col, cols, lo, hi);
+            store_codes8<WHOLE>(codes + (int64_t)row * ldq + col, col, cols, lo, hi);
         }
         if (sub == 0) scales[(int64_t)row * lds + group] = scale;
     }
 }
 
-// A thread a 4-byte word of the destination.
+// A thread 16 bytes of the destination.
 __global__ void __launch_bounds__(256) pad_bytes_kernel(const uint8_t *src, int64_t lds, uint8_t *dst, int64_t ldd,
-                                                        int64_t words, unsigned row_words, int64_t n) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / row_words;
-        const int64_t at = (i - row * row_words) * 4;
-        uint32_t word = 0;
+                                                        int64_t runs, unsigned row_runs, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < runs; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / row_runs;
+        const int64_t at = (i - row * row_runs) * 16;
+        u32x4 run = {0, 0, 0, 0};
+        if (at + 16 <= n) {
+            run = *reinterpret_cast<const u32x4_any *>(src + row * lds + at);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (at + e < n) word |= (uint32_t)src[row * lds + at + e] << (8 * e);
-        *reinterpret_cast<uint32_t *>(dst + row * ldd + at) = word;
+            for (int e = 0; e < 15; ++e)
+                if (at + e < n) run[e >> 2] |= (uint32_t)src[row * lds + at + e] << (8 * (e & 3));
+        }
+        *reinterpret_cast<u32x4 *>(dst + row * ldd + at) = run;
     }
 }
-
-bool at_16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace
 
 hipError_t launch_add_norm(const AddNormArgs &p, bool int8, int cus, hipStream_t stream) {
     if (p.rows == 0 || p.cols == 0) return hipSuccess;
-    const bool vec = p.cols % 8 == 0 && at_16(p.x) && p.ldx % 8 == 0 && at_16(p.w) && (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0 &&
-                     p.ldq % 8 == 0 && (!p.r || (at_16(p.r) && p.ldr % 8 == 0)) && (!p.ro || (at_16(p.ro) && p.ldro % 8 == 0));
+    const bool whole = p.cols % 8 == 0;
 #define SQ8_ADD_NORM(T, IT)                                                                                          \
     do {                                                                                                             \
         const int most = cus * (2048 / T), grid = p.rows < most ? p.rows : most;                                      \
-        if (int8 && vec) hipLaunchKernelGGL((add_norm_kernel<true, T, IT, true>), dim3(grid), dim3(T), 0, stream, p); \
+        if (int8 && whole) hipLaunchKernelGGL((add_norm_kernel<true, T, IT, true>), dim3(grid), dim3(T), 0, stream, p); \
         else if (int8) hipLaunchKernelGGL((add_norm_kernel<true, T, IT, false>), dim3(grid), dim3(T), 0, stream, p);  \
-        else if (vec) hipLaunchKernelGGL((add_norm_kernel<false, T, IT, true>), dim3(grid), dim3(T), 0, stream, p);   \
+        else if (whole) hipLaunchKernelGGL((add_norm_kernel<false, T, IT, true>), dim3(grid), dim3(T), 0, stream, p);   \
         else hipLaunchKernelGGL((add_norm_kernel<false, T, IT, false>), dim3(grid), dim3(T), 0, stream, p);           \
         return hipGetLastError();                                                                                    \
     } while (0)
@@ -283,10 +284,9 @@ hipError_t launch_quantize_groups(const void *x, bool x_bf16, int64_t ldx, int r
     if (rows == 0 || cols == 0) return hipSuccess;
     const int64_t groups = (cols + F8_GROUP - 1) / F8_GROUP, total = rows * groups;
     if (total > INT32_MAX - 65536 * 16) return hipErrorInvalidValue;
-    const bool vec = cols % 8 == 0 && at_16(x) && ldx % 8 == 0 && (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && ldq % 8 == 0;
     const int64_t want = (total + 15) / 16;
     const dim3 grid((unsigned)(want < 65536 ? want : 65536));
-    if (vec)
+    if (cols % 8 == 0)
         hipLaunchKernelGGL(quantize_groups_kernel<true>, grid, dim3(256), 0, stream, x, x_bf16, ldx, (unsigned)total,
                            (unsigned)groups, cols, codes, ldq, scales, lds);
     else
@@ -298,9 +298,9 @@ hipError_t launch_quantize_groups(const void *x, bool x_bf16, int64_t ldx, int r
 hipError_t launch_pad_bytes(const void *src, int64_t lds, void *dst, int64_t ldd, int64_t rows, int64_t n,
                             hipStream_t stream) {
     if (rows == 0 || ldd == 0) return hipSuccess;
-    const int64_t words = rows * (ldd / 4), want = (words + 255) / 256;
+    const int64_t runs = rows * (ldd / 16), want = (runs + 255) / 256;
     hipLaunchKernelGGL(pad_bytes_kernel, dim3((unsigned)(want < 65536 ? want : 65536)), dim3(256), 0, stream,
-                       static_cast<const uint8_t *>(src), lds, static_cast<uint8_t *>(dst), ldd, words, (unsigned)(ldd / 4), n);
+                       static_cast<const uint8_t *>(src), lds, static_cast<uint8_t *>(dst), ldd, runs, (unsigned)(ldd / 16), n);
     return hipGetLastError();
 }
 
