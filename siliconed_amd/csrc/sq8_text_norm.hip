@@ -8,8 +8,12 @@
 // The sums, the norm and the scales are fp32; s' is rounded to the stream's type only where it is stored, so the
 // norm sees the sum before that rounding. y/s is correctly rounded: an ulp of it decides a code where it lies
 // halfway between two, and among bf16 values that is common (448 = 7 · 64: y = 3·2^j · max|y| is such a
-// tie). It is under 449, which rounds to the largest code: none overflows to NaN. An infinity in a group (e4m3) or
-// row (int8) makes its scale infinite, and its finite values' codes 0.
+// tie). It is under 449, which rounds to the largest code: none overflows to NaN.
+//
+// What is not finite: a NaN y is a NaN e4m3 code, and the other codes of its group are as without it; int8 has no code
+// for one, so a row with a NaN y has a NaN scale, which makes its products NaN. An infinite y makes the scale of its
+// group (e4m3) or row (int8) infinite, and the finite values' codes 0. A NaN s' makes every y of its row NaN, an infinite
+// one itself NaN and the others 0 (1/sqrt is 0 there).
 #include <hip/hip_runtime.h>
 
 #include "sq8_device.h"
@@ -112,6 +116,9 @@ __device__ __forceinline__ void int8_codes(const float (&y)[8], float scale, uin
     }
 }
 
+// The larger of the two, a NaN if either is one (fmaxf would drop it).
+__device__ __forceinline__ float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 // Rows in turn over the grid, T threads a row, each holding IT runs of 8 columns 8·T apart in registers: one read
 // of x and r, w once a workgroup.
 //
@@ -179,18 +186,21 @@ __global__ void __launch_bounds__(T) add_norm_kernel(const AddNormArgs p) {
         for (int i = 0; i < IT; ++i) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[i][e] = (v[i][e] * r) * w[i][e];
-            if constexpr (INT8) top = fmaxf(top, max8(v[i]));
+            if constexpr (INT8) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = max_or_nan(top, fabsf(v[i][e]));
+            }
         }
         if constexpr (INT8) {
 #pragma unroll
-            for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+            for (int o = 32; o >= 1; o >>= 1) top = max_or_nan(top, __shfl_xor(top, o, 64));
             if constexpr (WAVES > 1) {
                 if (lane == 0) tops[turn][wave] = top;
                 __syncthreads();
 #pragma unroll
-                for (int i = 0; i < WAVES; ++i) top = fmaxf(top, tops[turn][i]);
+                for (int i = 0; i < WAVES; ++i) top = max_or_nan(top, tops[turn][i]);
             }
-            const float scale = quant::row_scale(top);
+            const float scale = top != top ? top : quant::row_scale(top);
             if (tid == 0) p.scales[row] = scale;
 #pragma unroll
             for (int i = 0; i < IT; ++i) {
