@@ -458,9 +458,9 @@ int sq8_append_kv(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_he
 
 /* **Attention of one new token per sequence over a paged cache.** o[b, h] = Σ_t softmax_t(s_t) · v_t over tokens t in
  * [max(0, len − window), len) (`window` 0: all) of sequence b, s_t = scale · q·k_t, capped to softcap · tanh(s_t /
- * softcap) unless softcap is 0; query head h reads kv head h / (q_heads / kv_heads). q, out bf16 [batch, q_heads, dim];
- * table int32 [batch, max_pages] (page indices in order; leading dimension table_row), lengths int32 [batch], cut to
- * [0, max_pages · page]. A length of 0 gives zeros; tokens on a page index outside the pools count as masked; masked
+ * softcap) unless softcap is 0 (or infinite: no cap); query head h reads kv head h / (q_heads / kv_heads). q, out bf16
+ * [batch, q_heads, dim]; table int32 [batch, max_pages] (page indices in order; leading dimension table_row), lengths
+ * int32 [batch], cut to [0, max_pages · page]. A length of 0 gives zeros; tokens on a page index outside the pools count as masked; masked
  * rows may hold anything. Scores, maxima and sums fp32; the probabilities are rounded to bf16 for their product with v.
  * dim up to 256, a multiple of 8 (past 128 and for e4m3: of 16); 16-byte aligned rows (else SQ8_EUNSUPPORTED). Partial
  * results of split sequences go to the context's scratch (sq8_linear says when it grows; its size follows from the

@@ -256,6 +256,10 @@ int sq8_paged_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_
     int st = check_cache(cache, q_heads);
     if (st != SQ8_OK) return st;
     if (q_heads % cache->kv_heads != 0) return SQ8_EINVAL;
+    // A cap that no score comes near is none (c · tanh(s / c) is s in fp32, and c · log2(e) may overflow). Capped by less
+    // than 2^-60, every exponential is 1: as good by 2^-60, whose reciprocal does not overflow.
+    if (softcap > 0x1p100f) softcap = 0.0f;
+    else if (softcap > 0.0f && softcap < 0x1p-60f) softcap = 0x1p-60f;
     const bool e4m3 = cache->dtype == SQ8_FP8_E4M3;
     if (cache->dim > 256 || cache->dim % (e4m3 || cache->dim > 128 ? 16 : 8) != 0) return SQ8_EUNSUPPORTED;
     // Token numbers, and the tiles of a batch over its heads, are 32-bit.

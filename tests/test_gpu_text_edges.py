@@ -1,0 +1,45 @@
+"""Arguments at the ends of their ranges: what the attention gives for them is what it gives for the plain value they mean."""
+import math
+
+import pytest
+import torch
+
+import siliconed_amd as sq
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF = torch.bfloat16
+F8 = torch.float8_e4m3fn
+
+
+def held(batch, page, most, heads, dim, dtype=BF, seed=0):
+    """A cache whose pages `table` [batch, most] scatters, and queries of two heads a key head."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    k, v = (torch.randn(batch * most, page, heads, dim, generator=g, device=DEV).to(dtype) for _ in "kv")
+    table = torch.randperm(batch * most, generator=g, device=DEV).to(torch.int32).view(batch, most)
+    q = torch.randn(batch, 2 * heads, dim, generator=g, device=DEV).to(BF)
+    return sq.PagedCache(k, v), table, q
+
+
+def lengths(*n):
+    return torch.tensor(n, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("dtype", [BF, F8], ids=["bf16", "e4m3"])
+def test_a_cap_that_no_score_comes_near_is_none(gemm, dtype):
+    cache, table, q = held(3, 16, 20, 2, 64, dtype)
+    n = lengths(300, 1, 0)
+    want = gemm.paged_attention(q, cache, table, n)
+    for cap in (math.inf, 3.4e38, 1e31):
+        assert torch.equal(gemm.paged_attention(q, cache, table, n, softcap=cap), want), cap
+    # Just inside: the formula's own value, s to a relative 2^-22 for |s| < 30, whose exponential is within 2^-16.
+    near = gemm.paged_attention(q, cache, table, n, softcap=1e30)
+    assert ((near.double() - want.double()).abs() <= 2.0 ** -7 * want.double().abs() + 2.0 ** -15 * 5).all()
+
+
+def test_a_cap_of_nothing_averages(gemm):
+    """Scores within 1e-20 of 0: every exponential is 1 in fp32, and the output the values' mean."""
+    cache, table, q = held(2, 16, 8, 1, 64)
+    want = gemm.paged_attention(q, cache, table, lengths(100, 3), scale=0.0)
+    for cap in (1e-20, 1e-39, 1e-45):
+        assert torch.equal(gemm.paged_attention(q, cache, table, lengths(100, 3), softcap=cap), want), cap
