@@ -55,6 +55,7 @@ SOURCES = [
     ("sq8_text_norm.hip", "sq8_text_norm", []),
     ("sq8_f8_gemm.hip", "sq8_f8_gemm", []),
     ("sq8_paged.hip", "sq8_paged", []),
+    ("sq8_text_plan.hip", "sq8_text_plan", []),
     ("sq8_text_api.hip", "sq8_text_api", []),
     ("sq8_api.hip", "sq8_api", []),
 ]

@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs p) {
 // lanes side by side (not by the 16 columns of the products), pairs to a load and a line for each counter the
 // sequence of 4096 went from 15.8 µs to 12.8, the ragged ones from 100 to 96.
 
-constexpr int TILE = 128;   // tokens a workgroup takes at a time
+constexpr int TILE = PAGED_TILE;
 constexpr int WAVES = 4;
 
 // Token / tokens a page, by a multiplication (page_divisor).
@@ -327,9 +327,6 @@ __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t d) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d, 1.0f, W != 0));
 }
 
-// A slot: maxima and sums [16][2], outputs [dp / 32][4][4][live][2]: pair, register and row of the first wave's lanes, head.
-__host__ __device__ constexpr int part_floats(int dp) { return 32 + 16 * dp; }
-
 // 1 / l, or 0 where nothing was added (a NaN stays one).
 __device__ __forceinline__ float inverse(float l) { return l > 0.0f ? __fdiv_rn(1.0f, l) : l == 0.0f ? 0.0f : l; }
 
@@ -339,7 +336,7 @@ __device__ __forceinline__ float inverse(float l) { return l > 0.0f ? __fdiv_rn(
 template <int DP>
 __device__ __forceinline__ void join_slots(const PagedArgs &p, int slot0, int g0, int g1, int live, float v_scale, uint16_t *out) {
     constexpr int DV = DP / 16, ROUND = 16;
-    auto slot_of = [&](int g) { return p.part + (int64_t)(g == g0 ? slot0 : 2 * g) * part_floats(DP); };
+    auto slot_of = [&](int g) { return p.part + (int64_t)(g == g0 ? slot0 : 2 * g) * paged_part_floats(DP); };
     // An item a thread: head c, row h of the lanes and register r, values d and d + 1.
     for (int i = threadIdx.x; i < live * 8 * DV; i += 64 * WAVES) {
         const int rest = i / live, c = i - rest * live;
@@ -385,11 +382,8 @@ __device__ __forceinline__ void join_slots(const PagedArgs &p, int slot0, int g0
     }
 }
 
-// Workgroups a CU holds (by their registers).
-constexpr int held(int dp) { return dp <= 128 ? 2 : 1; }
-
 template <int DP, bool E4M3, bool PAGE16>
-__global__ void __launch_bounds__(64 * WAVES, held(DP)) paged_attention_kernel(const PagedArgs p) {
+__global__ void __launch_bounds__(64 * WAVES, paged_held(DP)) paged_attention_kernel(const PagedArgs p) {
     constexpr int ES = E4M3 ? 1 : 2;
     constexpr int STEPS = DP / 32;                // MFMAs of a 16-token tile's scores
     constexpr int KRUNS = DP * ES / 64;           // 16-byte runs of a key a lane reads
@@ -693,7 +687,7 @@ __global__ void __launch_bounds__(64 * WAVES, held(DP)) paged_attention_kernel(c
                             *reinterpret_cast<uint32_t *>(dst + at + d) = pack_bf16_rne(o[d][r] * scale, o[d + 1][r] * scale);
                     }
                 } else {
-                    float *slot = p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * part_floats(DP);
+                    float *slot = p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * paged_part_floats(DP);
                     if (h == 0) put(slot + 2 * c, Pair{all, l});
 #pragma unroll
                     for (int d = 0; d < DV; d += 2)
@@ -754,8 +748,6 @@ __global__ void __launch_bounds__(256) zero_marks_kernel(int *marks, int64_t cou
 // Whether 16-token tiles lie in one page each, and a lane's offsets within one in 32 bits.
 bool by_pages(const PagedArgs &p) { return p.page % 16 == 0 && 32 * std::max(p.kc_tok, p.vc_tok) <= INT32_MAX; }
 
-int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-
 template <int DP, bool E4M3>
 hipError_t launch_attention(const PagedArgs &p, int groups, hipStream_t stream) {
     if (by_pages(p))
@@ -783,30 +775,6 @@ hipError_t launch_append_kv(const AppendArgs &p, bool e4m3, hipStream_t stream) 
     return hipGetLastError();
 }
 
-// n / page for n < 2^31 as (n · mul) >> shift: s with 2^(s-1) < page ≤ 2^s, mul = floor(2^(31+s) / page) + 1 ≤ 2^32 + 1,
-// the product's excess under n / 2^(31+s) < 2^-s ≤ 1/page.
-void page_divisor(PagedArgs &p) {
-    int s = 0;
-    while ((1ll << s) < p.page) ++s;
-    p.page_shift = 31 + s;
-    p.page_mul = ((1ull << (31 + s)) / (uint64_t)p.page) + 1;
-}
-
-int paged_groups(const PagedArgs &p, int cus) {
-    const int passes = (p.q_heads / p.kv_heads + 15) / 16;
-    int64_t tokens = (int64_t)p.max_pages * p.page;
-    if (p.window > 0 && tokens > p.window + 31) tokens = p.window + 31;
-    const int64_t most = (int64_t)p.batch * p.kv_heads * passes * ((tokens + TILE - 1) / TILE);
-    const int64_t full = held(padded_dim(p.dim)) * (int64_t)cus;
-    return (int)(most < 1 ? 1 : most < full ? most : full);
-}
-
-int64_t paged_part_bytes(const PagedArgs &p, int groups) {
-    return groups == 1 ? 0 : (int64_t)2 * groups * part_floats(padded_dim(p.dim)) * 4;
-}
-
-int64_t paged_marks(const PagedArgs &p) { return (int64_t)MARK * p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16); }
-
 hipError_t launch_zero_marks(int *marks, int64_t count, hipStream_t stream) {
     const int64_t blocks = (count + 255) / 256;
     hipLaunchKernelGGL(zero_marks_kernel, dim3((unsigned)(blocks < 1024 ? blocks : 1024)), dim3(256), 0, stream, marks, count);
@@ -815,7 +783,7 @@ hipError_t launch_zero_marks(int *marks, int64_t count, hipStream_t stream) {
 
 hipError_t launch_paged_attention(const PagedArgs &p, bool e4m3, int groups, hipStream_t stream) {
     if (p.batch == 0) return hipSuccess;
-    switch (padded_dim(p.dim)) {
+    switch (paged_dim(p.dim)) {
         case 64: return e4m3 ? launch_attention<64, true>(p, groups, stream) : launch_attention<64, false>(p, groups, stream);
         case 128: return e4m3 ? launch_attention<128, true>(p, groups, stream) : launch_attention<128, false>(p, groups, stream);
         default: return e4m3 ? launch_attention<256, true>(p, groups, stream) : launch_attention<256, false>(p, groups, stream);

@@ -81,7 +81,12 @@ struct F8Args {
     int c_vec;              // outputs a store may take: 8 or 4 (aligned base and rows), 0 for one at a time
     int sx_vec;             // four scales a load allowed (rows of whole fours)
 };
-// Which kernel a product runs on, and the parts its K is split in; part_bytes, marks: what F8Args::part and ::marks need.
+// A product's kernels: the tiles (F8_128_ONE: one workgroup a CU), the short kernel of 16 and of 32 columns, rows too far
+// apart for the tiles' offsets, and the short kernel that quantizes its values, of 16 and of 32 columns.
+enum { F8_256 = 0, F8_128, F8_128_ONE, F8_64x128, F8_64, F8_TILES, F8_SHORT = F8_TILES, F8_SHORT_WIDE, F8_FAR, F8_STAGED, F8_STAGED_WIDE };
+constexpr int F8_STAGED_GROUPS = 128;  // groups of 128 values that the staged kernel takes
+// sq8_text_plan.hip. Which kernel a product runs on, and the parts its K is split in; part_bytes, marks: what F8Args::part
+// and ::marks need.
 struct F8Plan {
     int kernel, splits;
     int64_t part_bytes, marks;
@@ -122,6 +127,12 @@ struct PagedArgs {
     uint64_t page_mul;                  // page_divisor()'s
     int page_shift;
 };
+constexpr int PAGED_TILE = 128;  // tokens a workgroup takes at a time
+constexpr int paged_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }  // the instance of a head's size
+constexpr int paged_held(int dp) { return dp <= 128 ? 2 : 1; }                        // workgroups a CU holds (by their registers)
+// A slot: maxima and sums [16][2], outputs [dp / 32][4][4][live][2]: pair, register and row of the first wave's lanes, head.
+__host__ __device__ constexpr int paged_part_floats(int dp) { return 32 + 16 * dp; }
+// sq8_text_plan.hip.
 void page_divisor(PagedArgs &p);
 // The workgroups a call of these sizes takes, and the partial results' bytes they need.
 int paged_groups(const PagedArgs &p, int cus);
