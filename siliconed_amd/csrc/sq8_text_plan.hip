@@ -93,7 +93,7 @@ void page_divisor(PagedArgs &p) {
 int paged_groups(const PagedArgs &p, int cus) {
     const int passes = (p.q_heads / p.kv_heads + 15) / 16;
     int64_t tokens = (int64_t)p.max_pages * p.page;
-    if (p.window > 0 && tokens > p.window + 31) tokens = p.window + 31;
+    if (p.window > 0) tokens = std::min<int64_t>(tokens, (int64_t)p.window + 31);  // (the window may be the largest int)
     const int64_t most = (int64_t)p.batch * p.kv_heads * passes * ((tokens + PAGED_TILE - 1) / PAGED_TILE);
     const int64_t full = paged_held(paged_dim(p.dim)) * (int64_t)cus;
     return (int)(most < 1 ? 1 : most < full ? most : full);

@@ -43,3 +43,13 @@ def test_a_cap_of_nothing_averages(gemm):
     want = gemm.paged_attention(q, cache, table, lengths(100, 3), scale=0.0)
     for cap in (1e-20, 1e-39, 1e-45):
         assert torch.equal(gemm.paged_attention(q, cache, table, lengths(100, 3), softcap=cap), want), cap
+
+
+@pytest.mark.parametrize("dtype", [BF, F8], ids=["bf16", "e4m3"])
+def test_a_window_past_every_length_is_none(gemm, dtype):
+    """Up to the largest int, the usual "no window"; the work is split as without one, so the bits are the same."""
+    cache, table, q = held(2, 16, 300, 1, 128, dtype)
+    n = lengths(4777, 130)
+    want = gemm.paged_attention(q, cache, table, n)
+    for window in (2 ** 31 - 1, 2 ** 31 - 31, 2 ** 31 - 32, 2 ** 30):
+        assert torch.equal(gemm.paged_attention(q, cache, table, n, window=window), want), window

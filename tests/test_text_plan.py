@@ -75,3 +75,17 @@ def test_short_products(plan):
     assert plan(1, 4096, 4096, values=True) == "staged/1" and plan(1, 4096, 6144, values=True) == "staged wide/1"
     assert plan(1, 16385, 4096, values=True) == "short/1" and plan(17, 128, 128, values=True) == "64/1"
     assert plan(4, 4096, 24576, glu=True, values=True) == "short/1"
+
+
+def test_windows_past_the_table_change_nothing(ask):
+    for case in ((2, 2, 1, 128, 16, 300), (1, 32, 8, 128, 64, 2048), (48, 40, 8, 64, 1, 100)):
+        want = int(ask("a", *case, 0))
+        assert want > 1
+        for window in (2 ** 31 - 1, 2 ** 31 - 31, 2 ** 31 - 32, 2 ** 30):
+            assert int(ask("a", *case, window)) == want, window
+
+
+def test_a_window_bounds_the_workgroups(ask):
+    assert ask("a", 1, 8, 1, 128, 16, 1000, 128) == "2"  # 159 tokens at most: two tiles
+    assert ask("a", 1, 8, 1, 128, 16, 1000, 1) == "1"
+    assert ask("a", 3, 8, 2, 128, 16, 0, 0) == "1"
