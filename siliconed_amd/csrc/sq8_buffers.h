@@ -64,6 +64,18 @@ inline void release(Buffer &b) {
     b = Buffer{nullptr, 0, false};
 }
 
+// reserve for counters, which calls find and leave at zero: new ones, `least` bytes or more, are cleared by clear(memory,
+// bytes), queued on the stream. Memory that could not be cleared is given back: the next call would take it for clean.
+// No graph may hold the clearing, so under capture `b` has to have grown before.
+template <typename Clear>
+hipError_t reserve_cleared(Buffer &b, size_t bytes, size_t least, hipStream_t stream, SetAside *&aside, Clear &&clear) {
+    if (b.bytes >= bytes) return reserve(b, bytes, stream, aside);
+    if (capturing(stream)) return hipErrorStreamCaptureUnsupported;
+    hipError_t e = reserve(b, bytes < least ? least : bytes, stream, aside);
+    if (e == hipSuccess && (e = clear(b.at, b.bytes)) != hipSuccess) release(b);
+    return e;
+}
+
 inline void release(SetAside *&aside) {
     while (aside) {
         SetAside *next = aside->next;

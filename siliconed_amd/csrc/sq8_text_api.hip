@@ -23,17 +23,10 @@ int64_t up_to(int64_t v, int64_t step) { return (v + step - 1) / step * step; }
 
 // `count` of the context's counters, zero between the calls that use them.
 int reserve_marks(sq8_ctx *ctx, int64_t count, int *&marks) {
-    const size_t bytes = (size_t)count * sizeof(int);
-    if (ctx->marks.bytes < bytes) {
-        // New counters are cleared once, and no graph may hold that.
-        if (sq8::capturing(ctx->stream)) return hip_status(hipErrorStreamCaptureUnsupported);
-        const int st = reserve(ctx, ctx->marks, bytes < 65536 ? 65536 : bytes);
-        if (st != SQ8_OK) return st;
-        const hipError_t e = sq8::launch_zero_marks(static_cast<int *>(ctx->marks.at), (int64_t)(ctx->marks.bytes / sizeof(int)), ctx->stream);
-        if (e != hipSuccess) return hip_status(e);
-    } else if (!ctx->marks.in_graph && sq8::capturing(ctx->stream)) {
-        ctx->marks.in_graph = true;
-    }
+    const hipError_t e = sq8::reserve_cleared(ctx->marks, (size_t)count * sizeof(int), 65536, ctx->stream, ctx->aside, [&](void *at, size_t bytes) {
+        return sq8::launch_zero_marks(static_cast<int *>(at), (int64_t)(bytes / sizeof(int)), ctx->stream);
+    });
+    if (e != hipSuccess) return hip_status(e);
     marks = static_cast<int *>(ctx->marks.at);
     return SQ8_OK;
 }
