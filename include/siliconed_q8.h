@@ -105,6 +105,9 @@ int sq8_destroy(sq8_ctx *ctx);
  * Replaces: the command queue passed at init (TensorGEMM.swift:206). */
 int sq8_set_stream(sq8_ctx *ctx, void *stream);
 
+/* The GPU of a context; -1 for a null one. Every address a call is given lies there. */
+int sq8_device(const sq8_ctx *ctx);
+
 /* 0 when `sq8_linear` runs this combination, else SQ8_EUNSUPPORTED / SQ8_EINVAL — the caller then
  * keeps the widened route. Replaces: the nil checks on `TensorGEMM.rounded`/`.int8`
  * (TensorGEMM.swift:218-229, `roundsActivations`, `readsBlocks`). */

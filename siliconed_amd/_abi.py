@@ -85,6 +85,7 @@ SIGNATURES = {
                            ctypes.POINTER(PagedCacheArgs), _P, _P, _P, _I64, _I, _I, _I, _I, _I]),
     "sq8_paged_attention": (_I, [_P, _P, _I64, _I64, ctypes.POINTER(PagedCacheArgs), _P, _I64, _I, _P, ctypes.c_float,
                                  ctypes.c_float, _I, _P, _I64, _I64, _I, _I]),
+    "sq8_device": (_I, [_P]),
     "sq8_synchronize": (_I, [_P]),
     "sq8_status_string": (ctypes.c_char_p, [_I]),
     "sq8_abi_version": (_I, []),
@@ -92,7 +93,7 @@ SIGNATURES = {
 
 # The entries that text_bind.cpp calls, in the order of its Entries.
 TEXT_ENTRIES = ("sq8_add_norm_quantized", "sq8_quantize_groups", "sq8_linear_f8", "sq8_linear_f8_quantized",
-                "sq8_append_kv", "sq8_paged_attention")
+                "sq8_append_kv", "sq8_paged_attention", "sq8_device")
 
 _lib = None
 text = None  # the text decoder's operators' native calls (text_bind.cpp), once the library is loaded

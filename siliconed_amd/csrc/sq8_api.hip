@@ -820,6 +820,8 @@ int sq8_set_stream(sq8_ctx *ctx, void *stream) {
     return SQ8_OK;
 }
 
+int sq8_device(const sq8_ctx *ctx) { return ctx ? ctx->device : -1; }
+
 int sq8_supports(const sq8_ctx *ctx, int a_dtype, int w_dtype, int w_layout, int scale_layout, int c_dtype,
                  int epilogue) {
     if (!ctx) return SQ8_EINVAL;

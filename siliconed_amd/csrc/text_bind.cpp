@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <type_traits>
 #include <utility>
 
@@ -30,6 +31,7 @@ struct Entries {
     decltype(&sq8_linear_f8_quantized) linear_f8_quantized;
     decltype(&sq8_append_kv) append_kv;
     decltype(&sq8_paged_attention) paged_attention;
+    decltype(&sq8_device) device;
 } entries;
 
 constexpr int64_t kGroup = 128;  // values of K that share a scale
@@ -108,6 +110,20 @@ T held(PyObject *o, const char *what) {
     return value;
 }
 sq8_ctx *context(PyObject *o) { return o == Py_None ? nullptr : held<sq8_ctx *>(o, "a context"); }
+
+// A call's tensors lie on the context's GPU: the kernels would fault on another's addresses. (A null context is the
+// library's to refuse.)
+struct Named {
+    const Tensor *t;
+    const char *what;
+};
+void on_device(const sq8_ctx *ctx, std::initializer_list<Named> all) {
+    if (!ctx) return;
+    const int device = entries.device(ctx);
+    for (const Named &n : all)
+        TORCH_CHECK_VALUE(!n.t || n.t->get_device() == device, n.what, " must be on the context's GPU, cuda:", device, ", not ",
+                          n.t->device());
+}
 
 double number(PyObject *o) {
     const double v = PyFloat_AsDouble(o);
@@ -190,6 +206,7 @@ PyObject *add_norm_quantized(PyObject *, PyObject *const *a, Py_ssize_t n) {
     }
     const float *const weights = vector_of<float>(w, cols, "w");
     const int x_type = activation(x, "x"), r32 = count32(rows, "x"), c32 = count32(cols, "x");
+    on_device(ctx, {{&x, "x"}, {&w, "w"}, {residual, "residual"}, {residual_out, "residual_out"}, {&codes, "codes"}, {&scales, "scales"}});
     const int status = call([&] {
         return entries.add_norm_quantized(ctx, x.data_ptr(), x_type, ldx, r, r_type, ldr, ro, ldro, weights, eps, codes.data_ptr(),
                                           int8 ? SQ8_INT8 : SQ8_FP8_E4M3, ldq, static_cast<float *>(scales.data_ptr()), lds, r32, c32);
@@ -216,6 +233,7 @@ PyObject *quantize_groups(PyObject *, PyObject *const *a, Py_ssize_t n) {
     TORCH_CHECK_VALUE(codes.scalar_type() == kF8 && scales.scalar_type() == at::kFloat, "codes must be float8_e4m3fn, scales float32");
     const int64_t ldq = rows_of(codes, "codes", rows, cols), lds = rows_of(scales, "scales", rows, groups(cols));
     const int x_type = activation(x, "x"), r32 = count32(rows, "x"), c32 = count32(cols, "x");
+    on_device(ctx, {{&x, "x"}, {&codes, "codes"}, {&scales, "scales"}});
     const int status = call([&] {
         return entries.quantize_groups(ctx, x.data_ptr(), x_type, ldx, r32, c32, codes.data_ptr(), ldq,
                                        static_cast<float *>(scales.data_ptr()), lds);
@@ -259,6 +277,7 @@ PyObject *product_f8(PyObject *, PyObject *const *a, Py_ssize_t n) {
     double seconds = 0.0, *const at = timed ? &seconds : nullptr;
     const uint8_t *const codes = static_cast<const uint8_t *>(w.data_ptr());
     const float *const sw = static_cast<const float *>(scale.data_ptr());
+    on_device(ctx, {{&x, "the activation"}, {sx, "sx"}, {&w, "w"}, {&scale, "scale"}, {bias, "bias"}, {&out, "out"}});
     const int status = call([&] {
         return sx ? entries.linear_f8(ctx, x.data_ptr(), lda, static_cast<const float *>(sx->data_ptr()), ldsx, codes, ldw, sw, lds, b,
                                       epilogue, out.data_ptr(), c_type, ldc, m32, k32, n32, at)
@@ -288,6 +307,7 @@ PyObject *append_kv(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int32_t *const at = vector_of<int32_t>(positions, tokens, "positions"), *const to = vector_of<int32_t>(slots, tokens, "slots");
     const int most = count32(table.size(0), "table"), rot = count32(table.size(1), "table"), interleaved = truth(a[9]);
     const int t32 = count32(tokens, "q"), h32 = count32(heads, "q");
+    on_device(ctx, {{&q, "q"}, {&k, "k"}, {&v, "v"}, {&positions, "positions"}, {&slots, "slots"}, {&table, "table"}, {&out, "q_out"}});
     const int status = call([&] {
         return entries.append_kv(ctx, qh.at, qh.row, qh.head, kh.at, kh.row, kh.head, vh.at, vh.row, vh.head, oh.at, oh.row, oh.head,
                                  &cache, at, to, static_cast<const float *>(table.data_ptr()), row, most, rot, interleaved, t32, h32);
@@ -313,6 +333,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int32_t *const held_tokens = vector_of<int32_t>(lengths, batch, "lengths");
     const float scale = (float)(a[5] == Py_None ? 1.0 / std::sqrt((double)cache.dim) : number(a[5])), softcap = (float)number(a[6]);
     const int window = integer(a[7]), most = count32(pages.size(1), "pages"), b32 = count32(batch, "q"), h32 = count32(heads, "q");
+    on_device(ctx, {{&q, "q"}, {&pages, "pages"}, {&lengths, "lengths"}, {&out, "out"}});
     const int status = call([&] {
         return entries.paged_attention(ctx, qh.at, qh.row, qh.head, &cache, static_cast<const int32_t *>(pages.data_ptr()), row, most,
                                        held_tokens, scale, softcap, window, oh.at, oh.row, oh.head, b32, h32);

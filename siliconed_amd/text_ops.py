@@ -22,12 +22,12 @@ _CACHES = {torch.bfloat16: abi.BF16, _F8: abi.FP8_E4M3}
 _EPILOGUES = {None: False, "none": False, "silu_glu": True, "swiglu": True}  # True: a GLU
 
 
-def _vector(t: Optional[torch.Tensor], count: int, what: str):
+def _vector(t: Optional[torch.Tensor], count: int, what: str, device: torch.device):
     """A contiguous fp32 vector's address (None: null)."""
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.numel() != count or not t.is_contiguous() or not t.is_cuda:
-        raise ValueError(f"{what} must be {count} contiguous float32 values on the GPU")
+    if t.dtype != torch.float32 or t.numel() != count or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{what} must be {count} contiguous float32 values on {device}")
     return t.data_ptr()
 
 
@@ -70,10 +70,10 @@ class PagedCache:
         if dtype == abi.BF16 and (k_scale is not None or v_scale is not None):
             raise ValueError("scales belong to float8_e4m3fn pools")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.pages, self.page, self.kv_heads, self.dim = pages, page, heads, dim
+        self.pages, self.page, self.kv_heads, self.dim, self.device = pages, page, heads, dim, k.device.index
         self._args = abi.PagedCacheArgs(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
-                                        _vector(k_scale, heads, "k_scale"), _vector(v_scale, heads, "v_scale"), dtype,
-                                        pages, page, heads, dim)
+                                        _vector(k_scale, heads, "k_scale", k.device), _vector(v_scale, heads, "v_scale", k.device),
+                                        dtype, pages, page, heads, dim)
 
 
 class TextOps:
@@ -117,6 +117,12 @@ class TextOps:
         return _done(abi.text.product_f8(self._h, x, None, w, scale, bias, _glu(epilogue), out, _is_f32(out_dtype),
                                          timed), "sq8_linear_f8_quantized")
 
+    def _args_of(self, cache: PagedCache):
+        """What the native calls take of a cache, which lies on this context's GPU."""
+        if cache.device != self.device:
+            raise ValueError(f"the cache must be on the context's GPU, cuda:{self.device}, not cuda:{cache.device}")
+        return cache._args
+
     def append_kv(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedCache, positions: torch.Tensor,
                   slots: torch.Tensor, table: torch.Tensor, *, q_out: Optional[torch.Tensor] = None,
                   interleaved: bool = False) -> torch.Tensor:
@@ -125,7 +131,7 @@ class TextOps:
         the turned q (`q_out`; q itself turns it in place). `table` float32 [positions, rot]: rot/2 cosines, then the
         sines, of a head's first rot values, paired (i, i + rot/2), or (2i, 2i + 1) when `interleaved`. positions,
         slots int32 [tokens]."""
-        return _done(abi.text.append_kv(self._h, q, k, v, cache._args, positions, slots, table, q_out, interleaved),
+        return _done(abi.text.append_kv(self._h, q, k, v, self._args_of(cache), positions, slots, table, q_out, interleaved),
                      "sq8_append_kv")
 
     def paged_attention(self, q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, lengths: torch.Tensor, *,
@@ -134,5 +140,5 @@ class TextOps:
         """Attention of each sequence's new token q [batch, q_heads, dim] (bf16) over its cached tokens: `pages` int32
         [batch, most pages] page indices in order, `lengths` int32 [batch] (0: zeros). `scale` defaults to
         1/sqrt(dim); `softcap` c > 0: scores c · tanh(s/c); `window` w > 0: the last w tokens only."""
-        return _done(abi.text.paged_attention(self._h, q, cache._args, pages, lengths, scale, softcap, window, out),
+        return _done(abi.text.paged_attention(self._h, q, self._args_of(cache), pages, lengths, scale, softcap, window, out),
                      "sq8_paged_attention")
