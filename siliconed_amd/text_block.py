@@ -10,7 +10,8 @@
 A layer takes and returns (y, x): the branch not yet added, and the fp32 residual stream, which it updates in place.
 Weights are e4m3 codes with an fp32 scale per 128 × 128 block, as published (random here); heads of a group share their
 keys and values. `step` runs one new token of each sequence and launches eight kernels (ten past a few sequences, whose
-operands two passes quantize), all of which a HIP graph can hold; `prompt` runs one sequence's first tokens. With the
+operands two passes quantize), all of which a HIP graph can hold; `prompt` runs one sequence's first tokens. Both queue
+everything on torch's current stream (a capture's: one that a step has run on before). With the
 sizes below a step's layer takes 76 us for one sequence of 2000 tokens, 103 for 16 and 125 for 64 of 1000; the weights
 alone, 192 MB, are 38.
 
@@ -86,12 +87,19 @@ class TextBlock:
         s = torch.full((self.kv_heads,), scale, device=dev) if dtype == F8 else None
         return PagedCache(k, v, s, s)
 
+    def _here(self) -> TensorGEMM:
+        """The context, on torch's current stream: what torch does before, between and after the library's kernels is
+        queued there (the context may be shared, and moved by whoever used it last)."""
+        self.ctx.set_stream(torch.cuda.current_stream(self.ctx.device))
+        return self.ctx
+
     def _append(self, y, x, cache, positions, slots, table):
         """The layer up to its attention: the turned q [tokens, heads, dim] and the stream."""
-        codes, sx, x = self.ctx.add_norm_quantized(y, self.w_in, EPS, residual=x)
-        qkv = self.ctx.product_f8(codes, sx, *self.qkv).view(-1, self.heads + 2 * self.kv_heads, self.dim)
+        ctx = self._here()
+        codes, sx, x = ctx.add_norm_quantized(y, self.w_in, EPS, residual=x)
+        qkv = ctx.product_f8(codes, sx, *self.qkv).view(-1, self.heads + 2 * self.kv_heads, self.dim)
         q, k, v = qkv.split([self.heads, self.kv_heads, self.kv_heads], 1)
-        return self.ctx.append_kv(q, k, v, cache, positions, slots, table, q_out=q), x
+        return ctx.append_kv(q, k, v, cache, positions, slots, table, q_out=q), x
 
     def _finish(self, o, x):
         """The layer after its attention."""
@@ -139,7 +147,7 @@ def main() -> None:
     most = -(-a.context // a.page)
     layers = [TextBlock(seed=i) for i in range(a.layers)]
     caches = [block.cache(a.batch * most, a.page) for block in layers]
-    d, dev, ctx = layers[0].d, layers[0].w_in.device, layers[0].ctx
+    d, dev = layers[0].d, layers[0].w_in.device
     i32 = dict(dtype=torch.int32, device=dev)
     pages = torch.randperm(a.batch * most, device=dev).to(torch.int32).view(a.batch, most)
     lengths = torch.full((a.batch,), a.context, **i32)
@@ -165,14 +173,13 @@ def main() -> None:
         return (time.perf_counter() - t) / a.steps * 1e6
 
     side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
-        ctx.set_stream(side)
         calls = timed(run)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=side):
             run()
         replays = timed(graph.replay)
-        ctx.set_stream(torch.cuda.default_stream())
     print(f"{a.layers} layers, {a.batch} sequences of {a.context} tokens: {calls:.0f} us a step as calls, "
           f"{replays:.0f} us as a graph ({replays / a.layers:.1f} a layer), {a.batch / replays * 1e6:.0f} tokens/s")
 

@@ -1,7 +1,9 @@
 """A text decoder's operators: the norm that writes a product's 8-bit operand, products of block-scaled e4m3 codes,
 and a paged key-value cache with its append and its attention (the sq8_* entries of include/siliconed_q8.h).
 
-`TensorGEMM` has them as methods; everything is queued on its stream. With them, a decoder layer's step is
+`TensorGEMM` has them as methods; everything is queued on its stream. Outputs that a call allocates are torch's, of its
+current stream: make calls with the context's stream current (`torch.cuda.stream`), or hand in outputs and order the two
+streams. With them, a decoder layer's step is
 
     codes, sx, x = ctx.add_norm_quantized(y, w_norm, eps, residual=x)
     qkv = ctx.product_f8(codes, sx, w_qkv, s_qkv)
