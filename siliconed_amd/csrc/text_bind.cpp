@@ -90,7 +90,8 @@ Heads heads_of(const Tensor &t, const char *what, int64_t rows, int64_t heads, i
                           t.size(2) == dim && t.is_cuda(),
                       what, " must be bfloat16 [", rows, ", ", heads, ", ", dim, "] on the GPU, not ", t.scalar_type(), " ", t.sizes());
     TORCH_CHECK_VALUE(t.stride(2) == 1 || dim <= 1, what, " must have contiguous heads");
-    return {static_cast<uint16_t *>(t.data_ptr()), t.stride(0), t.stride(1)};
+    // (Torch leaves the stride of a dimension of one anything.)
+    return {static_cast<uint16_t *>(t.data_ptr()), rows > 1 ? t.stride(0) : 0, heads > 1 ? t.stride(1) : 0};
 }
 int64_t queries(const Tensor &q) {
     TORCH_CHECK_VALUE(q.dim() == 3, "q must be [tokens, heads, dim], not ", q.sizes());

@@ -33,6 +33,11 @@ def _vector(t: Optional[torch.Tensor], count: int, what: str, device: torch.devi
     return t.data_ptr()
 
 
+def _strides(pool: torch.Tensor):
+    """A pool's strides but the last; of a dimension of one, which torch leaves anything, 0."""
+    return [stride if size > 1 else 0 for size, stride in zip(pool.shape[:3], pool.stride())]
+
+
 def _glu(epilogue) -> bool:
     if epilogue not in _EPILOGUES:
         raise ValueError(f"a block-scaled product's epilogue is None or 'silu_glu', not {epilogue!r}")
@@ -73,7 +78,7 @@ class PagedCache:
             raise ValueError("scales belong to float8_e4m3fn pools")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.page, self.kv_heads, self.dim, self.device = pages, page, heads, dim, k.device.index
-        self._args = abi.PagedCacheArgs(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3],
+        self._args = abi.PagedCacheArgs(k.data_ptr(), v.data_ptr(), *_strides(k), *_strides(v),
                                         _vector(k_scale, heads, "k_scale", k.device), _vector(v_scale, heads, "v_scale", k.device),
                                         dtype, pages, page, heads, dim)
 

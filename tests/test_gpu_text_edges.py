@@ -53,3 +53,21 @@ def test_a_window_past_every_length_is_none(gemm, dtype):
     want = gemm.paged_attention(q, cache, table, n)
     for window in (2 ** 31 - 1, 2 ** 31 - 31, 2 ** 31 - 32, 2 ** 30):
         assert torch.equal(gemm.paged_attention(q, cache, table, n, window=window), want), window
+
+
+def test_the_stride_of_a_single_row_is_nothing(gemm):
+    """One token's query, one key head, one page: torch leaves the stride of a dimension of one anything, odd values too."""
+    g = torch.Generator(device=DEV).manual_seed(3)
+    k, v = (torch.randn(2, 16, 1, 64, generator=g, device=DEV).to(BF) for _ in "kv")
+    q = torch.randn(1, 4, 64, generator=g, device=DEV).to(BF)
+    table = torch.tensor([[1, 0]], dtype=torch.int32, device=DEV)
+    want = gemm.paged_attention(q, sq.PagedCache(k, v), table, lengths(29))
+    odd = [t.as_strided(t.shape, (1024, 64, 3, 1)) for t in (k, v)]
+    out = torch.empty(4 * 64, dtype=BF, device=DEV).as_strided((1, 4, 64), (257, 64, 1))
+    gemm.paged_attention(q.as_strided(q.shape, (257, 64, 1)), sq.PagedCache(*odd), table, lengths(29), out=out)
+    assert torch.equal(out, want)
+    one = gemm.paged_attention(q[:, :1].as_strided((1, 1, 64), (5, 3, 1)), sq.PagedCache(*odd), table, lengths(29))
+    assert torch.equal(one, want[:, :1])
+    last = [t[1:].as_strided((1, 16, 1, 64), (7, 64, 3, 1), t[1:].storage_offset()) for t in (k, v)]
+    first = gemm.paged_attention(q, sq.PagedCache(*last), torch.zeros_like(table), lengths(16))
+    assert torch.equal(first, gemm.paged_attention(q, sq.PagedCache(k, v), table, lengths(16)))
