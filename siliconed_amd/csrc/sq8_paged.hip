@@ -174,8 +174,8 @@ __global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs p) {
 //
 // One pass over the cache with the running maximum and sum of the softmax, both fp32. The maximum is moved only when a
 // score passes it by 8 powers of two, so a probability may be up to 2^8 of what it will be divided by: the same bits
-// of it, and the sums rescaled hardly ever. The probabilities are rounded to bf16 for their product with v (the sum is of
-// the unrounded ones): at most 2^-8 of each, random over the tokens.
+// of it, and the sums rescaled hardly ever. For their product with v the probabilities are split into two bf16 numbers each,
+// 2^-17 of one at most left out: rounded to one they would cost the output as much as its own rounding to bf16.
 //
 // Bound by the cache's bytes. The query heads of one kv head (up to 16; more take several passes) are the columns of
 // both products, on v_mfma_f32_16x16x32_bf16:
@@ -612,8 +612,17 @@ __global__ void __launch_bounds__(64 * WAVES, paged_held(DP)) paged_attention_ke
 #pragma unroll
             for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(e[j] - from);
             sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-            const bf16x8 prob = __builtin_bit_cast(
-                bf16x8, u32x4{pack_bf16_rne(w[0], w[1]), pack_bf16_rne(w[2], w[3]), pack_bf16_rne(w[4], w[5]), pack_bf16_rne(w[6], w[7])});
+            // Each probability in two bf16 parts: its first 8 bits, and what they leave, rounded, at least 2^-126, so that an
+            // infinite value meets no zero and no other sign.
+            u32x4 part[2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t x = __float_as_uint(w[2 * j]), y = __float_as_uint(w[2 * j + 1]);
+                part[0][j] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+                part[1][j] = pack_bf16_rne(fmaxf(w[2 * j] - __uint_as_float(x & 0xFFFF0000u), 0x1p-126f),
+                                           fmaxf(w[2 * j + 1] - __uint_as_float(y & 0xFFFF0000u), 0x1p-126f));
+            }
+            const bf16x8 prob[2] = {__builtin_bit_cast(bf16x8, part[0]), __builtin_bit_cast(bf16x8, part[1])};
             // Value DV·c + d of the lane's eight tokens, two tokens a dword, two values at a time.
 #pragma unroll
             for (int d = 0; d < DV; d += 2) {
@@ -633,7 +642,9 @@ __global__ void __launch_bounds__(64 * WAVES, paged_held(DP)) paged_attention_ke
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    o[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t[i]), prob, o[d + i], 0, 0, 0);
+#pragma unroll
+                    for (int j = 1; j >= 0; --j)
+                        o[d + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t[i]), prob[j], o[d + i], 0, 0, 0);
             }
             if (more) load_v(next);
             at = next;
