@@ -96,7 +96,6 @@ TEXT_ENTRIES = ("sq8_add_norm_quantized", "sq8_quantize_groups", "sq8_linear_f8"
                 "sq8_append_kv", "sq8_paged_attention", "sq8_device")
 
 _lib = None
-text = None  # the text decoder's operators' native calls (text_bind.cpp), once the library is loaded
 
 
 class SQ8Error(RuntimeError):
@@ -112,7 +111,7 @@ class Unsupported(SQ8Error):
 
 
 def load() -> ctypes.CDLL:
-    global _lib, text
+    global _lib
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise ImportError(f"{LIB_PATH} is not built: run `python -c 'import __graft_entry__ as g; g.build()'`")
@@ -121,12 +120,26 @@ def load() -> ctypes.CDLL:
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args
-        import torch  # noqa: F401  (the libraries that the module is linked against)
-
-        from . import _text_bind
-        _text_bind.bind(*(ctypes.cast(getattr(lib, name), _P).value for name in TEXT_ENTRIES))
-        _lib, text = lib, _text_bind
+        _lib = lib
     return _lib
+
+
+def __getattr__(name: str):
+    """`text`: the text decoder's operators' native calls (text_bind.cpp), loaded when they are first asked for. The rest
+    of the library does without that module, which is built against one version of torch."""
+    if name != "text":
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    lib = load()
+    import torch  # noqa: F401  (the libraries that the module is linked against)
+
+    try:
+        from . import _text_bind
+    except ImportError as e:
+        raise ImportError(f"the text operators' host module does not load ({e}): build it again with "
+                          "`python -c 'import __graft_entry__ as g; g.build()'`") from e
+    _text_bind.bind(*(ctypes.cast(getattr(lib, entry), _P).value for entry in TEXT_ENTRIES))
+    globals()["text"] = _text_bind
+    return _text_bind
 
 
 def status_string(status: int) -> str:

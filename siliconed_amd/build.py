@@ -127,7 +127,6 @@ def build(verbose: bool = False, incremental: bool = False) -> str:
     with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, min(len(todo) + 1, os.cpu_count() or 1))) as pool:
         bind = pool.submit(_bind, incremental)
         list(pool.map(_compile, todo))
-        bind.result()
     objs = [os.path.join(OBJ, name + ".o") for _, name, _ in SOURCES]
     tmp = LIB + ".tmp"
     # rocBLAS: the bf16-weight product's plain GEMM.
@@ -136,6 +135,7 @@ def build(verbose: bool = False, incremental: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
+    bind.result()  # last: the library stands without it
     if verbose:
         print(f"built {LIB}", file=sys.stderr)
     return LIB

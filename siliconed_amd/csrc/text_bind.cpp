@@ -3,7 +3,8 @@
 // attributes of tensors, two allocations, a foreign call of twenty arguments) took 9 to 13: the calls, not the GPU,
 // set the pace of a decoder.
 //
-// The library is loaded by _abi.py, which hands over its entries' addresses (bind). A function here returns its
+// The library is loaded by _abi.py, which hands over its entries' addresses (bind) when a text operator is first
+// called: nothing else of the library needs this module. A function here returns its
 // outputs, or the status of a call that the library refused, an int, for _abi.py to raise. A tensor that does not fit
 // raises ValueError.
 #include <Python.h>
