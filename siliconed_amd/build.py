@@ -102,9 +102,8 @@ def _stale(item) -> bool:
 
 
 def _bind(incremental: bool = False) -> None:
-    deps = (os.path.join(CSRC, "text_bind.cpp"), os.path.join(ROOT, "include", "siliconed_q8.h"))
-    if incremental and os.path.exists(BIND) and all(os.path.getmtime(BIND) >= os.path.getmtime(d) for d in deps):
-        return
+    """Builds the host module, and beside it a note of the torch and the command it is built with; `incremental`: only
+    where that note, or a source's time, says otherwise."""
     import torch
 
     at = os.path.dirname(torch.__file__)
@@ -113,10 +112,17 @@ def _bind(incremental: bool = False) -> None:
            "-isystem", os.path.join(at, "include", "torch", "csrc", "api", "include"),
            "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, "text_bind.cpp"), "-o", BIND + ".tmp",
            "-L", os.path.join(at, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    note, noted = os.path.join(OBJ, "text_bind.txt"), " ".join([torch.__version__, sys.version, *cmd])
+    deps = (os.path.join(CSRC, "text_bind.cpp"), os.path.join(ROOT, "include", "siliconed_q8.h"))
+    if incremental and os.path.exists(BIND) and all(os.path.getmtime(BIND) >= os.path.getmtime(d) for d in deps):
+        if os.path.exists(note) and open(note).read() == noted:
+            return
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"the host module failed:\n{r.stderr}")
     os.replace(BIND + ".tmp", BIND)
+    with open(note, "w") as f:
+        f.write(noted)
 
 
 def build(verbose: bool = False, incremental: bool = False) -> str:

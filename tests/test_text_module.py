@@ -55,3 +55,28 @@ def test_the_library_is_built_whatever_becomes_of_the_module(tmp_path, monkeypat
     with pytest.raises(RuntimeError, match="no compiler"):
         build.build()
     assert len(linked) == 1 and (tmp_path / "lib.so").exists()
+
+
+def test_an_incremental_build_sees_another_torch(tmp_path, monkeypatch):
+    import torch
+    from siliconed_amd import build
+    built = []
+
+    def compiled(cmd, **_):
+        built.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(build, "BIND", str(tmp_path / "_text_bind.so"))
+    monkeypatch.setattr(build, "OBJ", str(tmp_path))
+    monkeypatch.setattr(build.subprocess, "run", compiled)
+    build._bind(incremental=True)
+    build._bind(incremental=True)
+    assert len(built) == 1  # the second call: nothing has changed
+    monkeypatch.setattr(torch, "__version__", "0.0.1+other")
+    build._bind(incremental=True)
+    assert len(built) == 2
+    build._bind(incremental=True)
+    assert len(built) == 2
+    build._bind()
+    assert len(built) == 3
