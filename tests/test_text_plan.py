@@ -6,6 +6,7 @@ import subprocess
 import pytest
 
 from conftest import ROOT
+from f8_shapes import FEW, LONG, VALUES
 
 CSRC = os.path.join(ROOT, "siliconed_amd", "csrc")
 PROBE = r"""
@@ -89,3 +90,13 @@ def test_a_window_bounds_the_workgroups(ask):
     assert ask("a", 1, 8, 1, 128, 16, 1000, 128) == "2"  # 159 tokens at most: two tiles
     assert ask("a", 1, 8, 1, 128, 16, 1000, 1) == "1"
     assert ask("a", 3, 8, 2, 128, 16, 0, 0) == "1"
+
+
+def test_the_kernels_that_the_gpu_tests_are_for(plan):
+    """The shapes of test_gpu_text_few_rows.py and test_gpu_text_long_k.py reach what they are named after."""
+    for shape, want in FEW:
+        assert plan(*shape) == plan(*shape, f32=True) == want, shape
+    for shape, want in VALUES:
+        assert plan(*shape, values=True) == plan(*shape, f32=True, values=True) == want, shape
+    for shape, bf16, f32 in LONG:
+        assert (plan(*shape), plan(*shape, f32=True)) == (bf16, f32), shape
