@@ -19,6 +19,9 @@ A recognized weight is `[N, K]` (published rows = outputs): `product_operands` g
 the fp32 scale (per output, or one) ready for `TensorGEMM.pack(..., layout="nk")` and
 `TensorGEMM.product(..., rotation=group)`, and `stage` puts them on the device; `to_map` writes
 them as a `.silicon` map ([K, N], the scale after the values).
+
+A text decoder's fp8 checkpoint by 128×128 blocks has no such weight (the reference refuses the file): its layers are
+read one by one, `stage_blocks`, for `TensorGEMM.product_f8`.
 """
 from __future__ import annotations
 
@@ -289,7 +292,8 @@ def recognize(st: Safetensors) -> Recognized:
         if e.dtype == "F8_E5M2":
             raise Refused(f"{name}: fp8 in E5M2; the product reads E4M3 codes only")
         if name.endswith(".weight_scale_inv"):
-            raise Refused(f"{name}: `weight_scale_inv` scales fp8 by 128×128 blocks, which the product does not take")
+            raise Refused(f"{name}: `weight_scale_inv` scales fp8 by 128×128 blocks, which the products of a recognized "
+                          f"weight do not take; `stage_blocks` reads such a weight for `product_f8`")
     for layer in sorted(comfy):
         f = comfy[layer].get("format")
         fmt = (f if isinstance(f, str) else "").lower()
@@ -467,6 +471,38 @@ def stage(st: Safetensors, g: QuantizedGroup, ctx=None, device: int = 0):
     n, k = q.shape
     return StagedWeight(name=g.values, packed=packed, scale=torch.from_numpy(s).to(dev), k=k, n=n,
                         group=g.rotation, dtype=g.kind)
+
+
+BLOCK = 128
+
+
+def block_operands(st: Safetensors, name: str):
+    """An fp8 weight by 128×128 blocks as published, w = code · scale of its block: `<l>.weight` F8_E4M3 [N, K] with
+    `<l>.weight_scale_inv` (F32, BF16 or F16) [⌈N/128⌉, ⌈K/128⌉]. The codes as uint8, the scales as fp32."""
+    scale = name + "_scale_inv"
+    w, s = st.entries.get(name), st.entries.get(scale)
+    if w is None or w.dtype != "F8_E4M3" or len(w.shape) != 2:
+        raise Refused(f"{name}: {'no such tensor' if w is None else f'{w.dtype} {w.shape}'} is not an fp8 [N, K] weight")
+    if s is None or _scale_type(s.dtype) is None:
+        raise Refused(f"{scale}: {'no such tensor' if s is None else f'a scale of type {s.dtype}'}")
+    want = [-(-d // BLOCK) for d in w.shape]
+    if s.shape != want:
+        raise Refused(f"{scale}: scales of shape {s.shape} for a weight of {w.shape}, which has {want} blocks of 128×128")
+    return np.ascontiguousarray(st.array(name)), np.ascontiguousarray(st.array(scale), dtype=np.float32)
+
+
+def stage_blocks(st: Safetensors, *names: str, device: int = 0):
+    """`product_f8`'s weight on the device, (codes float8_e4m3fn [N, K], scale fp32): one published weight, or a GLU's gate
+    and up, whose halves are blocked each by itself (`product_f8(..., epilogue="silu_glu")`)."""
+    import torch
+    if len(names) not in (1, 2):
+        raise ValueError("one weight, or a gate and an up")
+    parts = [block_operands(st, name) for name in names]
+    if any(q.shape != parts[0][0].shape for q, _ in parts):
+        raise Refused(f"{names[0]} and {names[1]}: {parts[0][0].shape} and {parts[1][0].shape} are not the halves of a GLU")
+    dev = torch.device("cuda", device)
+    codes, scale = (torch.from_numpy(np.concatenate(p)).to(dev) for p in zip(*parts))
+    return codes.view(torch.float8_e4m3fn), scale
 
 
 def to_map(st: Safetensors, r: Recognized, path: str, page: int = 16384) -> None:
