@@ -39,6 +39,9 @@ constexpr float kLaunch = 3.0f, kBytesMicrosecond = 5.0e6f, kIntoCU = 45.0e3f, k
 // time the bytes take. At M = 64, K = 12288, N = 4096: 64 × 64 tiles 37.6 µs whole and 17.5 in four parts; at M = 2048
 // of the same 256 × 256 160 and 128 × 128 120; at M = 8192, K = 4096, N = 24576 752 and 885.
 // Rows too far apart for the tile kernels' 32-bit offsets go to the short kernel.
+// Whole tiles sum K block by block, all alike, so rows have the same bits on any of them; a split's do not. From 4096 rows on
+// and past 1024 columns there is none, as for the other products: there chunks of a call's rows give the call's bits. (It
+// costs nothing: an fp32 C of 4097 × 2048 at K = 8192 takes 198 µs in two parts and 191 whole, at K = 16384 331 and 334.)
 F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
     F8Plan plan = {F8_FAR, 1, 0, 0, false};
     if (p.M <= 0 || p.H <= 0) return plan;
@@ -56,12 +59,13 @@ F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
     const bool near = 256 * std::max(std::max(p.lda, p.ldw), 4 * p.ldsx) + p.K <= INT32_MAX &&
                       (!glu || ((int64_t)p.H + 256) * p.ldw + p.K <= INT32_MAX);
     if (!near) return plan;
+    const bool whole = p.M >= 4096 && p.N > 1024;
     float best = 0.0f;
     for (int t = out_f32 ? F8_128 : F8_256; t < F8_TILES; ++t) {
         const TileCost &c = kTiles[t];
         const int64_t tiles = (int64_t)((p.M + c.rows - 1) / c.rows) * ((p.H * halves + c.columns - 1) / c.columns);
         for (int splits = 1; splits <= 8; ++splits) {
-            if (splits > 1 && (t < F8_64x128 || p.KB < 4 * splits)) break;
+            if (splits > 1 && (t < F8_64x128 || p.KB < 4 * splits || whole)) break;
             const int64_t groups = tiles * splits, slots = (int64_t)cus * c.held, rest = groups % slots;
             const int steps = (p.KB + splits - 1) / splits;
             const float one = out_f32 ? c.one_f32 : c.one, all = out_f32 ? c.all_f32 : c.all;

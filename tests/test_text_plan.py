@@ -100,3 +100,13 @@ def test_the_kernels_that_the_gpu_tests_are_for(plan):
         assert plan(*shape, values=True) == plan(*shape, f32=True, values=True) == want, shape
     for shape, bf16, f32 in LONG:
         assert (plan(*shape), plan(*shape, f32=True)) == (bf16, f32), shape
+
+
+def test_tall_products_sum_in_one_sequence(plan):
+    """From 4096 rows on and past 1024 columns a product's rows have the same bits however they are chunked."""
+    for n in (1025, 1500, 2048, 4098, 24576):
+        for m in (4096, 4097, 5000, 8192, 20000):
+            for k in (1024, 8192, 16384):
+                for glu in (False, True)[:2 - n % 2]:
+                    for f32 in (False, True):
+                        assert plan(m, k, n, glu, f32).endswith("/1"), (m, k, n, glu, f32)
