@@ -416,7 +416,8 @@ int sq8_quantize_groups(sq8_ctx *ctx, const void *x, int x_dtype, int64_t ldx, i
 /* **The product of e4m3 codes by e4m3 codes.** C[i, j] = act(Σ_b sx[i, b] · sw[j/128, b] · (Σ_{k in b} A[i, k] ·
  * W[j, k]) + bias[j]), b the blocks of 128 of K (the last may be short), sums fp32; for a bf16 C the matrix cores'
  * e4m3 instructions drop, within each 8 consecutive K, what is under 2^-13 of the largest product's power of two (1.4e-5
- * of a result's size on normal operands); for an fp32 C they do not. A: codes [m, k], leading dimension
+ * of a result's size on normal operands; at most 7 · 2^-13 of each eight's largest product, added up over K); an fp32 C is
+ * summed without that. A: codes [m, k], leading dimension
  * lda; sx fp32 [m, ⌈k/128⌉], ldsx. W: codes [n, k] as published, ldw; sw fp32 [⌈n/128⌉, ⌈k/128⌉], ldsw. `epilogue`
  * SQ8_EPI_NONE, or SQ8_EPI_SILU_GLU (n = 2h, output h: silu(gate)·up): the halves are then blocked each by itself, sw
  * [2·⌈h/128⌉, ⌈k/128⌉], gate's rows first (else SQ8_EUNSUPPORTED). bias fp32 [n] or NULL. C SQ8_BF16 or SQ8_F32, ldc.
@@ -451,8 +452,8 @@ typedef struct sq8_paged_cache {
  * `position` of `table` (fp32 [max_position, rot]: rot/2 cosines, then the sines; leading dimension table_row) — q to
  * q_out (bf16, may be q itself), k and v to slot slots[token] = page index · page + place, rounded once (e4m3: of value
  * / scale, saturated at ±448). A slot outside [0, pages · page) writes nothing (an idle row's −1); a position
- * outside the table takes its last row. dim and rot even, rot ≤ dim (else SQ8_EUNSUPPORTED). Two tokens with one slot
- * race. */
+ * outside the table takes its last row. dim and rot even (else SQ8_EUNSUPPORTED), rot ≤ dim (else SQ8_EINVAL). Two tokens
+ * with one slot race. */
 int sq8_append_kv(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head,
                   const uint16_t *k, int64_t k_token, int64_t k_head, const uint16_t *v, int64_t v_token, int64_t v_head,
                   uint16_t *q_out, int64_t qo_token, int64_t qo_head, const sq8_paged_cache *cache,

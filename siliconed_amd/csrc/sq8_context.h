@@ -14,8 +14,9 @@ struct sq8_ctx {
     hipEvent_t begin, end;
     sq8::Buffer scratch;    // bf16 copy of an fp32 activation (the reference's rounding scratch)
     sq8::Buffer wpack;      // [K, N] codes repacked for the weight-direct kernels, per product
-    sq8::Buffer part;       // partial sums: the skinny kernel's K split, a paged attention's split sequences
-    sq8::Buffer marks;      // a paged attention's counters, zero between its calls
+    sq8::Buffer part;       // partial sums: the skinny kernel's and a block-scaled product's K split, a paged attention's
+                            // split sequences
+    sq8::Buffer marks;      // the counters of those last two, zero between calls
     sq8::SetAside *aside;   // what these outgrew while a captured graph may use it
     rocblas_handle blas;    // the bf16-weight product's library GEMM (created on its first call)
     int wd_tile;            // measurement knobs, read once at sq8_create (SQ8_TILE, SQ8_Q8_TILE, SQ8_SPLITS): a

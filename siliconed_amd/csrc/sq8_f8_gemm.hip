@@ -7,8 +7,10 @@
 // added into the fp32 accumulator with one multiply-add by the two scales' rounded product. That instruction sums in
 // fp32 but for one thing, measured here: within each 8 consecutive K it aligns the products to the largest and drops
 // what is under 2^-13 of that one's power of two. On normal operands that is 1.4e-5 of a result's size, a hundredth of
-// what the rounding to bf16 then costs, and it runs at twice the bf16 rate. (v_mfma_f32_16x16x32_fp8_fp8 does the
-// same.) An fp32 C is for callers who want the sums as they are: its codes are widened to bf16, exactly, for
+// what the rounding to bf16 then costs; at worst it is 7 · 2^-13 of the largest product of each eight, where e4m3's own
+// rounding of a factor may have put that product off by 2^-4. It runs at twice the bf16 rate, and without the widening:
+// one row by K = 4096, N = 24576 (GLU) takes 21.6 µs so and 25.4 on the bf16 instructions. (v_mfma_f32_16x16x32_fp8_fp8
+// drops the same.) An fp32 C is for callers who want the sums as they are: its codes are widened to bf16, exactly, for
 // v_mfma_f32_16x16x32_bf16, whose products and sums are fp32.
 //
 // The weight is the first operand, so a lane ends with four consecutive outputs of one row; K is laid out alike for
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(64 * NW) f8_short_kernel(const F8Args p) {
         float s_x[U][TM], s_w[U][NT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int kb = min(k0 + u * NW, p.KB - 1);  // past the last: its scales are zeroed below
+            const int kb = min(k0 + u * NW, p.KB - 1);  // past the last: read, not used
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 w[u][j] = load_f8(wrow[j], kb, h, p.K);
@@ -330,8 +332,8 @@ __global__ void __launch_bounds__(512) f8_staged_kernel(const F8Args p) {
 // one burst behind the barrier they held up the small tiles' steps by a seventh), the next step's loads have landed,
 // and its first fragments are read under those instructions too.
 //
-// What bounds it: at M = 8192, K = 4096, N = 24576 (GLU) the 256 × 256 tile runs at the card's power limit, 703 to 757 µs
-// or 2.18 to 2.35 PFLOP/s on normal operands and 578 on zeros, its matrix instructions busy for 55 % of the cycles (a
+// What bounds it: at M = 8192, K = 4096, N = 24576 (GLU) the 256 × 256 tile runs at the card's power limit, 703 to 785 µs
+// or 2.10 to 2.35 PFLOP/s on normal operands and 578 on zeros, its matrix instructions busy for 55 % of the cycles (a
 // library's product of such codes with one scale a tensor, no GLU: 650). A 64-row tile's step is a chain of a barrier, reads, four
 // to eight matrix instructions a wave and their scaling, 0.36 µs where the instructions alone are 0.06, so few rows want
 // many workgroups: N = 24576 (GLU) has 192 of 64 × 128, 27.6 µs at M = 48 (100 MB, 3.7 TB/s), and N = 4096 takes its K in

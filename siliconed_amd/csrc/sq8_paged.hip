@@ -195,13 +195,17 @@ __global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs p) {
 // finds it.
 //
 // With 32 query heads on 8 of 128: two sequences of 131 072 tokens in bf16 (1074 MB) take 207 to 213 µs, 5.0 to 5.2 TB/s; 48
-// ragged ones of up to 8192 in e4m3 (414 MB) 96, 4.3 TB/s, of which some ten are the start (the launch, the lengths, the first
-// pages and rows) and the join, and the rest runs at what 128-byte pieces a kilobyte apart come in at; one of 777
-// tokens 8.6, a chain of those latencies (6.5 without a join), one of 4096 12.8 and of 16 384 25. The arithmetic is not
+// ragged ones of up to 8192 in e4m3 (414 MB) 96 to 97, 4.3 TB/s, of which some ten are the start (the launch, the lengths,
+// the first pages and rows) and the join, and the rest runs at what 128-byte pieces a kilobyte apart come in at; one of 777
+// tokens 8.9, a chain of those latencies (6.5 without a join), one of 4096 12.7 and of 16 384 25. The arithmetic is not
 // felt: without it the loads alone take as long. Neither are more workgroups a CU, or the heads of a sequence going through
 // the same pages at the same time. What the join costs is its slots' lines and its counters: with the values of a head's
 // lanes side by side (not by the 16 columns of the products), pairs to a load and a line for each counter the
 // sequence of 4096 went from 15.8 µs to 12.8, the ragged ones from 100 to 96.
+//
+// Pages that 16-token tiles do not fill are looked up row by row, by vector loads, which wait for the rows' loads under way:
+// the 48 sequences take 101 µs in pages of 24 or 8 tokens and 105 of one (in bf16 175, where pages of 16 and 64 take 165),
+// the two long ones 226 to 229.
 
 constexpr int TILE = PAGED_TILE;
 constexpr int WAVES = 4;

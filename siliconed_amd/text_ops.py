@@ -108,7 +108,8 @@ class TextOps:
     def product_f8(self, codes: torch.Tensor, sx: torch.Tensor, w: torch.Tensor, scale: torch.Tensor, *,
                    bias: Optional[torch.Tensor] = None, epilogue=None, out: Optional[torch.Tensor] = None,
                    out_dtype: torch.dtype = torch.bfloat16, timed: bool = False):
-        """act(Σ over blocks of 128 of K of sx · scale · (codes · wᵀ) + bias): codes float8_e4m3fn [m, k] with sx
+        """act(Σ over blocks of 128 of K of sx · scale · (codes · wᵀ) + bias), sums in fp32 with `out_dtype` float32 (a
+        bfloat16 output's leave out what is under 2^-13 of the largest of 8 products): codes float8_e4m3fn [m, k] with sx
         [m, ⌈k/128⌉] (add_norm_quantized's, quantize_groups'), w float8_e4m3fn [n, k] with scale [⌈n/128⌉, ⌈k/128⌉] as
         published. `epilogue="silu_glu"`: n = 2h rows, gate then up, each half blocked by itself (scale
         [2·⌈h/128⌉, ⌈k/128⌉]), output [m, h]."""
@@ -146,6 +147,6 @@ class TextOps:
                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of each sequence's new token q [batch, q_heads, dim] (bf16) over its cached tokens: `pages` int32
         [batch, most pages] page indices in order, `lengths` int32 [batch] (0: zeros). `scale` defaults to
-        1/sqrt(dim); `softcap` c > 0: scores c · tanh(s/c); `window` w > 0: the last w tokens only."""
+        1/sqrt(dim); `softcap` c > 0 (inf: none): scores c · tanh(s/c); `window` w > 0: the last w tokens only."""
         return _done(abi.text.paged_attention(self._h, q, self._args_of(cache), pages, lengths, scale, softcap, window, out),
                      "sq8_paged_attention")
