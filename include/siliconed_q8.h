@@ -474,6 +474,52 @@ int sq8_paged_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_
                         float scale, float softcap, int window,
                         uint16_t *out, int64_t o_token, int64_t o_head, int batch, int q_heads);
 
+/* **Heads normed, turned and appended in one pass.** sq8_append_kv with every query and key head normed before it is
+ * turned: y = x / sqrt(mean x² + eps) · w over the head's values, w = q_norm or k_norm (fp32 [dim]; NULL: that kind is not
+ * normed), values as they are. All fp32, one rounding, of the turned value. dim even and up to 512 (else SQ8_EUNSUPPORTED). */
+int sq8_norm_append_kv(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head,
+                       const uint16_t *k, int64_t k_token, int64_t k_head, const uint16_t *v, int64_t v_token, int64_t v_head,
+                       uint16_t *q_out, int64_t qo_token, int64_t qo_head, const sq8_paged_cache *cache,
+                       const int32_t *positions, const int32_t *slots, const float *table, int64_t table_row,
+                       int max_position, int rot, int interleaved, const float *q_norm, const float *k_norm, float eps,
+                       int tokens, int q_heads);
+
+/* **The same without a cache**: q [tokens, q_heads, dim] and k [tokens, kv_heads, dim] (bf16, strides in elements) normed and
+ * turned into q_out and k_out, which may be q and k themselves. rot 0: normed only (positions and table unused); kv_heads 0:
+ * q alone. */
+int sq8_norm_rotate(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head,
+                    const uint16_t *k, int64_t k_token, int64_t k_head, uint16_t *q_out, int64_t qo_token, int64_t qo_head,
+                    uint16_t *k_out, int64_t ko_token, int64_t ko_head, const int32_t *positions, const float *table,
+                    int64_t table_row, int max_position, int rot, int interleaved, const float *q_norm, const float *k_norm,
+                    float eps, int tokens, int q_heads, int kv_heads, int dim);
+
+/* **Attention of whole sequences over their own keys and values.** Sequence b's tokens are rows starts[b] .. starts[b + 1] −
+ * 1 (int32 [sequences + 1], ascending; cut to [0, tokens]; NULL with one sequence: all rows) of q, out [tokens, q_heads, dim]
+ * and k, v [tokens, kv_heads, dim] (bf16, strides in elements): o[i, h] = Σ_t softmax_t(s_t) · v_t over the sequence's tokens
+ * t — with `causal` those up to i, and of these the last `window` (0: all; a window needs `causal`) —, s_t = scale · q_i·k_t,
+ * capped to softcap · tanh(s_t / softcap) unless softcap is 0 (or infinite); query head h reads kv head h / (q_heads /
+ * kv_heads). Rows of no sequence are left as they were; a token that is not seen may hold anything. Scores, maxima and sums
+ * fp32; the probabilities are rounded to bf16 (by 2^-8 of each at most) for their product with v, or where few rows make the
+ * call wait for memory, to 17 bits. dim up to 256, a multiple of 8; q, k and v rows 16-byte aligned, out 8-byte (else
+ * SQ8_EUNSUPPORTED). No host copy of `starts` is needed: the call may be captured. */
+int sq8_prompt_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head,
+                         const uint16_t *k, int64_t k_token, int64_t k_head, const uint16_t *v, int64_t v_token, int64_t v_head,
+                         const int32_t *starts, int sequences, float scale, float softcap, int window, int causal,
+                         uint16_t *out, int64_t o_token, int64_t o_head, int tokens, int q_heads, int kv_heads, int dim);
+
+/* **Attention of chunks of new tokens over a paged cache.** Sequence b's new tokens are rows starts[b] .. starts[b + 1] − 1
+ * of q and out, as above, and the last of its lengths[b] cached tokens (int32 [sequences], these included, cut to [0,
+ * max_pages · page]); pages in `table` as sq8_paged_attention. A token sees the cached ones up to its own place, and of
+ * these the last `window` (0: all); one whose place would be before the first (a chunk longer than its length) gets zeros, and
+ * tokens on a page index outside the pools count as masked. The rest as sq8_prompt_attention (for e4m3 dim is a multiple of
+ * 16, rows 16-byte aligned). Units of a sequence that several workgroups share leave partial results in the context's
+ * scratch (sq8_linear says when it grows; its size follows from the arguments here, not from lengths or starts), with
+ * counters as sq8_linear_f8's, so sizes run once before they are captured. */
+int sq8_chunk_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head, const sq8_paged_cache *cache,
+                        const int32_t *table, int64_t table_row, int max_pages, const int32_t *lengths, const int32_t *starts,
+                        int sequences, float scale, float softcap, int window,
+                        uint16_t *out, int64_t o_token, int64_t o_head, int tokens, int q_heads);
+
 /* ---- codes with a scale per block of rows and column: GGUF Q8_0 (w = q · d, one fp16 d per 32
  * consecutive K of an output; Sources/Siliconed/Forge/GGUF.swift, `deinterleaveQ8_0`) ---- */
 

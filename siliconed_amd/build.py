@@ -55,6 +55,9 @@ SOURCES = [
     ("sq8_text_norm.hip", "sq8_text_norm", []),
     ("sq8_f8_gemm.hip", "sq8_f8_gemm", []),
     ("sq8_paged.hip", "sq8_paged", []),
+    *(("sq8_attend_inst.hip", f"sq8_attend_{i}", [f"-DSQ8_SOURCE={i}"]) for i in range(5)),
+    ("sq8_attend.hip", "sq8_attend", []),
+    ("sq8_heads.hip", "sq8_heads", []),
     ("sq8_text_plan.hip", "sq8_text_plan", []),
     ("sq8_text_api.hip", "sq8_text_api", []),
     ("sq8_api.hip", "sq8_api", []),

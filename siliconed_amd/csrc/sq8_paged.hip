@@ -11,12 +11,10 @@
 
 #include "sq8_device.h"
 #include "sq8_text.h"
-#include "sq8_text_quant.h"
+#include "sq8_text_device.h"
 
 namespace sq8 {
 namespace {
-
-__device__ __forceinline__ float bf16_f32(uint32_t bits) { return __uint_as_float(bits << 16); }
 
 // ---- append ------------------------------------------------------------------------------------------------------
 //
@@ -30,68 +28,6 @@ __device__ __forceinline__ float bf16_f32(uint32_t bits) { return __uint_as_floa
 // multiple of 16, W = 1 where not of 8). 8192 tokens of 32 query and
 // 8 key heads of 128 into a bf16 cache (206 MB) take 42.5 µs, 4.8 TB/s where a large copy runs at 5.0; 48 tokens
 // into an e4m3 one 3.2 µs, 2.3 of them the launch.
-template <int W>
-__device__ __forceinline__ void load_run(const uint16_t *src, float (&v)[W]) {
-    if constexpr (W == 1) {
-        v[0] = bf16_f32(src[0]);
-    } else {
-        typename std::conditional<W == 8, u32x4, u32x2>::type d;
-        if constexpr (W == 8) d = *reinterpret_cast<const u32x4_any *>(src);
-        else d = *reinterpret_cast<const u32x2_any *>(src);
-#pragma unroll
-        for (int e = 0; e < W / 2; ++e) {
-            v[2 * e] = bf16_f32(d[e] & 0xFFFFu);
-            v[2 * e + 1] = __uint_as_float(d[e] & 0xFFFF0000u);
-        }
-    }
-}
-
-template <int W>
-__device__ __forceinline__ void load_angles(const float *src, float (&v)[W]) {
-    if constexpr (W == 1) {
-        v[0] = src[0];
-    } else {
-#pragma unroll
-        for (int i = 0; i < W / 4; ++i) {
-            const u32x4 d = reinterpret_cast<const u32x4_any *>(src)[i];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * i + e] = __uint_as_float(d[e]);
-        }
-    }
-}
-
-template <int W>
-__device__ __forceinline__ void store_bf16(uint16_t *dst, const float (&v)[W]) {
-    if constexpr (W == 8)
-        *reinterpret_cast<u32x4_any *>(dst) = u32x4{pack_bf16_rne(v[0], v[1]), pack_bf16_rne(v[2], v[3]), pack_bf16_rne(v[4], v[5]),
-                                                    pack_bf16_rne(v[6], v[7])};
-    else if constexpr (W == 4)
-        *reinterpret_cast<u32x2_any *>(dst) = u32x2{pack_bf16_rne(v[0], v[1]), pack_bf16_rne(v[2], v[3])};
-    else
-        dst[0] = (uint16_t)(pack_bf16_rne(v[0], v[0]) & 0xFFFFu);
-}
-
-template <int W>
-__device__ __forceinline__ void store_e4m3(uint8_t *dst, const float (&v)[W], const Quotient &by) {
-    float q[W];
-#pragma unroll
-    for (int e = 0; e < W; ++e) {
-        const float near = v[e] * by.r;
-        const float t = fabsf(near) < INFINITY ? by.of(v[e]) : near;
-        q[e] = t != t ? t : fminf(fmaxf(t, -448.0f), 448.0f);
-    }
-    if constexpr (W > 1) {
-        auto four = [&](int e) {
-            const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[e], q[e + 1], 0, false);
-            return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[e + 2], q[e + 3], lo, true);
-        };
-        if constexpr (W == 8) *reinterpret_cast<u32x2_any *>(dst) = u32x2{four(0), four(4)};
-        else *reinterpret_cast<u32_any *>(dst) = four(0);
-    } else {
-        dst[0] = (uint8_t)((uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[0], 0, false) & 0xFFu);
-    }
-}
-
 template <int W, bool E4M3>
 __global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs p) {
     const unsigned per_head = (unsigned)p.dim / (2 * W);
@@ -231,33 +167,6 @@ __device__ __forceinline__ Span span_of(const PagedArgs &p, int length) {
     return s;
 }
 
-// How a batch's tiles are shared out: the first `more` of `groups` workgroups take each + 1, the others `each`, in
-// order. (Fewer workgroups of four tiles or more where there are not enough for all: slower, 20 µs against 12 at one
-// sequence of 777.)
-struct Share {
-    int groups, each, more;
-    __device__ __forceinline__ Share() {}
-    __device__ __forceinline__ Share(int total, int most) {
-        groups = min(most, total);
-        each = groups > 0 ? total / groups : 0;
-        more = groups > 0 ? total - each * groups : 0;
-    }
-    __device__ __forceinline__ int first(int g) const { return g * each + min(g, more); }
-    __device__ __forceinline__ int of(int tile) const {
-        return tile < more * (each + 1) ? tile / (each + 1) : more + (tile - more * (each + 1)) / each;
-    }
-};
-
-// The sum of v over this lane and those before it.
-__device__ __forceinline__ int wave_scan(int v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int t = __shfl_up(v, o, 64);
-        if (lane >= o) v += t;
-    }
-    return v;
-}
-
 // The batch's tiles of one head, by 64 sequences at a time in every wave.
 __device__ __forceinline__ int batch_tiles(const PagedArgs &p, int lane) {
     int total = 0;
@@ -324,15 +233,6 @@ __device__ __forceinline__ Raw<N> load_raw(const uint8_t *src) {
     }
     return r;
 }
-
-// Two e4m3 codes (bytes 2W, 2W + 1) as a bf16 pair, exactly.
-template <int W>
-__device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t d) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d, 1.0f, W != 0));
-}
-
-// 1 / l, or 0 where nothing was added (a NaN stays one).
-__device__ __forceinline__ float inverse(float l) { return l > 0.0f ? __fdiv_rn(1.0f, l) : l == 0.0f ? 0.0f : l; }
 
 // The results of workgroups g0 .. g1 over one sequence's head, in that order: the first's in slot `slot0`, the others' in
 // 2g (where a workgroup's tiles begin with that sequence's). A thread takes two values of a query head, side by side in

@@ -1,6 +1,6 @@
 // sq8_text.h — host/device interface of a text decoder's operators: the norm that adds the residual stream and
 // writes 8-bit codes, products of e4m3 codes with a scale per 128 of K, the paged cache's append with the position
-// rotation, and attention of one new token over that cache.
+// rotation, attention of one new token over that cache, heads normed and turned, and attention of prompts and chunks.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -133,12 +133,73 @@ constexpr int paged_held(int dp) { return dp <= 128 ? 2 : 1; }                  
 // A slot: maxima and sums [16][2], outputs [dp / 32][4][4][live][2]: pair, register and row of the first wave's lanes, head.
 __host__ __device__ constexpr int paged_part_floats(int dp) { return 32 + 16 * dp; }
 // sq8_text_plan.hip.
-void page_divisor(PagedArgs &p);
+void page_divisor(int page, uint64_t &mul, int &shift);
 // The workgroups a call of these sizes takes, and the partial results' bytes they need.
 int paged_groups(const PagedArgs &p, int cus);
 int64_t paged_part_bytes(const PagedArgs &p, int groups);
 int64_t paged_marks(const PagedArgs &p);
 hipError_t launch_zero_marks(int *marks, int64_t count, hipStream_t stream);
 hipError_t launch_paged_attention(const PagedArgs &p, bool e4m3, int groups, hipStream_t stream);
+
+// sq8_heads.hip. Strides in elements.
+struct HeadsArgs {
+    const uint16_t *q, *k, *v;          // bf16 [tokens, heads, dim]; v with a cache only
+    uint16_t *q_out, *k_out;            // k_out without a cache only
+    void *kc, *vc;                      // the cache's pools, or null
+    const float *k_scale, *v_scale;
+    const float *q_norm, *k_norm;       // [dim], or null: not normed
+    const float *table;                 // as AppendArgs
+    const int32_t *positions, *slots;
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head, qo_tok, qo_head, ko_tok, ko_head;
+    int64_t kc_page, kc_tok, kc_head, vc_page, vc_tok, vc_head, table_row;
+    int64_t slot_count;
+    float eps;
+    int tokens, q_heads, kv_heads, dim, rot, page, max_position;
+    int interleaved;
+    int lanes_log;                      // launch_norm_heads' own
+};
+constexpr int kNormHeadDim = 512;
+hipError_t launch_norm_heads(HeadsArgs p, bool e4m3, hipStream_t stream);
+
+// sq8_attend_kernel.h: attention of prompts over their own keys and values (pages null), or of chunks over a paged cache.
+struct AttendArgs {
+    const uint16_t *q;                  // bf16 [tokens, q_heads, dim]
+    const uint8_t *kc, *vc;             // bf16 [tokens, kv_heads, dim] (kc_page unused), or the cache's pools
+    const float *k_scale, *v_scale;
+    const int32_t *starts;              // [sequences + 1], or null: one sequence of all tokens
+    const int32_t *pages;               // [sequences, max_pages]
+    const int32_t *lengths;             // [sequences]
+    uint16_t *out;
+    float *part;                        // partial results of shared units
+    int *marks;                         // a counter a workgroup, zero before and after every call
+    int64_t q_tok, q_head, o_tok, o_head;
+    int64_t kc_page, kc_tok, kc_head, vc_page, vc_tok, vc_head, pages_row;
+    float scale, softcap;
+    int tokens, sequences, kv_heads, group, dim, page, page_count, max_pages, window, causal;
+    int share;                          // units are shared out over the workgroups
+    uint64_t page_mul;
+    int page_shift;
+};
+constexpr int attend_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }  // the instance of a head's size
+// Tokens of a tile, of WM sets of 32 rows and WT waves that share its tokens: a stage of 32 KB, or 64.
+constexpr int attend_tokens(int dp, int wm, int wt) { return dp == 64 ? (wt == 4 ? 256 : 128) : dp == 128 ? (wt == 4 ? 128 : 64) : 64; }
+// Waves a SIMD holds: two tiles' stages fit a CU's LDS, or one of 64 KB.
+constexpr int attend_waves(int dp, int wm, int wt) { return dp == 256 || wt == 4 ? 1 : 2; }
+// A slot of a shared unit: maxima and sums [rows][2], outputs.
+__host__ __device__ constexpr int attend_part_floats(int dp, int wm) { return 32 * wm * (2 + dp); }
+// sq8_text_plan.hip. The tile and the workgroups that a call takes, and what it needs of the context's buffers.
+struct AttendPlan {
+    int wm, groups, share;
+    int64_t part_bytes, marks;
+};
+AttendPlan attend_plan(const AttendArgs &p, int cus);
+hipError_t launch_attend(const AttendArgs &p, const AttendPlan &plan, bool e4m3, hipStream_t stream);
+namespace attend {
+// Where keys and values lie: rows of a projection; pages whose tokens are a multiple of 16 (16 tokens lie in one page); any
+// pages; in bf16 or e4m3.
+enum Source { ROWS = 0, PAGES16, PAGES, PAGES16_F8, PAGES_F8 };
+template <int SOURCE>
+hipError_t launch_source(const AttendArgs &p, const AttendPlan &plan, hipStream_t stream);
+}  // namespace attend
 
 }  // namespace sq8

@@ -152,6 +152,39 @@ int check_cache(const sq8_paged_cache *c, int q_heads) {
     return SQ8_OK;
 }
 
+// What prompt and chunk attention share once their keys and values are described: q, out and the call's sizes.
+int run_attend(sq8_ctx *ctx, sq8::AttendArgs &p, const uint16_t *q, int64_t q_token, int64_t q_head, float scale, float softcap,
+               uint16_t *out, int64_t o_token, int64_t o_head, int tokens, int sequences, int q_heads, bool e4m3) {
+    if (q_token < 0 || q_head < 0 || o_token < 0 || o_head < 0) return SQ8_EINVAL;
+    if (p.dim > 256 || p.dim % 8 != 0) return SQ8_EUNSUPPORTED;
+    if (!aligned(q, 16) || !aligned(out, 8) || (q_token | q_head) % 8 != 0 || (o_token | o_head) % 4 != 0) return SQ8_EUNSUPPORTED;
+    p.group = q_heads / p.kv_heads;
+    // Rows, and the tiles of keys of all tiles of rows, are 32-bit.
+    const double longest = p.pages ? (double)p.max_pages * p.page : (double)tokens;
+    const double rows = (double)tokens * p.group;
+    if (rows > INT32_MAX - 4096 || (rows / 32 + sequences) * p.kv_heads * (p.pages ? longest / 64 + 2 : 1.0) > INT32_MAX) return SQ8_EUNSUPPORTED;
+    // (As sq8_paged_attention: a cap that no score comes near is none, a tiny one averages.)
+    if (softcap > 0x1p100f) softcap = 0.0f;
+    else if (softcap > 0.0f && softcap < 0x1p-60f) softcap = 0x1p-60f;
+    DeviceScope scope(ctx->device);
+    if (scope.error != hipSuccess) return hip_status(scope.error);
+    p.q = q; p.out = out;
+    p.q_tok = q_token; p.q_head = q_head; p.o_tok = o_token; p.o_head = o_head;
+    p.scale = scale; p.softcap = softcap;
+    p.tokens = tokens; p.sequences = sequences;
+    sq8::page_divisor(p.page, p.page_mul, p.page_shift);
+    const sq8::AttendPlan plan = sq8::attend_plan(p, ctx->cus);
+    p.share = plan.share;
+    if (plan.part_bytes > 0) {
+        int st = reserve(ctx, ctx->part, (size_t)plan.part_bytes);
+        if (st != SQ8_OK) return st;
+        p.part = static_cast<float *>(ctx->part.at);
+        st = reserve_marks(ctx, plan.marks, p.marks);
+        if (st != SQ8_OK) return st;
+    }
+    return hip_status(sq8::launch_attend(p, plan, e4m3, ctx->stream));
+}
+
 }  // namespace
 
 extern "C" {
@@ -284,7 +317,7 @@ int sq8_paged_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_
     p.scale = scale; p.softcap = softcap;
     p.batch = batch; p.q_heads = q_heads; p.kv_heads = cache->kv_heads; p.dim = cache->dim;
     p.page = cache->page; p.page_count = cache->pages; p.max_pages = max_pages; p.window = window;
-    sq8::page_divisor(p);
+    sq8::page_divisor(p.page, p.page_mul, p.page_shift);
     const int groups = sq8::paged_groups(p, ctx->cus);
     const int64_t bytes = sq8::paged_part_bytes(p, groups);
     if (bytes > 0) {
@@ -295,6 +328,130 @@ int sq8_paged_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_
         if (st != SQ8_OK) return st;
     }
     return hip_status(sq8::launch_paged_attention(p, e4m3, groups, ctx->stream));
+}
+
+int sq8_norm_append_kv(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head, const uint16_t *k, int64_t k_token,
+                       int64_t k_head, const uint16_t *v, int64_t v_token, int64_t v_head, uint16_t *q_out, int64_t qo_token,
+                       int64_t qo_head, const sq8_paged_cache *cache, const int32_t *positions, const int32_t *slots,
+                       const float *table, int64_t table_row, int max_position, int rot, int interleaved, const float *q_norm,
+                       const float *k_norm, float eps, int tokens, int q_heads) {
+    if (!ctx || tokens < 0 || rot < 0) return SQ8_EINVAL;
+    const int st = check_cache(cache, q_heads);
+    if (st != SQ8_OK) return st;
+    if (rot > cache->dim) return SQ8_EINVAL;
+    if (cache->dim % 2 != 0 || rot % 2 != 0 || cache->dim > sq8::kNormHeadDim) return SQ8_EUNSUPPORTED;
+    if (tokens == 0) return SQ8_OK;
+    if (!q || !k || !v || !q_out || !slots || (rot > 0 && (!positions || !table || max_position <= 0 || table_row < rot)))
+        return SQ8_EINVAL;
+    if (q_token < 0 || q_head < 0 || k_token < 0 || k_head < 0 || v_token < 0 || v_head < 0 || qo_token < 0 || qo_head < 0)
+        return SQ8_EINVAL;
+    const int64_t slot_count = (int64_t)cache->pages * cache->page;
+    DeviceScope scope(ctx->device);
+    if (scope.error != hipSuccess) return hip_status(scope.error);
+    sq8::HeadsArgs p;
+    memset(&p, 0, sizeof(p));
+    p.q = q; p.k = k; p.v = v; p.q_out = q_out;
+    p.kc = cache->k; p.vc = cache->v;
+    if (slot_count == 0) p.kc = q_out;  // (no slot is inside: not written)
+    p.k_scale = cache->k_scale; p.v_scale = cache->v_scale;
+    p.q_norm = q_norm; p.k_norm = k_norm;
+    p.table = table; p.positions = positions; p.slots = slots;
+    p.q_tok = q_token; p.q_head = q_head; p.k_tok = k_token; p.k_head = k_head; p.v_tok = v_token; p.v_head = v_head;
+    p.qo_tok = qo_token; p.qo_head = qo_head;
+    p.kc_page = cache->k_page; p.kc_tok = cache->k_token; p.kc_head = cache->k_head;
+    p.vc_page = cache->v_page; p.vc_tok = cache->v_token; p.vc_head = cache->v_head;
+    p.table_row = table_row;
+    p.slot_count = slot_count;
+    p.eps = eps;
+    p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = cache->kv_heads; p.dim = cache->dim; p.rot = rot;
+    p.page = cache->page; p.max_position = max_position; p.interleaved = interleaved != 0;
+    const hipError_t e = sq8::launch_norm_heads(p, cache->dtype == SQ8_FP8_E4M3, ctx->stream);
+    return e == hipErrorInvalidValue ? SQ8_EUNSUPPORTED : hip_status(e);
+}
+
+int sq8_norm_rotate(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head, const uint16_t *k, int64_t k_token,
+                    int64_t k_head, uint16_t *q_out, int64_t qo_token, int64_t qo_head, uint16_t *k_out, int64_t ko_token,
+                    int64_t ko_head, const int32_t *positions, const float *table, int64_t table_row, int max_position, int rot,
+                    int interleaved, const float *q_norm, const float *k_norm, float eps, int tokens, int q_heads, int kv_heads,
+                    int dim) {
+    if (!ctx || tokens < 0 || rot < 0 || q_heads < 0 || kv_heads < 0 || dim < 0 || rot > dim) return SQ8_EINVAL;
+    if (dim % 2 != 0 || rot % 2 != 0 || dim > sq8::kNormHeadDim) return SQ8_EUNSUPPORTED;
+    if (tokens == 0 || dim == 0 || (q_heads == 0 && kv_heads == 0)) return SQ8_OK;
+    if ((q_heads > 0 && (!q || !q_out)) || (kv_heads > 0 && (!k || !k_out))) return SQ8_EINVAL;
+    if (rot > 0 && (!positions || !table || max_position <= 0 || table_row < rot)) return SQ8_EINVAL;
+    if (q_token < 0 || q_head < 0 || k_token < 0 || k_head < 0 || qo_token < 0 || qo_head < 0 || ko_token < 0 || ko_head < 0)
+        return SQ8_EINVAL;
+    if ((int64_t)q_heads + kv_heads > INT32_MAX) return SQ8_EUNSUPPORTED;
+    DeviceScope scope(ctx->device);
+    if (scope.error != hipSuccess) return hip_status(scope.error);
+    sq8::HeadsArgs p;
+    memset(&p, 0, sizeof(p));
+    p.q = q; p.k = k; p.q_out = q_out; p.k_out = k_out;
+    p.q_norm = q_norm; p.k_norm = k_norm;
+    p.table = table; p.positions = positions;
+    p.q_tok = q_token; p.q_head = q_head; p.k_tok = k_token; p.k_head = k_head;
+    p.qo_tok = qo_token; p.qo_head = qo_head; p.ko_tok = ko_token; p.ko_head = ko_head;
+    p.table_row = table_row;
+    p.eps = eps;
+    p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = kv_heads; p.dim = dim; p.rot = rot;
+    p.page = 1; p.max_position = max_position; p.interleaved = interleaved != 0;
+    const hipError_t e = sq8::launch_norm_heads(p, false, ctx->stream);
+    return e == hipErrorInvalidValue ? SQ8_EUNSUPPORTED : hip_status(e);
+}
+
+int sq8_prompt_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head, const uint16_t *k, int64_t k_token,
+                         int64_t k_head, const uint16_t *v, int64_t v_token, int64_t v_head, const int32_t *starts, int sequences,
+                         float scale, float softcap, int window, int causal, uint16_t *out, int64_t o_token, int64_t o_head,
+                         int tokens, int q_heads, int kv_heads, int dim) {
+    if (!ctx || tokens < 0 || sequences < 0 || dim <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0)
+        return SQ8_EINVAL;
+    if (!starts && sequences > 1) return SQ8_EINVAL;
+    if (window < 0 || (window > 0 && !causal) || !(softcap >= 0.0f)) return SQ8_EINVAL;
+    if (tokens == 0 || sequences == 0) return SQ8_OK;
+    if (!q || !k || !v || !out) return SQ8_EINVAL;
+    if (k_token < 0 || k_head < 0 || v_token < 0 || v_head < 0) return SQ8_EINVAL;
+    if (!aligned(k, 16) || !aligned(v, 16) || (k_token | k_head | v_token | v_head) % 8 != 0) return SQ8_EUNSUPPORTED;
+    sq8::AttendArgs p;
+    memset(&p, 0, sizeof(p));
+    p.kc = reinterpret_cast<const uint8_t *>(k);
+    p.vc = reinterpret_cast<const uint8_t *>(v);
+    p.kc_tok = k_token; p.kc_head = k_head; p.vc_tok = v_token; p.vc_head = v_head;
+    p.starts = starts;
+    p.page = 1;
+    p.kv_heads = kv_heads; p.dim = dim; p.window = window; p.causal = causal != 0;
+    return run_attend(ctx, p, q, q_token, q_head, scale, softcap, out, o_token, o_head, tokens, sequences, q_heads, false);
+}
+
+int sq8_chunk_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head, const sq8_paged_cache *cache,
+                        const int32_t *table, int64_t table_row, int max_pages, const int32_t *lengths, const int32_t *starts,
+                        int sequences, float scale, float softcap, int window, uint16_t *out, int64_t o_token, int64_t o_head,
+                        int tokens, int q_heads) {
+    if (!ctx || tokens < 0 || sequences < 0 || max_pages < 0 || window < 0 || !(softcap >= 0.0f)) return SQ8_EINVAL;
+    const int st = check_cache(cache, q_heads);
+    if (st != SQ8_OK) return st;
+    if (q_heads % cache->kv_heads != 0) return SQ8_EINVAL;
+    if (!starts && sequences > 1) return SQ8_EINVAL;
+    const bool e4m3 = cache->dtype == SQ8_FP8_E4M3;
+    if (e4m3 && cache->dim % 16 != 0) return SQ8_EUNSUPPORTED;
+    if ((int64_t)max_pages * cache->page > INT32_MAX - 4096) return SQ8_EUNSUPPORTED;  // token numbers are 32-bit
+    if (tokens == 0 || sequences == 0) return SQ8_OK;
+    if (!q || !out || !lengths || (max_pages > 0 && (!table || table_row < max_pages))) return SQ8_EINVAL;
+    const int64_t caches = cache->k_page | cache->k_token | cache->k_head | cache->v_page | cache->v_token | cache->v_head;
+    if (!aligned(cache->k, 16) || !aligned(cache->v, 16) || caches % (e4m3 ? 16 : 8) != 0) return SQ8_EUNSUPPORTED;
+    sq8::AttendArgs p;
+    memset(&p, 0, sizeof(p));
+    p.kc = static_cast<const uint8_t *>(cache->k);
+    p.vc = static_cast<const uint8_t *>(cache->v);
+    p.k_scale = cache->k_scale; p.v_scale = cache->v_scale;
+    p.kc_page = cache->k_page; p.kc_tok = cache->k_token; p.kc_head = cache->k_head;
+    p.vc_page = cache->v_page; p.vc_tok = cache->v_token; p.vc_head = cache->v_head;
+    p.starts = starts; p.lengths = lengths;
+    p.pages = table ? table : lengths;  // (with no pages, none is read)
+    p.pages_row = table_row;
+    p.max_pages = cache->pages == 0 ? 0 : max_pages;  // pages to read with no pool to read them from
+    p.page = cache->page; p.page_count = cache->pages;
+    p.kv_heads = cache->kv_heads; p.dim = cache->dim; p.window = window; p.causal = 1;
+    return run_attend(ctx, p, q, q_token, q_head, scale, softcap, out, o_token, o_head, tokens, sequences, q_heads, e4m3);
 }
 
 }  // extern "C"

@@ -87,11 +87,11 @@ F8Plan f8_plan(const F8Args &p, bool glu, bool out_f32, int cus) {
 
 // n / page for n < 2^31 as (n · mul) >> shift: s with 2^(s-1) < page ≤ 2^s, mul = floor(2^(31+s) / page) + 1 ≤ 2^32 + 1,
 // the product's excess under n / 2^(31+s) < 2^-s ≤ 1/page.
-void page_divisor(PagedArgs &p) {
+void page_divisor(int page, uint64_t &mul, int &shift) {
     int s = 0;
-    while ((1ll << s) < p.page) ++s;
-    p.page_shift = 31 + s;
-    p.page_mul = ((1ull << (31 + s)) / (uint64_t)p.page) + 1;
+    while ((1ll << s) < page) ++s;
+    shift = 31 + s;
+    mul = ((1ull << (31 + s)) / (uint64_t)page) + 1;
 }
 
 int paged_groups(const PagedArgs &p, int cus) {
@@ -108,5 +108,33 @@ int64_t paged_part_bytes(const PagedArgs &p, int groups) {
 }
 
 int64_t paged_marks(const PagedArgs &p) { return (int64_t)MARK * p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16); }
+
+AttendPlan attend_plan(const AttendArgs &p, int cus) {
+    AttendPlan plan = {4, 0, 0, 0, 0};
+    if (p.sequences <= 0 || p.tokens <= 0) return plan;
+    const int dp = attend_dim(p.dim);
+    const int64_t rows = (int64_t)p.tokens * p.group, each = (rows + p.sequences - 1) / p.sequences;
+    auto units = [&](int wm) { return (rows / (32 * wm) + p.sequences) * p.kv_heads; };  // at most
+    plan.share = p.pages != nullptr;
+    if (plan.share) {
+        plan.wm = each <= 32 ? 1 : each <= 64 ? 2 : each <= 128 ? 4 : 8;
+    } else {
+        auto some = [&](int wm) { return (each + 32 * wm - 1) / (32 * wm) * p.sequences * p.kv_heads; };  // if all were alike
+        plan.wm = some(8) >= cus ? 8 : some(4) >= cus ? 4 : some(2) >= cus ? 2 : 1;
+    }
+    if (dp == 256) plan.wm = plan.wm < 2 ? 2 : plan.wm > 4 ? 4 : plan.wm;
+    const int wt = plan.wm >= 4 ? 1 : plan.wm == 2 ? 2 : 4;
+    if (!plan.share) {
+        plan.groups = (int)units(plan.wm);
+        return plan;
+    }
+    const int tokens = attend_tokens(dp, plan.wm, wt), held = attend_waves(dp, plan.wm, wt) * 4 / (plan.wm * wt);
+    const int64_t longest = (int64_t)p.max_pages * p.page;
+    const int64_t most = units(plan.wm) * std::max<int64_t>(1, (longest + tokens - 1) / tokens), full = (int64_t)held * cus;
+    plan.groups = (int)std::min(most, full);
+    plan.part_bytes = (int64_t)2 * plan.groups * attend_part_floats(dp, plan.wm) * 4;
+    plan.marks = (int64_t)MARK * plan.groups;
+    return plan;
+}
 
 }  // namespace sq8

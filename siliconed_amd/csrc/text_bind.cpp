@@ -32,6 +32,10 @@ struct Entries {
     decltype(&sq8_linear_f8_quantized) linear_f8_quantized;
     decltype(&sq8_append_kv) append_kv;
     decltype(&sq8_paged_attention) paged_attention;
+    decltype(&sq8_norm_append_kv) norm_append_kv;
+    decltype(&sq8_norm_rotate) norm_rotate;
+    decltype(&sq8_prompt_attention) prompt_attention;
+    decltype(&sq8_chunk_attention) chunk_attention;
     decltype(&sq8_device) device;
 } entries;
 
@@ -345,6 +349,162 @@ PyObject *paged_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// A position table: its rows, positions and turned values.
+struct Table {
+    const float *at;
+    int64_t row;
+    int most, rot;
+};
+Table table_of(const Tensor &t) {
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat, "table must be float32 [positions, rot]");
+    const int64_t row = rows_of(t, "table");
+    return {static_cast<const float *>(t.data_ptr()), row, count32(t.size(0), "table"), count32(t.size(1), "table")};
+}
+const float *norm_of(const Tensor *t, int64_t dim, const char *what) { return t ? vector_of<float>(*t, dim, what) : nullptr; }
+
+// ctx, q, k, v, cache, positions, slots, table, q_norm, k_norm, eps, q_out, interleaved → q_out
+PyObject *norm_append_kv(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 13);
+    sq8_ctx *const ctx = context(a[0]);
+    const Tensor &q = tensor(a[1], "q"), &k = tensor(a[2], "k"), &v = tensor(a[3], "v");
+    const sq8_paged_cache cache = held<sq8_paged_cache>(a[4], "a cache's description");
+    const Tensor &positions = tensor(a[5], "positions"), &slots = tensor(a[6], "slots"), &table = tensor(a[7], "table");
+    const Tensor *const q_norm = maybe(a[8], "q_norm"), *const k_norm = maybe(a[9], "k_norm");
+    const float eps = (float)number(a[10]);
+    const int64_t tokens = queries(q), heads = q.size(1);
+    Tensor out = a[11] == Py_None ? at::empty({tokens, heads, cache.dim}, q.options()) : tensor(a[11], "q_out");
+    const Heads qh = heads_of(q, "q", tokens, heads, cache.dim), kh = heads_of(k, "k", tokens, cache.kv_heads, cache.dim);
+    const Heads vh = heads_of(v, "v", tokens, cache.kv_heads, cache.dim), oh = heads_of(out, "q_out", tokens, heads, cache.dim);
+    const Table angles = table_of(table);
+    const int32_t *const at = vector_of<int32_t>(positions, tokens, "positions"), *const to = vector_of<int32_t>(slots, tokens, "slots");
+    const float *const qn = norm_of(q_norm, cache.dim, "q_norm"), *const kn = norm_of(k_norm, cache.dim, "k_norm");
+    const int interleaved = truth(a[12]), t32 = count32(tokens, "q"), h32 = count32(heads, "q");
+    on_device(ctx, {{&q, "q"}, {&k, "k"}, {&v, "v"}, {&positions, "positions"}, {&slots, "slots"}, {&table, "table"},
+                    {q_norm, "q_norm"}, {k_norm, "k_norm"}, {&out, "q_out"}});
+    const int status = call([&] {
+        return entries.norm_append_kv(ctx, qh.at, qh.row, qh.head, kh.at, kh.row, kh.head, vh.at, vh.row, vh.head, oh.at, oh.row, oh.head,
+                                      &cache, at, to, angles.at, angles.row, angles.most, angles.rot, interleaved, qn, kn, eps, t32, h32);
+    });
+    if (status != SQ8_OK) return PyLong_FromLong(status);
+    return a[11] == Py_None ? give(std::move(out)) : same(a[11]);
+    END_HANDLE_TH_ERRORS
+}
+
+// ctx, q, k (or None), positions, table (None with positions: not turned), q_norm, k_norm, eps, q_out, k_out, interleaved →
+// (q_out, k_out)
+PyObject *norm_rotate(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 11);
+    sq8_ctx *const ctx = context(a[0]);
+    const Tensor &q = tensor(a[1], "q");
+    const Tensor *const k = maybe(a[2], "k"), *const positions = maybe(a[3], "positions"), *const table = maybe(a[4], "table");
+    const Tensor *const q_norm = maybe(a[5], "q_norm"), *const k_norm = maybe(a[6], "k_norm");
+    const float eps = (float)number(a[7]);
+    const int64_t tokens = queries(q), heads = q.size(1), dim = q.size(2), kv_heads = k && k->dim() == 3 ? k->size(1) : 0;
+    Tensor q_out = a[8] == Py_None ? at::empty({tokens, heads, dim}, q.options()) : tensor(a[8], "q_out"), k_out;
+    const Heads qh = heads_of(q, "q", tokens, heads, dim), oh = heads_of(q_out, "q_out", tokens, heads, dim);
+    Heads kh{}, ko{};
+    TORCH_CHECK_VALUE(k || (a[9] == Py_None && !k_norm), "k_out and k_norm belong to k");
+    if (k) {
+        kh = heads_of(*k, "k", tokens, kv_heads, dim);
+        k_out = a[9] == Py_None ? at::empty({tokens, kv_heads, dim}, k->options()) : tensor(a[9], "k_out");
+        ko = heads_of(k_out, "k_out", tokens, kv_heads, dim);
+    }
+    TORCH_CHECK_VALUE(!positions == !table, "positions and table belong together");
+    Table angles{};
+    const int32_t *at = nullptr;
+    if (table) {
+        angles = table_of(*table);
+        at = vector_of<int32_t>(*positions, tokens, "positions");
+    }
+    const float *const qn = norm_of(q_norm, dim, "q_norm"), *const kn = norm_of(k_norm, dim, "k_norm");
+    const int interleaved = truth(a[10]), t32 = count32(tokens, "q"), h32 = count32(heads, "q"), kv32 = count32(kv_heads, "k");
+    const int d32 = count32(dim, "q");
+    on_device(ctx, {{&q, "q"}, {k, "k"}, {positions, "positions"}, {table, "table"}, {q_norm, "q_norm"}, {k_norm, "k_norm"},
+                    {&q_out, "q_out"}, {k ? &k_out : nullptr, "k_out"}});
+    const int status = call([&] {
+        return entries.norm_rotate(ctx, qh.at, qh.row, qh.head, kh.at, kh.row, kh.head, oh.at, oh.row, oh.head, ko.at, ko.row, ko.head,
+                                   at, angles.at, angles.row, angles.most, angles.rot, interleaved, qn, kn, eps, t32, h32, kv32, d32);
+    });
+    if (status != SQ8_OK) return PyLong_FromLong(status);
+    PyObject *const all = PyTuple_New(2);
+    if (!all) throw python_error();
+    PyTuple_SET_ITEM(all, 0, a[8] == Py_None ? give(std::move(q_out)) : same(a[8]));
+    PyTuple_SET_ITEM(all, 1, k && a[9] == Py_None ? give(std::move(k_out)) : same(a[9]));
+    return all;
+    END_HANDLE_TH_ERRORS
+}
+
+// Where a batch's sequences begin: [sequences + 1], or null with one sequence of all rows.
+const int32_t *starts_of(const Tensor *t, int64_t &sequences) {
+    if (!t) {
+        sequences = 1;
+        return nullptr;
+    }
+    TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) >= 1, "starts must be int32 [sequences + 1]");
+    sequences = t->size(0) - 1;
+    return vector_of<int32_t>(*t, t->size(0), "starts");
+}
+
+// ctx, q, k, v, starts (None: one sequence), scale (None: 1/sqrt(dim)), softcap, window, causal, out → out
+PyObject *prompt_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 10);
+    sq8_ctx *const ctx = context(a[0]);
+    const Tensor &q = tensor(a[1], "q"), &k = tensor(a[2], "k"), &v = tensor(a[3], "v");
+    const Tensor *const starts = maybe(a[4], "starts");
+    const int64_t tokens = queries(q), heads = q.size(1), dim = q.size(2);
+    TORCH_CHECK_VALUE(k.dim() == 3, "k must be [tokens, kv heads, dim], not ", k.sizes());
+    const int64_t kv_heads = k.size(1);
+    Tensor out = a[9] == Py_None ? at::empty({tokens, heads, dim}, q.options()) : tensor(a[9], "out");
+    const Heads qh = heads_of(q, "q", tokens, heads, dim), kh = heads_of(k, "k", tokens, kv_heads, dim);
+    const Heads vh = heads_of(v, "v", tokens, kv_heads, dim), oh = heads_of(out, "out", tokens, heads, dim);
+    int64_t sequences;
+    const int32_t *const from = starts_of(starts, sequences);
+    const float scale = (float)(a[5] == Py_None ? 1.0 / std::sqrt((double)dim) : number(a[5])), softcap = (float)number(a[6]);
+    const int window = integer(a[7]), causal = truth(a[8]), t32 = count32(tokens, "q"), h32 = count32(heads, "q");
+    const int kv32 = count32(kv_heads, "k"), d32 = count32(dim, "q"), s32 = count32(sequences, "starts");
+    on_device(ctx, {{&q, "q"}, {&k, "k"}, {&v, "v"}, {starts, "starts"}, {&out, "out"}});
+    const int status = call([&] {
+        return entries.prompt_attention(ctx, qh.at, qh.row, qh.head, kh.at, kh.row, kh.head, vh.at, vh.row, vh.head, from, s32, scale,
+                                        softcap, window, causal, oh.at, oh.row, oh.head, t32, h32, kv32, d32);
+    });
+    if (status != SQ8_OK) return PyLong_FromLong(status);
+    return a[9] == Py_None ? give(std::move(out)) : same(a[9]);
+    END_HANDLE_TH_ERRORS
+}
+
+// ctx, q, cache, pages, lengths, starts (None: one sequence), scale (None: 1/sqrt(dim)), softcap, window, out → out
+PyObject *chunk_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 10);
+    sq8_ctx *const ctx = context(a[0]);
+    const Tensor &q = tensor(a[1], "q"), &pages = tensor(a[3], "pages"), &lengths = tensor(a[4], "lengths");
+    const sq8_paged_cache cache = held<sq8_paged_cache>(a[2], "a cache's description");
+    const Tensor *const starts = maybe(a[5], "starts");
+    const int64_t tokens = queries(q), heads = q.size(1);
+    Tensor out = a[9] == Py_None ? at::empty({tokens, heads, cache.dim}, q.options()) : tensor(a[9], "out");
+    const Heads qh = heads_of(q, "q", tokens, heads, cache.dim), oh = heads_of(out, "out", tokens, heads, cache.dim);
+    int64_t sequences;
+    const int32_t *const from = starts_of(starts, sequences);
+    TORCH_CHECK_VALUE(pages.scalar_type() == at::kInt && pages.dim() == 2 && pages.size(0) == sequences, "pages must be int32 [",
+                      sequences, ", most pages]");
+    const int64_t row = rows_of(pages, "pages");
+    const int32_t *const held_tokens = vector_of<int32_t>(lengths, sequences, "lengths");
+    const float scale = (float)(a[6] == Py_None ? 1.0 / std::sqrt((double)cache.dim) : number(a[6])), softcap = (float)number(a[7]);
+    const int window = integer(a[8]), most = count32(pages.size(1), "pages"), t32 = count32(tokens, "q"), h32 = count32(heads, "q");
+    const int s32 = count32(sequences, "starts");
+    on_device(ctx, {{&q, "q"}, {&pages, "pages"}, {&lengths, "lengths"}, {starts, "starts"}, {&out, "out"}});
+    const int status = call([&] {
+        return entries.chunk_attention(ctx, qh.at, qh.row, qh.head, &cache, static_cast<const int32_t *>(pages.data_ptr()), row, most,
+                                       held_tokens, from, s32, scale, softcap, window, oh.at, oh.row, oh.head, t32, h32);
+    });
+    if (status != SQ8_OK) return PyLong_FromLong(status);
+    return a[9] == Py_None ? give(std::move(out)) : same(a[9]);
+    END_HANDLE_TH_ERRORS
+}
+
 // The library's entries: their addresses, in the order of Entries.
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -365,7 +525,8 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 #define TEXT_OP(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {TEXT_OP(bind), TEXT_OP(add_norm_quantized), TEXT_OP(quantize_groups), TEXT_OP(product_f8),
-                         TEXT_OP(append_kv), TEXT_OP(paged_attention), {nullptr, nullptr, 0, nullptr}};
+                         TEXT_OP(append_kv), TEXT_OP(paged_attention), TEXT_OP(norm_append_kv), TEXT_OP(norm_rotate),
+                         TEXT_OP(prompt_attention), TEXT_OP(chunk_attention), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_text_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

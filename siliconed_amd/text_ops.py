@@ -150,3 +150,40 @@ class TextOps:
         1/sqrt(dim); `softcap` c > 0 (inf: none): scores c · tanh(s/c); `window` w > 0: the last w tokens only."""
         return _done(abi.text.paged_attention(self._h, q, self._args_of(cache), pages, lengths, scale, softcap, window, out),
                      "sq8_paged_attention")
+
+    def norm_append_kv(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedCache, positions: torch.Tensor,
+                       slots: torch.Tensor, table: torch.Tensor, *, q_norm: Optional[torch.Tensor] = None,
+                       k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, q_out: Optional[torch.Tensor] = None,
+                       interleaved: bool = False) -> torch.Tensor:
+        """append_kv with every query and key head's RMS norm (times `q_norm`, `k_norm` float32 [dim]; None: not normed) before
+        its turn, in the same pass: nothing is rounded in between. Heads of up to 512."""
+        return _done(abi.text.norm_append_kv(self._h, q, k, v, self._args_of(cache), positions, slots, table, q_norm, k_norm, eps,
+                                             q_out, interleaved), "sq8_norm_append_kv")
+
+    def norm_rotate(self, q: torch.Tensor, k: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                    table: Optional[torch.Tensor] = None, *, q_norm: Optional[torch.Tensor] = None,
+                    k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, q_out: Optional[torch.Tensor] = None,
+                    k_out: Optional[torch.Tensor] = None, interleaved: bool = False):
+        """The same without a cache: q [tokens, q_heads, dim] and k [tokens, kv_heads, dim] (None: q alone) normed and turned:
+        (q_out, k_out), which may be q and k themselves. No positions and table: normed only."""
+        return _done(abi.text.norm_rotate(self._h, q, k, positions, table, q_norm, k_norm, eps, q_out, k_out, interleaved),
+                     "sq8_norm_rotate")
+
+    def prompt_attention(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: Optional[torch.Tensor] = None, *,
+                         causal: bool = True, scale: Optional[float] = None, softcap: float = 0.0, window: int = 0,
+                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of whole sequences over their own keys and values: q [tokens, q_heads, dim], k and v [tokens, kv_heads,
+        dim] (bf16, any row and head strides of whole 16 bytes), sequence b in rows starts[b] to starts[b + 1] − 1 (`starts`
+        int32 [sequences + 1] on the GPU; None: one sequence). `causal`: a token sees those up to itself, with `window` w > 0
+        the last w of them; else all of its sequence. Rows of no sequence are left as they were: of an `out` that the call
+        allocates, anything. `scale` and `softcap` as paged_attention."""
+        return _done(abi.text.prompt_attention(self._h, q, k, v, starts, scale, softcap, window, causal, out), "sq8_prompt_attention")
+
+    def chunk_attention(self, q: torch.Tensor, cache: PagedCache, pages: torch.Tensor, lengths: torch.Tensor,
+                        starts: Optional[torch.Tensor] = None, *, scale: Optional[float] = None, softcap: float = 0.0,
+                        window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of each sequence's newest tokens over its cached ones, these included: q [tokens, q_heads, dim] (bf16) in
+        rows as prompt_attention's (`starts`), `pages` int32 [sequences, most pages] and `lengths` int32 [sequences] as
+        paged_attention's. A draft to verify, a piece of a long prompt, or both in one batch."""
+        return _done(abi.text.chunk_attention(self._h, q, self._args_of(cache), pages, lengths, starts, scale, softcap, window, out),
+                     "sq8_chunk_attention")
