@@ -520,6 +520,20 @@ int sq8_chunk_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_
                         int sequences, float scale, float softcap, int window,
                         uint16_t *out, int64_t o_token, int64_t o_head, int tokens, int q_heads);
 
+/* **Drawing the next token.** For each row of logits [rows, vocab] (SQ8_BF16 or SQ8_F32, leading dimension ld): weights w_i =
+ * exp((x_i − max x) / temperature); of the tokens in the order of falling logit, equal ones by index, the first top_k (0 or
+ * less: all), of these the fewest that hold top_p of their sum (1 or more: all), of these the ones with w ≥ min_p; then, by
+ * index, the first whose running sum of weights passes uniform · their whole. The first of the order is always kept. A
+ * temperature of 0 or less, or a top_k of 1, takes it. temperature, top_p, min_p fp32 [rows], top_k int32 [rows]: NULL for 1,
+ * 1, 0 and none; uniform fp32 [rows] in [0, 1) (cut to it). tokens int32 [rows]; logprobs fp32 [rows] or NULL: the log of the
+ * probability that the token was drawn with. A logit of -inf or NaN is never drawn; a row of nothing else gives token −1 and
+ * -inf; infinities share the whole. Weights and sums are whole numbers of 2^-43: the same logits and numbers give the same
+ * tokens always, the formula's but where u or a border lies within some 2^-40 of the whole of a sum. vocab up to 2^20 (else
+ * SQ8_EUNSUPPORTED), any alignment. */
+int sq8_sample_tokens(sq8_ctx *ctx, const void *logits, int dtype, int64_t ld, const float *uniform,
+                      const float *temperature, const int32_t *top_k, const float *top_p, const float *min_p,
+                      int32_t *tokens, float *logprobs, int rows, int vocab);
+
 /* ---- codes with a scale per block of rows and column: GGUF Q8_0 (w = q · d, one fp16 d per 32
  * consecutive K of an output; Sources/Siliconed/Forge/GGUF.swift, `deinterleaveQ8_0`) ---- */
 

@@ -93,6 +93,7 @@ SIGNATURES = {
                                   _I, _I, _P, _I64, _I64, _I, _I, _I, _I]),
     "sq8_chunk_attention": (_I, [_P, _P, _I64, _I64, ctypes.POINTER(PagedCacheArgs), _P, _I64, _I, _P, _P, _I, ctypes.c_float,
                                  ctypes.c_float, _I, _P, _I64, _I64, _I, _I]),
+    "sq8_sample_tokens": (_I, [_P, _P, _I, _I64, _P, _P, _P, _P, _P, _P, _P, _I, _I]),
     "sq8_device": (_I, [_P]),
     "sq8_synchronize": (_I, [_P]),
     "sq8_status_string": (ctypes.c_char_p, [_I]),
@@ -102,7 +103,7 @@ SIGNATURES = {
 # The entries that text_bind.cpp calls, in the order of its Entries.
 TEXT_ENTRIES = ("sq8_add_norm_quantized", "sq8_quantize_groups", "sq8_linear_f8", "sq8_linear_f8_quantized",
                 "sq8_append_kv", "sq8_paged_attention", "sq8_norm_append_kv", "sq8_norm_rotate", "sq8_prompt_attention",
-                "sq8_chunk_attention", "sq8_device")
+                "sq8_chunk_attention", "sq8_sample_tokens", "sq8_device")
 
 _lib = None
 

@@ -1,6 +1,7 @@
 // sq8_text.h — host/device interface of a text decoder's operators: the norm that adds the residual stream and
 // writes 8-bit codes, products of e4m3 codes with a scale per 128 of K, the paged cache's append with the position
-// rotation, attention of one new token over that cache, heads normed and turned, and attention of prompts and chunks.
+// rotation, attention of one new token over that cache, heads normed and turned, attention of prompts and
+// chunks, and the draw of a token.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -201,5 +202,19 @@ enum Source { ROWS = 0, PAGES16, PAGES, PAGES16_F8, PAGES_F8 };
 template <int SOURCE>
 hipError_t launch_source(const AttendArgs &p, const AttendPlan &plan, hipStream_t stream);
 }  // namespace attend
+
+// sq8_sample.hip.
+struct SampleArgs {
+    const void *logits;                 // [rows, vocab], rows ld apart, bf16 or fp32
+    const float *uniform;               // [rows]
+    const float *temperature, *top_p, *min_p;  // [rows] or null
+    const int32_t *top_k;               // [rows] or null
+    int32_t *tokens;                    // [rows]
+    float *logprobs;                    // [rows] or null
+    int64_t ld;
+    int rows, vocab, bf16;
+};
+constexpr int kSampleVocab = 1 << 20;
+hipError_t launch_sample(const SampleArgs &p, hipStream_t stream);
 
 }  // namespace sq8

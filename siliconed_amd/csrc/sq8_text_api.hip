@@ -454,4 +454,23 @@ int sq8_chunk_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_
     return run_attend(ctx, p, q, q_token, q_head, scale, softcap, out, o_token, o_head, tokens, sequences, q_heads, e4m3);
 }
 
+int sq8_sample_tokens(sq8_ctx *ctx, const void *logits, int dtype, int64_t ld, const float *uniform, const float *temperature,
+                      const int32_t *top_k, const float *top_p, const float *min_p, int32_t *tokens, float *logprobs, int rows,
+                      int vocab) {
+    if (!ctx || rows < 0 || vocab <= 0) return SQ8_EINVAL;
+    if (!is_activation(dtype) || vocab > sq8::kSampleVocab) return SQ8_EUNSUPPORTED;
+    if (rows == 0) return SQ8_OK;
+    if (!logits || !uniform || !tokens || ld < vocab) return SQ8_EINVAL;
+    DeviceScope scope(ctx->device);
+    if (scope.error != hipSuccess) return hip_status(scope.error);
+    sq8::SampleArgs p;
+    memset(&p, 0, sizeof(p));
+    p.logits = logits;
+    p.uniform = uniform; p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
+    p.tokens = tokens; p.logprobs = logprobs;
+    p.ld = ld;
+    p.rows = rows; p.vocab = vocab; p.bf16 = dtype == SQ8_BF16;
+    return hip_status(sq8::launch_sample(p, ctx->stream));
+}
+
 }  // extern "C"

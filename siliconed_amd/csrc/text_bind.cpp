@@ -36,6 +36,7 @@ struct Entries {
     decltype(&sq8_norm_rotate) norm_rotate;
     decltype(&sq8_prompt_attention) prompt_attention;
     decltype(&sq8_chunk_attention) chunk_attention;
+    decltype(&sq8_sample_tokens) sample_tokens;
     decltype(&sq8_device) device;
 } entries;
 
@@ -360,7 +361,8 @@ Table table_of(const Tensor &t) {
     const int64_t row = rows_of(t, "table");
     return {static_cast<const float *>(t.data_ptr()), row, count32(t.size(0), "table"), count32(t.size(1), "table")};
 }
-const float *norm_of(const Tensor *t, int64_t dim, const char *what) { return t ? vector_of<float>(*t, dim, what) : nullptr; }
+// A vector that may be left out.
+const float *maybe_vector(const Tensor *t, int64_t dim, const char *what) { return t ? vector_of<float>(*t, dim, what) : nullptr; }
 
 // ctx, q, k, v, cache, positions, slots, table, q_norm, k_norm, eps, q_out, interleaved → q_out
 PyObject *norm_append_kv(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -378,7 +380,7 @@ PyObject *norm_append_kv(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const Heads vh = heads_of(v, "v", tokens, cache.kv_heads, cache.dim), oh = heads_of(out, "q_out", tokens, heads, cache.dim);
     const Table angles = table_of(table);
     const int32_t *const at = vector_of<int32_t>(positions, tokens, "positions"), *const to = vector_of<int32_t>(slots, tokens, "slots");
-    const float *const qn = norm_of(q_norm, cache.dim, "q_norm"), *const kn = norm_of(k_norm, cache.dim, "k_norm");
+    const float *const qn = maybe_vector(q_norm, cache.dim, "q_norm"), *const kn = maybe_vector(k_norm, cache.dim, "k_norm");
     const int interleaved = truth(a[12]), t32 = count32(tokens, "q"), h32 = count32(heads, "q");
     on_device(ctx, {{&q, "q"}, {&k, "k"}, {&v, "v"}, {&positions, "positions"}, {&slots, "slots"}, {&table, "table"},
                     {q_norm, "q_norm"}, {k_norm, "k_norm"}, {&out, "q_out"}});
@@ -418,7 +420,7 @@ PyObject *norm_rotate(PyObject *, PyObject *const *a, Py_ssize_t n) {
         angles = table_of(*table);
         at = vector_of<int32_t>(*positions, tokens, "positions");
     }
-    const float *const qn = norm_of(q_norm, dim, "q_norm"), *const kn = norm_of(k_norm, dim, "k_norm");
+    const float *const qn = maybe_vector(q_norm, dim, "q_norm"), *const kn = maybe_vector(k_norm, dim, "k_norm");
     const int interleaved = truth(a[10]), t32 = count32(tokens, "q"), h32 = count32(heads, "q"), kv32 = count32(kv_heads, "k");
     const int d32 = count32(dim, "q");
     on_device(ctx, {{&q, "q"}, {k, "k"}, {positions, "positions"}, {table, "table"}, {q_norm, "q_norm"}, {k_norm, "k_norm"},
@@ -505,6 +507,38 @@ PyObject *chunk_attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ctx, logits, uniform, temperature, top_k, top_p, min_p (each or None), tokens, logprobs → (tokens, logprobs)
+PyObject *sample_tokens(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 9);
+    sq8_ctx *const ctx = context(a[0]);
+    const Tensor &logits = tensor(a[1], "logits"), &uniform = tensor(a[2], "uniform");
+    const Tensor *const temperature = maybe(a[3], "temperature"), *const top_k = maybe(a[4], "top_k");
+    const Tensor *const top_p = maybe(a[5], "top_p"), *const min_p = maybe(a[6], "min_p");
+    const int64_t ld = rows_of(logits, "logits"), rows = logits.size(0), vocab = logits.size(1);
+    const int type = activation(logits, "logits"), r32 = count32(rows, "logits"), v32 = count32(vocab, "logits");
+    Tensor tokens = a[7] == Py_None ? at::empty({rows}, logits.options().dtype(at::kInt)) : tensor(a[7], "tokens");
+    Tensor logprobs = a[8] == Py_None ? at::empty({rows}, logits.options().dtype(at::kFloat)) : tensor(a[8], "logprobs");
+    const float *const u = vector_of<float>(uniform, rows, "uniform"), *const t = maybe_vector(temperature, rows, "temperature");
+    const int32_t *const k = top_k ? vector_of<int32_t>(*top_k, rows, "top_k") : nullptr;
+    const float *const tp = maybe_vector(top_p, rows, "top_p"), *const mp = maybe_vector(min_p, rows, "min_p");
+    vector_of<int32_t>(tokens, rows, "tokens");
+    vector_of<float>(logprobs, rows, "logprobs");
+    on_device(ctx, {{&logits, "logits"}, {&uniform, "uniform"}, {temperature, "temperature"}, {top_k, "top_k"}, {top_p, "top_p"},
+                    {min_p, "min_p"}, {&tokens, "tokens"}, {&logprobs, "logprobs"}});
+    const int status = call([&] {
+        return entries.sample_tokens(ctx, logits.data_ptr(), type, ld, u, t, k, tp, mp, static_cast<int32_t *>(tokens.data_ptr()),
+                                     static_cast<float *>(logprobs.data_ptr()), r32, v32);
+    });
+    if (status != SQ8_OK) return PyLong_FromLong(status);
+    PyObject *const all = PyTuple_New(2);
+    if (!all) throw python_error();
+    PyTuple_SET_ITEM(all, 0, a[7] == Py_None ? give(std::move(tokens)) : same(a[7]));
+    PyTuple_SET_ITEM(all, 1, a[8] == Py_None ? give(std::move(logprobs)) : same(a[8]));
+    return all;
+    END_HANDLE_TH_ERRORS
+}
+
 // The library's entries: their addresses, in the order of Entries.
 PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -526,7 +560,7 @@ PyObject *bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
 #define TEXT_OP(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {TEXT_OP(bind), TEXT_OP(add_norm_quantized), TEXT_OP(quantize_groups), TEXT_OP(product_f8),
                          TEXT_OP(append_kv), TEXT_OP(paged_attention), TEXT_OP(norm_append_kv), TEXT_OP(norm_rotate),
-                         TEXT_OP(prompt_attention), TEXT_OP(chunk_attention), {nullptr, nullptr, 0, nullptr}};
+                         TEXT_OP(prompt_attention), TEXT_OP(chunk_attention), TEXT_OP(sample_tokens), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_text_bind", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

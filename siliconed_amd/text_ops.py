@@ -187,3 +187,16 @@ class TextOps:
         paged_attention's. A draft to verify, a piece of a long prompt, or both in one batch."""
         return _done(abi.text.chunk_attention(self._h, q, self._args_of(cache), pages, lengths, starts, scale, softcap, window, out),
                      "sq8_chunk_attention")
+
+    def sample_tokens(self, logits: torch.Tensor, uniform: torch.Tensor, *, temperature: Optional[torch.Tensor] = None,
+                      top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None,
+                      min_p: Optional[torch.Tensor] = None, tokens: Optional[torch.Tensor] = None,
+                      logprobs: Optional[torch.Tensor] = None):
+        """The next token of each row of logits [rows, vocab] (bfloat16 or float32), drawn with `uniform` float32 [rows] in [0, 1):
+        (tokens int32 [rows], the logs of the probabilities they were drawn with, float32 [rows]). Each row its own, float32
+        [rows]: `temperature` (None: 1; 0: the largest logit, the first of equal ones), `top_p` (None: 1), `min_p` (None: 0), and
+        `top_k` int32 [rows] (None or 0: all): of the tokens by falling logit the first top_k, of these the fewest that hold top_p
+        of their probability, of these the ones of at least min_p of the likeliest's. A row of nothing but -inf and NaN gives
+        −1. The same inputs give the same tokens always."""
+        return _done(abi.text.sample_tokens(self._h, logits, uniform, temperature, top_k, top_p, min_p, tokens, logprobs),
+                     "sq8_sample_tokens")
