@@ -36,19 +36,20 @@ template <int DP, int WM, int WT, int SRC>
 struct Shape {
     static constexpr int WAVES = WM * WT, THREADS = 64 * WAVES;
     static constexpr int M = 32 * WM;                                 // rows of a tile
-    static constexpr int TT = attend_tokens(DP, WM, WT);              // tokens of a tile
-    static constexpr int SUB = TT / (32 * WT);                        // 32-token parts a wave takes of it
+    static constexpr int TT = attend_tokens(WT);                      // tokens of a tile: 32 for each wave that shares it
+    static constexpr int STAGES = attend_stages(DP, WT);
     static constexpr int ROW = 2 * DP;                                // bytes of a token in LDS
     static constexpr int RUNS = DP / 8;                               // and its 16-byte runs
-    static constexpr int MATRIX = TT * ROW, STAGE = 2 * MATRIX;
+    static constexpr int MATRIX = TT * ROW;
     static constexpr bool F8 = SRC == PAGES16_F8 || SRC == PAGES_F8;
     static constexpr bool PAGED = SRC != ROWS, EACH = SRC == PAGES || SRC == PAGES_F8;  // EACH: rows are looked up one by one
+    // Half the waves load keys, half values.
     static constexpr int PER_LOAD = F8 ? 1024 / DP : 1024 / ROW;      // tokens a wave's load instruction fills
-    static constexpr int LOADS = TT / PER_LOAD / WAVES;               // a wave's of either matrix
-    static constexpr int MINE = TT / WAVES;                           // tokens a wave loads
+    static constexpr int MINE = TT / (WAVES / 2);                     // tokens a wave loads of a tile
+    static constexpr int LOADS = MINE / PER_LOAD;
     static constexpr int LANES = 64 / PER_LOAD;                       // lanes to a token
-    static constexpr int IDS = TT / 16;
-    static_assert(SUB >= 1 && SUB * 32 * WT == TT && LOADS >= 1 && LOADS * PER_LOAD * WAVES == TT, "whole parts");
+    static constexpr int IDS = EACH ? LOADS : PAGED ? (MINE + 15) / 16 : 1;  // page indices that a wave's loads take
+    static_assert(LOADS >= 1 && LOADS * PER_LOAD * (WAVES / 2) == TT, "whole loads");
     static_assert(MINE <= 16 || MINE % 16 == 0, "a load's tokens lie in one sixteen");
 };
 
@@ -64,10 +65,8 @@ __device__ __forceinline__ float over_halves(float v) {
     return SUM ? a + b : fmaxf(a, b);
 }
 
-// Whether either bf16 of a pair is an infinity or a NaN.
-__device__ __forceinline__ bool unbounded(uint32_t d) {
-    return (d & 0x7F80u) == 0x7F80u || (d & 0x7F800000u) == 0x7F800000u;
-}
+// Bits 15 and 31: whether that bf16 of a pair is an infinity or a NaN. (Other bits: anything.)
+__device__ __forceinline__ uint32_t unbounded(uint32_t d) { return (d & 0x7F807F80u) + 0x00800080u; }
 
 // A sequence's rows of q and the tokens it holds.
 struct Sequence {
@@ -92,31 +91,114 @@ __device__ __forceinline__ Sequence sequence(const AttendArgs &p, int b) {
     return s;
 }
 
-// Units of a sequence: a tile of rows by a kv head, the head running fastest. Shared out (p.share), each has as many tiles of
+// Units of a sequence: a tile of rows by a kv head, the head running fastest. Shared out (SHARE), each has as many tiles of
 // keys as the sequence's longest.
 struct Units {
     int tiles;   // of rows
     int run;     // tiles of keys of a unit that are numbered: 1 unless shared
 };
-template <int M, int TT>
+template <int M, int TT, bool SHARE>
 __device__ __forceinline__ Units units_of(const AttendArgs &p, const Sequence &s) {
     Units u;
     u.tiles = (int)(((int64_t)s.count * p.group + M - 1) / M);
     int base = 0;
     if (p.causal && p.window > 0) base = max(0, s.held - s.count - p.window + 1) & ~15;
-    u.run = p.share ? max(1, (s.held - base + TT - 1) / TT) : 1;
+    u.run = SHARE ? max(1, (s.held - base + TT - 1) / TT) : 1;
     return u;
 }
 
-template <int DP, int WM, int WT, int SRC, bool PRECISE>
-__global__ void __attribute__((amdgpu_flat_work_group_size(64 * WM * WT, 64 * WM * WT), amdgpu_waves_per_eu(attend_waves(DP, WM, WT), attend_waves(DP, WM, WT))))
+// Rows of which some, but not all, see a token whose value is an infinity or a NaN, done again by one wave without the matrix
+// cores, whose sums take in every token of a tile: a row at a time, 64 tokens a step, those that it sees.
+struct WildRows {
+    const uint16_t *q;
+    uint16_t *out;
+    const uint8_t *k, *v;       // the kv head's
+    const int32_t *pages;       // or null
+    float *slot;                // for a part of a unit; else null
+    int64_t q_tok, q_head, o_tok, o_head, k_page, k_tok, v_page, v_tok;  // keys' and values' in bytes
+    uint64_t page_mul;
+    float scale, cap, v_scale;  // in units of log2; cap 0: none
+    int page_shift, page, page_count, row0, wm, rows, group, dim, first, held, window, causal, from, to;
+};
+template <int DP, int WM, bool F8>
+__device__ __forceinline__ void wild_rows(const WildRows &w) {
+    constexpr int N = DP / 64;  // values of a lane
+    const int lane = threadIdx.x & 63;
+    auto row_of = [&](int t, int64_t page_bytes, int64_t tok_bytes, bool &bad) -> int64_t {
+        bad = false;
+        if (!w.pages) return t * tok_bytes;
+        const int page = (int)(((uint64_t)(uint32_t)t * w.page_mul) >> w.page_shift);
+        int id = w.pages[page];
+        bad = (unsigned)id >= (unsigned)w.page_count;
+        return (bad ? 0 : id) * page_bytes + (int64_t)(t - page * w.page) * tok_bytes;
+    };
+    auto value = [&](const uint8_t *at, int i) { return F8 ? widen1<W_FP8>(at[i]) : bf16_f32(reinterpret_cast<const uint16_t *>(at)[i]); };
+    for (int c = 0; c < 32; ++c) {
+        const int r = w.row0 + 32 * w.wm + c;
+        if (r >= w.rows) break;
+        const int tok = r / w.group, head = r - tok * w.group;
+        const uint16_t *const q = w.q + tok * w.q_tok + head * w.q_head;
+        const int hi = min(w.causal ? min(w.first + tok, w.held - 1) : w.held - 1, w.to - 1);
+        const int lo = max(w.window > 0 ? w.first + tok - w.window + 1 : 0, w.from);
+        float top = -INFINITY, sum = 0.0f, o[N] = {};
+        for (int t0 = lo; t0 <= hi; t0 += 64) {
+            bool bad;
+            const uint8_t *const k = w.k + row_of(min(t0 + lane, hi), w.k_page, w.k_tok, bad);
+            float s = 0.0f;
+            for (int i = 0; i < w.dim; ++i) s = __builtin_fmaf(bf16_f32(q[i]), value(k, i), s);
+            s *= w.scale;
+            if (w.cap > 0.0f) s = w.cap * tanh_rel(s);
+            if (bad || t0 + lane > hi) s = -INFINITY;
+            float m = s;
+#pragma unroll
+            for (int i = 32; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
+            m = fmaxf(m, top);
+            const float from = m == -INFINITY ? 0.0f : m, keep = __builtin_amdgcn_exp2f(top - from);
+            top = m;
+            float p = __builtin_amdgcn_exp2f(s - from), all = p;
+#pragma unroll
+            for (int i = 32; i >= 1; i >>= 1) all += __shfl_xor(all, i, 64);
+            sum = sum * keep + all;
+#pragma unroll
+            for (int i = 0; i < N; ++i) o[i] *= keep;
+            for (int j = 0; j < 64 && t0 + j <= hi; ++j) {
+                const uint8_t *const v = w.v + row_of(t0 + j, w.v_page, w.v_tok, bad);
+                if (bad) continue;
+                const float weight = __shfl(p, j, 64);
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (lane + 64 * i < w.dim) o[i] = __builtin_fmaf(weight, value(v, lane + 64 * i), o[i]);
+            }
+        }
+        if (!w.slot) {
+            const float by = inverse(sum) * w.v_scale;
+            uint16_t *const out = w.out + tok * w.o_tok + head * w.o_head;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (lane + 64 * i < w.dim) out[lane + 64 * i] = (uint16_t)(pack_bf16_rne(o[i] * by, 0.0f) & 0xFFFFu);
+        } else {
+            // As the first waves leave theirs.
+            if (lane == 0) put(w.slot + 2 * (32 * w.wm + c), Pair{top, sum});
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int x = lane + 64 * i, d = x >> 5, e = 4 * (x >> 3 & 3) + (x & 3), half = x >> 2 & 1;
+                __hip_atomic_store(w.slot + 64 * WM + 2 * (((w.wm * (DP / 32) + d) * 8 + e / 2) * 64 + c + 32 * half) + (e & 1), o[i],
+                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+    }
+    wd::wait_vmcnt<0>();
+}
+
+template <int DP, int WM, int WT, int SRC, bool PRECISE, bool SHARE>
+__global__ void __attribute__((amdgpu_flat_work_group_size(64 * WM * WT, 64 * WM * WT), amdgpu_waves_per_eu(attend_waves(DP, WT), attend_waves(DP, WT))))
 attend_kernel(const AttendArgs p) {
     using S = Shape<DP, WM, WT, SRC>;
-    constexpr int STEPS = DP / 16, DT = DP / 32, SUB = S::SUB, TT = S::TT, M = S::M;
+    constexpr int STEPS = DP / 16, DT = DP / 32, TT = S::TT, M = S::M;
     constexpr float LOG2E = 1.4426950408889634f;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * S::STAGE];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * S::STAGES * S::MATRIX];  // keys, then values
     __shared__ float tops[S::WAVES][32], totals[S::WAVES][32];
-    __shared__ int joins[2];
+    __shared__ int joins[2], wilds[S::WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, h = lane >> 5;
     const int wm = wave % WM, wt = wave / WM;
@@ -125,8 +207,8 @@ attend_kernel(const AttendArgs p) {
 
     // Runs past `dim` are zeros, written once: no load fills them.
     if (runs < S::RUNS) {
-        for (int i = tid; i < 2 * 2 * TT * S::RUNS; i += S::THREADS) {
-            const int token = i / S::RUNS % TT, run = i % S::RUNS, matrix = i / (S::RUNS * TT) & 1;
+        for (int i = tid; i < 2 * S::STAGES * TT * S::RUNS; i += S::THREADS) {
+            const int token = i / S::RUNS % TT, run = i % S::RUNS, matrix = i / (S::RUNS * TT * S::STAGES);
             if ((run ^ (matrix ? key_v(token) : key_k(token))) >= runs) *reinterpret_cast<u32x4 *>(lds + i * 16) = u32x4{0, 0, 0, 0};
         }
         __syncthreads();
@@ -136,7 +218,7 @@ attend_kernel(const AttendArgs p) {
     int total = 0, before = 0, b = 0;
     auto size_of = [&](int i) {
         if (i >= p.sequences) return 0;
-        const Units u = units_of<M, TT>(p, sequence(p, i));
+        const Units u = units_of<M, TT, SHARE>(p, sequence(p, i));
         return u.tiles * u.run;
     };
     for (int i = 0; i < p.sequences; i += 64) {
@@ -148,7 +230,7 @@ attend_kernel(const AttendArgs p) {
     total = __builtin_amdgcn_readfirstlane(total) * p.kv_heads;
     const Share share(total, gridDim.x);
     int start, end;
-    if (p.share) {
+    if constexpr (SHARE) {
         start = share.first(min((int)blockIdx.x, share.groups));
         end = share.first(min((int)blockIdx.x + 1, share.groups));
     } else {
@@ -178,7 +260,7 @@ attend_kernel(const AttendArgs p) {
         seq.row0 = __builtin_amdgcn_readfirstlane(s.row0);
         seq.count = __builtin_amdgcn_readfirstlane(s.count);
         seq.held = __builtin_amdgcn_readfirstlane(s.held);
-        units = units_of<M, TT>(p, seq);
+        units = units_of<M, TT, SHARE>(p, seq);
     };
     enter();
 
@@ -186,7 +268,9 @@ attend_kernel(const AttendArgs p) {
         int first, tiles;      // its numbered tiles (0: none)
         int row0, rows, kvh;   // first row of the tile in its sequence, the sequence's rows; its kv head
         int at;                // the sequence's first row of q
-    } parts[2] = {};
+    };
+    __shared__ Part parts[2];  // of the workgroup's first unit and of its last
+    if (SHARE && tid < 2) parts[tid].tiles = 0;
 
     for (int pos = start; pos < end;) {
         while (b + 1 < p.sequences && pos >= seq0 + units.tiles * units.run * p.kv_heads) {
@@ -198,7 +282,7 @@ attend_kernel(const AttendArgs p) {
         const int unit = in_seq / units.run, part0 = in_seq - unit * units.run;
         const int kvh = unit % p.kv_heads, tile = unit / p.kv_heads;
         if (in_seq < 0 || tile >= units.tiles) break;  // starts that do not ascend
-        const int numbered = p.share ? min(units.run - part0, end - pos) : 1;
+        const int numbered = SHARE ? min(units.run - part0, end - pos) : 1;
         const int rows = seq.count * p.group;  // of the sequence
         const int row0 = tile * M;
         const int first = seq.held - seq.count;  // the place of the chunk's first token
@@ -211,7 +295,7 @@ attend_kernel(const AttendArgs p) {
         const int base = (windowed ? max(0, first + tok0 - p.window + 1) : 0) & ~15;
         const int tiles = max(0, (stop - base + TT - 1) / TT);
         // Of the unit's numbered tiles, some may lie past these rows' last: none is read there.
-        const int t_from = p.share ? min(part0, tiles) : 0, t_to = p.share ? min(part0 + numbered, tiles) : tiles;
+        const int t_from = SHARE ? min(part0, tiles) : 0, t_to = SHARE ? min(part0 + numbered, tiles) : tiles;
 
         // ---- the wave's rows ----
         const int r = row0 + wm * 32 + c;
@@ -223,12 +307,15 @@ attend_kernel(const AttendArgs p) {
         const int lo = windowed ? first + tok - p.window + 1 : 0;                  // the first
         const int hi_min = __builtin_amdgcn_readfirstlane(p.causal ? first + min(w0, rows - 1) / p.group : seq.held - 1);
         const int hi_max = __builtin_amdgcn_readfirstlane(any ? (p.causal ? first + wN / p.group : seq.held - 1) : -1);
-        const int lo_min = windowed ? hi_min - p.window + 1 : 0, lo_max = windowed ? hi_max - p.window + 1 : 0;
+        const int lo_max = windowed ? hi_max - p.window + 1 : 0;
 
+        // Uniform, and kept in scalar registers.
+        auto scalar = [](float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); };
         float unit_scale = p.scale * (S::F8 && p.k_scale ? p.k_scale[kvh] : 1.0f);
         const bool minus = unit_scale < 0.0f;  // then Q is taken with the other sign: the largest score is that of S
         unit_scale = fabsf(unit_scale) * (capped ? 1.0f / p.softcap : LOG2E);
         if (unit_scale < 1e-30f) unit_scale = 1e-30f;  // (0 times a masked score would be a NaN)
+        unit_scale = scalar(unit_scale);
         bf16x8 q[STEPS];
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
@@ -239,71 +326,85 @@ attend_kernel(const AttendArgs p) {
             q[s] = __builtin_bit_cast(bf16x8, v);
         }
 
-        // ---- loads ----
-        const uint8_t *const kbase = p.kc + ((int64_t)kvh * p.kc_head + (S::PAGED ? 0 : (int64_t)seq.row0 * p.kc_tok)) * (S::F8 ? 1 : 2);
-        const uint8_t *const vbase = p.vc + ((int64_t)kvh * p.vc_head + (S::PAGED ? 0 : (int64_t)seq.row0 * p.vc_tok)) * (S::F8 ? 1 : 2);
-        const auto pages = (const __attribute__((address_space(4))) int32_t *)(p.pages + (int64_t)b * p.pages_row);
+        // ---- loads: the first half of the waves keys, the others values ----
         constexpr int ES = S::F8 ? 1 : 2;
+        const bool of_keys = wave < S::WAVES / 2;
+        const int slice = wave % (S::WAVES / 2);
+        const int64_t tok_bytes = (of_keys ? p.kc_tok : p.vc_tok) * ES, page_bytes = (of_keys ? p.kc_page : p.vc_page) * ES;
+        const uint8_t *const pool = (of_keys ? p.kc + (int64_t)kvh * p.kc_head * ES : p.vc + (int64_t)kvh * p.vc_head * ES) +
+                                    (S::PAGED ? 0 : (int64_t)seq.row0 * tok_bytes);
+        const auto pages = (const __attribute__((address_space(4))) int32_t *)(p.pages + (int64_t)b * p.pages_row);
         const int in_load = lane / S::LANES, run = lane % S::LANES;  // a lane's token of a load, and its place in LDS there
         auto page_of = [&](int token) { return (int)(((uint64_t)(uint32_t)token * p.page_mul) >> p.page_shift); };
-        // The pages of a tile: PAGES16's, one for each 16 tokens, uniform; EACH: lane l's is that of tokens l and 64 + l.
-        struct Where {
-            int id[S::EACH ? (TT + 63) / 64 : S::PAGED ? S::IDS : 1];
+        auto inside = [&](int id) { return (unsigned)id < (unsigned)p.page_count; };
+        // A lane's run of load i, in the order of LDS (bf16): turned by its token's number.
+        auto turned = [&](int i) {
+            const int row = i * S::PER_LOAD + in_load;  // (the wave's tokens begin at a multiple of eight)
+            return run ^ (of_keys ? key_k(row) : key_v(row));
         };
-        auto locate = [&](int token0) {
-            Where w;
-            if constexpr (S::EACH) {
+        // The page indices of a wave's loads of a tile (a uniform one for 16 tokens; EACH: a lane's own for each load).
+        struct Ids {
+            int id[S::IDS];
+        };
+        auto look_up = [&](int token0) {
+            Ids w;
 #pragma unroll
-                for (int i = 0; i < (TT + 63) / 64; ++i) w.id[i] = pages[page_of(min(token0 + 64 * i + lane, seq.held - 1))];
-            } else if constexpr (S::PAGED) {
-#pragma unroll
-                for (int i = 0; i < S::IDS; ++i) w.id[i] = pages[page_of(min(token0 + 16 * i, (seq.held - 1) & ~15))];
+            for (int i = 0; i < S::IDS; ++i) {
+                if constexpr (S::EACH) w.id[i] = pages[page_of(min(token0 + slice * S::MINE + i * S::PER_LOAD + in_load, seq.held - 1))];
+                else if constexpr (S::PAGED) w.id[i] = pages[page_of(min(token0 + ((slice * S::MINE) & ~15) + 16 * i, (seq.held - 1) & ~15))];
+                else w.id[i] = 0;
             }
             return w;
         };
-        auto inside = [&](int id) { return (unsigned)id < (unsigned)p.page_count; };
-        // The offsets (elements) of load i's tokens, the lane's among them.
-        auto offsets = [&](const Where &w, int token0, int i, int64_t &k, int64_t &v) {
-            const int local = wave * S::MINE + i * S::PER_LOAD;  // the load's first token in the tile
+        // Where load i's tokens lie: the lane's address.
+        auto address = [&](const Ids &w, int token0, int i) -> const uint8_t * {
+            const int local = slice * S::MINE + i * S::PER_LOAD;
+            const uint32_t in_bytes = (uint32_t)(in_load * (int)tok_bytes);
             if constexpr (S::EACH) {
-                const int mine = local + in_load;
-                const int t = min(token0 + mine, seq.held - 1);
-                int id = w.id[0];
-#pragma unroll
-                for (int j = 1; j < (TT + 63) / 64; ++j) id = (local >> 6) == j ? w.id[j] : id;
-                id = __shfl(id, mine & 63, 64);
-                id = inside(id) ? id : 0;
-                const int in = t - page_of(t) * p.page;
-                k = id * p.kc_page + in * p.kc_tok;
-                v = id * p.vc_page + in * p.vc_tok;
+                const int t = min(token0 + local + in_load, seq.held - 1);
+                const int id = inside(w.id[i]) ? w.id[i] : 0;
+                return pool + id * page_bytes + (int64_t)(t - page_of(t) * p.page) * tok_bytes;
             } else if constexpr (S::PAGED) {
                 const int t16 = min(token0 + (local & ~15), (seq.held - 1) & ~15);
-                int id = 0;
-#pragma unroll
-                for (int j = 0; j < S::IDS; ++j) id = (local >> 4) == j ? w.id[j] : id;
-                id = inside(id) ? id : 0;
-                const int in = t16 - page_of(t16) * p.page;
-                k = id * p.kc_page + in * p.kc_tok + (int64_t)((local & 15) + in_load) * p.kc_tok;
-                v = id * p.vc_page + in * p.vc_tok + (int64_t)((local & 15) + in_load) * p.vc_tok;
+                const int at = w.id[i * S::PER_LOAD / 16], id = inside(at) ? at : 0;
+                return pool + (id * page_bytes + (int64_t)(t16 - page_of(t16) * p.page + (local & 15)) * tok_bytes) + in_bytes;
             } else {
-                const int t = min(token0 + local + in_load, seq.held - 1);
-                k = t * p.kc_tok;
-                v = t * p.vc_tok;
+                // (Rows past the sequence's, up to the last of all, may be read: nothing sees them.)
+                const int from = token0 + local;
+                if (seq.row0 + token0 + TT <= p.tokens) return pool + from * tok_bytes + in_bytes;
+                return pool + min(from + in_load, seq.held - 1) * tok_bytes;
             }
         };
-        auto load = [&](const Where &w, int token0, int stage) {
+        // bf16: straight to LDS. e4m3: to registers, and widened into LDS later.
+        u32x4 codes[S::F8 ? S::LOADS : 1];
+        auto load = [&](const Ids &w, int token0, int slot) {
 #pragma unroll
             for (int i = 0; i < S::LOADS; ++i) {
-                int64_t ko, vo;
-                offsets(w, token0, i, ko, vo);
-                const int row = wave * S::MINE + i * S::PER_LOAD + in_load;
-                const int kr = run ^ key_k(row), vr = run ^ key_v(row);
-                uint8_t *const to = lds + stage * S::STAGE + (wave * S::LOADS + i) * 1024;
-                if (kr < runs) __builtin_amdgcn_global_load_lds((wd::glb_ptr)(kbase + ko * 2 + kr * 16), (wd::lds_ptr)to, 16, 0, 0);
-                if (vr < runs) __builtin_amdgcn_global_load_lds((wd::glb_ptr)(vbase + vo * 2 + vr * 16), (wd::lds_ptr)(to + S::MATRIX), 16, 0, 0);
+                const uint8_t *const at = address(w, token0, i);
+                if constexpr (S::F8) {
+                    codes[i] = *reinterpret_cast<const u32x4 *>(at + (16 * run < p.dim ? 16 * run : 0));
+                } else {
+                    const int r = turned(i);
+                    uint8_t *const to = lds + (of_keys ? 0 : S::STAGES * S::MATRIX) + slot + (slice * S::LOADS + i) * 1024;
+                    if (r < runs) __builtin_amdgcn_global_load_lds((wd::glb_ptr)(at + r * 16), (wd::lds_ptr)to, 16, 0, 0);
+                }
             }
         };
-        // The tile's tokens on a page outside the pools, a bit each of 64.
+        auto widen = [&](int slot) {
+            if (16 * run >= p.dim) return;
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) {
+                const int row = slice * S::MINE + i * S::PER_LOAD + in_load, key = of_keys ? key_k(row) : key_v(row);
+                uint8_t *const to = lds + (of_keys ? 0 : S::STAGES * S::MATRIX) + slot + row * S::ROW;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t x = codes[i][2 * half], y = codes[i][2 * half + 1];
+                    *reinterpret_cast<u32x4 *>(to + ((2 * run + half) ^ key) * 16) =
+                        u32x4{bf16_of_e4m3<0>(x), bf16_of_e4m3<1>(x), bf16_of_e4m3<0>(y), bf16_of_e4m3<1>(y)};
+                }
+            }
+        };
+        // A tile's tokens on a page outside the pools, a bit each.
         struct Bad {
             uint64_t bits[(TT + 63) / 64];
             __device__ __forceinline__ uint64_t from(int token) const {
@@ -319,65 +420,52 @@ attend_kernel(const AttendArgs p) {
                 return all != 0;
             }
         };
-        auto bad_of = [&](const Where &w) {
+        constexpr int BAD = !S::PAGED ? 1 : S::EACH ? (TT + 63) / 64 : TT / 16;
+        struct Pages {
+            int id[BAD];
+        };
+        auto pages_of = [&](int token0) {  // a tile's page indices, for its bad tokens
+            Pages w;
+#pragma unroll
+            for (int i = 0; i < BAD; ++i) {
+                if constexpr (S::EACH) w.id[i] = pages[page_of(min(token0 + 64 * i + lane, seq.held - 1))];
+                else if constexpr (S::PAGED) w.id[i] = pages[page_of(min(token0 + 16 * i, (seq.held - 1) & ~15))];
+                else w.id[i] = 0;
+            }
+            return w;
+        };
+        auto bad_of = [&](const Pages &w) {
             Bad bad;
 #pragma unroll
             for (int i = 0; i < (TT + 63) / 64; ++i) {
                 bad.bits[i] = 0;
                 if constexpr (S::EACH) {
-                    bad.bits[i] = __ballot(!inside(w.id[i]));
+                    bad.bits[i] = __ballot(64 * i + lane < TT && !inside(w.id[i]));
                 } else if constexpr (S::PAGED) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        if (4 * i + j < S::IDS && !inside(w.id[4 * i + j])) bad.bits[i] |= 0xFFFFull << (16 * j);
+                        if (4 * i + j < BAD && !inside(w.id[4 * i + j < BAD ? 4 * i + j : 0])) bad.bits[i] |= 0xFFFFull << (16 * j);
                 }
             }
             return bad;
         };
-        // Whether no row sees a tile's token, past the sequence's last or on such a page. Its values, which may be anything, are
-        // made zeros in LDS: 0 times an infinity or a NaN would not hide them.
-        auto gone = [&](int token0, const Bad &bad, int token) { return token0 + token >= seq.held || (S::PAGED && (bad.from(token) & 1)); };
-        auto clear = [&](int token0, const Bad &bad, int stage) {
-            if (token0 + TT <= seq.held && !bad.any()) return;
+        // The values of tokens that no row sees, past the sequence's last or on such a page, may be anything: they are made zeros
+        // in LDS by the wave that loaded them, as 0 times an infinity or a NaN would not hide them.
+        auto clear = [&](int token0, const Bad &bad, int slot) {
+            if (of_keys || (token0 + TT <= seq.held && !bad.any())) return;
 #pragma unroll
-            for (int i = 0; i < S::LOADS; ++i)
-                if (gone(token0, bad, wave * S::MINE + i * S::PER_LOAD + in_load))
-                    *reinterpret_cast<u32x4 *>(lds + stage * S::STAGE + S::MATRIX + (wave * S::LOADS + i) * 1024 + lane * 16) = u32x4{0, 0, 0, 0};
+            for (int i = 0; i < S::LOADS; ++i) {
+                const int row = slice * S::MINE + i * S::PER_LOAD + in_load;
+                if (token0 + row < seq.held && !(S::PAGED && (bad.from(row) & 1))) continue;
+                uint8_t *const at = lds + S::STAGES * S::MATRIX + slot + row * S::ROW;
+                constexpr int BYTES = S::ROW / S::LANES;  // a lane's share of a row: one run, or two of widened codes
+#pragma unroll
+                for (int j = 0; j < BYTES; j += 16) *reinterpret_cast<u32x4 *>(at + run * BYTES + j) = u32x4{0, 0, 0, 0};
+            }
         };
 
-        // e4m3: to registers, and widened into LDS later.
-        u32x4 k8[S::F8 ? S::LOADS : 1], v8[S::F8 ? S::LOADS : 1];
-        auto fetch = [&](const Where &w, int token0) {
-#pragma unroll
-            for (int i = 0; i < S::LOADS; ++i) {
-                int64_t ko, vo;
-                offsets(w, token0, i, ko, vo);
-                const int at = 16 * run < p.dim ? 16 * run : 0;
-                k8[i] = *reinterpret_cast<const u32x4 *>(kbase + ko + at);
-                v8[i] = *reinterpret_cast<const u32x4 *>(vbase + vo + at);
-            }
-        };
-        auto widen = [&](int token0, const Bad &bad, int stage) {
-            if (16 * run >= p.dim) return;
-            const bool some = token0 + TT > seq.held || bad.any();
-#pragma unroll
-            for (int i = 0; i < S::LOADS; ++i) {
-                const int row = wave * S::MINE + i * S::PER_LOAD + in_load;
-                uint8_t *const to = lds + stage * S::STAGE + row * S::ROW;
-                if (some && gone(token0, bad, row)) v8[i] = u32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    auto wide = [&](const u32x4 &d) {
-                        const uint32_t x = d[2 * half], y = d[2 * half + 1];
-                        return u32x4{bf16_of_e4m3<0>(x), bf16_of_e4m3<1>(x), bf16_of_e4m3<0>(y), bf16_of_e4m3<1>(y)};
-                    };
-                    *reinterpret_cast<u32x4 *>(to + ((2 * run + half) ^ key_k(row)) * 16) = wide(k8[i]);
-                    *reinterpret_cast<u32x4 *>(to + S::MATRIX + ((2 * run + half) ^ key_v(row)) * 16) = wide(v8[i]);
-                }
-            }
-        };
-        // ---- fragments: the lane's places in a stage ----
-        const int wave_token = wt * 32 * SUB;
+        // ---- fragments: the lane's places in a tile ----
+        const int wave_token = wt * 32;
         int k_at[4];  // run 2s + h of token c, by s mod 4 (further ones 128 bytes on)
 #pragma unroll
         for (int s = 0; s < 4; ++s) k_at[s] = (wave_token + c) * S::ROW + (((2 * s + h) ^ key_k(c)) * 16);
@@ -386,190 +474,190 @@ attend_kernel(const AttendArgs p) {
         const int v_run = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), v_key = key_v(v_token);
         int v_at[2];  // by d mod 2
 #pragma unroll
-        for (int d = 0; d < 2; ++d) v_at[d] = S::MATRIX + (wave_token + v_token) * S::ROW + (((4 * d + v_run) ^ v_key) * 16) + 8 * (lane & 1);
+        for (int d = 0; d < 2; ++d)
+            v_at[d] = S::STAGES * S::MATRIX + (wave_token + v_token) * S::ROW + (((4 * d + v_run) ^ v_key) * 16) + 8 * (lane & 1);
+        auto keys = [&](int at, int j) { return *reinterpret_cast<const bf16x8 *>(lds + at + k_at[j & 3] + (j >> 2) * 128); };
+        auto values = [&](int at, int ks, int d) {
+            const uint8_t *const from = lds + at + v_at[d & 1] + (d >> 1) * 128 + 16 * ks * S::ROW;
+            const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)from));
+            const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(from + 8 * S::ROW)));
+            return u32x4{x[0], x[1], y[0], y[1]};
+        };
 
         float top = -INFINITY, sum = 0.0f;
-        f32x16 o[DT];
+        f32x16 o[DT], s_even, s_odd;
+        bool wild = false;  // these rows are to be done again by wild_rows
+        bool far = false;  // a maximum is so far from 0 that the scaled scores' rounding counts
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
 
-        Where now, next;
-        if (t_from < t_to) {
-            now = locate(base + t_from * TT);
-            __syncthreads();  // the run before has been read
-            if constexpr (S::F8) {
-                fetch(now, base + t_from * TT);
-                widen(base + t_from * TT, bad_of(now), t_from & 1);
+        // The maximum moved, where a score passes it by 8 powers of two. `far`: a maximum is so far from 0 that the scaled scores'
+        // rounding, which a fused multiply-add does not share with it, would count: then the scores are taken as their scaled
+        // distance from it here.
+        auto raise = [&](f32x16 &s, float scale) {
+            float m = s[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) m = fmaxf(m, s[e]);
+            m *= scale;
+            const uint64_t move = __ballot(m > top + 8.0f);
+            float keep = 1.0f;
+            if (move) {
+                m = fmaxf(over_halves<false>(m), top);
+                keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - m);
+                top = m;
+                sum *= keep;
+                far = __any(fabsf(top) > 0x1p24f && fabsf(top) < INFINITY);
+            }
+            // In place, and past the compiler, which would keep a copy of every sum for the way that leaves them as they are. (They
+            // come from matrix instructions: 18 waits before they are read, and some before the next ones take them.)
+if (move)
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+                asm volatile("s_nop 15\n\ts_nop 1\n\t"
+                             "v_mul_f32 %0, %0, %16\n\tv_mul_f32 %1, %1, %16\n\tv_mul_f32 %2, %2, %16\n\tv_mul_f32 %3, %3, %16\n\t"
+                             "v_mul_f32 %4, %4, %16\n\tv_mul_f32 %5, %5, %16\n\tv_mul_f32 %6, %6, %16\n\tv_mul_f32 %7, %7, %16\n\t"
+                             "v_mul_f32 %8, %8, %16\n\tv_mul_f32 %9, %9, %16\n\tv_mul_f32 %10, %10, %16\n\tv_mul_f32 %11, %11, %16\n\t"
+                             "v_mul_f32 %12, %12, %16\n\tv_mul_f32 %13, %13, %16\n\tv_mul_f32 %14, %14, %16\n\tv_mul_f32 %15, %15, %16\n\t"
+                             "s_nop 3"
+                             : "+v"(o[d][0]), "+v"(o[d][1]), "+v"(o[d][2]), "+v"(o[d][3]), "+v"(o[d][4]), "+v"(o[d][5]), "+v"(o[d][6]),
+                               "+v"(o[d][7]), "+v"(o[d][8]), "+v"(o[d][9]), "+v"(o[d][10]), "+v"(o[d][11]), "+v"(o[d][12]), "+v"(o[d][13]),
+                               "+v"(o[d][14]), "+v"(o[d][15])
+                             : "v"(keep));
+        };
+        // The probabilities, two a dword in the order of the second product's tokens; what a bf16 leaves of each besides
+        // (PRECISE), at least 2^-126 of one that is not 0, so that an infinite value meets no zero and no other sign.
+        struct Weights {
+            u32x4 w[2], rest[2];
+        };
+        auto pair = [&](const f32x16 &s, Weights &p2, auto ec, float scale, float from) {
+            constexpr int e = decltype(ec)::value;
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e], scale, -from));
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e + 1], scale, -from));
+            sum += x + y;
+            if constexpr (PRECISE) {
+                const uint32_t a = __float_as_uint(x), z = __float_as_uint(y);
+                p2.w[e >> 2][e & 3] = __builtin_amdgcn_perm(z, a, 0x07060302u);
+                p2.rest[e >> 2][e & 3] = pack_bf16_rne(fmaxf(x - __uint_as_float(a & 0xFFFF0000u), fminf(x, 0x1p-126f)),
+                                                       fmaxf(y - __uint_as_float(z & 0xFFFF0000u), fminf(y, 0x1p-126f)));
             } else {
-                load(now, base + t_from * TT, t_from & 1);
+                p2.w[e >> 2][e & 3] = pack_bf16_rne(x, y);
             }
-            if (t_from + 1 < t_to) next = locate(base + (t_from + 1) * TT);
-        }
-#pragma clang loop unroll(disable)
-        for (int t = t_from; t < t_to; ++t) {
-            const int stage = (t & 1) * S::STAGE, token0 = base + t * TT;
-            const bool more = t + 1 < t_to;
-            const Bad bad = bad_of(now);
+        };
+        // Where some row does not see some token of the wave's, or scores are capped: the scores as they count.
+        auto edge = [&](f32x16 &s, float &scale, int mine, uint32_t bad, int v_from) {
+            if (capped) {
+                const float cap = scalar(p.softcap * LOG2E);
+                scale = 1.0f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = cap * tanh_rel(s[e] * unit_scale);
+            }
+            const int hi_rel = hi - mine - 4 * h, lo_rel = lo - mine - 4 * h;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int j = 8 * (e >> 2) + (e & 3);  // the token, 4h from the wave's
+                const bool dead = j > hi_rel || j < lo_rel || (S::PAGED && (bad >> (j + 4 * h) & 1));
+                s[e] = dead ? -INFINITY : s[e];
+            }
+            // A token that some rows do not see may hold an infinity or a NaN, which 0 times it would not hide: wild_rows.
+            uint32_t found = 0;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const u32x4 v = values(v_from, ks, d);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) found |= unbounded(v[i]);
+                }
+            wild = wild || __any((found & 0x80008000u) != 0);
+        };
+
+        // ---- the tiles. Keys are used a tile ahead of values: a tile's softmax goes beside the next one's first product ----
+        // At the barrier of tile t all are done with the tiles before it and with its keys, so the keys of t + STAGES and the values
+        // of t + STAGES − 1 are asked for; the keys of t + 1 and the values of t have come, and those that were asked for at the
+        // STAGES − 2 barriers before may be under way.
+        auto slot_of = [](int t) { return (t & (S::STAGES - 1)) * S::MATRIX; };
+        const int ahead = of_keys ? S::STAGES : S::STAGES - 1;
+        auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+        int t = t_from;
+        Ids ids = {};
+        Pages tile_pages = {}, next_pages = {};
+        auto step = [&](f32x16 &s, f32x16 &next) {
+            const Bad bad = bad_of(tile_pages);
+            next_pages = pages_of(base + (t + 1) * TT);
             if constexpr (!S::F8) {
-                wd::wait_vmcnt<0>();
-                clear(token0, bad, t & 1);
+                if (t + S::STAGES <= t_to) wd::wait_vmcnt<(S::STAGES - 2) * S::LOADS>();
+                else wd::wait_vmcnt<0>();
             }
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (more) {
-                if constexpr (S::F8) fetch(next, token0 + TT);
-                else load(next, token0 + TT, (t + 1) & 1);
-                now = next;
-                if (t + 2 < t_to) next = locate(token0 + 2 * TT);
+            clear(base + t * TT, bad, slot_of(t));
+            barrier();
+            if (t + ahead < t_to) {
+                load(ids, base + (t + ahead) * TT, slot_of(t + ahead));
+                ids = look_up(base + (t + 1 + ahead) * TT);
             }
-            const int mine = token0 + wave_token;  // the wave's first token
-            if (mine <= hi_max && mine + 32 * SUB > lo_min) {
-                f32x16 s[SUB];
+            const int k_from = slot_of(t + 1), v_from = slot_of(t);
+            const int mine = base + t * TT + wave_token;  // the wave's first token
+            float scale = unit_scale;
+            if (capped || mine + 31 > hi_min || mine < lo_max || bad.any()) edge(s, scale, mine, (uint32_t)bad.from(wave_token), v_from);
+            raise(s, scale);
+            float from = top == -INFINITY ? 0.0f : top;
+            if (far) {
 #pragma unroll
-                for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
-#pragma unroll
-                for (int j = 0; j < STEPS; ++j)
-#pragma unroll
-                    for (int u = 0; u < SUB; ++u) {
-                        const bf16x8 kk = *reinterpret_cast<const bf16x8 *>(lds + stage + k_at[j & 3] + (j >> 2) * 128 + u * 32 * S::ROW);
-                        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kk, q[j], s[u], 0, 0, 0);
-                    }
-                uint32_t bits[SUB], any_bad = 0;  // the wave's bad tokens
-#pragma unroll
-                for (int u = 0; u < SUB; ++u) any_bad |= bits[u] = S::PAGED ? (uint32_t)bad.from(wave_token + 32 * u) : 0u;
-                const bool edge = mine + 32 * SUB - 1 > hi_min || mine < lo_max || any_bad != 0;
-                float scale = unit_scale;
-                if (capped) {
-                    scale = 1.0f;
-#pragma unroll
-                    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) s[u][e] = p.softcap * LOG2E * tanh_rel(s[u][e] * unit_scale);
-                }
-                const int hi_rel = hi - mine - 4 * h, lo_rel = lo - mine - 4 * h;
-                auto dead_of = [&](int at, int u) {  // token 32u + at of the lane (4h apart from the wave's)
-                    const int j = 32 * u + at;
-                    bool dead = j > hi_rel || j < lo_rel;
-                    if constexpr (S::PAGED) dead = dead || (bits[u] >> (at + 4 * h) & 1);
-                    return dead;
-                };
-                if (edge) {
-#pragma unroll
-                    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) s[u][e] = dead_of(8 * (e >> 2) + (e & 3), u) ? -INFINITY : s[u][e];
-                }
-                float m = s[0][0];
-#pragma unroll
-                for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) m = fmaxf(m, s[u][e]);
-                m *= scale;
-                if (__any(m > top + 8.0f)) {
-                    m = fmaxf(over_halves<false>(m), top);
-                    const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - m);
-                    top = m;
-                    sum *= keep;
-#pragma unroll
-                    for (int d = 0; d < DT; ++d)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[d][e] *= keep;
-                }
-                float from = top == -INFINITY ? 0.0f : top;
-                if (__any(fabsf(from) > 0x1p16f)) {
-                    // So far out the scaled score's rounding, which a fused multiply-add does not share with `from`, would count.
-#pragma unroll
-                    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) s[u][e] = s[u][e] * scale - from;
-                    scale = 1.0f;
-                    from = 0.0f;
-                }
-                // The probabilities, two a dword in the order of the second product's tokens; what a bf16 leaves of each besides
-                // (PRECISE), at least 2^-126 of one that is not 0, so that an infinite value meets no zero and no other sign.
-                u32x4 w[SUB][2], rest[PRECISE ? SUB : 1][2];
-#pragma unroll
-                for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e], scale, -from));
-                        const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][e + 1], scale, -from));
-                        sum += x + y;
-                        if constexpr (PRECISE) {
-                            const uint32_t a = __float_as_uint(x), z = __float_as_uint(y);
-                            w[u][e >> 3][(e >> 1) & 3] = __builtin_amdgcn_perm(z, a, 0x07060302u);
-                            rest[u][e >> 3][(e >> 1) & 3] = pack_bf16_rne(fmaxf(x - __uint_as_float(a & 0xFFFF0000u), fminf(x, 0x1p-126f)),
-                                                                         fmaxf(y - __uint_as_float(z & 0xFFFF0000u), fminf(y, 0x1p-126f)));
-                        } else {
-                            w[u][e >> 3][(e >> 1) & 3] = pack_bf16_rne(x, y);
-                        }
-                    }
-                auto values = [&](int u, int ks, int d) {
-                    const uint8_t *const at = lds + stage + v_at[d & 1] + (d >> 1) * 128 + (32 * u + 16 * ks) * S::ROW;
-                    const i16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)at);
-                    const i16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(at + 8 * S::ROW));
-                    const u32x2 lo2 = __builtin_bit_cast(u32x2, x), hi2 = __builtin_bit_cast(u32x2, y);
-                    return u32x4{lo2[0], lo2[1], hi2[0], hi2[1]};
-                };
-                bool wild = false;  // a token that some rows do not see may hold an infinity or a NaN
-                if (edge) {
-                    bool found = false;
-#pragma unroll
-                    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                            for (int d = 0; d < DT; ++d) {
-                                const u32x4 v = values(u, ks, d);
-                                found = found || unbounded(v[0]) || unbounded(v[1]) || unbounded(v[2]) || unbounded(v[3]);
-                            }
-                    wild = __any(found);
-                }
-                if (!wild) {
-#pragma unroll
-                    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                            for (int d = 0; d < DT; ++d) {
-                                const bf16x8 v = __builtin_bit_cast(bf16x8, values(u, ks, d));
-                                if constexpr (PRECISE) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, rest[u][ks]), o[d], 0, 0, 0);
-                                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, w[u][ks]), o[d], 0, 0, 0);
-                            }
-                } else {
-                    // Token by token: a row takes the product with one it sees, and keeps what it had where it does not.
-#pragma unroll
-                    for (int u = 0; u < SUB; ++u)
-#pragma unroll
-                        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll 1
-                            for (int j = 0; j < 16; ++j) {
-                                // Token j of the 16: in half j / 4 mod 2, place 4·(j / 8) + j mod 4 of the lane's eight.
-                                const int place = 4 * (j >> 3) + (j & 3), half = (j >> 2) & 1;
-                                const int at = 16 * ks + j, rel = 32 * u + at;
-                                bool seen = rel <= hi - mine && rel >= lo - mine;
-                                if constexpr (S::PAGED) seen = seen && !(bits[u] >> at & 1);
-                                u32x4 keep;
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    keep[e] = h == half && (place >> 1) == e ? (place & 1 ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
-#pragma unroll
-                                for (int d = 0; d < DT; ++d) {
-                                    const bf16x8 v = __builtin_bit_cast(bf16x8, values(u, ks, d) & keep);
-                                    f32x16 with = o[d];
-                                    if constexpr (PRECISE) with = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, rest[u][ks] & keep), with, 0, 0, 0);
-                                    with = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, w[u][ks] & keep), with, 0, 0, 0);
-#pragma unroll
-                                    for (int e = 0; e < 16; ++e) o[d][e] = seen ? with[e] : o[d][e];
-                                }
-                            }
-                }
+                for (int e = 0; e < 16; ++e) s[e] = s[e] * scale - from;
+                scale = 1.0f;
+                from = 0.0f;
             }
+            // Written out in the order it runs: between the matrix instructions of the next tile's scores two values' softmax and a
+            // read four instructions ahead, and the first values' reads under the last of them. (The last tile's next one is
+            // whatever lies there.)
+            constexpr int LEAD = 4, PAIRS = 8, OUTS = 2 * DT;
+            bf16x8 k[LEAD], v[LEAD];
+            Weights p2;
+            static_for<0, LEAD>([&](auto jc) { k[decltype(jc)::value] = keys(k_from, decltype(jc)::value); });
+#pragma unroll
+            for (int e = 0; e < 16; ++e) next[e] = 0.0f;
+            __builtin_amdgcn_sched_barrier(0);
+            static_for<0, STEPS>([&](auto jc) {
+                constexpr int j = decltype(jc)::value;
+                next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[j % LEAD], q[j], next, 0, 0, 0);
+                if constexpr (j + LEAD < STEPS) k[j % LEAD] = keys(k_from, j + LEAD);
+                else v[j + LEAD - STEPS] = __builtin_bit_cast(bf16x8, values(v_from, (j + LEAD - STEPS) / DT, (j + LEAD - STEPS) % DT));
+                static_for<PAIRS * j / STEPS, PAIRS *(j + 1) / STEPS>([&](auto ec) { pair(s, p2, ec, scale, from); });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            static_for<0, OUTS>([&](auto jc) {
+                constexpr int j = decltype(jc)::value, ks = j / DT, d = j % DT;
+                if constexpr (PRECISE) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[j % LEAD], __builtin_bit_cast(bf16x8, p2.rest[ks]), o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[j % LEAD], __builtin_bit_cast(bf16x8, p2.w[ks]), o[d], 0, 0, 0);
+                if constexpr (j + LEAD < OUTS) v[j % LEAD] = __builtin_bit_cast(bf16x8, values(v_from, (j + LEAD) / DT, (j + LEAD) % DT));
+                __builtin_amdgcn_sched_barrier(0);
+            });
             if constexpr (S::F8) {
-                if (more) widen(token0 + TT, bad_of(now), (t + 1) & 1);
+                if (t + ahead < t_to) widen(slot_of(t + ahead));
+            }
+            tile_pages = next_pages;
+            ++t;
+        };
+        if (t < t_to) {
+            __syncthreads();  // the run before has been read
+            for (int i = t; i < min(t + ahead, t_to); ++i) {
+                load(look_up(base + i * TT), base + i * TT, slot_of(i));
+                if constexpr (S::F8) widen(slot_of(i));
+            }
+            ids = look_up(base + (t + ahead) * TT);  // (past the last tile: the last token's)
+            tile_pages = pages_of(base + t * TT);
+            if constexpr (!S::F8) wd::wait_vmcnt<0>();
+            barrier();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s_even[e] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) s_even = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys(slot_of(t), j), q[j], s_even, 0, 0, 0);
+            for (;;) {
+                step(s_even, s_odd);
+                if (t >= t_to) break;
+                step(s_odd, s_even);
+                if (t >= t_to) break;
             }
         }
 
@@ -579,6 +667,7 @@ attend_kernel(const AttendArgs p) {
             __syncthreads();  // the last tile has been read
             float *const mine = reinterpret_cast<float *>(lds) + ((wt - 1) * WM + wm) * (DT * 16 * 64) + lane;
             if (h == 0) { tops[wave][c] = top; totals[wave][c] = sum; }
+            if (lane == 0) wilds[wave] = wild;
             if (wt > 0) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
@@ -608,9 +697,11 @@ attend_kernel(const AttendArgs p) {
                         for (int e = 0; e < 16; ++e) o[d][e] = __builtin_fmaf(other[(d * 16 + e) * 64], weight, o[d][e]);
                 }
                 top = all;
+#pragma unroll
+                for (int i = 1; i < WT; ++i) wild = wild || wilds[i * WM + wm] != 0;
             }
         }
-        const bool whole = !p.share || numbered == units.run;
+        const bool whole = !SHARE || numbered == units.run;
         if (wt == 0) {
             if (whole) {
                 if (live) {
@@ -636,20 +727,28 @@ attend_kernel(const AttendArgs p) {
                         put(slot + 2 * M + 2 * (((wm * DT + d) * 8 + e / 2) * 64 + lane), Pair{o[d][e], o[d][e + 1]});
             }
         }
-        if (!whole) {
-            Part &part = pos == start ? parts[0] : parts[1];
-            part.first = seq0 + unit * units.run;
-            part.tiles = units.run;
-            part.row0 = row0;
-            part.rows = rows;
-            part.kvh = kvh;
-            part.at = seq.row0;
+        if (wt == 0 && __builtin_amdgcn_readfirstlane((int)wild)) {
+            const int64_t head0 = (int64_t)kvh * p.group;
+            const WildRows again = {p.q + seq.row0 * p.q_tok + head0 * p.q_head, p.out + seq.row0 * p.o_tok + head0 * p.o_head,
+                                    p.kc + (kvh * p.kc_head + (S::PAGED ? 0 : seq.row0 * p.kc_tok)) * ES,
+                                    p.vc + (kvh * p.vc_head + (S::PAGED ? 0 : seq.row0 * p.vc_tok)) * ES,
+                                    S::PAGED ? p.pages + b * p.pages_row : nullptr,
+                                    whole ? nullptr : p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * attend_part_floats(DP, WM),
+                                    p.q_tok, p.q_head, p.o_tok, p.o_head, p.kc_page * ES, p.kc_tok * ES, p.vc_page * ES, p.vc_tok * ES,
+                                    p.page_mul, minus ? -unit_scale : unit_scale, capped ? p.softcap * LOG2E : 0.0f,
+                                    S::F8 && p.v_scale ? p.v_scale[kvh] : 1.0f, p.page_shift, p.page, p.page_count, row0, wm, rows, p.group,
+                                    p.dim, first, seq.held, windowed ? p.window : 0, p.causal, base + t_from * TT, min(base + t_to * TT, seq.held)};
+            wild_rows<DP, WM, S::F8>(again);
         }
+        if (SHARE && !whole && tid == 0)
+            parts[pos == start ? 0 : 1] = Part{seq0 + unit * units.run, units.run, row0, rows, kvh, seq.row0};
         pos += numbered;
     }
 
     // ---- the parts' slots are written before their counters say so; the last workgroup to count joins ----
-    if (!p.share || (parts[0].tiles == 0 && parts[1].tiles == 0)) return;
+    if constexpr (!SHARE) return;
+    __syncthreads();
+    if (parts[0].tiles == 0 && parts[1].tiles == 0) return;
     wd::wait_vmcnt<0>();
     __syncthreads();
     if (tid < 2) {

@@ -182,10 +182,11 @@ struct AttendArgs {
     int page_shift;
 };
 constexpr int attend_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }  // the instance of a head's size
-// Tokens of a tile, of WM sets of 32 rows and WT waves that share its tokens: a stage of 32 KB, or 64.
-constexpr int attend_tokens(int dp, int wm, int wt) { return dp == 64 ? (wt == 4 ? 256 : 128) : dp == 128 ? (wt == 4 ? 128 : 64) : 64; }
-// Waves a SIMD holds: two tiles' stages fit a CU's LDS, or one of 64 KB.
-constexpr int attend_waves(int dp, int wm, int wt) { return dp == 256 || wt == 4 ? 1 : 2; }
+// Tokens of a tile that WT waves share, and the tiles that LDS holds: 64 KB of them, or 128 where one workgroup has a CU.
+constexpr int attend_tokens(int wt) { return 32 * wt; }
+constexpr int attend_stages(int dp, int wt) { return dp * wt >= 512 ? 2 : 4; }
+// Waves a SIMD holds.
+constexpr int attend_waves(int dp, int wt) { return dp * wt >= 256 ? 1 : 2; }
 // A slot of a shared unit: maxima and sums [rows][2], outputs.
 __host__ __device__ constexpr int attend_part_floats(int dp, int wm) { return 32 * wm * (2 + dp); }
 // sq8_text_plan.hip. The tile and the workgroups that a call takes, and what it needs of the context's buffers.
@@ -193,7 +194,7 @@ struct AttendPlan {
     int wm, groups, share;
     int64_t part_bytes, marks;
 };
-AttendPlan attend_plan(const AttendArgs &p, int cus);
+AttendPlan attend_plan(const AttendArgs &p, bool e4m3, int cus);
 hipError_t launch_attend(const AttendArgs &p, const AttendPlan &plan, bool e4m3, hipStream_t stream);
 namespace attend {
 // Where keys and values lie: rows of a projection; pages whose tokens are a multiple of 16 (16 tokens lie in one page); any

@@ -109,7 +109,7 @@ int64_t paged_part_bytes(const PagedArgs &p, int groups) {
 
 int64_t paged_marks(const PagedArgs &p) { return (int64_t)MARK * p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16); }
 
-AttendPlan attend_plan(const AttendArgs &p, int cus) {
+AttendPlan attend_plan(const AttendArgs &p, bool e4m3, int cus) {
     AttendPlan plan = {4, 0, 0, 0, 0};
     if (p.sequences <= 0 || p.tokens <= 0) return plan;
     const int dp = attend_dim(p.dim);
@@ -120,15 +120,16 @@ AttendPlan attend_plan(const AttendArgs &p, int cus) {
         plan.wm = each <= 32 ? 1 : each <= 64 ? 2 : each <= 128 ? 4 : 8;
     } else {
         auto some = [&](int wm) { return (each + 32 * wm - 1) / (32 * wm) * p.sequences * p.kv_heads; };  // if all were alike
-        plan.wm = some(8) >= cus ? 8 : some(4) >= cus ? 4 : some(2) >= cus ? 2 : 1;
+        plan.wm = some(8) >= cus ? 8 : some(4) >= cus ? 4 : 2;
     }
     if (dp == 256) plan.wm = plan.wm < 2 ? 2 : plan.wm > 4 ? 4 : plan.wm;
+    if (dp == 64 && e4m3 && plan.wm > 4) plan.wm = 4;  // (a tile's codes are fewer than eight waves' loads)
     const int wt = plan.wm >= 4 ? 1 : plan.wm == 2 ? 2 : 4;
     if (!plan.share) {
         plan.groups = (int)units(plan.wm);
         return plan;
     }
-    const int tokens = attend_tokens(dp, plan.wm, wt), held = attend_waves(dp, plan.wm, wt) * 4 / (plan.wm * wt);
+    const int tokens = attend_tokens(wt), held = attend_waves(dp, wt) * 4 / (plan.wm * wt);
     const int64_t longest = (int64_t)p.max_pages * p.page;
     const int64_t most = units(plan.wm) * std::max<int64_t>(1, (longest + tokens - 1) / tokens), full = (int64_t)held * cus;
     plan.groups = (int)std::min(most, full);

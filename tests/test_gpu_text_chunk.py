@@ -209,8 +209,14 @@ def test_infinite_and_nan_values_are_their_tokens(gemm, dtype):
     pool = b.cache.v.view(torch.uint8)
     pool[page, place, 0, :2 if dtype == BF else 1] = 0xFF  # a NaN
     out = b.run(gemm)
-    assert torch.equal(out[:20], clean[:20]) and torch.equal(out[40:], clean[40:])
-    assert torch.isnan(out[20:40, :2, 0]).all() and torch.equal(out[20:40, 2:], clean[20:40, 2:])
+    # Rows beside those that see it may be done without the matrix cores, their probabilities not rounded: the formula's tolerance
+    # covers either, another sequence keeps its bits.
+    want, tol = attended(b.q[:40], *b.values[0], 60)
+    within(out[:20], want[:20], tol[:20], "before the token")
+    within(out[20:40, 2:], want[20:, 2:], tol[20:, 2:], "another kv head")
+    assert torch.equal(out[40:], clean[40:])
+    assert torch.isnan(out[20:40, :2, 0]).all()
+    within(out[20:40, :2, 1:], want[20:, :2, 1:], tol[20:, :2, 1:], "its other values")
 
 
 def test_refusals(gemm):
