@@ -57,6 +57,7 @@ SOURCES = [
     ("sq8_paged.hip", "sq8_paged", []),
     *(("sq8_attend_inst.hip", f"sq8_attend_{i}", [f"-DSQ8_SOURCE={i}"]) for i in range(5)),
     ("sq8_attend.hip", "sq8_attend", []),
+    ("sq8_chunk.hip", "sq8_chunk", []),
     ("sq8_heads.hip", "sq8_heads", []),
     ("sq8_sample.hip", "sq8_sample", []),
     ("sq8_text_plan.hip", "sq8_text_plan", []),

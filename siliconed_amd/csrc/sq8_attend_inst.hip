@@ -7,19 +7,18 @@ namespace {
 
 template <int DP, int WM, int WT>
 hipError_t launch(const AttendArgs &p, int groups, hipStream_t stream) {
-    // Few rows wait for memory, and keep their probabilities to 17 bits.
-    hipLaunchKernelGGL((attend_kernel<DP, WM, WT, SQ8_SOURCE, WT == 4, SQ8_SOURCE != ROWS>), dim3(groups), dim3(64 * WM * WT), 0, stream, p);
+    hipLaunchKernelGGL((attend_kernel<DP, WM, WT, SQ8_SOURCE, SQ8_SOURCE != ROWS>), dim3(groups), dim3(64 * WM * WT), 0, stream, p);
     return hipGetLastError();
 }
 
 template <int DP>
 hipError_t pick(const AttendArgs &p, const AttendPlan &plan, hipStream_t stream) {
-    if (plan.wm == 4) return launch<DP, 4, 1>(p, plan.groups, stream);
-    if (plan.wm == 2) return launch<DP, 2, 2>(p, plan.groups, stream);
+    if (plan.rows == 128) return launch<DP, 4, 1>(p, plan.groups, stream);
     if constexpr (DP <= 128) {
+        if constexpr (SQ8_SOURCE == ROWS)
+            if (plan.rows == 64) return launch<DP, 2, 2>(p, plan.groups, stream);
         if constexpr (DP == 128 || SQ8_SOURCE <= PAGES)
-            if (plan.wm == 8) return launch<DP, 8, 1>(p, plan.groups, stream);
-        if (plan.wm == 1) return launch<DP, 1, 4>(p, plan.groups, stream);
+            if (plan.rows == 256) return launch<DP, 8, 1>(p, plan.groups, stream);
     }
     return hipErrorInvalidValue;
 }

@@ -21,6 +21,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include "sq8_attend_device.h"
 #include "sq8_device.h"
 #include "sq8_text.h"
 #include "sq8_text_device.h"
@@ -37,7 +38,7 @@ struct Shape {
     static constexpr int WAVES = WM * WT, THREADS = 64 * WAVES;
     static constexpr int M = 32 * WM;                                 // rows of a tile
     static constexpr int TT = attend_tokens(WT);                      // tokens of a tile: 32 for each wave that shares it
-    static constexpr int STAGES = attend_stages(DP, WT);
+    static constexpr int STAGES = kAttendStages;
     static constexpr int ROW = 2 * DP;                                // bytes of a token in LDS
     static constexpr int RUNS = DP / 8;                               // and its 16-byte runs
     static constexpr int MATRIX = TT * ROW;
@@ -65,132 +66,7 @@ __device__ __forceinline__ float over_halves(float v) {
     return SUM ? a + b : fmaxf(a, b);
 }
 
-// Bits 15 and 31: whether that bf16 of a pair is an infinity or a NaN. (Other bits: anything.)
-__device__ __forceinline__ uint32_t unbounded(uint32_t d) { return (d & 0x7F807F80u) + 0x00800080u; }
-
-// A sequence's rows of q and the tokens it holds.
-struct Sequence {
-    int row0, count, held;
-};
-__device__ __forceinline__ Sequence sequence(const AttendArgs &p, int b) {
-    Sequence s;
-    if (!p.starts) {
-        s.row0 = 0;
-        s.count = p.tokens;
-    } else {
-        const int lo = min(max(p.starts[b], 0), p.tokens), hi = min(max(p.starts[b + 1], lo), p.tokens);
-        s.row0 = lo;
-        s.count = hi - lo;
-    }
-    s.held = s.count;
-    if (p.lengths) {
-        const int64_t most = (int64_t)p.max_pages * p.page;
-        const int n = p.lengths[b];
-        s.held = (int)(n < 0 ? 0 : n > most ? most : n);
-    }
-    return s;
-}
-
-// Units of a sequence: a tile of rows by a kv head, the head running fastest. Shared out (SHARE), each has as many tiles of
-// keys as the sequence's longest.
-struct Units {
-    int tiles;   // of rows
-    int run;     // tiles of keys of a unit that are numbered: 1 unless shared
-};
-template <int M, int TT, bool SHARE>
-__device__ __forceinline__ Units units_of(const AttendArgs &p, const Sequence &s) {
-    Units u;
-    u.tiles = (int)(((int64_t)s.count * p.group + M - 1) / M);
-    int base = 0;
-    if (p.causal && p.window > 0) base = max(0, s.held - s.count - p.window + 1) & ~15;
-    u.run = SHARE ? max(1, (s.held - base + TT - 1) / TT) : 1;
-    return u;
-}
-
-// Rows of which some, but not all, see a token whose value is an infinity or a NaN, done again by one wave without the matrix
-// cores, whose sums take in every token of a tile: a row at a time, 64 tokens a step, those that it sees.
-struct WildRows {
-    const uint16_t *q;
-    uint16_t *out;
-    const uint8_t *k, *v;       // the kv head's
-    const int32_t *pages;       // or null
-    float *slot;                // for a part of a unit; else null
-    int64_t q_tok, q_head, o_tok, o_head, k_page, k_tok, v_page, v_tok;  // keys' and values' in bytes
-    uint64_t page_mul;
-    float scale, cap, v_scale;  // in units of log2; cap 0: none
-    int page_shift, page, page_count, row0, wm, rows, group, dim, first, held, window, causal, from, to;
-};
-template <int DP, int WM, bool F8>
-__device__ __forceinline__ void wild_rows(const WildRows &w) {
-    constexpr int N = DP / 64;  // values of a lane
-    const int lane = threadIdx.x & 63;
-    auto row_of = [&](int t, int64_t page_bytes, int64_t tok_bytes, bool &bad) -> int64_t {
-        bad = false;
-        if (!w.pages) return t * tok_bytes;
-        const int page = (int)(((uint64_t)(uint32_t)t * w.page_mul) >> w.page_shift);
-        int id = w.pages[page];
-        bad = (unsigned)id >= (unsigned)w.page_count;
-        return (bad ? 0 : id) * page_bytes + (int64_t)(t - page * w.page) * tok_bytes;
-    };
-    auto value = [&](const uint8_t *at, int i) { return F8 ? widen1<W_FP8>(at[i]) : bf16_f32(reinterpret_cast<const uint16_t *>(at)[i]); };
-    for (int c = 0; c < 32; ++c) {
-        const int r = w.row0 + 32 * w.wm + c;
-        if (r >= w.rows) break;
-        const int tok = r / w.group, head = r - tok * w.group;
-        const uint16_t *const q = w.q + tok * w.q_tok + head * w.q_head;
-        const int hi = min(w.causal ? min(w.first + tok, w.held - 1) : w.held - 1, w.to - 1);
-        const int lo = max(w.window > 0 ? w.first + tok - w.window + 1 : 0, w.from);
-        float top = -INFINITY, sum = 0.0f, o[N] = {};
-        for (int t0 = lo; t0 <= hi; t0 += 64) {
-            bool bad;
-            const uint8_t *const k = w.k + row_of(min(t0 + lane, hi), w.k_page, w.k_tok, bad);
-            float s = 0.0f;
-            for (int i = 0; i < w.dim; ++i) s = __builtin_fmaf(bf16_f32(q[i]), value(k, i), s);
-            s *= w.scale;
-            if (w.cap > 0.0f) s = w.cap * tanh_rel(s);
-            if (bad || t0 + lane > hi) s = -INFINITY;
-            float m = s;
-#pragma unroll
-            for (int i = 32; i >= 1; i >>= 1) m = fmaxf(m, __shfl_xor(m, i, 64));
-            m = fmaxf(m, top);
-            const float from = m == -INFINITY ? 0.0f : m, keep = __builtin_amdgcn_exp2f(top - from);
-            top = m;
-            float p = __builtin_amdgcn_exp2f(s - from), all = p;
-#pragma unroll
-            for (int i = 32; i >= 1; i >>= 1) all += __shfl_xor(all, i, 64);
-            sum = sum * keep + all;
-#pragma unroll
-            for (int i = 0; i < N; ++i) o[i] *= keep;
-            for (int j = 0; j < 64 && t0 + j <= hi; ++j) {
-                const uint8_t *const v = w.v + row_of(t0 + j, w.v_page, w.v_tok, bad);
-                if (bad) continue;
-                const float weight = __shfl(p, j, 64);
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if (lane + 64 * i < w.dim) o[i] = __builtin_fmaf(weight, value(v, lane + 64 * i), o[i]);
-            }
-        }
-        if (!w.slot) {
-            const float by = inverse(sum) * w.v_scale;
-            uint16_t *const out = w.out + tok * w.o_tok + head * w.o_head;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (lane + 64 * i < w.dim) out[lane + 64 * i] = (uint16_t)(pack_bf16_rne(o[i] * by, 0.0f) & 0xFFFFu);
-        } else {
-            // As the first waves leave theirs.
-            if (lane == 0) put(w.slot + 2 * (32 * w.wm + c), Pair{top, sum});
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int x = lane + 64 * i, d = x >> 5, e = 4 * (x >> 3 & 3) + (x & 3), half = x >> 2 & 1;
-                __hip_atomic_store(w.slot + 64 * WM + 2 * (((w.wm * (DP / 32) + d) * 8 + e / 2) * 64 + c + 32 * half) + (e & 1), o[i],
-                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-        }
-    }
-    wd::wait_vmcnt<0>();
-}
-
-template <int DP, int WM, int WT, int SRC, bool PRECISE, bool SHARE>
+template <int DP, int WM, int WT, int SRC, bool SHARE>
 __global__ void __attribute__((amdgpu_flat_work_group_size(64 * WM * WT, 64 * WM * WT), amdgpu_waves_per_eu(attend_waves(DP, WT), attend_waves(DP, WT))))
 attend_kernel(const AttendArgs p) {
     using S = Shape<DP, WM, WT, SRC>;
@@ -215,21 +91,9 @@ attend_kernel(const AttendArgs p) {
     }
 
     // ---- this workgroup's tiles and the sequence they begin in; all uniform ----
-    int total = 0, before = 0, b = 0;
-    auto size_of = [&](int i) {
-        if (i >= p.sequences) return 0;
-        const Units u = units_of<M, TT, SHARE>(p, sequence(p, i));
-        return u.tiles * u.run;
-    };
-    for (int i = 0; i < p.sequences; i += 64) {
-        int v = size_of(i + lane);
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-        total += v;
-    }
-    total = __builtin_amdgcn_readfirstlane(total) * p.kv_heads;
+    const int total = all_units<M, TT, SHARE>(p, lane) * p.kv_heads;
     const Share share(total, gridDim.x);
-    int start, end;
+    int start, end, b = 0, before = 0;
     if constexpr (SHARE) {
         start = share.first(min((int)blockIdx.x, share.groups));
         end = share.first(min((int)blockIdx.x + 1, share.groups));
@@ -240,19 +104,8 @@ attend_kernel(const AttendArgs p) {
         end = tile < tiles ? start + 1 : 0;
     }
     if (start >= end) return;
-    for (int i = 0; i < p.sequences; i += 64) {
-        const int v = size_of(i + lane), upto = wave_scan(v, lane);
-        const uint64_t past = __ballot((before + upto) * p.kv_heads > start);
-        if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
-            before += l > 0 ? __shfl(upto, l - 1, 64) : 0;
-            b = i + l;
-            break;
-        }
-        before += __shfl(upto, 63, 64);
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
-    int seq0 = __builtin_amdgcn_readfirstlane(before) * p.kv_heads;
+    find_unit<M, TT, SHARE>(p, start, lane, b, before);
+    int seq0 = before * p.kv_heads;
     Sequence seq;
     Units units;
     auto enter = [&]() {
@@ -264,11 +117,6 @@ attend_kernel(const AttendArgs p) {
     };
     enter();
 
-    struct Part {
-        int first, tiles;      // its numbered tiles (0: none)
-        int row0, rows, kvh;   // first row of the tile in its sequence, the sequence's rows; its kv head
-        int at;                // the sequence's first row of q
-    };
     __shared__ Part parts[2];  // of the workgroup's first unit and of its last
     if (SHARE && tid < 2) parts[tid].tiles = 0;
 
@@ -377,10 +225,19 @@ attend_kernel(const AttendArgs p) {
         };
         // bf16: straight to LDS. e4m3: to registers, and widened into LDS later.
         u32x4 codes[S::F8 ? S::LOADS : 1];
-        auto load = [&](const Ids &w, int token0, int slot) {
+        struct Addresses {
+            const uint8_t *at[S::LOADS];
+        };
+        auto addresses = [&](const Ids &w, int token0) {
+            Addresses all;
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) all.at[i] = address(w, token0, i);
+            return all;
+        };
+        auto load = [&](const Addresses &from, int slot) {
 #pragma unroll
             for (int i = 0; i < S::LOADS; ++i) {
-                const uint8_t *const at = address(w, token0, i);
+                const uint8_t *const at = from.at[i];
                 if constexpr (S::F8) {
                     codes[i] = *reinterpret_cast<const u32x4 *>(at + (16 * run < p.dim ? 16 * run : 0));
                 } else {
@@ -462,6 +319,7 @@ attend_kernel(const AttendArgs p) {
 #pragma unroll
                 for (int j = 0; j < BYTES; j += 16) *reinterpret_cast<u32x4 *>(at + run * BYTES + j) = u32x4{0, 0, 0, 0};
             }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         };
 
         // ---- fragments: the lane's places in a tile ----
@@ -485,7 +343,7 @@ attend_kernel(const AttendArgs p) {
         };
 
         float top = -INFINITY, sum = 0.0f;
-        f32x16 o[DT], s_even, s_odd;
+        f32x16 o[DT], s_now, s_next;
         bool wild = false;  // these rows are to be done again by wild_rows
         bool far = false;  // a maximum is so far from 0 that the scaled scores' rounding counts
 #pragma unroll
@@ -493,14 +351,22 @@ attend_kernel(const AttendArgs p) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
 
+        // The probabilities, two a dword in the order of the second product's tokens, rounded to bf16: by as much of the output as
+        // its own rounding is, which the sums of many hide and a second product for the rest would cost half the time again.
+        struct Weights {
+            u32x4 w[2];
+        };
+        auto pair = [&](const f32x16 &s, Weights &p2, auto ec, float scale, float from) {
+            constexpr int e = decltype(ec)::value;
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e], scale, -from));
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e + 1], scale, -from));
+            sum += x + y;
+            p2.w[e >> 2][e & 3] = pack_bf16_rne(x, y);
+        };
         // The maximum moved, where a score passes it by 8 powers of two. `far`: a maximum is so far from 0 that the scaled scores'
         // rounding, which a fused multiply-add does not share with it, would count: then the scores are taken as their scaled
         // distance from it here.
-        auto raise = [&](f32x16 &s, float scale) {
-            float m = s[0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) m = fmaxf(m, s[e]);
-            m *= scale;
+        auto raise = [&](float m, Weights &last) {
             const uint64_t move = __ballot(m > top + 8.0f);
             float keep = 1.0f;
             if (move) {
@@ -509,6 +375,12 @@ attend_kernel(const AttendArgs p) {
                 top = m;
                 sum *= keep;
                 far = __any(fabsf(top) > 0x1p24f && fabsf(top) < INFINITY);
+                // The probabilities that are still to be multiplied were taken from the maximum before: rounded once more here.
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t w = last.w[i >> 2][i & 3];
+                    last.w[i >> 2][i & 3] = pack_bf16_rne(__uint_as_float(w << 16) * keep, __uint_as_float(w & 0xFFFF0000u) * keep);
+                }
             }
             // In place, and past the compiler, which would keep a copy of every sum for the way that leaves them as they are. (They
             // come from matrix instructions: 18 waits before they are read, and some before the next ones take them.)
@@ -526,27 +398,14 @@ if (move)
                                "+v"(o[d][14]), "+v"(o[d][15])
                              : "v"(keep));
         };
-        // The probabilities, two a dword in the order of the second product's tokens; what a bf16 leaves of each besides
-        // (PRECISE), at least 2^-126 of one that is not 0, so that an infinite value meets no zero and no other sign.
-        struct Weights {
-            u32x4 w[2], rest[2];
+        auto largest = [](const f32x16 &s) {
+            float m = s[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) m = fmaxf(m, s[e]);
+            return m;
         };
-        auto pair = [&](const f32x16 &s, Weights &p2, auto ec, float scale, float from) {
-            constexpr int e = decltype(ec)::value;
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e], scale, -from));
-            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e + 1], scale, -from));
-            sum += x + y;
-            if constexpr (PRECISE) {
-                const uint32_t a = __float_as_uint(x), z = __float_as_uint(y);
-                p2.w[e >> 2][e & 3] = __builtin_amdgcn_perm(z, a, 0x07060302u);
-                p2.rest[e >> 2][e & 3] = pack_bf16_rne(fmaxf(x - __uint_as_float(a & 0xFFFF0000u), fminf(x, 0x1p-126f)),
-                                                       fmaxf(y - __uint_as_float(z & 0xFFFF0000u), fminf(y, 0x1p-126f)));
-            } else {
-                p2.w[e >> 2][e & 3] = pack_bf16_rne(x, y);
-            }
-        };
-        // Where some row does not see some token of the wave's, or scores are capped: the scores as they count.
-        auto edge = [&](f32x16 &s, float &scale, int mine, uint32_t bad, int v_from) {
+        // Where some row does not see some token of the wave's, or scores are capped: the scores as they count, and the largest.
+        auto edge = [&](f32x16 &s, float &most, float &scale, int mine, uint32_t bad, int v_from) {
             if (capped) {
                 const float cap = scalar(p.softcap * LOG2E);
                 scale = 1.0f;
@@ -560,6 +419,7 @@ if (move)
                 const bool dead = j > hi_rel || j < lo_rel || (S::PAGED && (bad >> (j + 4 * h) & 1));
                 s[e] = dead ? -INFINITY : s[e];
             }
+            most = largest(s);
             // A token that some rows do not see may hold an infinity or a NaN, which 0 times it would not hide: wild_rows.
             uint32_t found = 0;
 #pragma unroll
@@ -573,34 +433,50 @@ if (move)
             wild = wild || __any((found & 0x80008000u) != 0);
         };
 
-        // ---- the tiles. Keys are used a tile ahead of values: a tile's softmax goes beside the next one's first product ----
-        // At the barrier of tile t all are done with the tiles before it and with its keys, so the keys of t + STAGES and the values
-        // of t + STAGES − 1 are asked for; the keys of t + 1 and the values of t have come, and those that were asked for at the
-        // STAGES − 2 barriers before may be under way.
+        // ---- the tiles: beside tile t's softmax run the scores of t + 1 and the outputs of t − 1 ----
+        // At the barrier of tile t all are done with the scores of t and the outputs of t − 2, so the keys of t + STAGES and the values
+        // of t + STAGES − 2 are asked for; the keys of t + 2 and the values of t have come, and those that were asked for at the
+        // STAGES − 3 barriers before may be under way. So the first fragments of a step are read before its barrier.
         auto slot_of = [](int t) { return (t & (S::STAGES - 1)) * S::MATRIX; };
-        const int ahead = of_keys ? S::STAGES : S::STAGES - 1;
-        auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+        const int ahead = of_keys ? S::STAGES : S::STAGES - 2;
+        // (What a wave writes to LDS it waits for itself; fragments on their way are of tiles that stay.)
+        auto barrier = [] { asm volatile("s_barrier" ::: "memory"); };
+        auto written = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
         int t = t_from;
-        Ids ids = {};
+        Ids ids = {};            // of the tile after the one whose
+        Addresses asked = {};    // addresses these are: what the next barrier asks for
         Pages tile_pages = {}, next_pages = {};
+        Weights last = {};  // the probabilities of tile t − 1
+        auto output = [&](auto jc, bf16x8 v) {
+            constexpr int j = decltype(jc)::value;
+            o[j % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, last.w[j / DT]), o[j % DT], 0, 0, 0);
+        };
+        constexpr int LEAD = 4, OUTS = 2 * DT;  // reads go this many instructions ahead
+        float most = -INFINITY;                 // of the scores at hand
+        bf16x8 k[LEAD], v[LEAD];
+        auto first_fragments = [&]() {  // of step t
+            static_for<0, LEAD>([&](auto jc) {
+                constexpr int j = decltype(jc)::value;
+                k[j] = keys(slot_of(t + 1), j);
+                v[j] = __builtin_bit_cast(bf16x8, values(slot_of(t + S::STAGES - 1), j / DT, j % DT));
+            });
+        };
         auto step = [&](f32x16 &s, f32x16 &next) {
             const Bad bad = bad_of(tile_pages);
-            next_pages = pages_of(base + (t + 1) * TT);
+            tile_pages = next_pages;
             if constexpr (!S::F8) {
-                if (t + S::STAGES <= t_to) wd::wait_vmcnt<(S::STAGES - 2) * S::LOADS>();
-                else wd::wait_vmcnt<0>();
+                if (t + S::STAGES > t_to) wd::wait_vmcnt<0>();
+                else wd::wait_vmcnt<(S::STAGES - 3) * S::LOADS>();
             }
             clear(base + t * TT, bad, slot_of(t));
+            if constexpr (S::F8) written();
             barrier();
-            if (t + ahead < t_to) {
-                load(ids, base + (t + ahead) * TT, slot_of(t + ahead));
-                ids = look_up(base + (t + 1 + ahead) * TT);
-            }
-            const int k_from = slot_of(t + 1), v_from = slot_of(t);
+            if (t + ahead < t_to) load(asked, slot_of(t + ahead));
+            const int k_from = slot_of(t + 1), v_from = slot_of(t + S::STAGES - 1);
             const int mine = base + t * TT + wave_token;  // the wave's first token
             float scale = unit_scale;
-            if (capped || mine + 31 > hi_min || mine < lo_max || bad.any()) edge(s, scale, mine, (uint32_t)bad.from(wave_token), v_from);
-            raise(s, scale);
+            if (capped || mine + 31 > hi_min || mine < lo_max || bad.any()) edge(s, most, scale, mine, (uint32_t)bad.from(wave_token), slot_of(t));
+            raise(most * scale, last);
             float from = top == -INFINITY ? 0.0f : top;
             if (far) {
 #pragma unroll
@@ -608,13 +484,15 @@ if (move)
                 scale = 1.0f;
                 from = 0.0f;
             }
-            // Written out in the order it runs: between the matrix instructions of the next tile's scores two values' softmax and a
-            // read four instructions ahead, and the first values' reads under the last of them. (The last tile's next one is
-            // whatever lies there.)
-            constexpr int LEAD = 4, PAIRS = 8, OUTS = 2 * DT;
-            bf16x8 k[LEAD], v[LEAD];
+            // Written out in the order it runs, reads LEAD instructions ahead: between the matrix instructions of the next scores the
+            // softmax, two values each, and after every second one of the outputs; then the other outputs, and between them the
+            // largest of the next scores and what the next barrier asks for. (The last tile's next one is whatever lies there.)
             Weights p2;
-            static_for<0, LEAD>([&](auto jc) { k[decltype(jc)::value] = keys(k_from, decltype(jc)::value); });
+            auto outputs = [&](auto oc) {
+                constexpr int i = decltype(oc)::value;
+                output(oc, v[i % LEAD]);
+                if constexpr (i + LEAD < OUTS) v[i % LEAD] = __builtin_bit_cast(bf16x8, values(v_from, (i + LEAD) / DT, (i + LEAD) % DT));
+            };
 #pragma unroll
             for (int e = 0; e < 16; ++e) next[e] = 0.0f;
             __builtin_amdgcn_sched_barrier(0);
@@ -622,43 +500,63 @@ if (move)
                 constexpr int j = decltype(jc)::value;
                 next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[j % LEAD], q[j], next, 0, 0, 0);
                 if constexpr (j + LEAD < STEPS) k[j % LEAD] = keys(k_from, j + LEAD);
-                else v[j + LEAD - STEPS] = __builtin_bit_cast(bf16x8, values(v_from, (j + LEAD - STEPS) / DT, (j + LEAD - STEPS) % DT));
-                static_for<PAIRS * j / STEPS, PAIRS *(j + 1) / STEPS>([&](auto ec) { pair(s, p2, ec, scale, from); });
+                static_for<8 * j / STEPS, 8 *(j + 1) / STEPS>([&](auto ec) { pair(s, p2, ec, scale, from); });
+                if constexpr (j & 1) outputs(std::integral_constant<int, j / 2>{});
                 __builtin_amdgcn_sched_barrier(0);
             });
-            static_for<0, OUTS>([&](auto jc) {
-                constexpr int j = decltype(jc)::value, ks = j / DT, d = j % DT;
-                if constexpr (PRECISE) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[j % LEAD], __builtin_bit_cast(bf16x8, p2.rest[ks]), o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[j % LEAD], __builtin_bit_cast(bf16x8, p2.w[ks]), o[d], 0, 0, 0);
-                if constexpr (j + LEAD < OUTS) v[j % LEAD] = __builtin_bit_cast(bf16x8, values(v_from, (j + LEAD) / DT, (j + LEAD) % DT));
+            asked = addresses(ids, base + (t + 1 + ahead) * TT);  // (past the last tile: the last token's)
+            ids = look_up(base + (t + 2 + ahead) * TT);
+            next_pages = pages_of(base + (t + 2) * TT);
+            static_for<STEPS / 2, OUTS>([&](auto jc) {
+                constexpr int i = decltype(jc)::value;
+                outputs(jc);
+                if constexpr (i == STEPS / 2) most = -INFINITY;
+                else static_for<16 * (i - STEPS / 2 - 1) / (STEPS / 2 - 1), 16 * (i - STEPS / 2) / (STEPS / 2 - 1)>([&](auto ec) { most = fmaxf(most, next[decltype(ec)::value]); });
                 __builtin_amdgcn_sched_barrier(0);
             });
+            last = p2;
             if constexpr (S::F8) {
                 if (t + ahead < t_to) widen(slot_of(t + ahead));
             }
-            tile_pages = next_pages;
             ++t;
+            first_fragments();
         };
         if (t < t_to) {
             __syncthreads();  // the run before has been read
+            // No outputs of a tile before the first: values of zero.
+            // (Whole waves, in a loop whose end is uniform: the compiler has put copies of registers that live past a loop with an end
+            // of its own for each lane where no lane is active.)
+#pragma unroll
+            for (int i = 64 * wave; i < S::MATRIX / 16; i += S::THREADS)
+                *reinterpret_cast<u32x4 *>(lds + S::STAGES * S::MATRIX + slot_of(t + S::STAGES - 1) + (i + lane) * 16) = u32x4{0, 0, 0, 0};
             for (int i = t; i < min(t + ahead, t_to); ++i) {
-                load(look_up(base + i * TT), base + i * TT, slot_of(i));
+                load(addresses(look_up(base + i * TT), base + i * TT), slot_of(i));
                 if constexpr (S::F8) widen(slot_of(i));
             }
-            ids = look_up(base + (t + ahead) * TT);  // (past the last tile: the last token's)
+            asked = addresses(look_up(base + (t + ahead) * TT), base + (t + ahead) * TT);
+            ids = look_up(base + (t + 1 + ahead) * TT);
             tile_pages = pages_of(base + t * TT);
+            next_pages = pages_of(base + (t + 1) * TT);
             if constexpr (!S::F8) wd::wait_vmcnt<0>();
+            written();
             barrier();
+            first_fragments();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s_even[e] = 0.0f;
+            for (int e = 0; e < 16; ++e) s_now[e] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < STEPS; ++j) s_even = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys(slot_of(t), j), q[j], s_even, 0, 0, 0);
+            for (int j = 0; j < STEPS; ++j) s_now = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys(slot_of(t), j), q[j], s_now, 0, 0, 0);
+            most = largest(s_now);
             for (;;) {
-                step(s_even, s_odd);
+                step(s_now, s_next);
                 if (t >= t_to) break;
-                step(s_odd, s_even);
-                if (t >= t_to) break;
+                s_now = s_next;
             }
+            const int v_from = slot_of(t + S::STAGES - 1);
+            static_for<0, OUTS>([&](auto jc) {
+                constexpr int j = decltype(jc)::value;
+                if constexpr (j < LEAD) output(jc, v[j]);
+                else output(jc, __builtin_bit_cast(bf16x8, values(v_from, j / DT, j % DT)));
+            });
         }
 
         // ---- the waves of a row joined, by the first ----
@@ -718,7 +616,7 @@ if (move)
                         }
                 }
             } else {
-                float *const slot = p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * attend_part_floats(DP, WM);
+                float *const slot = p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * attend_part_floats(DP, M);
                 if (h == 0) put(slot + 2 * (wm * 32 + c), Pair{top, sum});
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
@@ -733,12 +631,15 @@ if (move)
                                     p.kc + (kvh * p.kc_head + (S::PAGED ? 0 : seq.row0 * p.kc_tok)) * ES,
                                     p.vc + (kvh * p.vc_head + (S::PAGED ? 0 : seq.row0 * p.vc_tok)) * ES,
                                     S::PAGED ? p.pages + b * p.pages_row : nullptr,
-                                    whole ? nullptr : p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * attend_part_floats(DP, WM),
+                                    whole ? nullptr : p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * attend_part_floats(DP, M),
                                     p.q_tok, p.q_head, p.o_tok, p.o_head, p.kc_page * ES, p.kc_tok * ES, p.vc_page * ES, p.vc_tok * ES,
                                     p.page_mul, minus ? -unit_scale : unit_scale, capped ? p.softcap * LOG2E : 0.0f,
-                                    S::F8 && p.v_scale ? p.v_scale[kvh] : 1.0f, p.page_shift, p.page, p.page_count, row0, wm, rows, p.group,
+                                    S::F8 && p.v_scale ? p.v_scale[kvh] : 1.0f, p.page_shift, p.page, p.page_count, row0 + 32 * wm, min(row0 + 32 * wm + 32, rows), p.group,
                                     p.dim, first, seq.held, windowed ? p.window : 0, p.causal, base + t_from * TT, min(base + t_to * TT, seq.held)};
-            wild_rows<DP, WM, S::F8>(again);
+            wild_rows<DP, S::F8>(again, [&](int r) { return 2 * (r - row0); }, [&](int r, int x) {
+                const int c = (r - row0) & 31, d = x >> 5, e = 4 * (x >> 3 & 3) + (x & 3), half = x >> 2 & 1;
+                return 2 * M + 2 * (((wm * DT + d) * 8 + e / 2) * 64 + c + 32 * half) + (e & 1);
+            });
         }
         if (SHARE && !whole && tid == 0)
             parts[pos == start ? 0 : 1] = Part{seq0 + unit * units.run, units.run, row0, rows, kvh, seq.row0};
@@ -748,69 +649,11 @@ if (move)
     // ---- the parts' slots are written before their counters say so; the last workgroup to count joins ----
     if constexpr (!SHARE) return;
     __syncthreads();
-    if (parts[0].tiles == 0 && parts[1].tiles == 0) return;
-    wd::wait_vmcnt<0>();
-    __syncthreads();
-    if (tid < 2) {
-        const Part part = tid == 0 ? parts[0] : parts[1];
-        bool last = false;
-        if (part.tiles != 0) {
-            // Of the units that more than one workgroup has, one begins in each: its counter is that workgroup's.
-            const int g0 = share.of(part.first), others = share.of(part.first + part.tiles - 1) - g0;
-            int *const mark = p.marks + (int64_t)g0 * MARK;
-            last = __hip_atomic_fetch_add(mark, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == others;
-            if (last) __hip_atomic_store(mark, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-        joins[tid] = last;
-    }
-    __syncthreads();
-#pragma unroll 1
-    for (int i = 0; i < 2; ++i) {
-        if (!joins[i]) continue;
-        const Part part = i == 0 ? parts[0] : parts[1];
-        const int g0 = share.of(part.first), g1 = share.of(part.first + part.tiles - 1);
-        const int slot0 = 2 * g0 + (share.first(g0) < part.first ? 1 : 0);
-        const float v_scale = S::F8 && p.v_scale ? p.v_scale[part.kvh] : 1.0f;
-        // A thread takes two values, side by side in a row, of every slot.
-        for (int item = tid; item < M * DP / 2; item += S::THREADS) {
-            const int l = item & 63, e = 2 * (item >> 6 & 7), d = (item >> 9) % DT, set = (item >> 9) / DT;
-            const int row = 32 * set + (l & 31), at = 32 * d + 8 * (e >> 2) + 4 * (l >> 5) + (e & 3);
-            if (part.row0 + row >= part.rows || at >= p.dim) continue;
-            float top = -INFINITY, sum = 0.0f, x = 0.0f, y = 0.0f;
-            constexpr int ROUND = 4;  // slots whose loads are under way at once
-            for (int g = g0; g <= g1; g += ROUND) {
-                Pair s[ROUND], v[ROUND];
-#pragma unroll
-                for (int k = 0; k < ROUND; ++k) {
-                    const int from = min(g + k, g1);
-                    const float *const slot = p.part + (int64_t)(from == g0 ? slot0 : 2 * from) * attend_part_floats(DP, WM);
-                    s[k] = get(slot + 2 * row);
-                    v[k] = get(slot + 2 * M + 2 * item);
-                }
-                float most = top;
-#pragma unroll
-                for (int k = 0; k < ROUND; ++k) most = fmaxf(most, s[k].a);
-                const float from = most == -INFINITY ? 0.0f : most;
-                const float keep = __builtin_amdgcn_exp2f(top - from);
-                top = most;
-                sum *= keep;
-                x *= keep;
-                y *= keep;
-#pragma unroll
-                for (int k = 0; k < ROUND; ++k) {
-                    if (g + k > g1) continue;
-                    const float weight = __builtin_amdgcn_exp2f(s[k].a - from);
-                    sum = __builtin_fmaf(s[k].b, weight, sum);
-                    x = __builtin_fmaf(v[k].a, weight, x);
-                    y = __builtin_fmaf(v[k].b, weight, y);
-                }
-            }
-            const float by = inverse(sum) * v_scale;
-            const int r = part.row0 + row, tok = r / p.group, head = part.kvh * p.group + (r - tok * p.group);
-            *reinterpret_cast<uint32_t *>(p.out + (int64_t)(part.at + tok) * p.o_tok + (int64_t)head * p.o_head + at) =
-                pack_bf16_rne(x * by, y * by);
-        }
-    }
+    join_parts<M, DP, S::THREADS, S::F8>(p, share, parts, joins, [](int item, int &row, int &at) {
+        const int l = item & 63, e = 2 * (item >> 6 & 7), d = (item >> 9) % DT, set = (item >> 9) / DT;
+        row = 32 * set + (l & 31);
+        at = 32 * d + 8 * (e >> 2) + 4 * (l >> 5) + (e & 3);
+    });
 }
 
 }  // namespace attend

@@ -182,17 +182,21 @@ struct AttendArgs {
     int page_shift;
 };
 constexpr int attend_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }  // the instance of a head's size
-// Tokens of a tile that WT waves share, and the tiles that LDS holds: 64 KB of them, or 128 where one workgroup has a CU.
+// Tokens of a tile that WT waves share, and the tiles that LDS holds (a slot of 64 tokens of 128 values or 32 of 256: 32 KB).
 constexpr int attend_tokens(int wt) { return 32 * wt; }
-constexpr int attend_stages(int dp, int wt) { return dp * wt >= 512 ? 2 : 4; }
+constexpr int kAttendStages = 4;
 // Waves a SIMD holds.
 constexpr int attend_waves(int dp, int wt) { return dp * wt >= 256 ? 1 : 2; }
+// sq8_chunk.hip: workgroups of `rows` rows (16 nc) that a CU holds, by their registers and LDS.
+constexpr int chunk_held(int dp, int nc) { return dp < 256 && dp * nc <= 256 ? 2 : 1; }
 // A slot of a shared unit: maxima and sums [rows][2], outputs.
-__host__ __device__ constexpr int attend_part_floats(int dp, int wm) { return 32 * wm * (2 + dp); }
+__host__ __device__ constexpr int attend_part_floats(int dp, int rows) { return rows * (2 + dp); }
 // sq8_text_plan.hip. The tile and the workgroups that a call takes, and what it needs of the context's buffers.
 struct AttendPlan {
-    int wm, groups, share;
+    int rows;                   // of a tile; narrow: of sq8_chunk.hip
+    int groups, share, narrow;
     int64_t part_bytes, marks;
+    double tiles;               // of all units, at most
 };
 AttendPlan attend_plan(const AttendArgs &p, bool e4m3, int cus);
 hipError_t launch_attend(const AttendArgs &p, const AttendPlan &plan, bool e4m3, hipStream_t stream);
@@ -200,6 +204,7 @@ namespace attend {
 // Where keys and values lie: rows of a projection; pages whose tokens are a multiple of 16 (16 tokens lie in one page); any
 // pages; in bf16 or e4m3.
 enum Source { ROWS = 0, PAGES16, PAGES, PAGES16_F8, PAGES_F8 };
+hipError_t launch_chunk(const AttendArgs &p, const AttendPlan &plan, bool e4m3, hipStream_t stream);
 template <int SOURCE>
 hipError_t launch_source(const AttendArgs &p, const AttendPlan &plan, hipStream_t stream);
 }  // namespace attend

@@ -159,10 +159,7 @@ int run_attend(sq8_ctx *ctx, sq8::AttendArgs &p, const uint16_t *q, int64_t q_to
     if (p.dim > 256 || p.dim % 8 != 0) return SQ8_EUNSUPPORTED;
     if (!aligned(q, 16) || !aligned(out, 8) || (q_token | q_head) % 8 != 0 || (o_token | o_head) % 4 != 0) return SQ8_EUNSUPPORTED;
     p.group = q_heads / p.kv_heads;
-    // Rows, and the tiles of keys of all tiles of rows, are 32-bit.
-    const double longest = p.pages ? (double)p.max_pages * p.page : (double)tokens;
-    const double rows = (double)tokens * p.group;
-    if (rows > INT32_MAX - 4096 || (rows / 32 + sequences) * p.kv_heads * (p.pages ? longest / 32 + 2 : 1.0) > INT32_MAX) return SQ8_EUNSUPPORTED;
+    if ((double)tokens * p.group > INT32_MAX - 4096) return SQ8_EUNSUPPORTED;  // rows are 32-bit, as is the number of tiles below
     // (As sq8_paged_attention: a cap that no score comes near is none, a tiny one averages.)
     if (softcap > 0x1p100f) softcap = 0.0f;
     else if (softcap > 0.0f && softcap < 0x1p-60f) softcap = 0x1p-60f;
@@ -174,6 +171,7 @@ int run_attend(sq8_ctx *ctx, sq8::AttendArgs &p, const uint16_t *q, int64_t q_to
     p.tokens = tokens; p.sequences = sequences;
     sq8::page_divisor(p.page, p.page_mul, p.page_shift);
     const sq8::AttendPlan plan = sq8::attend_plan(p, e4m3, ctx->cus);
+    if (plan.tiles > INT32_MAX / 2) return SQ8_EUNSUPPORTED;
     p.share = plan.share;
     if (plan.part_bytes > 0) {
         int st = reserve(ctx, ctx->part, (size_t)plan.part_bytes);

@@ -101,6 +101,43 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {
     return v;
 }
 
+// The larger (the sum) of a value over the four lanes of a column (16 apart): the swaps leave each row's neighbour's, and
+// each half's other's, in the second of the pair.
+template <bool SUM>
+__device__ __forceinline__ float over_rows(float v) {
+    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+    auto both = [](u32x2_t r) {
+        const float a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
+        return SUM ? a + b : fmaxf(a, b);
+    };
+    v = both(__builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    return both(__builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+}
+
+template <int N>
+struct Raw {
+    uint32_t d[N];
+};
+
+template <int N>
+__device__ __forceinline__ Raw<N> load_raw(const uint8_t *src) {
+    Raw<N> r;
+    if constexpr (N == 1) {
+        r.d[0] = *reinterpret_cast<const uint32_t *>(src);
+    } else if constexpr (N == 2) {
+        const u32x2 v = *reinterpret_cast<const u32x2 *>(src);
+        r.d[0] = v[0]; r.d[1] = v[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const u32x4 v = reinterpret_cast<const u32x4 *>(src)[i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r.d[4 * i + e] = v[e];
+        }
+    }
+    return r;
+}
+
 // Two e4m3 codes (bytes 2W, 2W + 1) as a bf16 pair, exactly.
 template <int W>
 __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t d) {

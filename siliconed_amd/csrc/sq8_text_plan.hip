@@ -110,30 +110,45 @@ int64_t paged_part_bytes(const PagedArgs &p, int groups) {
 int64_t paged_marks(const PagedArgs &p) { return (int64_t)MARK * p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16); }
 
 AttendPlan attend_plan(const AttendArgs &p, bool e4m3, int cus) {
-    AttendPlan plan = {4, 0, 0, 0, 0};
+    AttendPlan plan = {128, 0, 0, 0, 0, 0, 0.0};
     if (p.sequences <= 0 || p.tokens <= 0) return plan;
     const int dp = attend_dim(p.dim);
-    const int64_t rows = (int64_t)p.tokens * p.group, each = (rows + p.sequences - 1) / p.sequences;
-    auto units = [&](int wm) { return (rows / (32 * wm) + p.sequences) * p.kv_heads; };  // at most
+    const int64_t each = ((int64_t)p.tokens * p.group + p.sequences - 1) / p.sequences;  // rows of a sequence and kv head, if all are alike
     plan.share = p.pages != nullptr;
+    const int64_t longest = (int64_t)p.max_pages * p.page;
+    auto alike = [&](int rows) { return (double)((each + rows - 1) / rows * p.sequences) * p.kv_heads; };  // units, if all are alike
     if (plan.share) {
-        plan.wm = each <= 32 ? 1 : each <= 64 ? 2 : each <= 128 ? 4 : 8;
+        // (In µs, of 8 key and 32 query heads of 128 in bf16.) Up to 64 rows a sequence, sq8_chunk.hip, which reads the cache at
+        // the rate of memory: 32 sequences of 16 tokens behind 8192, 251 and 267 with tiles of 128 rows. With more, tiles of 128
+        // and 256 rows as soon as a workgroup has 64 tiles of keys or more (8 sequences of 64 tokens, 131 and 177): else the join
+        // of their large parts costs more than the cache's rows read once for every 64 (one sequence of 64 tokens, 155 and 55).
+        const int wide = each <= 128 || dp == 256 || (dp == 64 && e4m3) ? 128 : 256;  // (fewer codes than eight waves load; registers)
+        const double each_has = alike(wide) * (double)longest / 32.0 / (wide == 128 && dp < 256 ? 2.0 * cus : cus);
+        plan.narrow = (each <= (dp == 256 ? 32 : 64) || each_has < 64.0) && p.dim % (dp / 16) == 0;  // (a lane's values: a row's or past it)
+        plan.rows = wide;
+        if (plan.narrow) {
+            // The most rows that are there to share what is read, if a workgroup has 16 tiles or more: else fewer, and more of them
+            // (one sequence of 16 tokens behind 32 768: 86, 91 and 105 with 16, 32 and 64 rows; 32 of them behind 8192: 402,
+            // 292 and 251).
+            plan.rows = each <= 16 ? 16 : each <= 32 || dp == 256 ? 32 : 64;
+            while (plan.rows > 16 && alike(plan.rows) * (double)longest / 128.0 < 16.0 * cus * chunk_held(dp, plan.rows / 16)) plan.rows /= 2;
+        }
     } else {
-        auto some = [&](int wm) { return (each + 32 * wm - 1) / (32 * wm) * p.sequences * p.kv_heads; };  // if all were alike
-        plan.wm = some(8) >= cus ? 8 : some(4) >= cus ? 4 : 2;
+        plan.rows = alike(256) >= cus ? 256 : alike(128) >= cus ? 128 : 64;
+        if (dp == 256) plan.rows = 128;
     }
-    if (dp == 256) plan.wm = plan.wm < 2 ? 2 : plan.wm > 4 ? 4 : plan.wm;
-    if (dp == 64 && e4m3 && plan.wm > 4) plan.wm = 4;  // (a tile's codes are fewer than eight waves' loads)
-    const int wt = plan.wm >= 4 ? 1 : plan.wm == 2 ? 2 : 4;
+    const double units = (double)((int64_t)p.tokens * p.group / plan.rows + p.sequences) * p.kv_heads;  // at most
+    const int wt = !plan.narrow && plan.rows == 64 ? 2 : 1, waves = plan.rows / 32 * wt;
+    const int tokens = plan.narrow ? 128 : attend_tokens(wt);
+    const double run = plan.share ? (double)((longest + tokens - 1) / tokens + 1) : 1.0;
+    plan.tiles = units * run;
     if (!plan.share) {
-        plan.groups = (int)units(plan.wm);
+        plan.groups = (int)std::min(plan.tiles, 2e9);
         return plan;
     }
-    const int tokens = attend_tokens(wt), held = attend_waves(dp, wt) * 4 / (plan.wm * wt);
-    const int64_t longest = (int64_t)p.max_pages * p.page;
-    const int64_t most = units(plan.wm) * std::max<int64_t>(1, (longest + tokens - 1) / tokens), full = (int64_t)held * cus;
-    plan.groups = (int)std::min(most, full);
-    plan.part_bytes = (int64_t)2 * plan.groups * attend_part_floats(dp, plan.wm) * 4;
+    const int held = plan.narrow ? chunk_held(dp, plan.rows / 16) : attend_waves(dp, wt) * 4 / waves;
+    plan.groups = (int)std::min(plan.tiles, (double)held * cus);
+    plan.part_bytes = (int64_t)2 * plan.groups * attend_part_floats(dp, plan.rows) * 4;
     plan.marks = (int64_t)MARK * plan.groups;
     return plan;
 }

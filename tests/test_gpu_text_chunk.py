@@ -60,20 +60,28 @@ class Batch:
         self.starts = ints(*(sum(n for n, _ in chunks[:i]) for i in range(len(chunks) + 1)))
         self.q = normal(g, int(self.starts[-1]) + spare, qh, dim).to(BF)
 
-    def run(self, gemm, **options):
+    def roomy(self):
+        """The table with room for two million tokens: many rows a sequence then go by larger tiles."""
+        page = self.cache.k.shape[1]
+        room = torch.full((len(self.chunks), (1 << 21) // page), -5, dtype=torch.int32, device=DEV)
+        room[:, :self.table.shape[1]] = self.table
+        return room
+
+    def run(self, gemm, table=None, **options):
         out = torch.full_like(self.q, 7.0)
-        got = gemm.chunk_attention(self.q, self.cache, self.table, self.lengths, self.starts, out=out, **options)
+        got = gemm.chunk_attention(self.q, self.cache, self.table if table is None else table, self.lengths, self.starts, out=out, **options)
         assert got is out
         return out
 
     def check(self, gemm, **options):
         print(f"chunks {self.chunks[:6]} q {tuple(self.q.shape)} pools {tuple(self.cache.k.shape)} {self.cache.k.dtype} {options}", flush=True)
-        out = self.run(gemm, **options)
+        out, again = self.run(gemm, **options), self.run(gemm, self.roomy(), **options)
         for b, (n, m) in enumerate(self.chunks):
             lo = int(self.starts[b])
             want, tol = attended(self.q[lo:lo + n], *self.values[b], m - n, dead=self.dead[b], **options)
             within(out[lo:lo + n], want, tol, f"sequence {b}: {n} of {m}")
-        assert (out[len(out) - self.spare:] == 7.0).all()
+            within(again[lo:lo + n], want, tol, f"sequence {b}: {n} of {m}, a roomy table")
+        assert (out[len(out) - self.spare:] == 7.0).all() and (again[len(out) - self.spare:] == 7.0).all()
         return out
 
 
@@ -100,7 +108,7 @@ def test_narrow_dims_in_bf16(gemm, dim):
     Batch([(9, 90), (4, 4)], 4, 2, dim, 16, BF).check(gemm)
 
 
-# Each tile of rows: up to 32, 64, 128 and more rows a sequence.
+# Each tile of rows: 16, 32, 64, 128 and 256 rows (a sequence's, or as many as a table's room makes worth while).
 @BOTH
 @pytest.mark.parametrize("new", [1, 7, 13, 30, 70, 200])
 @pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (128, 24), (256, 32)])
@@ -173,15 +181,18 @@ def test_lengths_are_cut_and_chunks_past_them_give_zeros(gemm):
     assert (gemm.chunk_attention(q, empty, table, ints(5, 5, 5), starts) == 0).all()
 
 
+@pytest.mark.parametrize("roomy", [False, True])
 @pytest.mark.parametrize("starts", [[4, 2, 9, 3], [0, 12, 1, 11], [50, 60, 70, 80]])
-def test_starts_that_do_not_ascend_stay_inside(gemm, starts):
+def test_starts_that_do_not_ascend_stay_inside(gemm, starts, roomy):
     """Whatever is written, rows outside stay, and the counters that workgroups share are left as they were found."""
-    b = Batch([(4, 2000), (4, 900), (4, 3000)], 8, 1, 64, 16, BF, spare=4)
-    want = b.check(gemm)
-    out = torch.full((20, 8, 64), 3.0, dtype=BF, device=DEV)
-    gemm.chunk_attention(b.q[:12], b.cache, b.table, b.lengths, ints(*starts), out=out[:12])
+    b = Batch([(4, 2000), (4, 900), (4, 3000)], 24, 1, 64, 16, BF, spare=4)
+    b.check(gemm)
+    table = b.roomy() if roomy else b.table
+    want = b.run(gemm, table)
+    out = torch.full((20, 24, 64), 3.0, dtype=BF, device=DEV)
+    gemm.chunk_attention(b.q[:12], b.cache, table, b.lengths, ints(*starts), out=out[:12])
     assert (out[12:] == 3.0).all()
-    assert torch.equal(b.run(gemm), want)
+    assert torch.equal(b.run(gemm, table), want)
 
 
 def test_offsets_past_32_bits(gemm):
@@ -202,13 +213,16 @@ def test_offsets_past_32_bits(gemm):
 
 
 @BOTH
-def test_infinite_and_nan_values_are_their_tokens(gemm, dtype):
+@pytest.mark.parametrize("roomy", [False, True])
+def test_infinite_and_nan_values_are_their_tokens(gemm, dtype, roomy):
     b = Batch([(40, 100), (40, 100)], 4, 2, 64, 16, dtype)
-    clean = b.check(gemm)
+    b.check(gemm)
+    table = b.roomy() if roomy else None
+    clean = b.run(gemm, table)
     page, place = int(b.table[0, 5]), 0  # token 80 of the first sequence: the chunk's twentieth
     pool = b.cache.v.view(torch.uint8)
     pool[page, place, 0, :2 if dtype == BF else 1] = 0xFF  # a NaN
-    out = b.run(gemm)
+    out = b.run(gemm, table)
     # Rows beside those that see it may be done without the matrix cores, their probabilities not rounded: the formula's tolerance
     # covers either, another sequence keeps its bits.
     want, tol = attended(b.q[:40], *b.values[0], 60)
