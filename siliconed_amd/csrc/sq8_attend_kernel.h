@@ -366,7 +366,7 @@ attend_kernel(const AttendArgs p) {
         // The maximum moved, where a score passes it by 8 powers of two. `far`: a maximum is so far from 0 that the scaled scores'
         // rounding, which a fused multiply-add does not share with it, would count: then the scores are taken as their scaled
         // distance from it here.
-        auto raise = [&](float m, Weights &last) {
+        auto raise = [&](float m) {
             const uint64_t move = __ballot(m > top + 8.0f);
             float keep = 1.0f;
             if (move) {
@@ -375,18 +375,12 @@ attend_kernel(const AttendArgs p) {
                 top = m;
                 sum *= keep;
                 far = __any(fabsf(top) > 0x1p24f && fabsf(top) < INFINITY);
-                // The probabilities that are still to be multiplied were taken from the maximum before: rounded once more here.
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t w = last.w[i >> 2][i & 3];
-                    last.w[i >> 2][i & 3] = pack_bf16_rne(__uint_as_float(w << 16) * keep, __uint_as_float(w & 0xFFFF0000u) * keep);
-                }
             }
             // In place, and past the compiler, which would keep a copy of every sum for the way that leaves them as they are. (They
             // come from matrix instructions: 18 waits before they are read, and some before the next ones take them.)
-if (move)
+            if (move)
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+                for (int d = 0; d < DT; ++d)
                 asm volatile("s_nop 15\n\ts_nop 1\n\t"
                              "v_mul_f32 %0, %0, %16\n\tv_mul_f32 %1, %1, %16\n\tv_mul_f32 %2, %2, %16\n\tv_mul_f32 %3, %3, %16\n\t"
                              "v_mul_f32 %4, %4, %16\n\tv_mul_f32 %5, %5, %16\n\tv_mul_f32 %6, %6, %16\n\tv_mul_f32 %7, %7, %16\n\t"
@@ -433,12 +427,12 @@ if (move)
             wild = wild || __any((found & 0x80008000u) != 0);
         };
 
-        // ---- the tiles: beside tile t's softmax run the scores of t + 1 and the outputs of t − 1 ----
-        // At the barrier of tile t all are done with the scores of t and the outputs of t − 2, so the keys of t + STAGES and the values
-        // of t + STAGES − 2 are asked for; the keys of t + 2 and the values of t have come, and those that were asked for at the
-        // STAGES − 3 barriers before may be under way. So the first fragments of a step are read before its barrier.
+        // ---- the tiles: beside tile t's softmax run the scores of t + 1 ----
+        // At the barrier of tile t all are done with the scores of t and the outputs of t − 1, so the keys of t + STAGES and the values
+        // of t + STAGES − 1 are asked for; the keys of t + 2 and the values of t + 1 have come, and those that were asked for at the
+        // STAGES − 3 barriers before may be under way. So the first keys of a step are read before its barrier.
         auto slot_of = [](int t) { return (t & (S::STAGES - 1)) * S::MATRIX; };
-        const int ahead = of_keys ? S::STAGES : S::STAGES - 2;
+        const int ahead = of_keys ? S::STAGES : S::STAGES - 1;
         // (What a wave writes to LDS it waits for itself; fragments on their way are of tiles that stay.)
         auto barrier = [] { asm volatile("s_barrier" ::: "memory"); };
         auto written = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
@@ -446,20 +440,11 @@ if (move)
         Ids ids = {};            // of the tile after the one whose
         Addresses asked = {};    // addresses these are: what the next barrier asks for
         Pages tile_pages = {}, next_pages = {};
-        Weights last = {};  // the probabilities of tile t − 1
-        auto output = [&](auto jc, bf16x8 v) {
-            constexpr int j = decltype(jc)::value;
-            o[j % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(bf16x8, last.w[j / DT]), o[j % DT], 0, 0, 0);
-        };
         constexpr int LEAD = 4, OUTS = 2 * DT;  // reads go this many instructions ahead
         float most = -INFINITY;                 // of the scores at hand
-        bf16x8 k[LEAD], v[LEAD];
-        auto first_fragments = [&]() {  // of step t
-            static_for<0, LEAD>([&](auto jc) {
-                constexpr int j = decltype(jc)::value;
-                k[j] = keys(slot_of(t + 1), j);
-                v[j] = __builtin_bit_cast(bf16x8, values(slot_of(t + S::STAGES - 1), j / DT, j % DT));
-            });
+        bf16x8 k[LEAD];
+        auto first_keys = [&]() {  // of step t
+            static_for<0, LEAD>([&](auto jc) { k[decltype(jc)::value] = keys(slot_of(t + 1), decltype(jc)::value); });
         };
         auto step = [&](f32x16 &s, f32x16 &next) {
             const Bad bad = bad_of(tile_pages);
@@ -472,11 +457,11 @@ if (move)
             if constexpr (S::F8) written();
             barrier();
             if (t + ahead < t_to) load(asked, slot_of(t + ahead));
-            const int k_from = slot_of(t + 1), v_from = slot_of(t + S::STAGES - 1);
+            const int k_from = slot_of(t + 1), v_from = slot_of(t);
             const int mine = base + t * TT + wave_token;  // the wave's first token
             float scale = unit_scale;
-            if (capped || mine + 31 > hi_min || mine < lo_max || bad.any()) edge(s, most, scale, mine, (uint32_t)bad.from(wave_token), slot_of(t));
-            raise(most * scale, last);
+            if (capped || mine + 31 > hi_min || mine < lo_max || bad.any()) edge(s, most, scale, mine, (uint32_t)bad.from(wave_token), v_from);
+            raise(most * scale);
             float from = top == -INFINITY ? 0.0f : top;
             if (far) {
 #pragma unroll
@@ -485,14 +470,10 @@ if (move)
                 from = 0.0f;
             }
             // Written out in the order it runs, reads LEAD instructions ahead: between the matrix instructions of the next scores the
-            // softmax, two values each, and after every second one of the outputs; then the other outputs, and between them the
-            // largest of the next scores and what the next barrier asks for. (The last tile's next one is whatever lies there.)
+            // softmax, two values each; then the outputs, and between them the largest of the next scores and what the next
+            // barrier asks for. (The last tile's next one is whatever lies there.)
             Weights p2;
-            auto outputs = [&](auto oc) {
-                constexpr int i = decltype(oc)::value;
-                output(oc, v[i % LEAD]);
-                if constexpr (i + LEAD < OUTS) v[i % LEAD] = __builtin_bit_cast(bf16x8, values(v_from, (i + LEAD) / DT, (i + LEAD) % DT));
-            };
+            bf16x8 v[LEAD];
 #pragma unroll
             for (int e = 0; e < 16; ++e) next[e] = 0.0f;
             __builtin_amdgcn_sched_barrier(0);
@@ -500,35 +481,29 @@ if (move)
                 constexpr int j = decltype(jc)::value;
                 next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[j % LEAD], q[j], next, 0, 0, 0);
                 if constexpr (j + LEAD < STEPS) k[j % LEAD] = keys(k_from, j + LEAD);
+                else v[j + LEAD - STEPS] = __builtin_bit_cast(bf16x8, values(v_from, (j + LEAD - STEPS) / DT, (j + LEAD - STEPS) % DT));
                 static_for<8 * j / STEPS, 8 *(j + 1) / STEPS>([&](auto ec) { pair(s, p2, ec, scale, from); });
-                if constexpr (j & 1) outputs(std::integral_constant<int, j / 2>{});
                 __builtin_amdgcn_sched_barrier(0);
             });
             asked = addresses(ids, base + (t + 1 + ahead) * TT);  // (past the last tile: the last token's)
             ids = look_up(base + (t + 2 + ahead) * TT);
             next_pages = pages_of(base + (t + 2) * TT);
-            static_for<STEPS / 2, OUTS>([&](auto jc) {
+            static_for<0, OUTS>([&](auto jc) {
                 constexpr int i = decltype(jc)::value;
-                outputs(jc);
-                if constexpr (i == STEPS / 2) most = -INFINITY;
-                else static_for<16 * (i - STEPS / 2 - 1) / (STEPS / 2 - 1), 16 * (i - STEPS / 2) / (STEPS / 2 - 1)>([&](auto ec) { most = fmaxf(most, next[decltype(ec)::value]); });
+                o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v[i % LEAD], __builtin_bit_cast(bf16x8, p2.w[i / DT]), o[i % DT], 0, 0, 0);
+                if constexpr (i + LEAD < OUTS) v[i % LEAD] = __builtin_bit_cast(bf16x8, values(v_from, (i + LEAD) / DT, (i + LEAD) % DT));
+                if constexpr (i == 0) most = -INFINITY;
+                else static_for<16 * (i - 1) / (OUTS - 1), 16 * i / (OUTS - 1)>([&](auto ec) { most = fmaxf(most, next[decltype(ec)::value]); });
                 __builtin_amdgcn_sched_barrier(0);
             });
-            last = p2;
             if constexpr (S::F8) {
                 if (t + ahead < t_to) widen(slot_of(t + ahead));
             }
             ++t;
-            first_fragments();
+            first_keys();
         };
         if (t < t_to) {
             __syncthreads();  // the run before has been read
-            // No outputs of a tile before the first: values of zero.
-            // (Whole waves, in a loop whose end is uniform: the compiler has put copies of registers that live past a loop with an end
-            // of its own for each lane where no lane is active.)
-#pragma unroll
-            for (int i = 64 * wave; i < S::MATRIX / 16; i += S::THREADS)
-                *reinterpret_cast<u32x4 *>(lds + S::STAGES * S::MATRIX + slot_of(t + S::STAGES - 1) + (i + lane) * 16) = u32x4{0, 0, 0, 0};
             for (int i = t; i < min(t + ahead, t_to); ++i) {
                 load(addresses(look_up(base + i * TT), base + i * TT), slot_of(i));
                 if constexpr (S::F8) widen(slot_of(i));
@@ -540,7 +515,7 @@ if (move)
             if constexpr (!S::F8) wd::wait_vmcnt<0>();
             written();
             barrier();
-            first_fragments();
+            first_keys();
 #pragma unroll
             for (int e = 0; e < 16; ++e) s_now[e] = 0.0f;
 #pragma unroll
@@ -551,12 +526,6 @@ if (move)
                 if (t >= t_to) break;
                 s_now = s_next;
             }
-            const int v_from = slot_of(t + S::STAGES - 1);
-            static_for<0, OUTS>([&](auto jc) {
-                constexpr int j = decltype(jc)::value;
-                if constexpr (j < LEAD) output(jc, v[j]);
-                else output(jc, __builtin_bit_cast(bf16x8, values(v_from, j / DT, j % DT)));
-            });
         }
 
         // ---- the waves of a row joined, by the first ----
