@@ -12,7 +12,7 @@
 // changes a bit, so a cut or a draw is the formula's but where a border is nearer than some 2^-40 of the whole. (In fp32 the
 // weights' errors would move each of a hundred thousand borders by 1e-7 of the whole: one draw in a hundred would differ.)
 //
-// A workgroup of 16 waves takes a row.
+// A workgroup of 8 waves takes a row.
 #include <hip/hip_runtime.h>
 
 #include "sq8_device.h"
@@ -22,7 +22,9 @@
 namespace sq8 {
 namespace {
 
-constexpr int THREADS = 1024, BINS = 1024, LIST = 4096, CHUNKS = 4096;
+constexpr int THREADS = 512, WAVES = THREADS / 64, BINS = THREADS, LOG_BINS = 9, LIST = 4096, CHUNKS = 4096;
+static_assert(BINS == 1 << LOG_BINS, "a bin a thread");
+constexpr unsigned FEW = 256;  // of so many, each is compared with every other
 constexpr int ONE = 43;  // a weight of 1 is 2^43: 2^20 of them fit 64 bits
 
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -62,27 +64,43 @@ struct Row {
         float x = BF16 ? bf16_f32(static_cast<const uint16_t *>(at)[i]) : static_cast<const float *>(at)[i];
         return x == x ? x : -INFINITY;  // a NaN is not drawn
     }
+    __device__ __forceinline__ u32x4 fetch(int i) const {
+        if constexpr (BF16) return *reinterpret_cast<const u32x4_any *>(static_cast<const uint16_t *>(at) + i);
+        else return *reinterpret_cast<const u32x4_any *>(static_cast<const float *>(at) + i);
+    }
+    static __device__ __forceinline__ void logits(const u32x4 &d, float (&x)[E]) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float v = BF16 ? __uint_as_float(e & 1 ? d[e / 2 % 4] & 0xFFFF0000u : d[e / 2 % 4] << 16) : __uint_as_float(d[e % 4]);
+            x[e] = v == v ? v : -INFINITY;
+        }
+    }
     // Eight (four) logits from i on; past the row's end, and for NaN, -inf.
     __device__ __forceinline__ void load(int i, float (&x)[E]) const {
         if (i + E <= vocab) {
-            if constexpr (BF16) {
-                load_run<8>(static_cast<const uint16_t *>(at) + i, x);
-            } else {
-                const u32x4 d = *reinterpret_cast<const u32x4_any *>(static_cast<const float *>(at) + i);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(d[e]);
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = x[e] == x[e] ? x[e] : -INFINITY;
+            logits(fetch(i), x);
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) x[e] = i + e < vocab ? one(i + e) : -INFINITY;
         }
     }
-    // f(first index, logits) of a lane's runs; a wave's lie side by side.
+    // f(first index, logits) of a lane's runs; a wave's lie side by side, and a lane's loads of 32 logits are under way at once.
     template <typename F>
     __device__ __forceinline__ void runs(F &&f) const {
-        for (int i = tid * E; i < vocab; i += THREADS * E) {
+        constexpr int STEP = THREADS * E, MANY = 32 / E;
+        int first = 0;
+        for (; first + MANY * STEP <= vocab; first += MANY * STEP) {
+            u32x4 d[MANY];
+#pragma unroll
+            for (int j = 0; j < MANY; ++j) d[j] = fetch(first + j * STEP + tid * E);
+#pragma unroll
+            for (int j = 0; j < MANY; ++j) {
+                float x[E];
+                logits(d[j], x);
+                f(first + j * STEP + tid * E, x);
+            }
+        }
+        for (int i = first + tid * E; i < vocab; i += STEP) {
             float x[E];
             load(i, x);
             f(i, x);
@@ -91,17 +109,17 @@ struct Row {
 };
 
 template <bool BF16>
-__global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) {
+__global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) {
     using R = Row<BF16>;
     constexpr int E = R::E;
     __shared__ uint64_t list[LIST];   // key and index of the logits near the top
     __shared__ uint64_t acc[CHUNKS];  // sums: of bins, or of chunks of indices
     __shared__ uint32_t cnt[BINS];
-    __shared__ uint64_t wave_sum[16];
-    __shared__ uint32_t wave_cnt[16];
-    __shared__ float wave_a[16], wave_b[16];
+    __shared__ uint64_t wave_sum[WAVES];
+    __shared__ uint32_t wave_cnt[WAVES];
+    __shared__ float wave_a[WAVES], wave_b[WAVES];
     __shared__ double table[64];
-    __shared__ uint32_t listed, found, found_cnt, found_has;
+    __shared__ uint32_t listed, gathered, found, found_cnt, found_has;
     __shared__ uint64_t found_sum;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t b = blockIdx.x;
@@ -116,20 +134,24 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
     const bool by_count = want > 0 && want < p.vocab, by_sum = !(top_p >= 1.0f);
     const bool greedy = !(t > 0.0f) || (by_count && want == 1);
 
-    // ---- the largest logit, and the threads' own largest ones ----
-    float mine = -INFINITY;
-    int mine_at = INT32_MAX;
+    // ---- the largest logit, and each thread's own two ----
+    float half[2] = {-INFINITY, -INFINITY};  // of the logits at even places, and at odd ones
+    int half_at[2] = {INT32_MAX, INT32_MAX};
     row.runs([&](int i, const float (&x)[E]) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
-            if (x[e] > mine) {
-                mine = x[e];
-                mine_at = i + e;
+            if (x[e] > half[e & 1]) {
+                half[e & 1] = x[e];
+                half_at[e & 1] = i + e;
             }
     });
+    const float mine = fmaxf(half[0], half[1]);
+    const int mine_at = half[0] > half[1] || (half[0] == half[1] && half_at[0] < half_at[1]) ? half_at[0] : half_at[1];
     if (tid < 64) table[tid] = exp2((double)tid * (1.0 / 64.0));
     {
-        float top = mine, low = mine > -INFINITY ? mine : INFINITY;
+        float top = mine, low = INFINITY;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) low = half[e] > -INFINITY ? fminf(low, half[e]) : low;
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) {
             top = fmaxf(top, __shfl_xor(top, o, 64));
@@ -146,7 +168,7 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
     __syncthreads();
     float top = wave_a[0], low = wave_b[0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) {
+    for (int i = 1; i < WAVES; ++i) {
         top = fmaxf(top, wave_a[i]);
         low = fminf(low, wave_b[i]);
     }
@@ -164,24 +186,25 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
         if (lane == 0) wave_cnt[wave] = (uint32_t)at;
         __syncthreads();
         if (tid == 0) {
-            for (int i = 0; i < 16; ++i) at = min(at, (int)wave_cnt[i]);
+            for (int i = 0; i < WAVES; ++i) at = min(at, (int)wave_cnt[i]);
             p.tokens[b] = at;
             if (p.logprobs) p.logprobs[b] = 0.0f;
         }
         return;
     }
 
-    // A weight, in units of 2^-43: 2^(k/64) from the table times e^r, |r| ≤ ln 2 / 128, whose series to r⁴ is within 2^-44.
+    // A weight, in units of 2^-43: 2^(k/64) from the table times 2^r, |r| ≤ 1/128, whose series to r⁴ is within 2^-44. (k in the
+    // low bits of y + 1.5 · 2^52; the exponent added as a whole number; rounded to 2^-43 by the addition of 2^9.)
     const double per = -64.0 * 1.4426950408889634 / (double)t, top64 = (double)top;
     auto weight = [&](float x) -> uint64_t {
-        if (x == top) return 1ull << ONE;
-        const double y = (top64 - (double)x) * per;
-        if (!(y > -64.0 * (ONE + 2))) return 0;
-        const double k = rint(y), r = (y - k) * (0.6931471805599453 / 64.0);
-        const double e = fma(r, fma(r, fma(r, fma(r, 1.0 / 24.0, 1.0 / 6.0), 0.5), 1.0), 1.0);
-        const int n = (int)k;
-        const double v = ldexp(table[n & 63] * e, n >> 6) + 0x1p9;  // rounded to 2^-43
-        return (uint64_t)__double_as_longlong(v) - (uint64_t)__double_as_longlong(0x1p9);
+        constexpr double C = 0.6931471805599453 / 64.0;
+        const double y = fmax((top64 - (double)x) * per, -64.0 * (ONE + 3)), near = y + 0x1.8p52;
+        const int n = (int)(uint32_t)__double_as_longlong(near);
+        const double r = y - (near - 0x1.8p52);
+        const double e = fma(r, fma(r, fma(r, fma(r, C * C * C * C / 24.0, C * C * C / 6.0), C * C / 2.0), C), 1.0);
+        const double v = __longlong_as_double(__double_as_longlong(table[n & 63] * e) + ((int64_t)(n >> 6) << 52)) + 0x1p9;
+        const uint64_t w = (uint64_t)__double_as_longlong(v) - (uint64_t)__double_as_longlong(0x1p9);
+        return x == top ? 1ull << ONE : w;
     };
 
     // Over the bins of cnt and acc, from the first: the one in which the counts reach `need`, or with `sums` the sums T.
@@ -208,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
         all_cnt = 0;
         all_sum = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < WAVES; ++i) {
             before_cnt += i < wave ? wave_cnt[i] : 0;
             before_sum += i < wave ? wave_sum[i] : 0;
             all_cnt += wave_cnt[i];
@@ -257,8 +280,8 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
         cut.keep = by_count ? min(all_cnt, (unsigned)want) : all_cnt;
         if (by_sum) cut.keep = max(1u, (unsigned)fmin((double)cut.keep, ceil((double)fmaxf(top_p, 0.0f) * (double)cut.keep)));
     } else if (!all_of_it) {
-        // ---- bins of the distance from the top: first down to where some 2000 logits lie (by the threads' largest ones), and
-        // those in a list; where the cut is not among them, down to where weights end ----
+        // ---- bins of the distance from the top: first down to where some 2000 logits lie, or as many as
+        // top_k (by the threads' largest ones), and those in a list; where the cut is not among them, down to where weights end ----
         float by = 0.0f;
         unsigned last = BINS - 1;
         const bool short_row = p.vocab <= LIST;
@@ -266,9 +289,11 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
         if (!short_row) {
             by = top > low ? (float)(BINS - 1) / (top - low) : 0.0f;
             if (!(by < 3e38f)) by = 0.0f;
-            if (mine > -INFINITY) atomicAdd(&cnt[bin_of(mine)], 1u);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (half[e] > -INFINITY) atomicAdd(&cnt[bin_of(half[e])], 1u);
             scan();
-            const Place at = place(false, min(900u, all_cnt), 0.0);
+            const Place at = place(false, min(by_count ? min(max((unsigned)want, 64u), 900u) : 900u, all_cnt), 0.0);
             last = at.bin;
         }
         double T = 0.0;
@@ -294,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
             __syncthreads();
             least = wave_b[0];
 #pragma unroll
-            for (int i = 1; i < 16; ++i) least = fminf(least, wave_b[i]);
+            for (int i = 1; i < WAVES; ++i) least = fminf(least, wave_b[i]);
         };
         auto far_span = [&]() { return by_count ? top - least : fminf(top - least, t * 31.2f); };  // (2^-45 at 31.19 t)
         if (short_row) {
@@ -308,6 +333,45 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
         // From a bin of distances (by `with`) to one key, over the list or the row.
         auto refine = [&](Place at, float with, bool sums, unsigned need, double goal, bool in_list) {
             by = with;
+            if (in_list && at.has <= FEW) {
+                // Few in the bin: gathered behind the bins' sums, and every one compared with the others.
+                uint64_t *const keys = acc + BINS, *const weights = keys + FEW;
+                if (tid == 0) gathered = 0;
+                __syncthreads();
+                const unsigned n = listed;
+                for (unsigned i = tid; i < n; i += THREADS) {
+                    const uint32_t key = (uint32_t)(list[i] >> 32);
+                    const float x = of_key(key);
+                    if (bin_of(x) == at.bin) {
+                        const uint32_t slot = atomicAdd(&gathered, 1u);
+                        keys[slot] = key;
+                        weights[slot] = sums ? weight(x) : 0;
+                    }
+                }
+                __syncthreads();
+                if ((unsigned)tid < at.has) {
+                    const uint32_t key = (uint32_t)keys[tid];
+                    unsigned more = at.cnt, same = 0;
+                    uint64_t sum = at.sum;
+                    for (unsigned j = 0; j < at.has; ++j) {
+                        const uint32_t k = (uint32_t)keys[j];
+                        more += k > key;
+                        same += k == key;
+                        if (sums) sum += k > key ? weights[j] : 0;
+                    }
+                    const bool here = sums ? (double)sum < goal && (double)(sum + same * weights[tid]) >= goal : more < need && more + same >= need;
+                    if (here) {  // (its equals write the same)
+                        found = key;
+                        found_cnt = more;
+                        found_has = same;
+                        found_sum = sum;
+                    }
+                }
+                __syncthreads();
+                const Cut c = {found, 0, found_has, found_cnt, found_sum};
+                __syncthreads();
+                return c;
+            }
             // The bin's keys: bin_of falls with the key, so both ends are found by halving (64 keys a step).
             auto first_key = [&](unsigned bin) {  // the smallest key whose bin is `bin` or less
                 uint32_t lo = 0;                  // (key_of(-inf) and less are in the last bins)
@@ -327,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
             Cut c = {hi, 0, 0, at.cnt, at.sum};
             for (;;) {
                 const uint32_t range = hi - lo;
-                const int sh = range < BINS ? 0 : 32 - __builtin_clz(range) - 10;
+                const int sh = range < BINS ? 0 : 32 - __builtin_clz(range) - LOG_BINS;
                 auto put_in = [&](uint32_t key, float x) {
                     if (key < lo || key > hi) return;
                     atomicAdd(&cnt[(hi - key) >> sh], 1u);
@@ -366,23 +430,59 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
         for (int pass = 0; pass < 2; ++pass) {
             uint64_t rest = 0;
             const bool sum_all = by_sum && !by_count && !wide;
-            row.runs([&](int i, const float (&x)[E]) {
+            auto put_in = [&](float x) {
+                const unsigned bin = bin_of(x);
+                if (bin > last) return;
+                atomicAdd(&cnt[bin], 1u);
+                if (by_sum) atomicAdd(reinterpret_cast<unsigned long long *>(&acc[bin]), (unsigned long long)weight(x));
+            };
+            if (!wide) {
+                // The list first, a wave's places in it taken at once.
+                const float rough = top - (float)(last + 2) / by;  // (no less than any that is in; by 0 gives -inf or a NaN)
+                row.runs([&](int i, const float (&x)[E]) {
+                    if (!sum_all) {
+                        float m = x[0];
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    if (!(x[e] > -INFINITY)) continue;
-                    const unsigned bin = bin_of(x[e]);
-                    if (bin <= last) {
-                        atomicAdd(&cnt[bin], 1u);
-                        if (by_sum) atomicAdd(reinterpret_cast<unsigned long long *>(&acc[bin]), (unsigned long long)weight(x[e]));
-                        if (!wide) {
-                            const uint32_t slot = atomicAdd(&listed, 1u);
-                            if (slot < LIST) list[slot] = (uint64_t)key_of(x[e]) << 32 | (uint32_t)(i + e);
-                        }
-                    } else if (sum_all) {
-                        rest += weight(x[e]);
+                        for (int e = 1; e < E; ++e) m = fmaxf(m, x[e]);
+                        if (!__any(!(m < rough))) return;
                     }
-                }
-            });
+                    uint64_t hit[E];
+                    unsigned all = 0;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        hit[e] = __ballot(x[e] > -INFINITY && bin_of(x[e]) <= last);
+                        all += __popcll(hit[e]);
+                    }
+                    if (sum_all) {
+                        uint64_t w[E];  // (side by side: each is a long chain)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) w[e] = weight(x[e]);
+#pragma unroll
+                        for (int e = 0; e < E; ++e) rest += hit[e] >> lane & 1 ? 0 : w[e];
+                    }
+                    if (all == 0) return;
+                    uint32_t slot = 0;
+                    if (lane == 0) slot = atomicAdd(&listed, all);  // (the first lane has a run wherever another has)
+                    slot = __builtin_amdgcn_readfirstlane(slot);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const uint32_t to = slot + __popcll(hit[e] & ((1ull << lane) - 1));
+                        if ((hit[e] >> lane & 1) && to < LIST) list[to] = (uint64_t)key_of(x[e]) << 32 | (uint32_t)(i + e);
+                        slot += __popcll(hit[e]);
+                    }
+                });
+                __syncthreads();
+            }
+            if (!wide && listed <= LIST) {
+                const unsigned n = listed;
+                for (unsigned i = tid; i < n; i += THREADS) put_in(of_key((uint32_t)(list[i] >> 32)));
+            } else {
+                row.runs([&](int, const float (&x)[E]) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (x[e] > -INFINITY) put_in(x[e]);
+                });
+            }
             scan();
             const unsigned in_bins = all_cnt;
             const uint64_t sum_bins = all_sum;
@@ -396,7 +496,7 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
                 __syncthreads();
                 rest = 0;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) rest += wave_sum[i];
+                for (int i = 0; i < WAVES; ++i) rest += wave_sum[i];
                 total = sum_bins + rest;
                 __syncthreads();
             }
@@ -490,6 +590,46 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
     const int chunks = (p.vocab + R::CHUNK - 1) / R::CHUNK;
     auto select = [&](auto &&value, auto &&goal, uint64_t &all) {
         __syncthreads();
+        if (from_list) {
+            // Few that count: each sums the others before it.
+            uint64_t *const values = acc, *const places = acc + FEW;
+            if (tid == 0) {
+                gathered = 0;
+                found_cnt = (uint32_t)p.vocab - 1;
+            }
+            __syncthreads();
+            const unsigned n = listed;
+            for (unsigned i = tid; i < n; i += THREADS) {
+                const uint32_t key = (uint32_t)(list[i] >> 32), at = (uint32_t)list[i];
+                const uint64_t v = value(key, of_key(key), at);
+                if (v) {
+                    const uint32_t slot = atomicAdd(&gathered, 1u);
+                    if (slot < FEW) {
+                        values[slot] = v;
+                        places[slot] = at;
+                    }
+                }
+            }
+            __syncthreads();
+            const unsigned few = gathered;
+            if (few <= FEW) {
+                uint64_t sum = 0, before = 0;
+                if ((unsigned)tid < few || tid == 0) {
+                    const uint64_t own = (unsigned)tid < few ? places[tid] : 0;
+                    for (unsigned j = 0; j < few; ++j) {
+                        sum += values[j];
+                        before += places[j] < own ? values[j] : 0;
+                    }
+                    if (tid == 0) wave_sum[0] = sum;
+                    if ((unsigned)tid < few && !goal(before, sum) && goal(before + values[tid], sum)) found_cnt = (uint32_t)own;
+                }
+                __syncthreads();
+                all = wave_sum[0];
+                const uint32_t at = found_cnt;
+                __syncthreads();
+                return at;
+            }
+        }
         for (int i = tid; i < CHUNKS; i += THREADS) acc[i] = 0;
         __syncthreads();
         if (from_list) {
@@ -500,7 +640,7 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
                 if (v) atomicAdd(reinterpret_cast<unsigned long long *>(&acc[at / R::CHUNK]), (unsigned long long)v);
             }
         } else {
-            for (int c = wave; c < chunks; c += 16) {
+            for (int c = wave; c < chunks; c += WAVES) {
                 float x[E];
                 const int i = c * R::CHUNK + lane * E;
                 row.load(i, x);
@@ -524,7 +664,7 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
         uint64_t at = 0;
         all = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < WAVES; ++i) {
             at += i < wave ? wave_sum[i] : 0;
             all += wave_sum[i];
         }
@@ -554,7 +694,7 @@ __global__ void __launch_bounds__(THREADS, 4) sample_kernel(const SampleArgs p) 
             }
         }
         __syncthreads();
-        return chunk != 0xFFFFFFFFu ? found_cnt : (uint32_t)p.vocab - 1;
+        return chunk != 0xFFFFFFFFu ? (uint32_t)found_cnt : (uint32_t)p.vocab - 1;
     };
     uint64_t total = 0;
     uint32_t last_at = 0xFFFFFFFFu;  // of the logits equal to the cut's, the last index kept
