@@ -20,7 +20,8 @@ per-output-channel product of this library (weights w ~ N(0, 0.02), s = amax/127
 q = clamp(rint(w/s), −127, 127), staged once in the packed layout). The residual stream is fp32 as
 in the reference; the products' operands are bf16. The modulated norms (eps 1e-6, MossImage.swift:49),
 the per-head norms and the gated residual updates are this library's elementwise passes; the
-attention is torch's fused flash / memory-efficient SDPA in bf16. RoPE is left out: an elementwise
+attention is torch's fused flash / memory-efficient SDPA in bf16, or with `attend="own"` this library's
+(sq8_norm_rotate, both per-head norms in one pass, and sq8_prompt_attention). RoPE is left out: an elementwise
 rotation of q and k, small next to the products.
 """
 from __future__ import annotations
@@ -50,14 +51,17 @@ class DiTBlock:
     """The block's weights (int8 packed, fp32 scales, fp32 norm weights) on one device."""
 
     def __init__(self, d: int = 3072, heads: int = 24, mlp: int = 4, seed: int = 0, device: int = 0,
-                 ctx: TensorGEMM | None = None, route: str = "bf16", group: int = 0, keep_codes: bool = False):
+                 ctx: TensorGEMM | None = None, route: str = "bf16", group: int = 0, keep_codes: bool = False,
+                 attend: str = "torch"):
         """`keep_codes`: also keep each weight's int8 codes [N, K] (key "q") beside the packed copy the
         forward reads — for a checker that widens them itself; off, only the packed codes stay resident."""
         if d % heads or (d // heads) % 8:
             raise ValueError("d must split into heads of a multiple of 8")
         if route not in ("bf16", "w8a8"):
             raise ValueError("route is 'bf16' or 'w8a8'")
-        self.route, self.group = route, group
+        if attend not in ("torch", "own"):
+            raise ValueError("attend is 'torch' or 'own'")
+        self.route, self.group, self.attend = route, group, attend
         self.d, self.heads, self.hd = d, heads, d // heads
         self.ctx = ctx or context(device)
         dev = torch.device("cuda", device)
@@ -89,6 +93,18 @@ class DiTBlock:
         return self.ctx.product_w8a8(codes, sx, lin["packed"], lin["s"], bias=lin["b"], epilogue=epilogue,
                                      out_dtype=out_dtype)
 
+    def _attend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """The per-head norms of q and k (in place) and the attention, [S, d] each."""
+        S = q.shape[0]
+        if self.attend == "own":
+            heads = lambda t: t.view(S, self.heads, self.hd)
+            self.ctx.norm_rotate(heads(q), heads(k), q_norm=self.norm_q, k_norm=self.norm_k, eps=EPS, q_out=heads(q), k_out=heads(k))
+            return self.ctx.prompt_attention(heads(q), heads(k), heads(v), causal=False).view(S, self.d)
+        self.ctx.rms_rows(q.view(S * self.heads, self.hd), self.norm_q, EPS)
+        self.ctx.rms_rows(k.view(S * self.heads, self.hd), self.norm_k, EPS)
+        heads = lambda t: t.view(S, self.heads, self.hd).transpose(0, 1)                        # [heads, S, hd]
+        return attention(heads(q), heads(k), heads(v)).transpose(0, 1).reshape(S, self.d)
+
     def _forward_w8a8(self, x: torch.Tensor, temb: torch.Tensor) -> torch.Tensor:
         S, d = x.shape
         ctx, g = self.ctx, self.group
@@ -96,10 +112,7 @@ class DiTBlock:
         shift_a, scale_a, gate_a, shift_f, scale_f, gate_f = mod.chunk(6)
         n8 = ctx.norm_modulate_quantized(x, self.norm_a, scale_a, shift_a, EPS, g)
         q, k, v = ctx.product_w8a8_qkv(n8[0], n8[1], self.qkv["packed"], self.qkv["s"], bias=self.qkv["b"])
-        ctx.rms_rows(q.view(S * self.heads, self.hd), self.norm_q, EPS)
-        ctx.rms_rows(k.view(S * self.heads, self.hd), self.norm_k, EPS)
-        heads = lambda t: t.view(S, self.heads, self.hd).transpose(0, 1)
-        o = attention(heads(q), heads(k), heads(v)).transpose(0, 1).reshape(S, d)
+        o = self._attend(q, k, v)
         o8 = ctx.quantize_rows(o, g)
         ctx.product_w8a8_residual(x, o8[0], o8[1], self.out["packed"], self.out["s"], bias=self.out["b"], gate=gate_a)
         m8 = ctx.norm_modulate_quantized(x, self.norm_f, scale_f, shift_f, EPS, g)
@@ -121,10 +134,7 @@ class DiTBlock:
         shift_a, scale_a, gate_a, shift_f, scale_f, gate_f = mod.chunk(6)
         n = ctx.norm_modulate(x, self.norm_a, scale_a, shift_a, EPS)
         q, k, v = ctx.product_qkv(n, self.qkv["packed"], self.qkv["s"], bias=self.qkv["b"])   # [S, d] each
-        ctx.rms_rows(q.view(S * self.heads, self.hd), self.norm_q, EPS)
-        ctx.rms_rows(k.view(S * self.heads, self.hd), self.norm_k, EPS)
-        heads = lambda t: t.view(S, self.heads, self.hd).transpose(0, 1)                        # [heads, S, hd]
-        o = attention(heads(q), heads(k), heads(v)).transpose(0, 1).reshape(S, d)
+        o = self._attend(q, k, v)
         ctx.product_residual(x, o, self.out["packed"], self.out["s"], bias=self.out["b"], gate=gate_a)
         m = ctx.norm_modulate(x, self.norm_f, scale_f, shift_f, EPS)
         h = self._product(m, self.up, epilogue="gelu_tanh")
