@@ -22,7 +22,7 @@
 namespace sq8 {
 namespace {
 
-constexpr int THREADS = 512, WAVES = THREADS / 64, BINS = THREADS, LOG_BINS = 9, LIST = 4096, CHUNKS = 4096;
+constexpr int THREADS = 512, WAVES = THREADS / 64, BINS = THREADS, LOG_BINS = 9, LIST = 4096, SEG = LIST / WAVES, CHUNKS = 4096;
 static_assert(BINS == 1 << LOG_BINS, "a bin a thread");
 constexpr unsigned FEW = 256;  // of so many, each is compared with every other
 constexpr int ONE = 43;  // a weight of 1 is 2^43: 2^20 of them fit 64 bits
@@ -112,14 +112,14 @@ template <bool BF16>
 __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) {
     using R = Row<BF16>;
     constexpr int E = R::E;
-    __shared__ uint64_t list[LIST];   // key and index of the logits near the top
+    __shared__ uint64_t list[LIST];   // key and index of the logits near the top, a segment a wave
     __shared__ uint64_t acc[CHUNKS];  // sums: of bins, or of chunks of indices
     __shared__ uint32_t cnt[BINS];
     __shared__ uint64_t wave_sum[WAVES];
     __shared__ uint32_t wave_cnt[WAVES];
     __shared__ float wave_a[WAVES], wave_b[WAVES];
     __shared__ double table[64];
-    __shared__ uint32_t listed, gathered, found, found_cnt, found_has;
+    __shared__ uint32_t crowded, gathered, found, found_cnt, found_has;
     __shared__ uint64_t found_sum;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t b = blockIdx.x;
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
     }
     cnt[tid] = 0;
     acc[tid] = 0;
-    if (tid == 0) listed = 0;
+    if (tid == 0) crowded = 0;  // a wave's segment is too short
     __syncthreads();
     float top = wave_a[0], low = wave_b[0];
 #pragma unroll
@@ -266,6 +266,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
     const uint32_t top_key = key_of(top);
     Cut cut = {0, 0, 0, 0, 0};
     bool from_list = false;   // what is kept lies in the list
+    uint64_t *const segment = list + wave * SEG;
+    uint32_t listed = 0;      // of the wave's
 
     if (!all_of_it && top == INFINITY) {
         // The infinities share everything.
@@ -338,9 +340,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                 uint64_t *const keys = acc + BINS, *const weights = keys + FEW;
                 if (tid == 0) gathered = 0;
                 __syncthreads();
-                const unsigned n = listed;
-                for (unsigned i = tid; i < n; i += THREADS) {
-                    const uint32_t key = (uint32_t)(list[i] >> 32);
+                for (unsigned i = lane; i < listed; i += 64) {
+                    const uint32_t key = (uint32_t)(segment[i] >> 32);
                     const float x = of_key(key);
                     if (bin_of(x) == at.bin) {
                         const uint32_t slot = atomicAdd(&gathered, 1u);
@@ -398,9 +399,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                     if (sums) atomicAdd(reinterpret_cast<unsigned long long *>(&acc[(hi - key) >> sh]), (unsigned long long)weight(x));
                 };
                 if (in_list) {
-                    const unsigned n = listed;
-                    for (unsigned i = tid; i < n; i += THREADS) {
-                        const uint32_t key = (uint32_t)(list[i] >> 32);
+                    for (unsigned i = lane; i < listed; i += 64) {
+                        const uint32_t key = (uint32_t)(segment[i] >> 32);
                         put_in(key, of_key(key));
                     }
                 } else {
@@ -428,7 +428,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
             return c;
         };
         for (int pass = 0; pass < 2; ++pass) {
-            uint64_t rest = 0;
+            double rest32 = 0.0;  // what lies past the bins, from exponentials in fp32
+            const float per32 = fminf(1.4426950408889634f / t, 3e38f);
             const bool sum_all = by_sum && !by_count && !wide;
             auto put_in = [&](float x) {
                 const unsigned bin = bin_of(x);
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                 if (by_sum) atomicAdd(reinterpret_cast<unsigned long long *>(&acc[bin]), (unsigned long long)weight(x));
             };
             if (!wide) {
-                // The list first, a wave's places in it taken at once.
+                // The list first.
                 const float rough = top - (float)(last + 2) / by;  // (no less than any that is in; by 0 gives -inf or a NaN)
                 row.runs([&](int i, const float (&x)[E]) {
                     if (!sum_all) {
@@ -446,36 +447,36 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                         for (int e = 1; e < E; ++e) m = fmaxf(m, x[e]);
                         if (!__any(!(m < rough))) return;
                     }
-                    uint64_t hit[E];
-                    unsigned all = 0;
+                    bool in[E];
+                    uint64_t hit[E], all = 0;
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        hit[e] = __ballot(x[e] > -INFINITY && bin_of(x[e]) <= last);
-                        all += __popcll(hit[e]);
+                        in[e] = x[e] > -INFINITY && bin_of(x[e]) <= last;
+                        hit[e] = __ballot(in[e]);
+                        all |= hit[e];
                     }
                     if (sum_all) {
-                        uint64_t w[E];  // (side by side: each is a long chain)
+                        float w[E], sum = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < E; ++e) w[e] = weight(x[e]);
+                        for (int e = 0; e < E; ++e) w[e] = in[e] ? 0.0f : __builtin_amdgcn_exp2f((x[e] - top) * per32);
 #pragma unroll
-                        for (int e = 0; e < E; ++e) rest += hit[e] >> lane & 1 ? 0 : w[e];
+                        for (int e = 0; e < E; ++e) sum += w[e];
+                        rest32 += (double)sum;
                     }
                     if (all == 0) return;
-                    uint32_t slot = 0;
-                    if (lane == 0) slot = atomicAdd(&listed, all);  // (the first lane has a run wherever another has)
-                    slot = __builtin_amdgcn_readfirstlane(slot);
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        const uint32_t to = slot + __popcll(hit[e] & ((1ull << lane) - 1));
-                        if ((hit[e] >> lane & 1) && to < LIST) list[to] = (uint64_t)key_of(x[e]) << 32 | (uint32_t)(i + e);
-                        slot += __popcll(hit[e]);
+                        const uint32_t to = __builtin_amdgcn_mbcnt_hi((uint32_t)(hit[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit[e], listed));
+                        if (in[e] && to < SEG) segment[to] = (uint64_t)key_of(x[e]) << 32 | (uint32_t)(i + e);
+                        listed += __popcll(hit[e]);
                     }
                 });
+                listed = __builtin_amdgcn_readfirstlane(listed);  // (a lane past the row's end has not counted to the last)
+                if (listed > SEG && lane == 0) crowded = 1;
                 __syncthreads();
             }
-            if (!wide && listed <= LIST) {
-                const unsigned n = listed;
-                for (unsigned i = tid; i < n; i += THREADS) put_in(of_key((uint32_t)(list[i] >> 32)));
+            if (!wide && !crowded) {
+                for (unsigned i = lane; i < listed; i += 64) put_in(of_key((uint32_t)(segment[i] >> 32)));
             } else {
                 row.runs([&](int, const float (&x)[E]) {
 #pragma unroll
@@ -486,19 +487,62 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
             scan();
             const unsigned in_bins = all_cnt;
             const uint64_t sum_bins = all_sum;
-            const bool held = !wide && listed <= LIST;
+            const bool held = !wide && !crowded;
+            // Sums over the workgroup of what the threads have.
+            auto of_all = [&](uint64_t v) {
+#pragma unroll
+                for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+                __syncthreads();
+                if (lane == 0) wave_sum[wave] = v;
+                __syncthreads();
+                v = 0;
+#pragma unroll
+                for (int i = 0; i < WAVES; ++i) v += wave_sum[i];
+                __syncthreads();
+                return v;
+            };
+            bool settled = false;
             if (sum_all) {
-                // What lies past the bins.
+                // The cut for the least and the most that the rest can be: a weight in fp32 is within 2^-17 of its value (its exponent,
+                // at most 45, three roundings; the exponential; eight in a sum), and a whole number of them within one. The same cut
+                // for both is the cut; else the rest is summed exactly.
+                const double est = (double)of_all((uint64_t)(rest32 * 0x1p43)), off = est * 0x1p-16 + (double)p.vocab + WAVES * 64.0;
+                const double share_of = (double)fmaxf(top_p, 0.0f), held_sum = (double)sum_bins;
+                const double low_T = fmax(share_of * (held_sum + fmax(est - off, 0.0)), 1.0), high_T = fmax(share_of * (held_sum + est + off), 1.0);
+                if (held_sum >= high_T && held) {
+                    const Place lo = place(true, 0, low_T), hi = place(true, 0, high_T);
+                    if (lo.bin == hi.bin && lo.has <= FEW) {
+                        const unsigned bc = before_cnt, sc = scan_cnt;
+                        const uint64_t bs = before_sum, ss = scan_sum;
+                        Cut cuts[2];
+#pragma unroll 1
+                        for (int i = 0; i < 2; ++i) {
+                            const double goal = i == 0 ? low_T : high_T;
+                            Cut c = refine(lo, by, true, 0, goal, true);
+                            const uint64_t w = weight(of_key(c.key));
+                            c.keep = w ? (unsigned)fmin(fmax(ceil((goal - (double)c.sum) / (double)w), 1.0), (double)c.ties) : c.ties;
+                            if (i == 0) cuts[0] = c;
+                            else cuts[1] = c;
+                        }
+                        settled = cuts[0].key == cuts[1].key && cuts[0].keep == cuts[1].keep;
+                        if (settled) cut = cuts[0];
+                        before_cnt = bc; scan_cnt = sc; before_sum = bs; scan_sum = ss;
+                    }
+                }
+                if (settled) {
+                    p_place.bin = BINS + 2;
+                    p_list = true;
+                } else {
+                    uint64_t rest = 0;
+                    row.runs([&](int, const float (&x)[E]) {
+                        uint64_t w[E];  // (side by side: each is a long chain)
 #pragma unroll
-                for (int o = 32; o >= 1; o >>= 1) rest += __shfl_xor(rest, o, 64);
-                __syncthreads();
-                if (lane == 0) wave_sum[wave] = rest;
-                __syncthreads();
-                rest = 0;
+                        for (int e = 0; e < E; ++e) w[e] = weight(x[e]);
 #pragma unroll
-                for (int i = 0; i < WAVES; ++i) rest += wave_sum[i];
-                total = sum_bins + rest;
-                __syncthreads();
+                        for (int e = 0; e < E; ++e) rest += x[e] > -INFINITY && bin_of(x[e]) <= last ? 0 : w[e];
+                    });
+                    total = sum_bins + of_all(rest);
+                }
             }
             bool short_of = false;  // what is looked for lies past the bins
             if (by_count && k_place.bin == BINS) {
@@ -525,9 +569,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                         uint64_t sum = 0;
                         auto take = [&](uint32_t key, float x) { sum += key > c.key ? weight(x) : 0; };
                         if (k_list) {
-                            const unsigned n = listed;
-                            for (unsigned i = tid; i < n; i += THREADS) {
-                                const uint32_t key = (uint32_t)(list[i] >> 32);
+                            for (unsigned i = lane; i < listed; i += 64) {
+                                const uint32_t key = (uint32_t)(segment[i] >> 32);
                                 take(key, of_key(key));
                             }
                         } else {
@@ -566,7 +609,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
         }
 
         // ---- the cut's key, and how many of the logits equal to it are kept ----
-        if (by_sum && p_place.bin < BINS) {
+        if (by_sum && p_place.bin == BINS + 2) {
+            from_list = p_list;  // settled above
+        } else if (by_sum && p_place.bin < BINS) {
             const Cut k_cut = cut;
             cut = refine(p_place, p_by, true, 0, T, p_list);
             const uint64_t w = weight(of_key(cut.key));
@@ -581,7 +626,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
         } else {
             cut.key = 0;  // all
             cut.ties = cut.keep = 0;
-            from_list = short_row && listed <= LIST;
+            from_list = short_row && !crowded;
         }
     }
 
@@ -598,9 +643,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                 found_cnt = (uint32_t)p.vocab - 1;
             }
             __syncthreads();
-            const unsigned n = listed;
-            for (unsigned i = tid; i < n; i += THREADS) {
-                const uint32_t key = (uint32_t)(list[i] >> 32), at = (uint32_t)list[i];
+            for (unsigned i = lane; i < listed; i += 64) {
+                const uint32_t key = (uint32_t)(segment[i] >> 32), at = (uint32_t)segment[i];
                 const uint64_t v = value(key, of_key(key), at);
                 if (v) {
                     const uint32_t slot = atomicAdd(&gathered, 1u);
@@ -633,9 +677,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
         for (int i = tid; i < CHUNKS; i += THREADS) acc[i] = 0;
         __syncthreads();
         if (from_list) {
-            const unsigned n = listed;
-            for (unsigned i = tid; i < n; i += THREADS) {
-                const uint32_t key = (uint32_t)(list[i] >> 32), at = (uint32_t)list[i];
+            for (unsigned i = lane; i < listed; i += 64) {
+                const uint32_t key = (uint32_t)(segment[i] >> 32), at = (uint32_t)segment[i];
                 const uint64_t v = value(key, of_key(key), at);
                 if (v) atomicAdd(reinterpret_cast<unsigned long long *>(&acc[at / R::CHUNK]), (unsigned long long)v);
             }
