@@ -57,6 +57,14 @@ struct Shape {
 __device__ __forceinline__ int key_k(int row) { return row & 7; }
 __device__ __forceinline__ int key_v(int row) { return 2 * (row & 3); }
 
+// 16 bytes a lane from memory to LDS, to the wave's place and 16 bytes on for each lane. Written out: beside the builtin, the
+// compiler waits for all loads under way before it reads anything transposed from LDS. (No register is loaded; whoever reads the
+// place waits for it by itself.)
+__device__ __forceinline__ void to_lds(const uint8_t *from, const uint8_t *place) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t *)place);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory", "m0");
+}
+
 // A value's maximum (sum) over the two lanes of a row.
 template <bool SUM>
 __device__ __forceinline__ float over_halves(float v) {
@@ -243,7 +251,7 @@ attend_kernel(const AttendArgs p) {
                 } else {
                     const int r = turned(i);
                     uint8_t *const to = lds + (of_keys ? 0 : S::STAGES * S::MATRIX) + slot + (slice * S::LOADS + i) * 1024;
-                    if (r < runs) __builtin_amdgcn_global_load_lds((wd::glb_ptr)(at + r * 16), (wd::lds_ptr)to, 16, 0, 0);
+                    if (r < runs) to_lds(at + r * 16, to);
                 }
             }
         };
@@ -431,7 +439,9 @@ attend_kernel(const AttendArgs p) {
         // At the barrier of tile t all are done with the scores of t and the outputs of t − 1, so the keys of t + STAGES and the values
         // of t + STAGES − 1 are asked for; the keys of t + 2 and the values of t + 1 have come, and those that were asked for at the
         // STAGES − 3 barriers before may be under way. So the first keys of a step are read before its barrier.
-        auto slot_of = [](int t) { return (t & (S::STAGES - 1)) * S::MATRIX; };
+        // A tile's slot goes by its number from the run's first, and the loop below is written out for each: the slots' places are
+        // then parts of the instructions, and the two sets of scores need no copies.
+        auto slot_of = [](int n) { return (n & (S::STAGES - 1)) * S::MATRIX; };
         const int ahead = of_keys ? S::STAGES : S::STAGES - 1;
         // (What a wave writes to LDS it waits for itself; fragments on their way are of tiles that stay.)
         auto barrier = [] { asm volatile("s_barrier" ::: "memory"); };
@@ -443,21 +453,23 @@ attend_kernel(const AttendArgs p) {
         constexpr int LEAD = 4, OUTS = 2 * DT;  // reads go this many instructions ahead
         float most = -INFINITY;                 // of the scores at hand
         bf16x8 k[LEAD];
-        auto first_keys = [&]() {  // of step t
-            static_for<0, LEAD>([&](auto jc) { k[decltype(jc)::value] = keys(slot_of(t + 1), decltype(jc)::value); });
+        auto first_keys = [&](auto nc) {  // of the step of slot n
+            static_for<0, LEAD>([&](auto jc) { k[decltype(jc)::value] = keys(slot_of(decltype(nc)::value + 1), decltype(jc)::value); });
         };
-        auto step = [&](f32x16 &s, f32x16 &next) {
+        static_assert(S::STAGES == 4, "a step for each");
+        auto step = [&](auto nc, f32x16 &s, f32x16 &next) {
+            constexpr int n = decltype(nc)::value;
             const Bad bad = bad_of(tile_pages);
             tile_pages = next_pages;
             if constexpr (!S::F8) {
                 if (t + S::STAGES > t_to) wd::wait_vmcnt<0>();
                 else wd::wait_vmcnt<(S::STAGES - 3) * S::LOADS>();
             }
-            clear(base + t * TT, bad, slot_of(t));
+            clear(base + t * TT, bad, slot_of(n));
             if constexpr (S::F8) written();
             barrier();
-            if (t + ahead < t_to) load(asked, slot_of(t + ahead));
-            const int k_from = slot_of(t + 1), v_from = slot_of(t);
+            if (t + ahead < t_to) load(asked, of_keys ? slot_of(n + S::STAGES) : slot_of(n + S::STAGES - 1));
+            const int k_from = slot_of(n + 1), v_from = slot_of(n);
             const int mine = base + t * TT + wave_token;  // the wave's first token
             float scale = unit_scale;
             if (capped || mine + 31 > hi_min || mine < lo_max || bad.any()) edge(s, most, scale, mine, (uint32_t)bad.from(wave_token), v_from);
@@ -486,6 +498,9 @@ attend_kernel(const AttendArgs p) {
                 __builtin_amdgcn_sched_barrier(0);
             });
             asked = addresses(ids, base + (t + 1 + ahead) * TT);  // (past the last tile: the last token's)
+            // Here, not where it is used.
+#pragma unroll
+            for (int i = 0; i < S::LOADS; ++i) asm volatile("" : "+v"(asked.at[i]));
             ids = look_up(base + (t + 2 + ahead) * TT);
             next_pages = pages_of(base + (t + 2) * TT);
             static_for<0, OUTS>([&](auto jc) {
@@ -494,19 +509,20 @@ attend_kernel(const AttendArgs p) {
                 if constexpr (i + LEAD < OUTS) v[i % LEAD] = __builtin_bit_cast(bf16x8, values(v_from, (i + LEAD) / DT, (i + LEAD) % DT));
                 if constexpr (i == 0) most = -INFINITY;
                 else static_for<16 * (i - 1) / (OUTS - 1), 16 * i / (OUTS - 1)>([&](auto ec) { most = fmaxf(most, next[decltype(ec)::value]); });
+                asm volatile("" : "+v"(most));
                 __builtin_amdgcn_sched_barrier(0);
             });
             if constexpr (S::F8) {
-                if (t + ahead < t_to) widen(slot_of(t + ahead));
+                if (t + ahead < t_to) widen(of_keys ? slot_of(n + S::STAGES) : slot_of(n + S::STAGES - 1));
             }
             ++t;
-            first_keys();
+            first_keys(std::integral_constant<int, n + 1>{});
         };
         if (t < t_to) {
             __syncthreads();  // the run before has been read
             for (int i = t; i < min(t + ahead, t_to); ++i) {
-                load(addresses(look_up(base + i * TT), base + i * TT), slot_of(i));
-                if constexpr (S::F8) widen(slot_of(i));
+                load(addresses(look_up(base + i * TT), base + i * TT), slot_of(i - t));
+                if constexpr (S::F8) widen(slot_of(i - t));
             }
             asked = addresses(look_up(base + (t + ahead) * TT), base + (t + ahead) * TT);
             ids = look_up(base + (t + 1 + ahead) * TT);
@@ -515,16 +531,21 @@ attend_kernel(const AttendArgs p) {
             if constexpr (!S::F8) wd::wait_vmcnt<0>();
             written();
             barrier();
-            first_keys();
+            first_keys(std::integral_constant<int, 0>{});
 #pragma unroll
             for (int e = 0; e < 16; ++e) s_now[e] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < STEPS; ++j) s_now = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys(slot_of(t), j), q[j], s_now, 0, 0, 0);
+            for (int j = 0; j < STEPS; ++j) s_now = __builtin_amdgcn_mfma_f32_32x32x16_bf16(keys(slot_of(0), j), q[j], s_now, 0, 0, 0);
             most = largest(s_now);
             for (;;) {
-                step(s_now, s_next);
+                step(std::integral_constant<int, 0>{}, s_now, s_next);
                 if (t >= t_to) break;
-                s_now = s_next;
+                step(std::integral_constant<int, 1>{}, s_next, s_now);
+                if (t >= t_to) break;
+                step(std::integral_constant<int, 2>{}, s_now, s_next);
+                if (t >= t_to) break;
+                step(std::integral_constant<int, 3>{}, s_next, s_now);
+                if (t >= t_to) break;
             }
         }
 
