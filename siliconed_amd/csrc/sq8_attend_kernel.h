@@ -60,9 +60,8 @@ __device__ __forceinline__ int key_v(int row) { return 2 * (row & 3); }
 // 16 bytes a lane from memory to LDS, to the wave's place and 16 bytes on for each lane. Written out: beside the builtin, the
 // compiler waits for all loads under way before it reads anything transposed from LDS. (No register is loaded; whoever reads the
 // place waits for it by itself.)
-__device__ __forceinline__ void to_lds(const uint8_t *from, const uint8_t *place) {
-    const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t *)place);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(at) : "memory", "m0");
+__device__ __forceinline__ void to_lds(const uint8_t *from, uint32_t place) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(place) : "memory", "m0");
 }
 
 // A value's maximum (sum) over the two lanes of a row.
@@ -225,14 +224,13 @@ attend_kernel(const AttendArgs p) {
                 const int at = w.id[i * S::PER_LOAD / 16], id = inside(at) ? at : 0;
                 return pool + (id * page_bytes + (int64_t)(t16 - page_of(t16) * p.page + (local & 15)) * tok_bytes) + in_bytes;
             } else {
-                // (Rows past the sequence's, up to the last of all, may be read: nothing sees them.)
-                const int from = token0 + local;
-                if (seq.row0 + token0 + TT <= p.tokens) return pool + from * tok_bytes + in_bytes;
-                return pool + min(from + in_load, seq.held - 1) * tok_bytes;
+                return pool + min(token0 + local + in_load, seq.held - 1) * tok_bytes;
             }
         };
+        const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)lds;
         // bf16: straight to LDS. e4m3: to registers, and widened into LDS later.
         u32x4 codes[S::F8 ? S::LOADS : 1];
+        const uint8_t *const last_row = pool + (seq.held - 1) * tok_bytes;
         struct Addresses {
             const uint8_t *at[S::LOADS];
         };
@@ -250,8 +248,7 @@ attend_kernel(const AttendArgs p) {
                     codes[i] = *reinterpret_cast<const u32x4 *>(at + (16 * run < p.dim ? 16 * run : 0));
                 } else {
                     const int r = turned(i);
-                    uint8_t *const to = lds + (of_keys ? 0 : S::STAGES * S::MATRIX) + slot + (slice * S::LOADS + i) * 1024;
-                    if (r < runs) to_lds(at + r * 16, to);
+                    if (r < runs) to_lds(at + r * 16, lds_at + (of_keys ? 0 : S::STAGES * S::MATRIX) + slice * S::LOADS * 1024 + slot + i * 1024);
                 }
             }
         };
@@ -369,7 +366,9 @@ attend_kernel(const AttendArgs p) {
             const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e], scale, -from));
             const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * e + 1], scale, -from));
             sum += x + y;
-            p2.w[e >> 2][e & 3] = pack_bf16_rne(x, y);
+            uint32_t both = pack_bf16_rne(x, y);
+            asm volatile("" : "+v"(both));  // here, not where it is used
+            p2.w[e >> 2][e & 3] = both;
         };
         // The maximum moved, where a score passes it by 8 powers of two. `far`: a maximum is so far from 0 that the scaled scores'
         // rounding, which a fused multiply-add does not share with it, would count: then the scores are taken as their scaled
@@ -497,7 +496,11 @@ attend_kernel(const AttendArgs p) {
                 static_for<8 * j / STEPS, 8 *(j + 1) / STEPS>([&](auto ec) { pair(s, p2, ec, scale, from); });
                 __builtin_amdgcn_sched_barrier(0);
             });
-            asked = addresses(ids, base + (t + 1 + ahead) * TT);  // (past the last tile: the last token's)
+            // (Past the last tile: the last token's.) Rows of a projection lie a tile's bytes on, the last token's at most.
+            if constexpr (S::PAGED) asked = addresses(ids, base + (t + 1 + ahead) * TT);
+            else
+#pragma unroll
+                for (int i = 0; i < S::LOADS; ++i) asked.at[i] = std::min(asked.at[i] + TT * tok_bytes, last_row);
             // Here, not where it is used.
 #pragma unroll
             for (int i = 0; i < S::LOADS; ++i) asm volatile("" : "+v"(asked.at[i]));
