@@ -137,13 +137,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
     // ---- the largest logit, and each thread's own two ----
     float half[2] = {-INFINITY, -INFINITY};  // of the logits at even places, and at odd ones
     int half_at[2] = {INT32_MAX, INT32_MAX};
+    float under = INFINITY;                    // the smallest but -inf
     row.runs([&](int i, const float (&x)[E]) {
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+        for (int e = 0; e < E; ++e) {
+            under = fminf(under, x[e] > -INFINITY ? x[e] : INFINITY);
             if (x[e] > half[e & 1]) {
                 half[e & 1] = x[e];
                 half_at[e & 1] = i + e;
             }
+        }
     });
     const float mine = fmaxf(half[0], half[1]);
     const int mine_at = half[0] > half[1] || (half[0] == half[1] && half_at[0] < half_at[1]) ? half_at[0] : half_at[1];
@@ -308,12 +311,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
         };
         float least = 0.0f;  // the row's smallest logit, where it is needed
         auto find_least = [&]() {
-            float v = INFINITY;
-            row.runs([&](int, const float (&x)[E]) {
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (x[e] > -INFINITY) v = fminf(v, x[e]);
-            });
+            float v = under;
 #pragma unroll
             for (int o = 32; o >= 1; o >>= 1) v = fminf(v, __shfl_xor(v, o, 64));
             __syncthreads();
@@ -479,9 +477,18 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                 for (unsigned i = lane; i < listed; i += 64) put_in(of_key((uint32_t)(segment[i] >> 32)));
             } else {
                 row.runs([&](int, const float (&x)[E]) {
+                    uint64_t w[E] = {};
+                    if (by_sum) {
 #pragma unroll
-                    for (int e = 0; e < E; ++e)
-                        if (x[e] > -INFINITY) put_in(x[e]);
+                        for (int e = 0; e < E; ++e) w[e] = weight(x[e]);  // (side by side: each is a long chain)
+                    }
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        const unsigned bin = bin_of(x[e]);
+                        if (!(x[e] > -INFINITY) || bin > last) continue;
+                        atomicAdd(&cnt[bin], 1u);
+                        if (by_sum) atomicAdd(reinterpret_cast<unsigned long long *>(&acc[bin]), (unsigned long long)w[e]);
+                    }
                 });
             }
             scan();
@@ -532,7 +539,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                 if (settled) {
                     p_place.bin = BINS + 2;
                     p_list = true;
-                } else {
+                } else if (held_sum >= low_T) {
                     uint64_t rest = 0;
                     row.runs([&](int, const float (&x)[E]) {
                         uint64_t w[E];  // (side by side: each is a long chain)
@@ -542,8 +549,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                         for (int e = 0; e < E; ++e) rest += x[e] > -INFINITY && bin_of(x[e]) <= last ? 0 : w[e];
                     });
                     total = sum_bins + of_all(rest);
+                } else {
+                    total = ~0ull;  // whatever it is, the cut lies past the bins
                 }
             }
+            if (wide && by_sum && !by_count) total = sum_bins;
             bool short_of = false;  // what is looked for lies past the bins
             if (by_count && k_place.bin == BINS) {
                 k_place = place(false, want, 0.0);
@@ -689,8 +699,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                 row.load(i, x);
                 uint64_t v = 0;
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (x[e] > -INFINITY) v += value(key_of(x[e]), x[e], (uint32_t)(i + e));
+                for (int e = 0; e < E; ++e) {
+                    const uint64_t one = value(key_of(x[e]), x[e], (uint32_t)(i + e));
+                    v += x[e] > -INFINITY ? one : 0;
+                }
 #pragma unroll
                 for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
                 if (lane == 0) acc[c] = v;
@@ -749,9 +761,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
     const double least_weight = (double)min_p * (double)(1ull << ONE), u = (double)fminf(fmaxf(p.uniform[b], 0.0f), 0x1.fffffep-1f);
     const uint32_t token = select(
         [&](uint32_t key, float x, uint32_t at) -> uint64_t {
-            if (key < cut.key || (key == cut.key && at > last_at)) return 0;
             const uint64_t w = weight(x);
-            return key == top_key || (double)w >= least_weight ? w : 0;
+            const bool taken = key > cut.key || (key == cut.key && at <= last_at);
+            return taken && (key == top_key || (double)w >= least_weight) ? w : 0;
         },
         [&](uint64_t s, uint64_t all) { return (double)s > u * (double)all; }, total);
     if (tid == 0) {
