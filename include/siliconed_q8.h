@@ -499,8 +499,8 @@ int sq8_norm_rotate(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_
  * t — with `causal` those up to i, and of these the last `window` (0: all; a window needs `causal`) —, s_t = scale · q_i·k_t,
  * capped to softcap · tanh(s_t / softcap) unless softcap is 0 (or infinite); query head h reads kv head h / (q_heads /
  * kv_heads). Rows of no sequence are left as they were; a token that is not seen may hold anything. Scores, maxima and sums
- * fp32; the probabilities are rounded to bf16 (by 2^-8 of each at most) for their product with v, or where few rows make the
- * call wait for memory, to 17 bits. dim up to 256, a multiple of 8; q, k and v rows 16-byte aligned, out 8-byte (else
+ * fp32; the probabilities are rounded to bf16 (by 2^-8 of each at most) for their product with v, or in chunks of few rows,
+ * which wait for memory, to 17 bits. dim up to 256, a multiple of 8; q, k and v rows 16-byte aligned, out 8-byte (else
  * SQ8_EUNSUPPORTED). No host copy of `starts` is needed: the call may be captured. */
 int sq8_prompt_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head,
                          const uint16_t *k, int64_t k_token, int64_t k_head, const uint16_t *v, int64_t v_token, int64_t v_head,

@@ -14,9 +14,26 @@
 // register r), and the second product takes its tokens in that order, so the probabilities are its operand as they lie and a
 // row's maximum and sum cross only two lanes.
 //
-// A workgroup has WM · WT waves: WM sets of 32 rows, and WT waves that share a tile's tokens and are joined at the end. Tiles
-// of keys and values go to LDS in two stages, the next tile's loads under way while one is used, in runs of 16 bytes whose
-// places are turned by the row's number, so that neither reads nor transposed reads meet in a bank.
+// A workgroup has WM · WT waves: WM sets of 32 rows, and WT waves that share a tile's tokens and are joined at the end. Tiles of
+// keys and values lie in four slots of LDS each, in runs of 16 bytes whose places are turned by the row's number; half the waves
+// load keys, half values, without registers, and bf16 tiles are asked for three and four barriers before their use (e4m3 codes
+// go through registers, widened on the way). One barrier a tile. Beside the softmax of a tile run the scores of the next, beside
+// its outputs the search of the next one's maximum and the addresses of what is asked for next; the loop is written out in that
+// order for each slot. What it took, of 8192 causal tokens with 32 heads on 8 of 128: keys a tile ahead of the values and no
+// spilled register (a reload waits for all loads under way) from 1.2 ms to 636 µs; the compiler's own waits out of the way (its
+// LDS loads made transposed reads of other slots wait for them) and maxima and conversions kept between the matrix instructions,
+// 571; addresses stepped instead of multiplied, 549.
+//
+// There it does 1000 TFLOP/s of the products that the mask leaves, where a large library product of normal values does 1384, both
+// at the power limit (1.8 GHz of 2.4): the matrix pipes are busy 48 % of the cycles, the vector ALUs 40 %. Without exponentials
+// it would take 8 % less, without loads 5 %, without three quarters of the second product 21 %: no one thing bounds it. Tried
+// and not faster: outputs a tile late beside the next tile's softmax (6 % slower), reads six instructions ahead, wave
+// priorities, places turned so that no read meets another in a bank (the counted conflicts went from 68 M to none, the time stayed),
+// loads between the matrix instructions. 4608 tokens of 24 heads, not causal, take 283 µs: 432 tiles on 256 CUs, two rounds
+// of which the second is two thirds full. 2048 new tokens behind 30 720 in pages of 64, 1.12 ms (960 TFLOP/s).
+//
+// Tiles of rows (sq8_text_plan.hip): 256, 128 or 64 for prompts, by how many there are for the card's CUs (100 tokens, 32 heads on
+// 8: 12 µs with 64, of which the launch and a chain of loads are most); 256 and 128 for chunks, and for few rows sq8_chunk.hip.
 #pragma once
 
 #include <hip/hip_runtime.h>

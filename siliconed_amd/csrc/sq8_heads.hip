@@ -6,6 +6,10 @@
 //
 // All in fp32. A head's units of two runs of W values (the halves of W pairs) lie in as many consecutive lanes, a power of
 // two of them, so the sum of squares crosses lanes by a few exchanges and everything is read and written once.
+//
+// Bound by memory: 8192 tokens of 32 and 8 heads of 128 into an e4m3 cache (189 MB with v) take 36.4 µs alone and 44 in turns
+// with other tensors (5.2 and 4.3 TB/s; a copy runs at 4.9); 4608 tokens of 24 and 24 beside the heads (116 MB) 26 and 31. One
+// token 2.9 to 3.5 µs, a launch.
 #include <hip/hip_runtime.h>
 
 #include "sq8_device.h"

@@ -1,5 +1,6 @@
 """A text decoder's operators: the norm that writes a product's 8-bit operand, products of block-scaled e4m3 codes,
-and a paged key-value cache with its append and its attention (the sq8_* entries of include/siliconed_q8.h).
+and a paged key-value cache with its append and its attention; heads normed in the pass that turns and appends them, attention of
+packed prompts and of chunks over the cache, and the draw of the next tokens (the sq8_* entries of include/siliconed_q8.h).
 
 `TensorGEMM` has them as methods; everything is queued on its stream. Outputs that a call allocates are torch's, of its
 current stream: make calls with the context's stream current (`torch.cuda.stream`), or hand in outputs and order the two
@@ -10,6 +11,10 @@ streams. With them, a decoder layer's step is
     q = ctx.append_kv(q, k, v, cache, positions, slots, table)
     o = ctx.paged_attention(q, cache, pages, lengths)
     y = ctx.product_f8_quantized(o.flatten(1), w_out, s_out)
+
+with normed heads norm_append_kv, with several new tokens of a sequence chunk_attention, and after the last layer
+
+    tokens, logprobs = ctx.sample_tokens(logits, uniform, temperature=t, top_p=p)
 """
 from __future__ import annotations
 
