@@ -132,45 +132,55 @@ __device__ __forceinline__ void wild_rows(const WildRows &w, PairAt pair_at, Val
     wd::wait_vmcnt<0>();
 }
 
-// The tiles of all sequences for one kv head, by 64 sequences at a time in every wave.
+// The tiles of all sequences for one kv head, by 64 sequences at a time in every wave; `upto`: of the first 64, those of a lane's and
+// before. Starts that do not ascend may count rows many times over: where the tiles of all kv heads would pass 32 bits, there
+// are none (the host has refused sizes that could by themselves).
 template <int M, int TT, bool SHARE>
-__device__ __forceinline__ int all_units(const AttendArgs &p, int lane) {
-    int total = 0;
+__device__ __forceinline__ int all_units(const AttendArgs &p, int lane, int &upto) {
+    auto of = [&](int i) {
+        if (i >= p.sequences) return 0;
+        const Units u = units_of<M, TT, SHARE>(p, sequence(p, i));
+        return u.tiles * u.run;
+    };
+    int64_t total = 0, most = INT32_MAX / p.kv_heads;
     for (int i = 0; i < p.sequences; i += 64) {
-        int v = 0;
-        if (i + lane < p.sequences) {
-            const Units u = units_of<M, TT, SHARE>(p, sequence(p, i + lane));
-            v = u.tiles * u.run;
+        const int v = of(i + lane);
+        // 64 values of up to 2^25 fit a scan; larger ones are summed one by one in 64 bits.
+        if (__any(v >> 25)) {
+            for (int l = 0; l < 64; ++l) total += __builtin_amdgcn_readlane(v, l);
+            if (i == 0 && total <= most) upto = wave_scan(v, lane);
+        } else {
+            const int sum = wave_scan(v, lane);
+            if (i == 0) upto = sum;
+            total += __builtin_amdgcn_readlane(sum, 63);
         }
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-        total += v;
+        if (total > most) return 0;
     }
-    return __builtin_amdgcn_readfirstlane(total);
+    return (int)total;
 }
 
 // The sequence that holds tile number `start` of all, and the tiles of one kv head in the sequences before it.
 template <int M, int TT, bool SHARE>
-__device__ __forceinline__ void find_unit(const AttendArgs &p, int start, int lane, int &b, int &before) {
+__device__ __forceinline__ void find_unit(const AttendArgs &p, int start, int lane, int upto, int &b, int &before) {
     before = b = 0;
     for (int i = 0; i < p.sequences; i += 64) {
-        int v = 0;
-        if (i + lane < p.sequences) {
-            const Units u = units_of<M, TT, SHARE>(p, sequence(p, i + lane));
-            v = u.tiles * u.run;
+        if (i > 0) {
+            int v = 0;
+            if (i + lane < p.sequences) {
+                const Units u = units_of<M, TT, SHARE>(p, sequence(p, i + lane));
+                v = u.tiles * u.run;
+            }
+            upto = wave_scan(v, lane);
         }
-        const int upto = wave_scan(v, lane);
         const uint64_t past = __ballot((before + upto) * p.kv_heads > start);
         if (past) {
             const int l = __ffsll((unsigned long long)past) - 1;
-            before += l > 0 ? __shfl(upto, l - 1, 64) : 0;
+            before += l > 0 ? __builtin_amdgcn_readlane(upto, l - 1) : 0;
             b = i + l;
-            break;
+            return;
         }
-        before += __shfl(upto, 63, 64);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
-    b = __builtin_amdgcn_readfirstlane(b);
-    before = __builtin_amdgcn_readfirstlane(before);
 }
 
 // A part of a unit: at most a workgroup's first unit and its last are parts.

@@ -115,7 +115,8 @@ attend_kernel(const AttendArgs p) {
     }
 
     // ---- this workgroup's tiles and the sequence they begin in; all uniform ----
-    const int total = all_units<M, TT, SHARE>(p, lane) * p.kv_heads;
+    int upto = 0;
+    const int total = all_units<M, TT, SHARE>(p, lane, upto) * p.kv_heads;
     const Share share(total, gridDim.x);
     int start, end, b = 0, before = 0;
     if constexpr (SHARE) {
@@ -128,7 +129,7 @@ attend_kernel(const AttendArgs p) {
         end = tile < tiles ? start + 1 : 0;
     }
     if (start >= end) return;
-    find_unit<M, TT, SHARE>(p, start, lane, b, before);
+    find_unit<M, TT, SHARE>(p, start, lane, upto, b, before);
     int seq0 = before * p.kv_heads;
     Sequence seq;
     Units units;

@@ -55,12 +55,13 @@ __global__ void __launch_bounds__(64 * WAVES, chunk_held(DP, NC)) chunk_kernel(c
 #pragma unroll
     for (int i = 0; i < 4; ++i) v_lane[i] = (uint32_t)((4 * h + i) * p.vc_tok * ES) + v_run;
 
-    const int total = all_units<M, TILE, true>(p, lane) * p.kv_heads;
+    int upto = 0;
+    const int total = all_units<M, TILE, true>(p, lane, upto) * p.kv_heads;
     const Share share(total, gridDim.x);
     const int start = share.first(min((int)blockIdx.x, share.groups)), end = share.first(min((int)blockIdx.x + 1, share.groups));
     if (start >= end) return;
     int b, before;
-    find_unit<M, TILE, true>(p, start, lane, b, before);
+    find_unit<M, TILE, true>(p, start, lane, upto, b, before);
     int seq0 = before * p.kv_heads;
     Sequence seq;
     Units units;

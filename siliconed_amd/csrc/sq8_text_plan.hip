@@ -134,7 +134,10 @@ AttendPlan attend_plan(const AttendArgs &p, bool e4m3, int cus) {
             while (plan.rows > 16 && alike(plan.rows) * (double)longest / 128.0 < 16.0 * cus * chunk_held(dp, plan.rows / 16)) plan.rows /= 2;
         }
     } else {
-        plan.rows = alike(256) >= cus ? 256 : alike(128) >= cus ? 128 : 64;
+        // Tiles of 128 rows, two workgroups a CU, whose beginnings and ends lie beside each other's tiles: sequences of 512, 1024 and 2048
+        // tokens, 16 384 in all, take 167, 231 and 349 µs (with 256 rows 190, 251 and 365). Of 4096 and more both hardly count, and
+        // 256 rows read keys and values half as often: one of 4096 takes 154 (165), two of 8192 1101 (1119).
+        plan.rows = p.tokens / p.sequences >= 4096 && alike(256) >= cus ? 256 : alike(128) >= cus ? 128 : 64;
         if (dp == 256) plan.rows = 128;
     }
     const double units = (double)((int64_t)p.tokens * p.group / plan.rows + p.sequences) * p.kv_heads;  // at most

@@ -195,6 +195,20 @@ def test_starts_that_do_not_ascend_stay_inside(gemm, starts, roomy):
     assert torch.equal(b.run(gemm, table), want)
 
 
+def test_starts_that_count_more_tiles_than_32_bits_hold(gemm):
+    """4096 sequences of 32 768 tokens that all claim the same 4096 rows: nothing past the rows is written, and calls go on."""
+    good = Batch([(4, 2000), (4, 900)], 32, 8, 64, 16, BF)
+    want = good.check(gemm)
+    k, v = (torch.zeros(2, 16, 8, 64, dtype=BF, device=DEV) for _ in "kv")
+    table = torch.zeros(4096, 2048, dtype=torch.int32, device=DEV)
+    starts = torch.tensor([0, 4096] * 2048 + [0], dtype=torch.int32, device=DEV)
+    out = torch.full((4104, 32, 64), 3.0, dtype=BF, device=DEV)
+    q = torch.zeros(4096, 32, 64, dtype=BF, device=DEV)
+    gemm.chunk_attention(q, sq.PagedCache(k, v), table, torch.full((4096,), 32768, dtype=torch.int32, device=DEV), starts, out=out[:4096])
+    assert (out[4096:] == 3.0).all()
+    assert torch.equal(good.run(gemm, good.roomy()), good.run(gemm, good.roomy())) and torch.equal(good.run(gemm), want)
+
+
 def test_offsets_past_32_bits(gemm):
     """A pool of 5 GB, the sequence's pages at its end."""
     pages, page, dim = 40000, 64, 128

@@ -47,9 +47,10 @@ def plan(tmp_path_factory):
 
 
 def test_prompts(plan):
-    """Tiles of 256 rows if they are as many as the card's 256 units, else of 128, else of 64; heads of 256: 128."""
-    assert plan(8192, 1)[:2] == (256, 0) and plan(4096, 1)[:2] == (256, 0) and plan(2048, 1)[:2] == (256, 0)
-    assert plan(2047, 1)[:2] == (256, 0) and plan(1900, 1)[0] == 128 and plan(700, 1)[0] == 64 and plan(1, 1)[0] == 64
+    """Of long sequences tiles of 256 rows, else of 128, if they are as many as the card's 256 units; else of 64; heads of 256: 128."""
+    assert plan(8192, 1)[:2] == (256, 0) and plan(4096, 1)[:2] == (256, 0) and plan(4095, 1)[:2] == (128, 0)
+    assert plan(8192, 2)[:2] == (256, 0) and plan(8192, 3)[:2] == (128, 0) and plan(4096, 1, kv=1, group=1)[0] == 64
+    assert plan(1000, 1)[0] == 128 and plan(900, 1)[0] == 64 and plan(700, 1)[0] == 64 and plan(1, 1)[0] == 64
     assert plan(8192, 1, dim=256)[0] == 128 and plan(5, 1, dim=200)[0] == 128
     assert plan(8192, 1)[2:5] == (8 * (32768 // 256 + 1), 0, 0)  # a workgroup a tile, nothing of the context
     assert plan(0, 3)[2] == 0 and plan(7, 0)[2] == 0
