@@ -195,7 +195,6 @@ attend_kernel(const AttendArgs p) {
             u32x4 v = {0, 0, 0, 0};
             if (live && 2 * s + h < runs)
                 v = *reinterpret_cast<const u32x4 *>(p.q + (int64_t)(seq.row0 + tok) * p.q_tok + (int64_t)head * p.q_head + 16 * s + 8 * h);
-            if (minus) v ^= u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
             q[s] = __builtin_bit_cast(bf16x8, v);
         }
 
@@ -553,6 +552,11 @@ attend_kernel(const AttendArgs p) {
             written();
             barrier();
             first_keys(std::integral_constant<int, 0>{});
+            if (minus) {  // (here, where the rows have come)
+#pragma unroll
+                for (int j = 0; j < STEPS; ++j)
+                    q[j] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, q[j]) ^ u32x4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u});
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) s_now[e] = 0.0f;
 #pragma unroll
@@ -611,20 +615,32 @@ attend_kernel(const AttendArgs p) {
             }
         }
         const bool whole = !SHARE || numbered == units.run;
+        if (WT == 1 && whole) __syncthreads();  // the last tile has been read
         if (wt == 0) {
             if (whole) {
-                if (live) {
-                    const float by = inverse(sum) * (S::F8 && p.v_scale ? p.v_scale[kvh] : 1.0f);
-                    uint16_t *const dst = p.out + (int64_t)(seq.row0 + tok) * p.o_tok + (int64_t)head * p.o_head;
+                // By way of LDS (a place of the wave's own), so that rows are written in whole runs: written as they lie, 16 bytes a row
+                // and instruction, they took 1.5 µs of a unit.
+                uint8_t *const mine = lds + (WT > 1 ? S::STAGES * S::MATRIX : 0) + wm * 32 * S::ROW;
+                const float by = inverse(sum) * (S::F8 && p.v_scale ? p.v_scale[kvh] : 1.0f);
+                auto key = [](int row) { return row & (S::RUNS < 16 ? S::RUNS - 1 : 15); };
 #pragma unroll
-                    for (int d = 0; d < DT; ++d)
+                for (int d = 0; d < DT; ++d)
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            const int at = 32 * d + 2 * e + 4 * h;
-                            if (at < p.dim)
-                                *reinterpret_cast<u32x2 *>(dst + at) = u32x2{pack_bf16_rne(o[d][e] * by, o[d][e + 1] * by),
-                                                                             pack_bf16_rne(o[d][e + 2] * by, o[d][e + 3] * by)};
-                        }
+                    for (int e = 0; e < 16; e += 4)
+                        *reinterpret_cast<u32x2 *>(mine + c * S::ROW + ((4 * d + e / 4) ^ key(c)) * 16 + 8 * h) =
+                            u32x2{pack_bf16_rne(o[d][e] * by, o[d][e + 1] * by), pack_bf16_rne(o[d][e + 2] * by, o[d][e + 3] * by)};
+                const int w_tok = w0 / p.group, w_head = w0 - w_tok * p.group;  // of the wave's first row
+                const float per = 1.0f / (float)p.group;
+                const int run = lane % S::RUNS;
+#pragma unroll
+                for (int i = 0; i < S::RUNS / 2; ++i) {
+                    const int row = i * (64 / S::RUNS) + lane / S::RUNS;
+                    const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + row * S::ROW + (run ^ key(row)) * 16);
+                    if (w0 + row >= rows || run >= runs) continue;
+                    // (w_head + row) / group: small numbers, or the next token at most.
+                    const int x = w_head + row, next = p.group >= 32 ? (x >= p.group ? 1 : 0) : (int)(((float)x + 0.5f) * per);
+                    uint16_t *const dst = p.out + (int64_t)(seq.row0 + w_tok + next) * p.o_tok + (int64_t)(kvh * p.group + x - next * p.group) * p.o_head;
+                    *reinterpret_cast<u32x4_any *>(dst + 8 * run) = v;
                 }
             } else {
                 float *const slot = p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * attend_part_floats(DP, M);
