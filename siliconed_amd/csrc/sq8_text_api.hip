@@ -163,6 +163,8 @@ int run_attend(sq8_ctx *ctx, sq8::AttendArgs &p, const uint16_t *q, int64_t q_to
     // (As sq8_paged_attention: a cap that no score comes near is none, a tiny one averages.)
     if (softcap > 0x1p100f) softcap = 0.0f;
     else if (softcap > 0.0f && softcap < 0x1p-60f) softcap = 0x1p-60f;
+    // A window that no sequence fills is none (and a place less it stays in 32 bits).
+    if (p.window > (p.pages ? (double)p.max_pages * p.page : (double)tokens)) p.window = 0;
     DeviceScope scope(ctx->device);
     if (scope.error != hipSuccess) return hip_status(scope.error);
     p.q = q; p.out = out;

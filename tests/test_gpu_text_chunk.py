@@ -174,6 +174,11 @@ def test_lengths_are_cut_and_chunks_past_them_give_zeros(gemm):
     flat = lambda pool, b: pool[table[b].long()].flatten(0, 1)  # noqa: E731
     o, tol = attended(q[2:4], flat(k, 0)[:2], flat(v, 0)[:2], 0)
     within(got[2:4], o, tol, "the two that are there")
+    for window in (5, (1 << 31) - 1):  # eleven new tokens, of which three are there, the others nowhere
+        wide = gemm.chunk_attention(q[:11], cache, table[:1], ints(3), window=window)
+        o, tol = attended(q[8:11], flat(k, 0)[:3], flat(v, 0)[:3], 0)
+        assert (wide[:8] == 0).all()
+        within(wide[8:], o, tol, "the three that are there")
     assert gemm.chunk_attention(q[:0], cache, table, ints(5, 5, 5), ints(0, 0, 0, 0)).shape == (0, 2, 64)
     none = gemm.chunk_attention(q, cache, table[:, :0], ints(5, 5, 5), starts)
     assert (none == 0).all()
