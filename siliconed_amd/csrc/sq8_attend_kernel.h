@@ -22,18 +22,20 @@
 // order for each slot. What it took, of 8192 causal tokens with 32 heads on 8 of 128: keys a tile ahead of the values and no
 // spilled register (a reload waits for all loads under way) from 1.2 ms to 636 µs; the compiler's own waits out of the way (its
 // LDS loads made transposed reads of other slots wait for them) and maxima and conversions kept between the matrix instructions,
-// 571; addresses stepped instead of multiplied, 549.
+// 571; addresses stepped instead of multiplied, 549; rows
+// written in whole runs, 533.
 //
-// There it does 1000 TFLOP/s of the products that the mask leaves, where a large library product of normal values does 1384, both
+// There it does 1030 TFLOP/s of the products that the mask leaves, where a large library product of normal values does 1384, both
 // at the power limit (1.8 GHz of 2.4): the matrix pipes are busy 48 % of the cycles, the vector ALUs 40 %. Without exponentials
 // it would take 8 % less, without loads 5 %, without three quarters of the second product 21 %: no one thing bounds it. Tried
 // and not faster: outputs a tile late beside the next tile's softmax (6 % slower), reads six instructions ahead, wave
 // priorities, places turned so that no read meets another in a bank (the counted conflicts went from 68 M to none, the time stayed),
-// loads between the matrix instructions. 4608 tokens of 24 heads, not causal, take 283 µs: 432 tiles on 256 CUs, two rounds
-// of which the second is two thirds full. 2048 new tokens behind 30 720 in pages of 64, 1.12 ms (960 TFLOP/s).
+// loads between the matrix instructions. 4608 tokens of 24 heads, not causal, take 275 µs: 432 tiles on 256 CUs, two rounds
+// of which the second is two thirds full. 2048 new tokens behind 30 720 in pages of 64, 1.10 ms (970 TFLOP/s).
 //
 // Tiles of rows (sq8_text_plan.hip): 256, 128 or 64 for prompts, by how many there are for the card's CUs (100 tokens, 32 heads on
-// 8: 12 µs with 64, of which the launch and a chain of loads are most); 256 and 128 for chunks, and for few rows sq8_chunk.hip.
+// 8: 11.6 µs with 64: the launch, 3 µs of loads one after another, four
+// tiles whose instructions are read for the first time, the join of two waves); 256 and 128 for chunks, and for few rows sq8_chunk.hip.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -231,7 +233,7 @@ attend_kernel(const AttendArgs p) {
         // Where load i's tokens lie: the lane's address.
         auto address = [&](const Ids &w, int token0, int i) -> const uint8_t * {
             const int local = slice * S::MINE + i * S::PER_LOAD;
-            const uint32_t in_bytes = (uint32_t)(in_load * (int)tok_bytes);
+            const int64_t in_bytes = in_load * tok_bytes;
             if constexpr (S::EACH) {
                 const int t = min(token0 + local + in_load, seq.held - 1);
                 const int id = inside(w.id[i]) ? w.id[i] : 0;

@@ -18,8 +18,8 @@
 // is a part of is first bounded by fp32 exponentials; only where the bounds disagree on the cut is it summed exactly. A wide
 // nucleus goes by bins over the row.
 //
-// 128 rows of 128 000 fp32 logits, every option set, take 36 µs: the first pass runs at the memory's rate (11 µs), the second, from
-// the last cache level, 14, the rest is barriers and scans. One row of 32 000 with a nucleus 24 to 27 µs, of which the list and the
+// 128 rows of 128 000 fp32 logits, every option set, take 37 µs: the first pass runs at the memory's rate (11 µs), the second, from
+// the last cache level, 14, the rest is barriers and scans. One row of 32 000 with a nucleus 23 to 27 µs, of which the list and the
 // fp32 sum are 10 (one CU's vector ALU) and the exact sum, one time in ten, 15 more. A nucleus past the list: 2 rows of 157 420
 // 240 µs, two passes of 64-bit exponentials of 50 each, three of keys; another workgroup a row would halve it. With sixteen
 // waves a row, whose registers spilled, and an atomic a listed logit the first two were 102 and 47.

@@ -121,7 +121,7 @@ AttendPlan attend_plan(const AttendArgs &p, bool e4m3, int cus) {
         // (In µs, of 8 key and 32 query heads of 128 in bf16.) Up to 64 rows a sequence, sq8_chunk.hip, which reads the cache at
         // the rate of memory: 32 sequences of 16 tokens behind 8192, 251 and 267 with tiles of 128 rows. With more, tiles of 128
         // and 256 rows as soon as a workgroup has 64 tiles of keys or more (8 sequences of 64 tokens, 131 and 177): else the join
-        // of their large parts costs more than the cache's rows read once for every 64 (one sequence of 64 tokens, 155 and 55).
+        // of their large parts costs more than the cache's rows read once for every 64 (one sequence of 64 tokens, 155 and 57).
         const int wide = each <= 128 || dp == 256 || (dp == 64 && e4m3) ? 128 : 256;  // (fewer codes than eight waves load; registers)
         const double each_has = alike(wide) * (double)longest / 32.0 / (wide == 128 && dp < 256 ? 2.0 * cus : cus);
         plan.narrow = (each <= (dp == 256 ? 32 : 64) || each_has < 64.0) && p.dim % (dp / 16) == 0;  // (a lane's values: a row's or past it)
@@ -135,8 +135,8 @@ AttendPlan attend_plan(const AttendArgs &p, bool e4m3, int cus) {
         }
     } else {
         // Tiles of 128 rows, two workgroups a CU, whose beginnings and ends lie beside each other's tiles: sequences of 512, 1024 and 2048
-        // tokens, 16 384 in all, take 167, 231 and 349 µs (with 256 rows 190, 251 and 365). Of 4096 and more both hardly count, and
-        // 256 rows read keys and values half as often: one of 4096 takes 154 (165), two of 8192 1101 (1119).
+        // tokens, 16 384 in all, take 151, 210 and 331 µs (with 256 rows 172, 231 and 340). Of 4096 and more both hardly count, and
+        // 256 rows read keys and values half as often: one of 4096 takes 147 (160), two of 8192 1055 (1080).
         plan.rows = p.tokens / p.sequences >= 4096 && alike(256) >= cus ? 256 : alike(128) >= cus ? 128 : 64;
         if (dp == 256) plan.rows = 128;
     }
