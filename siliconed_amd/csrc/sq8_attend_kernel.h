@@ -107,14 +107,15 @@ attend_kernel(const AttendArgs p) {
     const bool capped = p.softcap > 0.0f;
     const int runs = p.dim / 8;  // 16-byte runs of a token that hold values
 
-    // Runs past `dim` are zeros, written once: no load fills them.
-    if (runs < S::RUNS) {
+    // Runs past `dim` are zeros, which no load fills: written here, and again where a unit's outputs went by way of LDS.
+    auto clear_ends = [&]() {
+        if (runs >= S::RUNS) return;
         for (int i = tid; i < 2 * S::STAGES * TT * S::RUNS; i += S::THREADS) {
             const int token = i / S::RUNS % TT, run = i % S::RUNS, matrix = i / (S::RUNS * TT * S::STAGES);
             if ((run ^ (matrix ? key_v(token) : key_k(token))) >= runs) *reinterpret_cast<u32x4 *>(lds + i * 16) = u32x4{0, 0, 0, 0};
         }
-        __syncthreads();
-    }
+    };
+    clear_ends();
 
     // ---- this workgroup's tiles and the sequence they begin in; all uniform ----
     int upto = 0;
@@ -542,6 +543,7 @@ attend_kernel(const AttendArgs p) {
         };
         if (t < t_to) {
             __syncthreads();  // the run before has been read
+            if (SHARE && DP <= 128 && pos != start) clear_ends();
             for (int i = t; i < min(t + ahead, t_to); ++i) {
                 load(addresses(look_up(base + i * TT), base + i * TT), slot_of(i - t));
                 if constexpr (S::F8) widen(slot_of(i - t));
@@ -617,32 +619,48 @@ attend_kernel(const AttendArgs p) {
             }
         }
         const bool whole = !SHARE || numbered == units.run;
-        if (WT == 1 && whole) __syncthreads();  // the last tile has been read
+        if (WT == 1 && DP <= 128 && whole) __syncthreads();  // the last tile has been read
         if (wt == 0) {
             if (whole) {
-                // By way of LDS (a place of the wave's own), so that rows are written in whole runs: written as they lie, 16 bytes a row
-                // and instruction, they took 1.5 µs of a unit.
-                uint8_t *const mine = lds + (WT > 1 ? S::STAGES * S::MATRIX : 0) + wm * 32 * S::ROW;
                 const float by = inverse(sum) * (S::F8 && p.v_scale ? p.v_scale[kvh] : 1.0f);
-                auto key = [](int row) { return row & (S::RUNS < 16 ? S::RUNS - 1 : 15); };
+                if constexpr (DP > 128) {
+                    // As they lie: the way below takes registers that spill (8192 tokens of 16 heads of 256, 976 and 923 µs).
+                    if (live) {
+                        uint16_t *const dst = p.out + (int64_t)(seq.row0 + tok) * p.o_tok + (int64_t)head * p.o_head;
 #pragma unroll
-                for (int d = 0; d < DT; ++d)
+                        for (int d = 0; d < DT; ++d)
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        *reinterpret_cast<u32x2 *>(mine + c * S::ROW + ((4 * d + e / 4) ^ key(c)) * 16 + 8 * h) =
-                            u32x2{pack_bf16_rne(o[d][e] * by, o[d][e + 1] * by), pack_bf16_rne(o[d][e + 2] * by, o[d][e + 3] * by)};
-                const int w_tok = w0 / p.group, w_head = w0 - w_tok * p.group;  // of the wave's first row
-                const float per = 1.0f / (float)p.group;
-                const int run = lane % S::RUNS;
+                            for (int e = 0; e < 16; e += 4) {
+                                const int at = 32 * d + 2 * e + 4 * h;
+                                if (at < p.dim)
+                                    *reinterpret_cast<u32x2 *>(dst + at) = u32x2{pack_bf16_rne(o[d][e] * by, o[d][e + 1] * by),
+                                                                                 pack_bf16_rne(o[d][e + 2] * by, o[d][e + 3] * by)};
+                            }
+                    }
+                } else {
+                    // By way of LDS (a place of the wave's own), so that rows are written in whole runs: written as they lie, 16 bytes a row
+                    // and instruction, they took 1.5 µs of a unit.
+                    uint8_t *const mine = lds + (WT > 1 ? S::STAGES * S::MATRIX : 0) + wm * 32 * S::ROW;
+                    auto key = [](int row) { return row & (S::RUNS < 16 ? S::RUNS - 1 : 15); };
 #pragma unroll
-                for (int i = 0; i < S::RUNS / 2; ++i) {
-                    const int row = i * (64 / S::RUNS) + lane / S::RUNS;
-                    const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + row * S::ROW + (run ^ key(row)) * 16);
-                    if (w0 + row >= rows || run >= runs) continue;
-                    // (w_head + row) / group: small numbers, or the next token at most.
-                    const int x = w_head + row, next = p.group >= 32 ? (x >= p.group ? 1 : 0) : (int)(((float)x + 0.5f) * per);
-                    uint16_t *const dst = p.out + (int64_t)(seq.row0 + w_tok + next) * p.o_tok + (int64_t)(kvh * p.group + x - next * p.group) * p.o_head;
-                    *reinterpret_cast<u32x4_any *>(dst + 8 * run) = v;
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            *reinterpret_cast<u32x2 *>(mine + c * S::ROW + ((4 * d + e / 4) ^ key(c)) * 16 + 8 * h) =
+                                u32x2{pack_bf16_rne(o[d][e] * by, o[d][e + 1] * by), pack_bf16_rne(o[d][e + 2] * by, o[d][e + 3] * by)};
+                    const int w_tok = w0 / p.group, w_head = w0 - w_tok * p.group;  // of the wave's first row
+                    const float per = 1.0f / (float)p.group;
+                    const int run = lane % S::RUNS;
+#pragma unroll
+                    for (int i = 0; i < S::RUNS / 2; ++i) {
+                        const int row = i * (64 / S::RUNS) + lane / S::RUNS;
+                        const u32x4 v = *reinterpret_cast<const u32x4 *>(mine + row * S::ROW + (run ^ key(row)) * 16);
+                        if (w0 + row >= rows || run >= runs) continue;
+                        // (w_head + row) / group: small numbers, or the next token at most.
+                        const int x = w_head + row, next = p.group >= 32 ? (x >= p.group ? 1 : 0) : (int)(((float)x + 0.5f) * per);
+                        uint16_t *const dst = p.out + (int64_t)(seq.row0 + w_tok + next) * p.o_tok + (int64_t)(kvh * p.group + x - next * p.group) * p.o_head;
+                        *reinterpret_cast<u32x4_any *>(dst + 8 * run) = v;
+                    }
                 }
             } else {
                 float *const slot = p.part + (int64_t)(2 * blockIdx.x + (pos == start ? 0 : 1)) * attend_part_floats(DP, M);

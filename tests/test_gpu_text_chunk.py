@@ -308,3 +308,21 @@ def test_a_graph_s_replays_beside_other_attention(gemm):
             assert torch.equal(out, o) and torch.equal(single, s), i
         ctx.set_stream(torch.cuda.default_stream())
     torch.cuda.current_stream().wait_stream(side)
+
+
+@BOTH
+@pytest.mark.parametrize("dim", [80, 96, 48])
+def test_a_sequence_s_nan_stays_with_it(gemm, dtype, dim):
+    """Heads narrower than their tiles, many sequences to a workgroup: a NaN in every seventh's cache is in no other's output."""
+    b = Batch([(20, 70)] * 300, 16, 4, dim, 64, dtype)
+    room = torch.full((300, 1 << 15), -5, dtype=torch.int32, device=DEV)
+    room[:, :b.table.shape[1]] = b.table
+    for table in (None, room):
+        clean = b.run(gemm, table).view(300, 20, 16, dim)
+        pool, kept = b.cache.v.view(torch.uint8), b.cache.v.view(torch.uint8).clone()
+        for i in range(0, 300, 7):
+            pool[int(b.table[i, 0]), 0] = 0xFF  # the first token, which every row sees
+        out = b.run(gemm, table).view(300, 20, 16, dim)
+        pool.copy_(kept)
+        others = torch.arange(300, device=DEV) % 7 != 0
+        assert torch.equal(out[others], clean[others]) and torch.isnan(out[~others]).all()
