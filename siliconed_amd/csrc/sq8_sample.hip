@@ -259,10 +259,10 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
         unsigned bin, cnt, has;  // the bin, those before it and in it
         uint64_t sum;            // and the weights before it
     };
-    auto place = [&](bool sums, unsigned need, double T) {  // after scan()
+    auto place = [&](bool sums, unsigned need, double T, double T2) {  // after scan(); T2 ≥ T: the bin that holds both
         if (tid == 0) found = BINS;
         __syncthreads();
-        const bool here = sums ? (double)before_sum < T && (double)scan_sum >= T : before_cnt < need && scan_cnt >= need;
+        const bool here = sums ? (double)before_sum < T && (double)scan_sum >= T2 : before_cnt < need && scan_cnt >= need;
         if (here) {
             found = tid;
             found_cnt = before_cnt;
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
             for (int e = 0; e < 2; ++e)
                 if (half[e] > -INFINITY) atomicAdd(&cnt[bin_of(half[e])], 1u);
             scan();
-            const Place at = place(false, min(by_count ? min(max((unsigned)want, 64u), 900u) : 900u, all_cnt), 0.0);
+            const Place at = place(false, min(by_count ? min(max((unsigned)want, 64u), 900u) : 900u, all_cnt), 0.0, 0.0);
             last = at.bin;
         }
         double T = 0.0;
@@ -341,12 +341,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
         bool k_list = false, p_list = false;
 
         // From a bin of distances (by `with`) to one key, over the list or the row.
-        auto refine = [&](Place at, float with, bool sums, unsigned need, double goal, bool in_list) {
+        // (`goal2` ≥ goal, among few: the key that holds both, or 0.)
+        auto refine = [&](Place at, float with, bool sums, unsigned need, double goal, double goal2, bool in_list) {
             by = with;
             if (in_list && at.has <= FEW) {
                 // Few in the bin: gathered behind the bins' sums, and every one compared with the others.
                 uint64_t *const keys = acc + BINS, *const weights = keys + FEW;
-                if (tid == 0) gathered = 0;
+                if (tid == 0) gathered = found = 0;
                 __syncthreads();
                 for (unsigned i = lane; i < listed; i += 64) {
                     const uint32_t key = (uint32_t)(segment[i] >> 32);
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                         same += k == key;
                         if (sums) sum += k > key ? weights[j] : 0;
                     }
-                    const bool here = sums ? (double)sum < goal && (double)(sum + same * weights[tid]) >= goal : more < need && more + same >= need;
+                    const bool here = sums ? (double)sum < goal && (double)(sum + same * weights[tid]) >= goal2 : more < need && more + same >= need;
                     if (here) {  // (its equals write the same)
                         found = key;
                         found_cnt = more;
@@ -419,7 +420,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                     });
                 }
                 scan();
-                const Place q = place(sums, need - c.above, goal - (double)c.sum);
+                const Place q = place(sums, need - c.above, goal - (double)c.sum, goal - (double)c.sum);
                 // (Rounding may leave the goal a hair past the bin's sums: then its last keys.)
                 const unsigned bin = q.bin < BINS ? q.bin : range >> sh;
                 if (q.bin < BINS) {
@@ -527,23 +528,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                 const double share_of = (double)fmaxf(top_p, 0.0f), held_sum = (double)sum_bins;
                 const double low_T = fmax(share_of * (held_sum + fmax(est - off, 0.0)), 1.0), high_T = fmax(share_of * (held_sum + est + off), 1.0);
                 if (held_sum >= high_T && held) {
-                    const Place lo = place(true, 0, low_T), hi = place(true, 0, high_T);
-                    if (lo.bin == hi.bin && lo.has <= FEW) {
-                        const unsigned bc = before_cnt, sc = scan_cnt;
-                        const uint64_t bs = before_sum, ss = scan_sum;
-                        Cut cuts[2];
-#pragma unroll 1
-                        for (int i = 0; i < 2; ++i) {
-                            const double goal = i == 0 ? low_T : high_T;
-                            Cut c = refine(lo, by, true, 0, goal, true);
-                            const uint64_t w = weight(of_key(c.key));
-                            c.keep = w ? (unsigned)fmin(fmax(ceil((goal - (double)c.sum) / (double)w), 1.0), (double)c.ties) : c.ties;
-                            if (i == 0) cuts[0] = c;
-                            else cuts[1] = c;
+                    const Place both = place(true, 0, low_T, high_T);
+                    if (both.bin < BINS && both.has <= FEW) {
+                        const Cut c = refine(both, by, true, 0, low_T, high_T, true);
+                        const uint64_t w = weight(of_key(c.key));
+                        auto keep = [&](double goal) { return w ? (unsigned)fmin(fmax(ceil((goal - (double)c.sum) / (double)w), 1.0), (double)c.ties) : c.ties; };
+                        settled = c.key != 0 && keep(low_T) == keep(high_T);
+                        if (settled) {
+                            cut = c;
+                            cut.keep = keep(low_T);
                         }
-                        settled = cuts[0].key == cuts[1].key && cuts[0].keep == cuts[1].keep;
-                        if (settled) cut = cuts[0];
-                        before_cnt = bc; scan_cnt = sc; before_sum = bs; scan_sum = ss;
                     }
                 }
                 if (settled) {
@@ -566,7 +560,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
             if (wide && by_sum && !by_count) total = sum_bins;
             bool short_of = false;  // what is looked for lies past the bins
             if (by_count && k_place.bin == BINS) {
-                k_place = place(false, want, 0.0);
+                k_place = place(false, want, 0.0, 0.0);
                 if (k_place.bin == BINS) {
                     if (last == BINS - 1 && (wide || short_row)) {
                         // Fewer logits than top_k: all of them.
@@ -584,7 +578,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                         // The sum of the first top_k; the bins are needed again for the cut by sums.
                         const unsigned bc = before_cnt, sc = scan_cnt;
                         const uint64_t bs = before_sum, ss = scan_sum;
-                        const Cut c = refine(k_place, k_by, false, want, 0.0, k_list);
+                        const Cut c = refine(k_place, k_by, false, want, 0.0, 0.0, k_list);
                         // The weights above the cut: over the source.
                         uint64_t sum = 0;
                         auto take = [&](uint32_t key, float x) { sum += key > c.key ? weight(x) : 0; };
@@ -611,7 +605,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
             if (by_sum && !short_of && p_place.bin == BINS) {
                 T = fmax((double)fmaxf(top_p, 0.0f) * (double)total, 1.0);
                 if ((double)sum_bins >= T) {
-                    p_place = place(true, 0, T);
+                    p_place = place(true, 0, T, T);
                     p_by = by;
                     p_list = held;
                 } else if (wide || (short_row && last == BINS - 1)) {
@@ -633,14 +627,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
             from_list = p_list;  // settled above
         } else if (by_sum && p_place.bin < BINS) {
             const Cut k_cut = cut;
-            cut = refine(p_place, p_by, true, 0, T, p_list);
+            cut = refine(p_place, p_by, true, 0, T, T, p_list);
             const uint64_t w = weight(of_key(cut.key));
             const double left = T - (double)cut.sum;
             cut.keep = w ? (unsigned)fmin(fmax(ceil(left / (double)w), 1.0), (double)cut.ties) : cut.ties;
             if (by_count && k_place.bin < BINS && cut.key == k_cut.key) cut.keep = min(cut.keep, want - k_cut.above);
             from_list = p_list;
         } else if (by_count && k_place.bin < BINS) {
-            if (!by_sum) cut = refine(k_place, k_by, false, want, 0.0, k_list);
+            if (!by_sum) cut = refine(k_place, k_by, false, want, 0.0, 0.0, k_list);
             cut.keep = min(cut.ties, want - cut.above);
             from_list = k_list;
         } else {
