@@ -19,9 +19,10 @@
 // nucleus goes by bins over the row.
 //
 // 128 rows of 128 000 fp32 logits, every option set, take 37 µs: the first pass runs at the memory's rate (11 µs), the second, from
-// the last cache level, 14, the rest is barriers and scans. One row of 32 000 with a nucleus 23 to 27 µs, of which the list and the
+// the last cache level, 14, the rest is barriers and scans. One row of 32 000 with a nucleus 23 to 26 µs, of which the list and the
 // fp32 sum are 10 (one CU's vector ALU) and the exact sum, one time in ten, 15 more. A nucleus past the list: 2 rows of 157 420
-// 240 µs, two passes of 64-bit exponentials of 50 each, three of keys; another workgroup a row would halve it. With sixteen
+// 236 µs, two passes of 64-bit exponentials of 50 each, three of keys; another workgroup a row would halve it. 64 rows of 128 000
+// with min_p alone 46 (92 where runs of logits under what it leaves were not passed over). With sixteen
 // waves a row, whose registers spilled, and an atomic a listed logit the first two were 102 and 47.
 #include <hip/hip_runtime.h>
 
@@ -647,7 +648,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
     // ---- by index: the first whose running sum of values over what is taken passes a goal ----
     // value(key, logit, index) of every logit; sums of chunks of indices, then the chunk in which they reach the goal, by one wave.
     const int chunks = (p.vocab + R::CHUNK - 1) / R::CHUNK;
-    auto select = [&](auto &&value, auto &&goal, uint64_t &all) {
+    // (Logits under `least_x` have value 0: a run of nothing else is passed over.)
+    auto select = [&](float least_x, auto &&value, auto &&goal, uint64_t &all) {
         __syncthreads();
         if (from_list) {
             // Few that count: each sums the others before it.
@@ -701,14 +703,19 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                 float x[E];
                 const int i = c * R::CHUNK + lane * E;
                 row.load(i, x);
+                float most = x[0];
+#pragma unroll
+                for (int e = 1; e < E; ++e) most = fmaxf(most, x[e]);
                 uint64_t v = 0;
+                if (__any(most >= least_x)) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const uint64_t one = value(key_of(x[e]), x[e], (uint32_t)(i + e));
-                    v += x[e] > -INFINITY ? one : 0;
+                    for (int e = 0; e < E; ++e) {
+                        const uint64_t one = value(key_of(x[e]), x[e], (uint32_t)(i + e));
+                        v += x[e] > -INFINITY ? one : 0;
+                    }
+#pragma unroll
+                    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
                 }
-#pragma unroll
-                for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
                 if (lane == 0) acc[c] = v;
             }
         }
@@ -759,11 +766,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
     uint32_t last_at = 0xFFFFFFFFu;  // of the logits equal to the cut's, the last index kept
     if (cut.keep < cut.ties) {
         const unsigned need = cut.keep;
-        last_at = select([&](uint32_t key, float, uint32_t) { return (uint64_t)(key == cut.key); },
+        last_at = select(of_key(cut.key), [&](uint32_t key, float, uint32_t) { return (uint64_t)(key == cut.key); },
                          [&](uint64_t s, uint64_t) { return s >= need; }, total);
     }
     const double least_weight = (double)min_p * (double)(1ull << ONE), u = (double)fminf(fmaxf(p.uniform[b], 0.0f), 0x1.fffffep-1f);
+    // What min_p leaves lies above top + t · ln(min_p), less a ten-thousandth of t for all roundings (a weight's is half a unit of
+    // thousands).
+    float least_x = cut.key != 0 ? of_key(cut.key) : -INFINITY;
+    if (min_p > 1e-9f && top < INFINITY) least_x = fmaxf(least_x, top - t * (1e-4f - logf(min_p)) - 1e-6f * fabsf(top));
+    if (!(least_x <= top)) least_x = -INFINITY;
     const uint32_t token = select(
+        least_x,
         [&](uint32_t key, float x, uint32_t at) -> uint64_t {
             const uint64_t w = weight(x);
             const bool taken = key > cut.key || (key == cut.key && at <= last_at);
