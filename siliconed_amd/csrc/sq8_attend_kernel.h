@@ -189,9 +189,9 @@ attend_kernel(const AttendArgs p) {
         auto scalar = [](float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); };
         float unit_scale = p.scale * (S::F8 && p.k_scale ? p.k_scale[kvh] : 1.0f);
         const bool minus = unit_scale < 0.0f;  // then Q is taken with the other sign: the largest score is that of S
-        unit_scale = fabsf(unit_scale) * (capped ? 1.0f / p.softcap : LOG2E);
-        if (unit_scale < 1e-30f) unit_scale = 1e-30f;  // (0 times a masked score would be a NaN)
-        unit_scale = scalar(unit_scale);
+        unit_scale = scalar(fabsf(unit_scale) * (capped ? 1.0f / p.softcap : LOG2E));
+        // Scaled before the masked ones become -inf: capped scores, and those by a scale of 0 (or a NaN), which -inf would make NaNs of.
+        const bool early = capped || !(unit_scale >= 0x1p-126f);
         bf16x8 q[STEPS];
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
@@ -425,13 +425,17 @@ attend_kernel(const AttendArgs p) {
             for (int e = 1; e < 16; ++e) m = fmaxf(m, s[e]);
             return m;
         };
-        // Where some row does not see some token of the wave's, or scores are capped: the scores as they count, and the largest.
+        // Where some row does not see some token of the wave's, or scores are scaled early: the scores as they count, and the largest.
         auto edge = [&](f32x16 &s, float &most, float &scale, int mine, uint32_t bad, int v_from) {
             if (capped) {
                 const float cap = scalar(p.softcap * LOG2E);
                 scale = 1.0f;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] = cap * tanh_rel(s[e] * unit_scale);
+            } else if (early) {
+                scale = 1.0f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] *= unit_scale;
             }
             const int hi_rel = hi - mine - 4 * h, lo_rel = lo - mine - 4 * h;
 #pragma unroll
@@ -491,7 +495,7 @@ attend_kernel(const AttendArgs p) {
             const int k_from = slot_of(n + 1), v_from = slot_of(n);
             const int mine = base + t * TT + wave_token;  // the wave's first token
             float scale = unit_scale;
-            if (capped || mine + 31 > hi_min || mine < lo_max || bad.any()) edge(s, most, scale, mine, (uint32_t)bad.from(wave_token), v_from);
+            if (early || mine + 31 > hi_min || mine < lo_max || bad.any()) edge(s, most, scale, mine, (uint32_t)bad.from(wave_token), v_from);
             raise(most * scale);
             float from = top == -INFINITY ? 0.0f : top;
             if (far) {
