@@ -439,8 +439,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
         };
         for (int pass = 0; pass < 2; ++pass) {
             double rest32 = 0.0;  // what lies past the bins, from exponentials in fp32
-            const float per32 = fminf(1.4426950408889634f / t, 3e38f);
             const bool sum_all = by_sum && !by_count && !wide;
+            // (Only where fp32 holds what the exponents are made of: at temperatures past these, 1 / t may be 0, which -inf would make
+            // NaNs of, or a difference past the largest number may weigh something.)
+            const bool estimated = sum_all && t >= 0x1p-100f && t <= 0x1p100f;
+            const float per32 = 1.4426950408889634f / t;
             auto put_in = [&](float x) {
                 const unsigned bin = bin_of(x);
                 if (bin > last) return;
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                 // The list first.
                 const float rough = top - (float)(last + 2) / by;  // (no less than any that is in; by 0 gives -inf or a NaN)
                 row.runs([&](int i, const float (&x)[E]) {
-                    if (!sum_all) {
+                    if (!estimated) {
                         float m = x[0];
 #pragma unroll
                         for (int e = 1; e < E; ++e) m = fmaxf(m, x[e]);
@@ -465,7 +468,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
                         hit[e] = __ballot(in[e]);
                         all |= hit[e];
                     }
-                    if (sum_all) {
+                    if (estimated) {
                         float w[E], sum = 0.0f;
 #pragma unroll
                         for (int e = 0; e < E; ++e) w[e] = in[e] ? 0.0f : __builtin_amdgcn_exp2f((x[e] - top) * per32);
@@ -524,11 +527,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
             if (sum_all) {
                 // The cut for the least and the most that the rest can be: a weight in fp32 is within 2^-17 of its value (its exponent,
                 // at most 45, three roundings; the exponential; eight in a sum), and a whole number of them within one. The same cut
-                // for both is the cut; else the rest is summed exactly.
+                // for both is the cut; else, or without an estimate, the rest is summed exactly.
                 const double est = (double)of_all((uint64_t)(rest32 * 0x1p43)), off = est * 0x1p-16 + (double)p.vocab + WAVES * 64.0;
                 const double share_of = (double)fmaxf(top_p, 0.0f), held_sum = (double)sum_bins;
-                const double low_T = fmax(share_of * (held_sum + fmax(est - off, 0.0)), 1.0), high_T = fmax(share_of * (held_sum + est + off), 1.0);
-                if (held_sum >= high_T && held) {
+                const double low_T = estimated ? fmax(share_of * (held_sum + fmax(est - off, 0.0)), 1.0) : 0.0, high_T = fmax(share_of * (held_sum + est + off), 1.0);
+                if (estimated && held_sum >= high_T && held) {
                     const Place both = place(true, 0, low_T, high_T);
                     if (both.bin < BINS && both.has <= FEW) {
                         const Cut c = refine(both, by, true, 0, low_T, high_T, true);
