@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
     const float top_p = p.top_p ? p.top_p[b] : 1.0f, min_p = p.min_p ? p.min_p[b] : 0.0f;
     const int want = p.top_k ? p.top_k[b] : 0;
     const bool by_count = want > 0 && want < p.vocab, by_sum = !(top_p >= 1.0f);
-    const bool greedy = !(t > 0.0f) || (by_count && want == 1);
+    const bool greedy = !(t > 0.0f) || (by_count && want == 1) || min_p > 1.0f;  // (no weight is more than 1: the first of the order is left)
 
     // ---- the largest logit, and each thread's own two ----
     float half[2] = {-INFINITY, -INFINITY};  // of the logits at even places, and at odd ones

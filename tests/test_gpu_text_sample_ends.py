@@ -1,4 +1,4 @@
-"""The draw at the ends of what a temperature may be, against the definition in 64 bits (test_gpu_text_sample.py)."""
+"""The draw at the ends of what a temperature and a min_p may be, against the definition in 64 bits (test_gpu_text_sample.py)."""
 import math
 
 import pytest
@@ -50,3 +50,21 @@ def test_a_nucleus_at_temperatures_of_next_to_nothing(gemm, vocab):
         row = (x * t).float()
         for p in (0.05, 0.5, 0.97):
             run(gemm, row, uniform(g, 4), [t] * 4, None, [p] * 4, what=f"tiny {t} top_p {p}")
+
+
+@TYPES
+@pytest.mark.parametrize("vocab", [3, 700, 9000])
+def test_a_min_p_above_one_keeps_the_first(gemm, dtype, vocab):
+    """No weight is as much, and the first of the order is always kept: of equal largest logits the lowest index alone."""
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.randn(6, vocab, generator=g).to(dtype)
+    x[0, 1:] = 9.0
+    x[1, vocab // 2::2] = 7.5
+    x[2] = -2.5
+    x[3, vocab - 2:] = math.inf
+    x[4, ::2] = -math.inf
+    m = [1.5, 1.0 + 2.0 ** -23, math.inf, 2.0, 3e38, 1.0001]
+    for u in (0.0, 0.5, 0.999):
+        run(gemm, x, [u] * 6, None, None, None, m, what=f"min_p {u}")
+        run(gemm, x, [u] * 6, [2.0, 0.5, math.inf, 1.0, 1e-3, 1.0], [0, 2, 5, vocab, 3, 0], [0.9, 1.0, 0.5, 0.7, 0.99, 0.0], m, what=f"all {u}")
+        run(gemm, x, [u] * 6, None, None, None, [1.0] * 6, what=f"one {u}")  # every one of the largest
