@@ -360,10 +360,13 @@ attend_kernel(const AttendArgs p) {
         for (int d = 0; d < 2; ++d)
             v_at[d] = S::STAGES * S::MATRIX + (wave_token + v_token) * S::ROW + (((4 * d + v_run) ^ v_key) * 16) + 8 * (lane & 1);
         auto keys = [&](int at, int j) { return *reinterpret_cast<const bf16x8 *>(lds + at + k_at[j & 3] + (j >> 2) * 128); };
+        // Four tokens of a lane, from `token` + 4h on.
+        auto four = [&](int at, int token, int d) {
+            const uint8_t *const from = lds + at + v_at[d & 1] + (d >> 1) * 128 + token * S::ROW;
+            return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)from));
+        };
         auto values = [&](int at, int ks, int d) {
-            const uint8_t *const from = lds + at + v_at[d & 1] + (d >> 1) * 128 + 16 * ks * S::ROW;
-            const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)from));
-            const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4)(from + 8 * S::ROW)));
+            const u32x2 x = four(at, 16 * ks, d), y = four(at, 16 * ks + 8, d);
             return u32x4{x[0], x[1], y[0], y[1]};
         };
 
@@ -426,7 +429,7 @@ attend_kernel(const AttendArgs p) {
             return m;
         };
         // Where some row does not see some token of the wave's, or scores are scaled early: the scores as they count, and the largest.
-        auto edge = [&](f32x16 &s, float &most, float &scale, int mine, uint32_t bad, int v_from) {
+        auto edge = [&](f32x16 &s, float &most, float &scale, int mine, uint32_t bad, int v_from, bool partly) {
             if (capped) {
                 const float cap = scalar(p.softcap * LOG2E);
                 scale = 1.0f;
@@ -437,6 +440,10 @@ attend_kernel(const AttendArgs p) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[e] *= unit_scale;
             }
+            if (!partly) {
+                most = largest(s);
+                return;
+            }
             const int hi_rel = hi - mine - 4 * h, lo_rel = lo - mine - 4 * h;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
@@ -445,17 +452,25 @@ attend_kernel(const AttendArgs p) {
                 s[e] = dead ? -INFINITY : s[e];
             }
             most = largest(s);
-            // A token that some rows do not see may hold an infinity or a NaN, which 0 times it would not hide: wild_rows.
+            // A token that some rows do not see may hold an infinity or a NaN, which 0 times it would not hide: wild_rows. (One that all
+            // see belongs in their sums.)
+            const int past = hi_min - mine, before = lo_max - mine;
+            uint32_t unseen = (past < 0 ? ~0u : past < 31 ? ~1u << past : 0u) | (before > 31 ? ~0u : before > 0 ? (1u << before) - 1 : 0u);
+            unseen = unseen >> (4 * h);
             uint32_t found = 0;
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
+            for (int n = 0; n < 4; ++n) {  // tokens 8n + 4h on
+                u32x2 some = {0, 0};
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
-                    const u32x4 v = values(v_from, ks, d);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) found |= unbounded(v[i]);
+                    const u32x2 v = four(v_from, 8 * n, d);
+                    some[0] |= unbounded(v[0]);
+                    some[1] |= unbounded(v[1]);
                 }
-            wild = wild || __any((found & 0x80008000u) != 0);
+                some = some & u32x2{0x80008000u, 0x80008000u};
+                found |= (some[0] >> 15 | some[0] >> 30 | some[1] >> 13 | some[1] >> 28) & unseen >> (8 * n) & 15u;
+            }
+            wild = wild || __any(found != 0);
         };
 
         // ---- the tiles: beside tile t's softmax run the scores of t + 1 ----
@@ -495,7 +510,8 @@ attend_kernel(const AttendArgs p) {
             const int k_from = slot_of(n + 1), v_from = slot_of(n);
             const int mine = base + t * TT + wave_token;  // the wave's first token
             float scale = unit_scale;
-            if (early || mine + 31 > hi_min || mine < lo_max || bad.any()) edge(s, most, scale, mine, (uint32_t)bad.from(wave_token), v_from);
+            const bool partly = mine + 31 > hi_min || mine < lo_max || bad.any();
+            if (early || partly) edge(s, most, scale, mine, (uint32_t)bad.from(wave_token), v_from, partly);
             raise(most * scale);
             float from = top == -INFINITY ? 0.0f : top;
             if (far) {
