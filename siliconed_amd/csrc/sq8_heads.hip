@@ -159,7 +159,9 @@ hipError_t launch_norm_heads(HeadsArgs p, bool e4m3, hipStream_t stream) {
     const int run = (p.dim | p.rot) % 16 == 0 ? 8 : (p.dim | p.rot) % 8 == 0 ? 4 : 1;
     p.lanes_log = 0;
     while (p.lanes_log < 6 && (1 << p.lanes_log) < p.dim / (2 * run)) ++p.lanes_log;
-    const int64_t heads = (int64_t)(p.q_heads + (p.kc ? 2 : 1) * p.kv_heads) * p.tokens, per_group = 256 >> p.lanes_log;
+    const int64_t each = (int64_t)p.q_heads + (int64_t)(p.kc ? 2 : 1) * p.kv_heads;
+    if (each > INT32_MAX) return hipErrorInvalidValue;  // a token's heads are counted in 32 bits
+    const int64_t heads = each * p.tokens, per_group = 256 >> p.lanes_log;
     const int64_t blocks = (heads + per_group - 1) / per_group;
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
     const int dest = !p.kc ? BESIDE : e4m3 ? CACHE_E4M3 : CACHE_BF16;

@@ -640,7 +640,9 @@ hipError_t launch_attention(const PagedArgs &p, int groups, hipStream_t stream) 
 hipError_t launch_append_kv(const AppendArgs &p, bool e4m3, hipStream_t stream) {
     if (p.tokens == 0) return hipSuccess;
     const int run = (p.dim | p.rot) % 16 == 0 ? 8 : (p.dim | p.rot) % 8 == 0 ? 4 : 1;
-    const int64_t units = (int64_t)(p.q_heads + 2 * p.kv_heads) * (p.dim / (2 * run)) * p.tokens;
+    const int64_t each = (int64_t)p.q_heads + 2 * (int64_t)p.kv_heads, per_head = p.dim / (2 * run);
+    if (each > INT32_MAX / per_head) return hipErrorInvalidValue;  // a token's units are counted in 32 bits
+    const int64_t units = each * per_head * p.tokens;
     const int64_t blocks = (units + 255) / 256;
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks);

@@ -1,0 +1,25 @@
+"""Sizes at the end of what 32 bits count: refused before anything is launched, or done in parts. (Expanded tensors: their rows or heads
+all lie in one place, so that such sizes take no memory.)"""
+import pytest
+import torch
+
+import siliconed_amd as sq
+from siliconed_amd import _abi as abi
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF = torch.bfloat16
+MOST = (1 << 31) - 1
+
+
+@pytest.mark.parametrize("dim", [64, 24, 10])
+def test_more_heads_of_a_token_than_32_bits_count(gemm, dim):
+    many = torch.zeros(1, 1, dim, dtype=BF, device=DEV).expand(1, MOST, dim)
+    few = torch.zeros(1, 2, dim, dtype=BF, device=DEV)
+    at, table = torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros(1, dim, device=DEV)
+    cache = sq.PagedCache(*(torch.zeros(1, 16, 2, dim, dtype=BF, device=DEV) for _ in "kv"))
+    for append in (gemm.append_kv, gemm.norm_append_kv):
+        with pytest.raises(abi.Unsupported):
+            append(many, few, few, cache, at, at, table, q_out=many)
+    with pytest.raises(abi.Unsupported):
+        gemm.norm_rotate(many, few, q_out=many, k_out=few)
