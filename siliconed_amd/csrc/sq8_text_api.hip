@@ -165,6 +165,8 @@ int run_attend(sq8_ctx *ctx, sq8::AttendArgs &p, const uint16_t *q, int64_t q_to
     else if (softcap > 0.0f && softcap < 0x1p-60f) softcap = 0x1p-60f;
     // A window that no sequence fills is none (and a place less it stays in 32 bits).
     if (p.window > (p.pages ? (double)p.max_pages * p.page : (double)tokens)) p.window = 0;
+    // (A chunk's first row lies up to `tokens` places before its sequence's first, its window's start as many before that.)
+    if (p.pages && (double)tokens + p.window > INT32_MAX) return SQ8_EUNSUPPORTED;
     DeviceScope scope(ctx->device);
     if (scope.error != hipSuccess) return hip_status(scope.error);
     p.q = q; p.out = out;

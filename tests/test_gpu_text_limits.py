@@ -23,3 +23,13 @@ def test_more_heads_of_a_token_than_32_bits_count(gemm, dim):
             append(many, few, few, cache, at, at, table, q_out=many)
     with pytest.raises(abi.Unsupported):
         gemm.norm_rotate(many, few, q_out=many, k_out=few)
+
+
+def test_windows_that_begin_before_what_32_bits_count(gemm):
+    """2^31 - 4097 new tokens of a sequence that holds fewer: with a window their places less it would wrap."""
+    tokens = MOST - 4096
+    q = torch.zeros(1, 1, 8, dtype=BF, device=DEV).expand(tokens, 1, 8)
+    cache = sq.PagedCache(*(torch.zeros(1, 64, 1, 8, dtype=BF, device=DEV) for _ in "kv"))
+    pages, length = torch.zeros(1, 256, dtype=torch.int32, device=DEV), torch.full((1,), 16000, dtype=torch.int32, device=DEV)
+    with pytest.raises(abi.Unsupported):
+        gemm.chunk_attention(q, cache, pages, length, window=16000, out=q)
