@@ -799,10 +799,25 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
 }  // namespace
 
 hipError_t launch_sample(const SampleArgs &p, hipStream_t stream) {
-    if (p.rows == 0) return hipSuccess;
-    if (p.bf16) hipLaunchKernelGGL(sample_kernel<true>, dim3(p.rows), dim3(THREADS), 0, stream, p);
-    else hipLaunchKernelGGL(sample_kernel<false>, dim3(p.rows), dim3(THREADS), 0, stream, p);
-    return hipGetLastError();
+    // A launch is of fewer than 2^32 threads: of more, the runtime would start what is left of their number without it, and say nothing.
+    constexpr int64_t MOST = UINT32_MAX / THREADS;
+    for (int64_t first = 0; first < p.rows; first += MOST) {
+        SampleArgs part = p;
+        part.logits = static_cast<const char *>(p.logits) + first * p.ld * (p.bf16 ? 2 : 4);
+        part.uniform += first;
+        if (p.temperature) part.temperature += first;
+        if (p.top_p) part.top_p += first;
+        if (p.min_p) part.min_p += first;
+        if (p.top_k) part.top_k += first;
+        part.tokens += first;
+        if (p.logprobs) part.logprobs += first;
+        const unsigned rows = (unsigned)(p.rows - first < MOST ? p.rows - first : MOST);
+        if (p.bf16) hipLaunchKernelGGL(sample_kernel<true>, dim3(rows), dim3(THREADS), 0, stream, part);
+        else hipLaunchKernelGGL(sample_kernel<false>, dim3(rows), dim3(THREADS), 0, stream, part);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace sq8

@@ -33,3 +33,16 @@ def test_windows_that_begin_before_what_32_bits_count(gemm):
     pages, length = torch.zeros(1, 256, dtype=torch.int32, device=DEV), torch.full((1,), 16000, dtype=torch.int32, device=DEV)
     with pytest.raises(abi.Unsupported):
         gemm.chunk_attention(q, cache, pages, length, window=16000, out=q)
+
+
+def test_more_rows_of_logits_than_one_launch_takes(gemm):
+    """A launch is of fewer than 2^32 threads: 2^23 rows of 512. Two equal logits: the first for numbers under a half."""
+    rows = (1 << 23) + 3
+    x, u = torch.zeros(rows, 2, device=DEV), torch.rand(rows, device=DEV)
+    k = torch.zeros(rows, dtype=torch.int32, device=DEV)
+    k[::5] = 1
+    tokens, logprobs = gemm.sample_tokens(x, u, top_k=k)
+    want = (u >= 0.5).int()
+    want[::5] = 0
+    assert torch.equal(tokens, want)
+    assert (logprobs[::5] == 0).all() and ((logprobs + 0.6931472).abs() < 1e-6)[k == 0].all()
