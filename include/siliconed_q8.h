@@ -476,7 +476,8 @@ int sq8_paged_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_
 
 /* **Heads normed, turned and appended in one pass.** sq8_append_kv with every query and key head normed before it is
  * turned: y = x / sqrt(mean x² + eps) · w over the head's values, w = q_norm or k_norm (fp32 [dim]; NULL: that kind is not
- * normed), values as they are. All fp32, one rounding, of the turned value. dim even and up to 512 (else SQ8_EUNSUPPORTED). */
+ * normed), values as they are. All fp32, one rounding, of the turned value. dim even and up to 512, heads of all tokens together
+ * what a launch of 2^32 threads holds (2^29 of 128 values; else SQ8_EUNSUPPORTED). */
 int sq8_norm_append_kv(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head,
                        const uint16_t *k, int64_t k_token, int64_t k_head, const uint16_t *v, int64_t v_token, int64_t v_head,
                        uint16_t *q_out, int64_t qo_token, int64_t qo_head, const sq8_paged_cache *cache,
@@ -501,7 +502,8 @@ int sq8_norm_rotate(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_
  * kv_heads). Rows of no sequence are left as they were; a token that is not seen may hold anything. Scores, maxima and sums
  * fp32; the probabilities are rounded to bf16 (by 2^-8 of each at most) for their product with v, or in chunks of few rows,
  * which wait for memory, to 17 bits. dim up to 256, a multiple of 8; q, k and v rows 16-byte aligned, out 8-byte (else
- * SQ8_EUNSUPPORTED). No host copy of `starts` is needed: the call may be captured. */
+ * SQ8_EUNSUPPORTED, as are more tiles than a launch of 2^32 threads has: 2^24 sequences times kv heads). No host copy of
+ * `starts` is needed: the call may be captured. */
 int sq8_prompt_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head,
                          const uint16_t *k, int64_t k_token, int64_t k_head, const uint16_t *v, int64_t v_token, int64_t v_head,
                          const int32_t *starts, int sequences, float scale, float softcap, int window, int causal,

@@ -163,7 +163,7 @@ hipError_t launch_norm_heads(HeadsArgs p, bool e4m3, hipStream_t stream) {
     if (each > INT32_MAX) return hipErrorInvalidValue;  // a token's heads are counted in 32 bits
     const int64_t heads = each * p.tokens, per_group = 256 >> p.lanes_log;
     const int64_t blocks = (heads + per_group - 1) / per_group;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    if (blocks > kMostThreads / 256) return hipErrorInvalidValue;
     const int dest = !p.kc ? BESIDE : e4m3 ? CACHE_E4M3 : CACHE_BF16;
     return run == 8   ? launch_heads<8>(p, dest, (unsigned)blocks, stream)
            : run == 4 ? launch_heads<4>(p, dest, (unsigned)blocks, stream)

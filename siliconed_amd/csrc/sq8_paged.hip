@@ -644,7 +644,7 @@ hipError_t launch_append_kv(const AppendArgs &p, bool e4m3, hipStream_t stream) 
     if (each > INT32_MAX / per_head) return hipErrorInvalidValue;  // a token's units are counted in 32 bits
     const int64_t units = each * per_head * p.tokens;
     const int64_t blocks = (units + 255) / 256;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    if (blocks > kMostThreads / 256) return hipErrorInvalidValue;
     const dim3 grid((unsigned)blocks);
     if (e4m3 && run == 8) hipLaunchKernelGGL((append_kv_kernel<8, true>), grid, dim3(256), 0, stream, p);
     else if (e4m3 && run == 4) hipLaunchKernelGGL((append_kv_kernel<4, true>), grid, dim3(256), 0, stream, p);

@@ -799,8 +799,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs p) 
 }  // namespace
 
 hipError_t launch_sample(const SampleArgs &p, hipStream_t stream) {
-    // A launch is of fewer than 2^32 threads: of more, the runtime would start what is left of their number without it, and say nothing.
-    constexpr int64_t MOST = UINT32_MAX / THREADS;
+    constexpr int64_t MOST = kMostThreads / THREADS;
     for (int64_t first = 0; first < p.rows; first += MOST) {
         SampleArgs part = p;
         part.logits = static_cast<const char *>(p.logits) + first * p.ld * (p.bf16 ? 2 : 4);

@@ -10,6 +10,8 @@
 namespace sq8 {
 
 constexpr int F8_GROUP = 128;  // values of K that share a scale
+// A launch's threads. (Of 2^32 or more the runtime starts what is left of their number without it, and says nothing.)
+constexpr int64_t kMostThreads = UINT32_MAX;
 
 // Correctly rounded quotients by one divisor s: from r = fl(1/s), q0 = fl(y·r) is within two ulps, one step
 // q1 = q0 + r·(y − q0·s) within one, and the next is then the rounded quotient (Markstein 1990: r correctly rounded,
@@ -197,6 +199,7 @@ struct AttendPlan {
     int groups, share, narrow;
     int64_t part_bytes, marks;
     double tiles;               // of all units, at most
+    int threads;                // of a workgroup
 };
 AttendPlan attend_plan(const AttendArgs &p, bool e4m3, int cus);
 hipError_t launch_attend(const AttendArgs &p, const AttendPlan &plan, bool e4m3, hipStream_t stream);

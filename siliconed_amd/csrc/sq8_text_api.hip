@@ -175,7 +175,7 @@ int run_attend(sq8_ctx *ctx, sq8::AttendArgs &p, const uint16_t *q, int64_t q_to
     p.tokens = tokens; p.sequences = sequences;
     sq8::page_divisor(p.page, p.page_mul, p.page_shift);
     const sq8::AttendPlan plan = sq8::attend_plan(p, e4m3, ctx->cus);
-    if (plan.tiles > INT32_MAX / 2) return SQ8_EUNSUPPORTED;
+    if (plan.tiles > INT32_MAX / 2 || (!plan.share && (double)plan.groups * plan.threads > (double)sq8::kMostThreads)) return SQ8_EUNSUPPORTED;
     p.share = plan.share;
     if (plan.part_bytes > 0) {
         int st = reserve(ctx, ctx->part, (size_t)plan.part_bytes);

@@ -110,7 +110,7 @@ int64_t paged_part_bytes(const PagedArgs &p, int groups) {
 int64_t paged_marks(const PagedArgs &p) { return (int64_t)MARK * p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16); }
 
 AttendPlan attend_plan(const AttendArgs &p, bool e4m3, int cus) {
-    AttendPlan plan = {128, 0, 0, 0, 0, 0, 0.0};
+    AttendPlan plan = {128, 0, 0, 0, 0, 0, 0.0, 0};
     if (p.sequences <= 0 || p.tokens <= 0) return plan;
     const int dp = attend_dim(p.dim);
     const int64_t each = ((int64_t)p.tokens * p.group + p.sequences - 1) / p.sequences;  // rows of a sequence and kv head, if all are alike
@@ -145,6 +145,7 @@ AttendPlan attend_plan(const AttendArgs &p, bool e4m3, int cus) {
     const int tokens = plan.narrow ? 128 : attend_tokens(wt);
     const double run = plan.share ? (double)((longest + tokens - 1) / tokens + 1) : 1.0;
     plan.tiles = units * run;
+    plan.threads = plan.narrow ? 256 : 64 * waves;
     if (!plan.share) {
         plan.groups = (int)std::min(plan.tiles, 2e9);
         return plan;

@@ -46,3 +46,24 @@ def test_more_rows_of_logits_than_one_launch_takes(gemm):
     want[::5] = 0
     assert torch.equal(tokens, want)
     assert (logprobs[::5] == 0).all() and ((logprobs + 0.6931472).abs() < 1e-6)[k == 0].all()
+
+
+def test_more_heads_than_one_launch_takes(gemm):
+    tokens, dim = (1 << 28) + 1, 64
+    q = torch.zeros(1, 1, dim, dtype=BF, device=DEV).expand(tokens, 4, dim)
+    with pytest.raises(abi.Unsupported):
+        gemm.norm_rotate(q, q_out=q)
+    k = q[:, :1]
+    slots = torch.full((tokens,), -1, dtype=torch.int32, device=DEV)
+    cache = sq.PagedCache(*(torch.zeros(1, 16, 1, dim, dtype=BF, device=DEV) for _ in "kv"))
+    table = torch.zeros(1, dim, device=DEV)
+    for append in (gemm.append_kv, gemm.norm_append_kv):
+        with pytest.raises(abi.Unsupported):
+            append(q, k, k, cache, slots, slots, table, q_out=q)
+
+
+def test_more_prompts_than_one_launch_takes(gemm):
+    """A tile of each kv head for every sequence, were none empty."""
+    q, k = torch.zeros(4, 8, 64, dtype=BF, device=DEV), torch.zeros(4, 8, 64, dtype=BF, device=DEV)
+    with pytest.raises(abi.Unsupported):
+        gemm.prompt_attention(q, k, k, torch.zeros((1 << 21) + 2, dtype=torch.int32, device=DEV))
