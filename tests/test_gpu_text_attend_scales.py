@@ -88,3 +88,14 @@ def test_a_tiny_scale_of_large_heads(gemm, by, scale):
     b.cache.k.copy_((b.cache.k.float() * by).to(BF))
     b.values = [[(k * by).to(BF).float(), v] for k, v in b.values]
     check_chunk(gemm, b, scale=scale)
+
+
+@pytest.mark.parametrize("cap", [1e-20, 1e-39, 1e-45])
+def test_a_cap_of_nothing_averages(gemm, cap):
+    """Scores within 1e-18 of 0: every exponential is 1 in fp32."""
+    q, k, v = (normal(torch.Generator().manual_seed(7 + h), 150, h, 64).to(BF) for h in (8, 2, 2))
+    assert torch.equal(gemm.prompt_attention(q, k, v, softcap=cap), gemm.prompt_attention(q, k, v, scale=0.0))
+    for dtype in (BF, F8):
+        b = Batch([(1, 1), (9, 140), (40, 500)], 8, 2, 128, 16, dtype)
+        for table in (None, b.roomy()):
+            assert torch.equal(b.run(gemm, table, softcap=cap), b.run(gemm, table, scale=0.0))
