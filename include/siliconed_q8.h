@@ -465,7 +465,7 @@ int sq8_append_kv(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_he
  * softcap) unless softcap is 0 (or infinite: no cap); query head h reads kv head h / (q_heads / kv_heads). q, out bf16
  * [batch, q_heads, dim]; table int32 [batch, max_pages] (page indices in order; leading dimension table_row), lengths
  * int32 [batch], cut to [0, max_pages · page]. A length of 0 gives zeros; tokens on a page index outside the pools count as masked; masked
- * rows may hold anything. Scores, maxima and sums fp32, the probabilities to 17 bits in their product with v.
+ * rows may hold anything. Scores, maxima and sums fp32, the probabilities to 16 bits in their product with v.
  * dim up to 256, a multiple of 8 (past 128 and for e4m3: of 16); 16-byte aligned rows (else SQ8_EUNSUPPORTED). Partial
  * results of split sequences go to the context's scratch (sq8_linear says when it grows; its size follows from the
  * arguments here, not from the lengths), with sq8_linear_f8's counters. */
@@ -501,7 +501,7 @@ int sq8_norm_rotate(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_
  * capped to softcap · tanh(s_t / softcap) unless softcap is 0 (or infinite); query head h reads kv head h / (q_heads /
  * kv_heads). Rows of no sequence are left as they were; a token that is not seen may hold anything. Scores, maxima and sums
  * fp32; the probabilities are rounded to bf16 (by 2^-8 of each at most) for their product with v, or in chunks of few rows,
- * which wait for memory, to 17 bits. dim up to 256, a multiple of 8; q, k and v rows 16-byte aligned, out 8-byte (else
+ * which wait for memory, to 16 bits. dim up to 256, a multiple of 8; q, k and v rows 16-byte aligned, out 8-byte (else
  * SQ8_EUNSUPPORTED, as are more tiles than a launch of 2^32 threads has: 2^24 sequences times kv heads). No host copy of
  * `starts` is needed: the call may be captured. */
 int sq8_prompt_attention(sq8_ctx *ctx, const uint16_t *q, int64_t q_token, int64_t q_head,

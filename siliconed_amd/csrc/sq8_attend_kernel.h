@@ -22,19 +22,20 @@
 // order for each slot. What it took, of 8192 causal tokens with 32 heads on 8 of 128: keys a tile ahead of the values and no
 // spilled register (a reload waits for all loads under way) from 1.2 ms to 636 µs; the compiler's own waits out of the way (its
 // LDS loads made transposed reads of other slots wait for them) and maxima and conversions kept between the matrix instructions,
-// 571; addresses stepped instead of multiplied, 549; rows
-// written in whole runs, 533.
+// 571; addresses stepped instead of multiplied, 571 to 554 on another card; rows written in whole runs, 563 to 556 on a third.
 //
-// There it does 1030 TFLOP/s of the products that the mask leaves, where a large library product of normal values does 1384, both
-// at the power limit (1.8 GHz of 2.4): the matrix pipes are busy 48 % of the cycles, the vector ALUs 40 %. Without exponentials
-// it would take 8 % less, without loads 5 %, without three quarters of the second product 21 %: no one thing bounds it. Tried
+// There it takes 544 to 602 µs, from card to card, 1010 to 910 TFLOP/s of the products that the mask leaves, where a large library
+// product of normal values does 1384, both at the power limit (1.8 GHz of 2.4): the matrix pipes are busy 45 % of the cycles, the
+// vector ALUs 40 %. Without exponentials it would take 8 % less, without loads 5 %, without three quarters of the second
+// product 21 %: no one thing bounds it. Tried
 // and not faster: outputs a tile late beside the next tile's softmax (6 % slower), reads six instructions ahead, wave
 // priorities, places turned so that no read meets another in a bank (the counted conflicts went from 68 M to none, the time stayed),
-// loads between the matrix instructions. 4608 tokens of 24 heads, not causal, take 275 µs: 432 tiles on 256 CUs, two rounds
-// of which the second is two thirds full. 2048 new tokens behind 30 720 in pages of 64, 1.10 ms (970 TFLOP/s).
+// loads between the matrix instructions. 4608 tokens of 24 heads, not causal, take 281 to 306 µs: 432 tiles on 256 CUs, two rounds
+// of which the second is two thirds full. 2048 new tokens behind 30 720 in pages of 64, 1.13 to 1.22 ms (950 to 870 TFLOP/s). Capped scores
+// take a hyperbolic tangent each: of 30, the two calls take 1120 and 2170 µs (with values looked over in every tile 1275 and 2940).
 //
 // Tiles of rows (sq8_text_plan.hip): 256, 128 or 64 for prompts, by how many there are for the card's CUs (100 tokens, 32 heads on
-// 8: 11.6 µs with 64: the launch, 3 µs of loads one after another, four
+// 8: 11.8 µs with 64: the launch, 3 µs of loads one after another, four
 // tiles whose instructions are read for the first time, the join of two waves); 256 and 128 for chunks, and for few rows sq8_chunk.hip.
 #pragma once
 
@@ -380,7 +381,8 @@ attend_kernel(const AttendArgs p) {
             for (int e = 0; e < 16; ++e) o[d][e] = 0.0f;
 
         // The probabilities, two a dword in the order of the second product's tokens, rounded to bf16: by as much of the output as
-        // its own rounding is, which the sums of many hide and a second product for the rest would cost half the time again.
+        // its own rounding is. A second product for what that leaves out costs a third more time (8192 causal tokens 601 and
+        // 806 µs, 12 packed prompts 222 and 279); chunks of few rows, which wait for memory, have it.
         struct Weights {
             u32x4 w[2];
         };

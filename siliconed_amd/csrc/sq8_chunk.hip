@@ -12,12 +12,12 @@
 //
 // A tile is 128 tokens, 32 a wave; the tiles of all units are shared out evenly, and units that several workgroups have are joined
 // by the last (sq8_attend_device.h). Softmax in fp32, its maximum moved only past 8 powers of two; probabilities in two bf16
-// parts, which leave out 2^-17 of one at most. A new token's rows see different tokens: only tiles at the ends of what they see
+// parts, which leave out 2^-16 of one at most. A new token's rows see different tokens: only tiles at the ends of what they see
 // compare places, and a value there that some rows do not see is looked over for infinities and NaN (wild_rows).
 //
 // 32 sequences of 4 new tokens behind ragged contexts of up to 8192, 32 heads on 8 of 128 in e4m3 (287 MB), take 81 µs, 3.5 TB/s
 // (69 from the last cache level), of which some ten are the start and the join; 32 of 8 behind 8192 in bf16 (1074 MB) 263, 4.1 TB/s;
-// 16 tokens of one sequence behind 500 12.1 µs, a chain of latencies (with tiles of 64 rows 33: a quarter of the workgroups, and
+// 16 tokens of one sequence behind 500 12.1 µs, a chain of latencies (with tiles of 64 rows 26: a quarter of the workgroups, and
 // four times the join). Before, tiles of 64 rows in LDS took 170 and 33 for the first and the last. How many rows share what is read: sq8_text_plan.hip.
 // A row's lookups of pages that 16 tokens do not fill cost 5 to 10 % more.
 #include "sq8_attend_device.h"

@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(256) append_kv_kernel(const AppendArgs p) {
 // One pass over the cache with the running maximum and sum of the softmax, both fp32. The maximum is moved only when a
 // score passes it by 8 powers of two, so a probability may be up to 2^8 of what it will be divided by: the same bits
 // of it, and the sums rescaled hardly ever. For their product with v the probabilities are split into two bf16 numbers each,
-// 2^-17 of one at most left out: rounded to one they would cost the output as much as its own rounding to bf16.
+// 2^-16 of one at most left out: rounded to one they would cost the output as much as its own rounding to bf16.
 //
 // Bound by the cache's bytes. The query heads of one kv head (up to 16; more take several passes) are the columns of
 // both products, on v_mfma_f32_16x16x32_bf16:
